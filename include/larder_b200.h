@@ -339,6 +339,68 @@ int lb2_qsa_select(const void* q, const void* pooled, int64_t pool_bstride, int 
                    int64_t offset, int cr, int k, float div, void* workspace, size_t workspace_bytes, int32_t* top,
                    void* stream);
 
+/* ------------------------------------------------------------------------------------------------------------
+ * The serving steps around a paged 8-bit KV cache (no counterpart in the reference, whose caches are contiguous
+ * 16-bit arrays): rotary positions, append, attention over the pages, causal attention over packed prompts.
+ *
+ * Rotary positions: y = x with the first R of each head's D values rotated by the row's position.
+ *   x, y      [B, H, T, D]  strides x_st / y_st [0..2] for B, H, T; unit stride on D; y may be x (same strides)
+ *   positions int32 [B, T] (batch stride pos_st; 0 for one row of positions), >= 0
+ *   turns     64-bit words [R / 2] on the device: pair i turns by position * turns[i] / 2^64 of a full turn (mod 1)
+ * Pairs are (i, i + R / 2), or (2 i, 2 i + 1) with `interleaved`; y0 = amp (x0 cos - x1 sin), y1 = amp (x1 cos +
+ * x0 sin), fp32, rounded once. `inverse` negates the angle: the gradient of the forward call with the same amp.
+ * dtype LB2_F32 / BF16 / F16; D even, up to 1024; R even, 2 <= R <= D. 16-byte accesses where D and R are multiples of
+ * two 16-byte groups and bases and strides are 16-byte aligned, else element accesses. */
+int lb2_rope(const void* x, const int64_t* x_st, void* y, const int64_t* y_st, const int32_t* positions, int64_t pos_st,
+             const uint64_t* turns, int B, int H, int T, int D, int R, int dtype, int interleaved, int inverse,
+             float amp, void* stream);
+
+/* Append to the paged 8-bit cache.
+ *   pages  e4m3 codes [num_pages, 2 (K, V), Hkv, page, D], contiguous, 16-byte aligned; scales fp32 [num_pages, 2, Hkv]
+ *   table  int32 [B, max_pages] (row stride table_st): sequence b's tokens i page .. i page + page - 1 are in
+ *          pages[table[b][i]]
+ *   k, v   [B, Hkv, T, D] (strides k_st / v_st for B, H, T; unit on D), dtype LB2_F32 / BF16 / F16: sequence b's new
+ *          tokens, as its positions start[b] .. start[b] + n_b - 1; n_b = T, or lens[b] (int32 [B]), or, with cu
+ *          (int32 [B + 1]), the rows cu[b] .. cu[b + 1] - 1 of one packed row axis ([1, Hkv, T, D])
+ *   turns  as lb2_rope with R dims (keys are rotated by their positions before they are rounded), or R = 0
+ * A held value is code * scale, scale the least power of two s with max |x| <= 448 s over the page's tokens of that head
+ * (K and V apart). A page that already holds tokens (start[b] inside it) keeps max(s, s_new); its codes are divided by
+ * s_new / s where it grew, exactly but for e4m3 subnormals. start[b] at a page's beginning starts the page afresh: its
+ * former scale and codes count for nothing. What lies past the new tokens in a page is left as it is. Infinities are
+ * held as +-448 s, NaN as NaN; neither sets the scale. A page id outside [0, num_pages), or a position past the table's
+ * end, is skipped and lb2_status reports LB2_EINVAL. No two sequences of a call may append to the same page. */
+int lb2_kv8_append(uint8_t* pages, float* scales, const void* k, const int64_t* k_st, const void* v, const int64_t* v_st,
+                   const int32_t* table, int64_t table_st, const int32_t* start, const int32_t* lens, const int32_t* cu,
+                   const uint64_t* turns, int B, int Hkv, int T, int D, int R, int page, int num_pages, int max_pages,
+                   int dtype, int interleaved, float amp, void* stream);
+
+/* Attention over the paged 8-bit cache: o = softmax(scale q K^T) V over each sequence's first kv_len[b] tokens (int32
+ * [B]; this call's own among them).
+ *   q, o [B, Hq, T, D], strides q_st / o_st for B, H, T; unit on D; dtype LB2_BF16 / F16, or LB2_F32 (exact CUDA-core
+ *   kernel); pages, scales, table as lb2_kv8_append. causal: row t sees keys 0 .. kv_len[b] - T + t, else all; a row
+ *   that sees none gives zeros. D in {64, 128, 256}, page in {16, 32, 64, 128}, any Hq / Hkv and T.
+ *   workspace: lb2_kv8_attend_workspace_size() bytes, 256-byte aligned, any contents. Calls that share a workspace must
+ *   be ordered on one stream.
+ * Codes past kv_len are never used, whatever they hold. A page id outside [0, num_pages) is not read: lb2_status
+ * reports LB2_EINVAL and the sequence's output is unspecified. */
+size_t lb2_kv8_attend_workspace_size(int B, int Hq, int Hkv, int T, int D, int page, int max_pages);
+int lb2_kv8_attend(const void* q, const int64_t* q_st, const uint8_t* pages, const float* scales, const int32_t* table,
+                   int64_t table_st, const int32_t* kv_len, void* o, const int64_t* o_st, int B, int Hq, int Hkv, int T,
+                   int D, int page, int num_pages, int max_pages, int dtype, float scale, int causal, void* workspace,
+                   size_t workspace_bytes, void* stream);
+
+/* Causal attention over S whole prompts packed on one row axis: prompt s is rows cu[s] .. cu[s + 1] - 1 (int32
+ * [S + 1] on the device, rising from 0 to T; empty prompts allowed), and row i of a prompt sees its rows 0 .. i.
+ *   q, o [Hq, T, D], k, v [Hkv, T, D]: strides [0..1] for H, T; unit on D; dtype LB2_BF16 / F16 (row strides multiples
+ *   of 8 elements, 16-byte aligned bases) or LB2_F32 (exact CUDA-core kernel); D in {64, 128, 256}.
+ *   workspace: lb2_attn_packed_workspace_size(S, T) bytes, 256-byte aligned, any contents.
+ * Rows of no prompt (cu[S] < T) give zeros. No value of one prompt reaches another's rows, infinities and NaN among
+ * them, nor a later row's an earlier row. */
+size_t lb2_attn_packed_workspace_size(int S, int T);
+int lb2_attn_packed(const void* q, const int64_t* q_st, const void* k, const int64_t* k_st, const void* v,
+                    const int64_t* v_st, void* o, const int64_t* o_st, const int32_t* cu, int S, int Hq, int Hkv, int T,
+                    int D, int dtype, float scale, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

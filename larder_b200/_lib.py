@@ -69,6 +69,14 @@ SIGNATURES = {
     "lb2_qsa_select_workspace_size": ([_i, _i, _i], _sz),
     "lb2_qsa_select": ([_p, _p, ctypes.c_int64, _i, _i, _i, _i, _i, ctypes.c_int64, _i, _i, _f, _p, _sz, _p, _p],
                        _i),
+    "lb2_rope": ([_p, _i64p, _p, _i64p, _p, ctypes.c_int64, _p, _i, _i, _i, _i, _i, _i, _i, _i, _f, _p], _i),
+    "lb2_kv8_append": ([_p, _p, _p, _i64p, _p, _i64p, _p, ctypes.c_int64, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _i,
+                        _i, _i, _f, _p], _i),
+    "lb2_kv8_attend_workspace_size": ([_i, _i, _i, _i, _i, _i, _i], _sz),
+    "lb2_kv8_attend": ([_p, _i64p, _p, _p, _p, ctypes.c_int64, _p, _p, _i64p, _i, _i, _i, _i, _i, _i, _i, _i, _i, _f, _i,
+                        _p, _sz, _p], _i),
+    "lb2_attn_packed_workspace_size": ([_i, _i], _sz),
+    "lb2_attn_packed": ([_p, _i64p, _p, _i64p, _p, _i64p, _p, _i64p, _p, _i, _i, _i, _i, _i, _i, _f, _p, _sz, _p], _i),
 }
 
 _lib = None

@@ -21,6 +21,9 @@
 #include "kv_runs.cuh"
 #include "attn_tiles.cuh"
 #include "gdn_glue.cuh"
+#include "rope.cuh"
+#include "kv8.cuh"
+#include "attn_rows.cuh"
 
 namespace lb2 {
 
@@ -1450,6 +1453,216 @@ int lb2_qsa_select(const void* q, const void* pooled, int64_t pool_bstride, int 
   LB2_CUDA(cudaLaunchKernelEx(&cfg, topk_for(qsasel::topk_per(n_blocks, cl)), static_cast<const float*>(scores),
                               n_blocks, k, top));
   return LB2_OK;
+}
+
+// ------------------------------------------------------------------------------------------------ rotary positions
+
+}  // extern "C"
+
+namespace {
+
+template <typename T, int V>
+int rope_launch(const rope::Params& p0, cudaStream_t st) {
+  rope::Params p = p0;
+  // A block takes about 1024 units (four a thread), whole tokens of as many heads as that allows; small calls are cut
+  // finer so that they fill the SMs.
+  const int upr = p.D / (2 * V), rows = p.B * p.T;
+  p.hg = p.H;
+  p.tok = std::max(1, std::min(rows, 1024 / std::max(1, upr * p.H)));
+  const int smem = p.tok * (p.R / 2) * int(sizeof(float2));
+  const dim3 grid(unsigned((rows + p.tok - 1) / p.tok), unsigned((p.H + p.hg - 1) / p.hg));
+  rope::rope_kernel<T, V><<<grid, rope::THREADS, smem, st>>>(p);
+  LB2_CUDA(cudaGetLastError());
+  return LB2_OK;
+}
+
+template <typename T>
+int rope_run(const rope::Params& p, cudaStream_t st) {
+  constexpr int V = 16 / int(sizeof(T));
+  bool wide = p.D % (2 * V) == 0 && p.R % (2 * V) == 0 && aligned16(p.x) && aligned16(p.y);
+  for (int i = 0; i < 3; ++i) wide = wide && p.x_st[i] % V == 0 && p.y_st[i] % V == 0;
+  return wide ? rope_launch<T, V>(p, st) : rope_launch<T, 1>(p, st);
+}
+
+}  // namespace
+
+extern "C" {
+
+int lb2_rope(const void* x, const int64_t* x_st, void* y, const int64_t* y_st, const int32_t* positions,
+             int64_t pos_st, const uint64_t* turns, int B, int H, int T, int D, int R, int dtype, int interleaved,
+             int inverse, float amp, void* stream) {
+  LB2_CHECK_ARG(B >= 0 && H >= 0 && T >= 0, "rope: shape");
+  LB2_CHECK_ARG(D >= 2 && D <= 1024 && D % 2 == 0, "rope: an even head dim up to 1024");
+  LB2_CHECK_ARG(R >= 2 && R <= D && R % 2 == 0, "rope: an even number of rotated dims, at most the head dim");
+  if (B == 0 || H == 0 || T == 0) return LB2_OK;
+  LB2_CHECK_ARG(x && y && positions && turns && x_st && y_st, "rope: missing argument");
+  LB2_CHECK_ARG(int64_t(B) * T < (int64_t(1) << 31), "rope: too many rows");
+  rope::Params p{};
+  p.x = x;
+  p.y = y;
+  for (int i = 0; i < 3; ++i) p.x_st[i] = x_st[i], p.y_st[i] = y_st[i];
+  p.pos = positions;
+  p.p_st = pos_st;
+  p.turns = turns;
+  p.B = B, p.H = H, p.T = T, p.D = D, p.R = R;
+  p.interleaved = interleaved != 0;
+  p.inverse = inverse != 0;
+  p.amp = amp;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  switch (dtype) {
+    case LB2_F32: return rope_run<float>(p, st);
+    case LB2_BF16: return rope_run<__nv_bfloat16>(p, st);
+    case LB2_F16: return rope_run<__half>(p, st);
+    default: return fail(LB2_EINVAL, "rope: dtype");
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ paged 8-bit cache
+
+static int kv8_shape(int B, int Hkv, int T, int D, int page, int num_pages, int max_pages, const char* what) {
+  const std::string w = what;
+  LB2_CHECK_ARG(B >= 0 && Hkv > 0 && T >= 0, w + ": shape");
+  LB2_CHECK_ARG(D == 64 || D == 128 || D == 256, w + ": head dim must be 64, 128 or 256");
+  LB2_CHECK_ARG(page == 16 || page == 32 || page == 64 || page == 128, w + ": pages of 16, 32, 64 or 128 tokens");
+  LB2_CHECK_ARG(num_pages > 0 && max_pages > 0, w + ": empty pool or page table");
+  LB2_CHECK_ARG(int64_t(max_pages) * page <= 0x7fffffff, w + ": sequences of at most 2^31 - 1 tokens");
+  return LB2_OK;
+}
+
+int lb2_kv8_append(uint8_t* pages, float* scales, const void* k, const int64_t* k_st, const void* v,
+                   const int64_t* v_st, const int32_t* table, int64_t table_st, const int32_t* start,
+                   const int32_t* lens, const int32_t* cu, const uint64_t* turns, int B, int Hkv, int T, int D, int R,
+                   int page, int num_pages, int max_pages, int dtype, int interleaved, float amp, void* stream) {
+  const int rc = kv8_shape(B, Hkv, T, D, page, num_pages, max_pages, "kv8_append");
+  if (rc) return rc;
+  LB2_CHECK_ARG(R >= 0 && R <= D && R % 2 == 0, "kv8_append: an even number of rotated dims, at most the head dim");
+  LB2_CHECK_ARG(R == 0 || turns != nullptr, "kv8_append: rotated dims need their turns");
+  LB2_CHECK_ARG(!(lens && cu), "kv8_append: lens or cu, not both");
+  LB2_CHECK_ARG(dtype == LB2_F32 || dtype == LB2_BF16 || dtype == LB2_F16, "kv8_append: dtype");
+  if (B == 0 || T == 0) return LB2_OK;
+  LB2_CHECK_ARG(pages && scales && k && v && k_st && v_st && table && start, "kv8_append: missing argument");
+  LB2_CHECK_ARG(aligned16(pages), "kv8_append: pages must be 16-byte aligned");
+  LB2_CHECK_ARG(Hkv < 32768, "kv8_append: too many heads");
+  kv8::AppendParams p{};
+  p.pages = pages;
+  p.scales = scales;
+  p.table = table;
+  p.table_st = table_st;
+  p.x[0] = k, p.x[1] = v;
+  for (int i = 0; i < 3; ++i) p.st[0][i] = k_st[i], p.st[1][i] = v_st[i];
+  p.start = start;
+  p.lens = lens;
+  p.cu = cu;
+  p.turns = turns;
+  p.B = B, p.Hkv = Hkv, p.T = T, p.D = D, p.R = R;
+  p.page = page, p.num_pages = num_pages, p.max_pages = max_pages;
+  p.touched = int((int64_t(T) + page - 2) / page) + 1;
+  p.interleaved = interleaved != 0;
+  p.amp = amp;
+  LB2_CHECK_ARG(int64_t(B) * p.touched < (int64_t(1) << 31), "kv8_append: too many rows");
+  const dim3 grid(unsigned(B) * unsigned(p.touched), unsigned(2 * Hkv));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (dtype == LB2_F32) kv8::append_kernel<float><<<grid, 128, 0, st>>>(p);
+  else if (dtype == LB2_BF16) kv8::append_kernel<__nv_bfloat16><<<grid, 128, 0, st>>>(p);
+  else kv8::append_kernel<__half><<<grid, 128, 0, st>>>(p);
+  LB2_CUDA(cudaGetLastError());
+  return LB2_OK;
+}
+
+}  // extern "C"
+
+template <typename T>
+static int paged_rows(const arows::PagedParams& p, int D, cudaStream_t st) {
+  const int64_t blocks = (int64_t(p.B) * p.Hq * p.T + 3) / 4;
+  LB2_CHECK_ARG(blocks < (int64_t(1) << 31), "kv8_attend: too many rows");
+  if (D == 64) arows::paged_kernel<T, 64><<<unsigned(blocks), 128, 0, st>>>(p);
+  else if (D == 128) arows::paged_kernel<T, 128><<<unsigned(blocks), 128, 0, st>>>(p);
+  else arows::paged_kernel<T, 256><<<unsigned(blocks), 128, 0, st>>>(p);
+  LB2_CUDA(cudaGetLastError());
+  return LB2_OK;
+}
+
+extern "C" {
+
+size_t lb2_kv8_attend_workspace_size(int B, int Hq, int Hkv, int T, int D, int page, int max_pages) {
+  if (B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || T <= 0 || D <= 0 || page <= 0 || max_pages <= 0) return 0;
+  return 256;
+}
+
+int lb2_kv8_attend(const void* q, const int64_t* q_st, const uint8_t* pages, const float* scales, const int32_t* table,
+                   int64_t table_st, const int32_t* kv_len, void* o, const int64_t* o_st, int B, int Hq, int Hkv, int T,
+                   int D, int page, int num_pages, int max_pages, int dtype, float scale, int causal, void* workspace,
+                   size_t workspace_bytes, void* stream) {
+  const int rc = kv8_shape(B, Hkv, T, D, page, num_pages, max_pages, "kv8_attend");
+  if (rc) return rc;
+  LB2_CHECK_ARG(Hq > 0 && Hq % Hkv == 0, "kv8_attend: Hq must be a multiple of Hkv");
+  LB2_CHECK_ARG(dtype == LB2_F32 || dtype == LB2_BF16 || dtype == LB2_F16, "kv8_attend: dtype");
+  if (B == 0 || T == 0) return LB2_OK;
+  LB2_CHECK_ARG(q && q_st && pages && scales && table && kv_len && o && o_st, "kv8_attend: missing argument");
+  LB2_CHECK_ARG(aligned16(pages), "kv8_attend: pages must be 16-byte aligned");
+  LB2_CHECK_ARG(workspace != nullptr &&
+                    workspace_bytes >= lb2_kv8_attend_workspace_size(B, Hq, Hkv, T, D, page, max_pages),
+                "kv8_attend: workspace too small");
+  arows::PagedParams p{};
+  p.q = q;
+  p.o = o;
+  for (int i = 0; i < 3; ++i) p.q_st[i] = q_st[i], p.o_st[i] = o_st[i];
+  p.pages = pages;
+  p.scales = scales;
+  p.table = table;
+  p.table_st = table_st;
+  p.kv_len = kv_len;
+  p.B = B, p.Hq = Hq, p.Hkv = Hkv, p.T = T;
+  p.page = page, p.num_pages = num_pages, p.max_pages = max_pages;
+  p.causal = causal != 0;
+  p.scale = scale;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (dtype == LB2_F32) return paged_rows<float>(p, D, st);
+  return dtype == LB2_BF16 ? paged_rows<__nv_bfloat16>(p, D, st) : paged_rows<__half>(p, D, st);
+}
+
+// ------------------------------------------------------------------------------------------------ packed prompts
+
+}  // extern "C"
+
+template <typename T>
+static int packed_rows(const arows::PackedParams& p, int D, cudaStream_t st) {
+  const int64_t blocks = (int64_t(p.Hq) * p.T + 3) / 4;
+  LB2_CHECK_ARG(blocks < (int64_t(1) << 31), "attn_packed: too many rows");
+  if (D == 64) arows::packed_kernel<T, 64><<<unsigned(blocks), 128, 0, st>>>(p);
+  else if (D == 128) arows::packed_kernel<T, 128><<<unsigned(blocks), 128, 0, st>>>(p);
+  else arows::packed_kernel<T, 256><<<unsigned(blocks), 128, 0, st>>>(p);
+  LB2_CUDA(cudaGetLastError());
+  return LB2_OK;
+}
+
+extern "C" {
+
+size_t lb2_attn_packed_workspace_size(int S, int T) {
+  if (S <= 0 || T <= 0) return 0;
+  return 256;
+}
+
+int lb2_attn_packed(const void* q, const int64_t* q_st, const void* k, const int64_t* k_st, const void* v,
+                    const int64_t* v_st, void* o, const int64_t* o_st, const int32_t* cu, int S, int Hq, int Hkv, int T,
+                    int D, int dtype, float scale, void* workspace, size_t workspace_bytes, void* stream) {
+  LB2_CHECK_ARG(S >= 1 && Hq > 0 && Hkv > 0 && T >= 0, "attn_packed: shape");
+  LB2_CHECK_ARG(Hq % Hkv == 0, "attn_packed: Hq must be a multiple of Hkv");
+  LB2_CHECK_ARG(D == 64 || D == 128 || D == 256, "attn_packed: head dim must be 64, 128 or 256");
+  LB2_CHECK_ARG(dtype == LB2_F32 || dtype == LB2_BF16 || dtype == LB2_F16, "attn_packed: dtype");
+  if (T == 0) return LB2_OK;
+  LB2_CHECK_ARG(q && k && v && o && q_st && k_st && v_st && o_st && cu, "attn_packed: missing argument");
+  LB2_CHECK_ARG(workspace != nullptr && workspace_bytes >= lb2_attn_packed_workspace_size(S, T),
+                "attn_packed: workspace too small");
+  arows::PackedParams p{};
+  p.q = q, p.k = k, p.v = v, p.o = o;
+  for (int i = 0; i < 2; ++i) p.q_st[i] = q_st[i], p.k_st[i] = k_st[i], p.v_st[i] = v_st[i], p.o_st[i] = o_st[i];
+  p.cu = cu;
+  p.S = S, p.Hq = Hq, p.Hkv = Hkv, p.T = T;
+  p.scale = scale;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (dtype == LB2_F32) return packed_rows<float>(p, D, st);
+  return dtype == LB2_BF16 ? packed_rows<__nv_bfloat16>(p, D, st) : packed_rows<__half>(p, D, st);
 }
 
 }  // extern "C"
