@@ -1,0 +1,647 @@
+// Attention of a few query rows over the paged 8-bit KV cache (kv8.cuh), split over the keys: HBM-bound.
+//
+//   o = softmax(scale q (code_k s_k)^T) (code_v s_v)
+//
+// A persistent CTA an SM streams its run of 64-key tiles. The call's tiles, ordered (b, KV head, row block, tile), are cut
+// into equal runs, one a CTA, cut again where a (b, head, row block) ends, so that every SM streams the same number of
+// bytes whatever the lengths; the partials (max, sum, unnormalised o) of a run's pieces are merged by combine_kernel,
+// launched behind as a programmatic dependent. All G T query rows of a KV head share each pass over its codes.
+//
+// The codes reach shared memory as they lie (TMA boxes of a page's rows, 128-byte swizzled, 64-byte at D = 64), 1 byte a
+// value, and turn into f16 MMA operands in registers: every e4m3 value is an f16 value, so nothing is rounded there, and
+// cvt.rn.f16x2.e4m3x2 runs at 64 lanes a clock on an SM (measured), 128 codes against the 23 codes a clock that HBM
+// delivers an SM. Products run on mma.sync m16n8k16 f16 (fp32 accumulate) with the keys, then the head dim, in M = 16 and
+// the query rows in N = 8 columns. (mma.sync m16n8k32 on e4m3 itself would need the query and the weights split into two
+// or three e4m3 terms.)
+//  - S^T = K Q^T: a lane takes 16 consecutive bytes of a key, its share of four k-steps: the dims inside a 64-byte segment
+//    are permuted alike in the query's fragments. The key of row q of an 8-row block is chosen so that neighbouring quads
+//    read different halves of the 128-byte lines (no bank conflicts).
+//  - O^T += V^T P^T: ldmatrix.trans on 16-bit units gives a lane two dims of two keys; one byte permute and two
+//    conversions make them the operand pairs of two dims (rows quad and quad + 8 of the MMA are dims 2 quad, 2 quad + 1).
+// Query rows go to f16 exactly: a row is shifted by a power of two (its largest value to [2^14, 2^15)), which the score's
+// factor undoes; bf16's 8 bits fit f16's 11 down to 2^-28 of the row's largest value.
+//
+// Softmax in base 2, fp32. The weights carry the values' scale: p'_n = 2^(s_n + log2 s_v - m), m the running maximum of
+// s_n + log2 s_v, and l = sum p'_n / s_v, so that o = sum p'_n code_n / l; the weights of pages with scales far apart thus
+// never leave f16's range, where p' is rounded (2^-11 relative; the sums are fp32).
+//
+// A NaN code under a weight of 0 would spread to rows that do not see it: values past the length are zeroed in shared
+// memory; with several rows of different horizons, combine_kernel takes a row that came out NaN again, key by key
+// (attn_rows.cuh), which reads only what the row sees.
+#pragma once
+
+#include "attn_rows.cuh"
+#include "common.cuh"
+#include "kv8.cuh"
+
+namespace lb2 {
+namespace kv8attn {
+
+constexpr int BK = 64;       // keys a tile
+constexpr int MAX_B = 1024;  // sequences a launch (the prefix table in shared memory); larger batches go in several
+constexpr int STATUS = 112;  // where (lb2_status): 112 page id, 113.. waits
+
+// NT: 8-row tiles of query rows a warp; RG: row groups (sets of four warps taking the same tile for other rows); KG: key
+// groups (sets of four warps taking alternate tiles).
+template <int D, int NT, int RG, int KG>
+struct Cfg {
+  static constexpr int RP = 8 * NT * RG;  // rows of a block, padded
+  static constexpr int WARPS = 4 * RG * KG;
+  static constexpr int THREADS = (WARPS + 1) * 32;
+  static constexpr int BW = D < 128 ? D : 128;  // bytes a box row
+  static constexpr int TILE = BK * D;           // bytes of a K (or V) tile
+  static constexpr int STAGE = 2 * TILE;
+  static constexpr bool Q_REGS = NT * D <= 256;
+  static constexpr int QBYTES = Q_REGS ? 0 : RG * NT * (D / 64) * 32 * 32;
+  static constexpr int PART_REGS = NT * (D / 16 + 1);           // float4 a lane: O and (m, l) of a warp's rows
+  static constexpr int PART = WARPS / 2 * PART_REGS * 32 * 16;  // half the warps' parts
+  static constexpr int FIXED = QBYTES + PART + (2 * MAX_B + 1) * 4 + 1024 + 1024;
+  static constexpr int FIT = (232448 - FIXED) / (STAGE + 48);
+  static constexpr int STAGES = (FIT > 10 ? 10 : FIT) / KG * KG;
+  static constexpr int Q_OFF = STAGES * STAGE;
+  static constexpr int PART_OFF = Q_OFF + QBYTES;
+  static constexpr int SC_OFF = PART_OFF + PART;                 // [STAGES][4 slices][K, V] fp32
+  static constexpr int PREFIX_OFF = SC_OFF + STAGES * 32;        // [MAX_B + 1]
+  static constexpr int LENS_OFF = PREFIX_OFF + (MAX_B + 1) * 4;  // [MAX_B]
+  static constexpr int BAR_OFF = (LENS_OFF + MAX_B * 4 + 15) / 16 * 16;
+  static constexpr int SMEM = BAR_OFF + 2 * STAGES * 8 + 16 + 1024;
+  static_assert(STAGES >= 2 && SMEM <= 232448, "shared memory budget");
+};
+
+struct Params {
+  arows::PagedParams a;  // the call's arguments
+  float* ws_o;           // [slots][rpb][D]
+  float* ws_ml;          // [slots][rpb][2]
+  int G, rows;           // query rows a KV head: G T
+  int nrb, rpb;          // row blocks a KV head, rows a block
+  int grid;
+  int box;     // tokens a TMA box: min(page, BK)
+  int lpage;   // log2(page)
+  int wide_q;  // q rows may be read 16 bytes at a time
+  float scale_log2;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ void mma16816(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t movm_t(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+__device__ __forceinline__ void ldsm_x4_t(uint32_t addr, uint32_t* r) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+
+// Byte offset of (key row r, 16-byte chunk c) in a tile: boxes of BW bytes a row, [D / BW][BK][BW], swizzled.
+template <int D>
+__device__ __forceinline__ uint32_t at(int r, int c) {
+  if constexpr (D == 64) return uint32_t(r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
+  return uint32_t((c >> 3) * (BK * 128) + r * 128 + (((c ^ r) & 7) << 4));
+}
+
+// The key (0..7) in row i of an 8-key block: consecutive rows differ in bit 2 (bit 0 at D = 64), see above.
+template <int D>
+__device__ __forceinline__ int key_of(int i) {
+  if constexpr (D == 64) return i;
+  return (i >> 1) | ((i & 1) << 2);
+}
+
+// How many runs the call's tiles are cut into: one a CTA, but none without a tile (the grid is sized by the table's
+// width, the lengths are read on the device). Every slot between a pair's first and last run is thus written.
+__device__ __forceinline__ int64_t runs_of(const Params& p, int64_t total) { return min(int64_t(p.grid), total); }
+
+// One piece of work: tiles [i0, i1) of sequence b for head-and-row-block hb (KV head hb / nrb, block hb % nrb).
+struct Item {
+  int b, hb, i0, i1, len, slot;
+};
+
+// The CTA's items in order; prefix[b] counts, for one head and row block, the tiles of the sequences before b.
+struct Sched {
+  const int* prefix;
+  const int* lens;
+  int B, H, cur, end;
+  __device__ __forceinline__ Sched(const Params& p, const int* prefix_, const int* lens_)
+      : prefix(prefix_), lens(lens_), B(p.a.B), H(p.a.Hkv * p.nrb) {
+    const int64_t total = int64_t(prefix[B]) * H, runs = runs_of(p, total), c = blockIdx.x;
+    cur = c < runs ? int(c * total / runs) : 0;
+    end = c < runs ? int((c + 1) * total / runs) : 0;
+  }
+  __device__ __forceinline__ bool next(Item& it) {
+    if (cur >= end) return false;
+    const int key = cur / H;
+    int lo = 0, hi = B;  // the largest b with prefix[b] <= key
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (prefix[mid] <= key) lo = mid; else hi = mid;
+    }
+    const int base = prefix[lo] * H, nt = prefix[lo + 1] - prefix[lo];
+    it.b = lo;
+    it.len = lens[lo];
+    it.hb = (cur - base) / nt;
+    it.i0 = cur - base - it.hb * nt;
+    const int stop = min(end, base + (it.hb + 1) * nt);
+    it.i1 = it.i0 + stop - cur;
+    it.slot = int(blockIdx.x) + lo * H + it.hb;
+    cur = stop;
+    return true;
+  }
+};
+
+__device__ __forceinline__ int seq_len(const Params& p, int b) {
+  return int(min(int64_t(max(p.a.kv_len[b], 0)), int64_t(p.a.max_pages) << p.lpage));
+}
+
+template <typename T, int D, int NT, int RG, int KG>
+__global__ void __launch_bounds__(Cfg<D, NT, RG, KG>::THREADS, 1)
+    attend_kernel(const __grid_constant__ CUtensorMap map, const Params p) {
+  using C = Cfg<D, NT, RG, KG>;
+  constexpr int STAGES = C::STAGES, WARPS = C::WARPS, SEG = D / 64;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  int* prefix = reinterpret_cast<int*>(sm + C::PREFIX_OFF);
+  int* lens = reinterpret_cast<int*>(sm + C::LENS_OFF);
+  float* scl = reinterpret_cast<float*>(sm + C::SC_OFF);
+  float4* part = reinterpret_cast<float4*>(sm + C::PART_OFF);  // [WARPS / 2][PART_REGS][32 lanes]
+  uint64_t* full = reinterpret_cast<uint64_t*>(sm + C::BAR_OFF);
+  uint64_t* empty = full + STAGES;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(empty + STAGES);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < STAGES; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 4 * RG);
+    }
+    *abort_flag = 0;
+    fence_barrier_init();
+    prefetch_tensormap(&map);
+  }
+  // A programmatic dependent of the stream's previous kernel: global memory is read only past this point.
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  for (int b = threadIdx.x; b < p.a.B; b += C::THREADS) {
+    const int len = seq_len(p, b);
+    lens[b] = len;
+    prefix[b + 1] = (len + BK - 1) / BK;
+  }
+  __syncthreads();
+  if (warp == 0) {
+    int run = 0;
+    for (int base = 0; base < p.a.B; base += 32) {
+      int x = base + lane < p.a.B ? prefix[base + lane + 1] : 0;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+      }
+      if (base + lane < p.a.B) prefix[base + lane + 1] = run + x;
+      run += __shfl_sync(0xffffffffu, x, 31);
+    }
+    if (lane == 0) prefix[0] = 0;
+  }
+  __syncthreads();
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  Sched sched(p, prefix, lens);
+  Item it;
+
+  if (warp == WARPS) {
+    // ------------------------------------------------------------------ producer warp
+    // Page ids and scales come 32 pages at a time, a lane a page, the next 32 loaded while these are used. A tile's boxes
+    // (a page's rows, K or V, 128 bytes wide) are issued by a lane each.
+    constexpr int NB = D / C::BW;  // boxes across a row
+    const int sub = BK / p.box;    // boxes down a tile
+    const int per = p.box < (1 << p.lpage) ? (1 << p.lpage) / p.box : 1;  // tiles a page (128-token pages: 2)
+    int gt = 0;
+    bool ok = true;
+    while (ok && sched.next(it)) {
+      const int hk = it.hb / p.nrb;
+      const int32_t* row = p.a.table + it.b * p.a.table_st;
+      const int npages = (it.len + (1 << p.lpage) - 1) >> p.lpage;
+      // page j of the sequence: id (-1: past the sequence), K scale, V scale
+      auto fetch = [&](int j, int& id, float& ks, float& vs) {
+        id = -1, ks = vs = 0.f;
+        if (j < npages) {
+          id = row[j];
+          if (id < 0 || id >= p.a.num_pages) {
+            report_bad_index(STATUS);
+            id = -1;
+          } else {
+            const float* s = p.a.scales + int64_t(id) * 2 * p.a.Hkv + hk;
+            ks = s[0], vs = s[p.a.Hkv];
+          }
+        }
+      };
+      int j0 = (it.i0 * BK) >> p.lpage;  // first page of the current 32
+      int id, nid;
+      float ks, vs, nks, nvs;
+      fetch(j0 + lane, id, ks, vs);
+      fetch(j0 + 32 + lane, nid, nks, nvs);
+      for (int i = it.i0; i < it.i1; ++i, ++gt) {
+        const int j = (i * BK) >> p.lpage;  // first page of the tile
+        if (j - j0 >= 32) {                 // (a tile's pages never straddle: sub divides 32)
+          j0 += 32;
+          id = nid, ks = nks, vs = nvs;
+          fetch(j0 + 32 + lane, nid, nks, nvs);
+        }
+        const int st = gt % STAGES;
+        bool w = true;
+        if (lane == 0 && gt >= STAGES) w = !*abort_flag && mbar_wait(&empty[st], ((gt / STAGES) - 1) & 1, STATUS + 1);
+        if (!__shfl_sync(0xffffffffu, w, 0)) {
+          ok = false;
+          break;
+        }
+        uint8_t* base = sm + st * C::STAGE;
+        // lane = ((page in tile) NB + box) 2 + (K, V)
+        const int kv = lane & 1, bx = (lane >> 1) % NB, pg = (lane >> 1) / NB;
+        const int pid = __shfl_sync(0xffffffffu, id, (j - j0 + (pg < sub ? pg : 0)) & 31);
+        const bool go = pg < sub && pid >= 0;
+        if (go)
+          tma_load_4d(base + kv * C::TILE + bx * (BK * C::BW) + pg * p.box * C::BW, &map, bx * C::BW,
+                      per > 1 ? (i & (per - 1)) * BK : 0, kv * p.a.Hkv + hk, pid, &full[st]);
+        // slice of 16 keys: its page's scales
+        const int sp = (lane & 3) * 16 >= p.box ? (lane & 3) * 16 / p.box : 0;
+        const float a = __shfl_sync(0xffffffffu, ks, (j - j0 + sp) & 31), c = __shfl_sync(0xffffffffu, vs, (j - j0 + sp) & 31);
+        if (lane < 4) *reinterpret_cast<float2*>(scl + (st * 4 + lane) * 2) = make_float2(a, c);
+        const uint32_t n = __popc(__ballot_sync(0xffffffffu, go));
+        __syncwarp();  // the scales are written before lane 0's arrival
+        if (lane == 0) mbar_arrive_expect_tx(&full[st], n * uint32_t(p.box * C::BW));
+      }
+    }
+    if (!ok && lane == 0) *abort_flag = 1;
+    // Drain: the last copies issued have landed before the CTA ends.
+    if (lane == 0)
+      for (int g = max(0, gt - STAGES); g < gt; ++g) mbar_wait(&full[g % STAGES], (g / STAGES) & 1, STATUS + 2);
+    return;
+  }
+
+  // ------------------------------------------------------------------ consumer warps
+  const int quad = lane >> 2, qid = lane & 3;
+  const int wq = warp & 3, rg = (warp >> 2) % RG, kg = (warp >> 2) / RG;
+  const int Tq = p.a.T;
+  uint32_t qf[C::Q_REGS ? NT : 1][C::Q_REGS ? SEG : 1][8];  // this row's 16 dims of each 64-dim segment
+  uint4* qsm = reinterpret_cast<uint4*>(sm + C::Q_OFF);     // [RG][NT][SEG][2][32 lanes]
+  int gt = 0;
+  bool ok = true;
+  while (sched.next(it)) {
+    const int hk = it.hb / p.nrb, rb = it.hb - hk * p.nrb;
+    const int r0 = rb * p.rpb, r1 = min(p.rows, r0 + p.rpb);  // the block's rows
+    // Query fragments: lane (quad, qid) holds dims 64 s + 16 qid .. + 15 of row quad of each row tile.
+    float fac[NT][2];
+    int lim[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int r = r0 + (rg * NT + nt) * 8 + quad;
+      float x[SEG][16], mx = 0.f;
+      const bool live = r < r1;
+      const int g = live ? r / Tq : 0, t = live ? r - g * Tq : 0;
+      const T* src = static_cast<const T*>(p.a.q) + it.b * p.a.q_st[0] + int64_t(hk * p.G + g) * p.a.q_st[1] +
+                     t * p.a.q_st[2] + 16 * qid;
+#pragma unroll
+      for (int s = 0; s < SEG; ++s) {
+        if (!live) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) x[s][e] = 0.f;
+        } else if (p.wide_q) {
+          rope::ld_vec<T, 8>(src + 64 * s, x[s]);
+          rope::ld_vec<T, 8>(src + 64 * s + 8, x[s] + 8);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) x[s][e] = to_f<T>(src[64 * s + e]);
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) mx = fmaxf(mx, kv8::finite_abs(x[s][e]));
+      }
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      // multiply by 2^(14 - floor(log2 mx)), in two factors where that leaves fp32's range of exponents
+      const int ex = mx > 0.f ? min(max(int(__float_as_uint(mx) >> 23) - 127, -112), 127) : 14;
+      const float up = __uint_as_float(uint32_t(127 + 14 - ex) << 23);  // 14 - ex in [-113, 126]
+#pragma unroll
+      for (int s = 0; s < SEG; ++s) {
+        uint32_t w[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = pack2<__half>(x[s][2 * e] * up, x[s][2 * e + 1] * up);
+        if constexpr (C::Q_REGS) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) qf[nt][s][e] = w[e];
+        } else if (wq == 0 && kg == 0) {
+          uint4* d = qsm + ((rg * NT + nt) * SEG + s) * 64 + lane;
+          d[0] = make_uint4(w[0], w[1], w[2], w[3]);
+          d[32] = make_uint4(w[4], w[5], w[6], w[7]);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {  // for columns 2 qid + e: the row whose fragments quad 2 qid + e holds
+        const int exr = __shfl_sync(0xffffffffu, ex, (2 * qid + e) * 4);
+        // scale 2^(ex - 14), the two powers apart so that neither leaves fp32's range
+        fac[nt][e] = p.scale_log2 * __uint_as_float(uint32_t(127 + (exr - 14) / 2) << 23) *
+                     __uint_as_float(uint32_t(127 + (exr - 14) - (exr - 14) / 2) << 23);
+        const int rr = r0 + (rg * NT + nt) * 8 + 2 * qid + e;
+        lim[nt][e] = rr >= r1 ? -1 : p.a.causal ? it.len - Tq + rr % Tq : it.len - 1;
+      }
+    }
+    if constexpr (!C::Q_REGS) asm volatile("bar.sync 1, %0;" ::"n"(WARPS * 32) : "memory");
+
+    float m_run[NT][2], l_run[NT][2], acc[NT][D / 16][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      m_run[nt][0] = m_run[nt][1] = -INFINITY;
+      l_run[nt][0] = l_run[nt][1] = 0.f;
+#pragma unroll
+      for (int j = 0; j < D / 16; ++j) acc[nt][j][0] = acc[nt][j][1] = acc[nt][j][2] = acc[nt][j][3] = 0.f;
+    }
+    for (int i = it.i0; i < it.i1; ++i, ++gt) {
+      if (KG > 1 && gt % KG != kg) continue;
+      const int st = gt % STAGES;
+      if (!ok || *abort_flag || !mbar_wait(&full[st], (gt / STAGES) & 1, STATUS + 3)) {
+        ok = false;
+        gt += it.i1 - i;
+        break;
+      }
+      uint8_t* kt = sm + st * C::STAGE;
+      uint8_t* vt = kt + C::TILE;
+      const int kbase = i * BK + wq * 16;
+      const int nvalid = min(16, max(0, it.len - kbase));
+      const float2 sc2 = *reinterpret_cast<const float2*>(scl + (st * 4 + wq) * 2);
+      if (nvalid < 16) {  // values past the length: zeros (rows by key, so that P = 0 meets no NaN code)
+        for (int e = lane; e < (16 - nvalid) * (D / 16); e += 32) {
+          const int r = wq * 16 + nvalid + e / (D / 16), c = e % (D / 16);
+          *reinterpret_cast<uint4*>(vt + at<D>(r, c)) = make_uint4(0, 0, 0, 0);
+        }
+        __syncwarp();
+      }
+      float s[NT][4];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+      const int kr = wq * 16 + key_of<D>(quad);
+#pragma unroll
+      for (int sg = 0; sg < SEG; ++sg) {
+        const uint4 ka = *reinterpret_cast<const uint4*>(kt + at<D>(kr, 4 * sg + qid));
+        const uint4 kb = *reinterpret_cast<const uint4*>(kt + at<D>(kr + 8, 4 * sg + qid));
+        const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
+        uint32_t qs[NT][8];
+        if constexpr (!C::Q_REGS) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            const uint4* d = qsm + ((rg * NT + nt) * SEG + sg) * 64 + lane;
+            const uint4 u = d[0], v = d[32];
+            qs[nt][0] = u.x, qs[nt][1] = u.y, qs[nt][2] = u.z, qs[nt][3] = u.w;
+            qs[nt][4] = v.x, qs[nt][5] = v.y, qs[nt][6] = v.z, qs[nt][7] = v.w;
+          }
+        }
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          uint32_t a0, a1, a2, a3;
+          kv8::dec4(wa[w], a0, a2);
+          kv8::dec4(wb[w], a1, a3);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            const uint32_t* q = C::Q_REGS ? qf[C::Q_REGS ? nt : 0][C::Q_REGS ? sg : 0] : qs[nt];
+            mma16816(s[nt], a0, a1, a2, a3, q[2 * w], q[2 * w + 1]);
+          }
+        }
+      }
+      // the values' scale as a power of two: its logarithm (at least -100), what that leaves of it, its reciprocal
+      const float vs = sc2.y;
+      const float lv = fmaxf(log2f(vs), -100.f);
+      const float iv = ex2(-lv), rest = lv == -100.f ? vs * 0x1p100f : 1.f;
+      uint32_t pb[NT][2];
+      const int key0 = kbase + key_of<D>(quad), key1 = key0 + 8;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float f = fac[nt][e] * sc2.x;
+          float x0 = key0 <= lim[nt][e] ? fmaf(s[nt][e], f, lv) : -INFINITY;
+          float x1 = key1 <= lim[nt][e] ? fmaf(s[nt][2 + e], f, lv) : -INFINITY;
+          float mx = fmaxf(x0, x1);
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+          const float mn = fmaxf(m_run[nt][e], mx);
+          const float mu = mn == -INFINITY ? 0.f : mn;
+          const float corr = ex2(m_run[nt][e] - mu);
+          m_run[nt][e] = mn;
+          x0 = ex2(x0 - mu);
+          x1 = ex2(x1 - mu);
+          l_run[nt][e] = fmaf(x0 + x1, iv, l_run[nt][e] * corr);
+          s[nt][e] = x0 * rest;
+          s[nt][2 + e] = x1 * rest;
+#pragma unroll
+          for (int j = 0; j < D / 16; ++j) {
+            acc[nt][j][e] *= corr;
+            acc[nt][j][2 + e] *= corr;
+          }
+        }
+        pb[nt][0] = movm_t(pack2<__half>(s[nt][0], s[nt][1]));
+        pb[nt][1] = movm_t(pack2<__half>(s[nt][2], s[nt][3]));
+      }
+      const uint32_t vbase = smem_u32(vt);
+#pragma unroll
+      for (int c = 0; c < D / 16; c += 2) {  // 32 dims: matrices (keys 0-7, 8-15) x (chunks c, c + 1)
+        uint32_t v[4];
+        const int r = wq * 16 + ((lane >> 3) & 1) * 8 + key_of<D>(lane & 7);
+        ldsm_x4_t(vbase + at<D>(r, c + (lane >> 4)), v);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t a0, a1, a2, a3;
+          kv8::dec4(__byte_perm(v[2 * h], 0, 0x3120), a0, a1);
+          kv8::dec4(__byte_perm(v[2 * h + 1], 0, 0x3120), a2, a3);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) mma16816(acc[nt][c + h], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
+        }
+      }
+      if (nvalid < 16) fence_proxy_async_shared();  // the zeros precede the next copy into this stage
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[st]);
+    }
+
+    // ------------------------------------------------------------------ the item's partial
+    // The parts of a row (one a key slice and key group) meet in a tree through shared memory, each warp's registers as
+    // they lie (a lane's counterpart is the same lane); the warps of part 0 write the merged partial.
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        l_run[nt][e] += __shfl_xor_sync(0xffffffffu, l_run[nt][e], 4);
+        l_run[nt][e] += __shfl_xor_sync(0xffffffffu, l_run[nt][e], 8);
+        l_run[nt][e] += __shfl_xor_sync(0xffffffffu, l_run[nt][e], 16);
+      }
+    uint32_t all_ok;  // every warp's waits held: else all leave. (Also: the previous item's parts have been read.)
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.and.pred q, 1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(all_ok)
+        : "r"(uint32_t(ok)), "n"(WARPS * 32)
+        : "memory");
+    if (!all_ok) {
+      if (lane == 0) *abort_flag = 1;
+      break;
+    }
+    const int pi = kg * 4 + wq;
+#pragma unroll
+    for (int half = 2 * KG; half > 0; half >>= 1) {
+      if (pi >= half && pi < 2 * half) {
+        float4* d = part + ((pi - half) * RG + rg) * C::PART_REGS * 32 + lane;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          *d = make_float4(m_run[nt][0], m_run[nt][1], l_run[nt][0], l_run[nt][1]);
+          d += 32;
+#pragma unroll
+          for (int j = 0; j < D / 16; ++j, d += 32) *d = make_float4(acc[nt][j][0], acc[nt][j][1], acc[nt][j][2], acc[nt][j][3]);
+        }
+      }
+      asm volatile("bar.sync 1, %0;" ::"n"(WARPS * 32) : "memory");
+      if (pi < half) {
+        const float4* d = part + (pi * RG + rg) * C::PART_REGS * 32 + lane;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const float4 x = *d;
+          d += 32;
+          const float xm[2] = {x.x, x.y}, xl[2] = {x.z, x.w};
+          float f[2], g[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float mn = fmaxf(m_run[nt][e], xm[e]), mu = mn == -INFINITY ? 0.f : mn;
+            f[e] = ex2(m_run[nt][e] - mu);
+            g[e] = ex2(xm[e] - mu);
+            m_run[nt][e] = mn;
+            l_run[nt][e] = l_run[nt][e] * f[e] + xl[e] * g[e];
+          }
+#pragma unroll
+          for (int j = 0; j < D / 16; ++j, d += 32) {
+            const float4 o = *d;
+            acc[nt][j][0] = acc[nt][j][0] * f[0] + o.x * g[0];
+            acc[nt][j][1] = acc[nt][j][1] * f[1] + o.y * g[1];
+            acc[nt][j][2] = acc[nt][j][2] * f[0] + o.z * g[0];
+            acc[nt][j][3] = acc[nt][j][3] * f[1] + o.w * g[1];
+          }
+        }
+      }
+      if (half > 1) asm volatile("bar.sync 1, %0;" ::"n"(WARPS * 32) : "memory");
+    }
+    if (pi == 0) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int r = (rg * NT + nt) * 8 + 2 * qid + e;
+          if (r >= r1 - r0) continue;
+          const size_t out = size_t(it.slot) * p.rpb + r;
+          if (quad == 0) *reinterpret_cast<float2*>(p.ws_ml + 2 * out) = make_float2(m_run[nt][e], l_run[nt][e]);
+#pragma unroll
+          for (int j = 0; j < D / 16; ++j)
+            *reinterpret_cast<float2*>(p.ws_o + out * D + 16 * j + 2 * quad) =
+                make_float2(acc[nt][j][e], acc[nt][j][2 + e]);
+        }
+    }
+  }
+}
+
+// Merges the partials of each (b, KV head, row block): a block each, a warp a row. The pair's partials sit in consecutive
+// slots, found from its first and last tile.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) combine_kernel(const Params p) {
+  constexpr int E = D / 32, HELD = 8;
+  __shared__ int s_tiles[2][8];
+  const int H = p.a.Hkv * p.nrb, b = blockIdx.x / H, hb = blockIdx.x - b * H;
+  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
+  int before = 0, total = 0;
+  for (int i = tid; i < p.a.B; i += 256) {
+    const int t = (seq_len(p, i) + BK - 1) / BK;
+    total += t;
+    if (i < b) before += t;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    before += __shfl_xor_sync(0xffffffffu, before, o);
+    total += __shfl_xor_sync(0xffffffffu, total, o);
+  }
+  if (lane == 0) s_tiles[0][w] = before, s_tiles[1][w] = total;
+  __syncthreads();
+  before = total = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) before += s_tiles[0][i], total += s_tiles[1][i];
+  const int len = seq_len(p, b), nt = (len + BK - 1) / BK;
+  int first = 0, nparts = 0;
+  if (nt > 0) {  // CTA of tile t: the largest c with floor(c total / runs) <= t, i.e. ((t + 1) runs - 1) / total
+    const int64_t tt = int64_t(total) * H, t0 = int64_t(before) * H + int64_t(hb) * nt, runs = runs_of(p, tt);
+    const int c0 = int(((t0 + 1) * runs - 1) / tt), c1 = int(((t0 + nt) * runs - 1) / tt);
+    first = c0 + blockIdx.x;
+    nparts = c1 - c0 + 1;
+  }
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int hk = hb / p.nrb, r0 = (hb - hk * p.nrb) * p.rpb, nrows = min(p.rows - r0, p.rpb);
+  for (int r = w; r < nrows; r += 8) {
+    float x[E], M = -INFINITY, L = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) x[e] = 0.f;
+    for (int k0 = 0; k0 < nparts; k0 += HELD) {  // HELD partials' loads in flight at once
+      float2 ml[HELD];
+      float y[HELD][E];
+#pragma unroll
+      for (int k = 0; k < HELD; ++k) {
+        const size_t at = size_t(first + min(k0 + k, nparts - 1)) * p.rpb + r;
+        ml[k] = *reinterpret_cast<const float2*>(p.ws_ml + 2 * at);
+        const float2* src = reinterpret_cast<const float2*>(p.ws_o + at * D + lane * E);
+#pragma unroll
+        for (int e = 0; e < E; e += 2) {
+          const float2 v = src[e / 2];
+          y[k][e] = v.x, y[k][e + 1] = v.y;
+        }
+      }
+      float m1 = M;
+#pragma unroll
+      for (int k = 0; k < HELD; ++k) m1 = fmaxf(m1, k0 + k < nparts ? ml[k].x : -INFINITY);
+      const float mu = m1 == -INFINITY ? 0.f : m1, f = ex2(M - mu);
+      L *= f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) x[e] *= f;
+#pragma unroll
+      for (int k = 0; k < HELD; ++k) {
+        if (k0 + k >= nparts) continue;
+        const float g = ex2(ml[k].x - mu);
+        L = fmaf(ml[k].y, g, L);
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[e] = fmaf(y[k][e], g, x[e]);
+      }
+      M = m1;
+    }
+    const float inv = L > 0.f || L != L ? 1.f / L : 0.f;
+    bool nan = false;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      x[e] *= inv;
+      nan = nan || x[e] != x[e];
+    }
+    const int rr = r0 + r, h = hk * p.G + rr / p.a.T, t = rr % p.a.T;
+    if (p.a.causal && p.a.T > 1 && __any_sync(0xffffffffu, nan)) {
+      // A NaN: the row's own, or a later token's under a weight of 0. The row again, reading only what it sees.
+      const T* q = static_cast<const T*>(p.a.q) + b * p.a.q_st[0] + h * p.a.q_st[1] + t * p.a.q_st[2] + lane * E;
+#pragma unroll
+      for (int e = 0; e < E; ++e) x[e] = to_f<T>(q[e]);
+      arows::PagedKeys<E> keys{p.a.pages, p.a.scales, p.a.table + b * p.a.table_st, p.a.Hkv, hk, p.a.page,
+                               p.a.num_pages, lane * E};
+      arows::attend_row<E>(keys, len - p.a.T + 1 + t, p.a.scale, x);
+    }
+    T* o = static_cast<T*>(p.a.o) + b * p.a.o_st[0] + h * p.a.o_st[1] + t * p.a.o_st[2] + lane * E;
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = from_f<T>(x[e]);
+  }
+}
+
+}  // namespace kv8attn
+}  // namespace lb2

@@ -24,6 +24,7 @@
 #include "rope.cuh"
 #include "kv8.cuh"
 #include "attn_rows.cuh"
+#include "kv8_attend.cuh"
 
 namespace lb2 {
 
@@ -1582,11 +1583,125 @@ static int paged_rows(const arows::PagedParams& p, int D, cudaStream_t st) {
   return LB2_OK;
 }
 
+namespace lb2 {
+namespace kv8attn {
+
+// Rows a block and the kernel's shape: up to 8 and 16 rows by one set of four warps a tile and two sets on alternate
+// tiles, up to 32 by two sets sharing each tile; more rows take further passes over the codes (from L2 as far as it holds
+// them).
+struct Plan {
+  int nrb, rpb, grid;
+  int64_t slots;
+  size_t ml, o, total;
+};
+
+static Plan plan(int B, int rows, int Hkv, int D, int page, int max_pages) {
+  Plan pl{};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  pl.nrb = (rows + 31) / 32;
+  pl.rpb = ((rows + pl.nrb - 1) / pl.nrb + 7) / 8 * 8;
+  const int nb = std::min(B, MAX_B);
+  const int64_t H = int64_t(Hkv) * pl.nrb, tiles = int64_t(nb) * H * ((int64_t(max_pages) * page + BK - 1) / BK);
+  pl.grid = int(std::max<int64_t>(1, std::min<int64_t>(sm_count(dev), tiles / 2)));
+  pl.slots = pl.grid + nb * H;
+  pl.ml = 0;
+  pl.o = align_up(size_t(pl.slots) * pl.rpb * 2 * sizeof(float), 256);
+  pl.total = pl.o + size_t(pl.slots) * pl.rpb * D * sizeof(float);
+  return pl;
+}
+
+template <typename T, int D, int NT, int RG, int KG>
+static int launch_t(const CUtensorMap& map, const Params& p, cudaStream_t st) {
+  using C = Cfg<D, NT, RG, KG>;
+  auto kern = attend_kernel<T, D, NT, RG, KG>;
+  static int attr_dev = -1;
+  int dev = 0;
+  LB2_CUDA(cudaGetDevice(&dev));
+  if (attr_dev != dev) {
+    LB2_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+    attr_dev = dev;
+  }
+  cudaLaunchAttribute pdl[1];
+  pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  pdl[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(p.grid));
+  cfg.blockDim = dim3(C::THREADS);
+  cfg.dynamicSmemBytes = C::SMEM;
+  cfg.stream = st;
+  cfg.attrs = pdl;
+  cfg.numAttrs = 1;
+  LB2_CUDA(cudaLaunchKernelEx(&cfg, kern, map, p));
+  cfg.gridDim = dim3(unsigned(p.a.B * p.a.Hkv * p.nrb));
+  cfg.blockDim = dim3(256);
+  cfg.dynamicSmemBytes = 0;
+  LB2_CUDA(cudaLaunchKernelEx(&cfg, combine_kernel<T, D>, p));
+  return LB2_OK;
+}
+
+template <typename T, int D>
+static int launch_d(const CUtensorMap& map, const Params& p, cudaStream_t st) {
+  if (p.rpb <= 8) return launch_t<T, D, 1, 1, 2>(map, p, st);
+  if (p.rpb <= 16) return launch_t<T, D, 2, 1, 2>(map, p, st);
+  return launch_t<T, D, 2, 2, 1>(map, p, st);
+}
+
+template <typename T>
+static int launch(const CUtensorMap& map, const Params& p, int D, cudaStream_t st) {
+  return D == 64 ? launch_d<T, 64>(map, p, st) : D == 128 ? launch_d<T, 128>(map, p, st) : launch_d<T, 256>(map, p, st);
+}
+
+static int run(const arows::PagedParams& a, int D, int dtype, void* workspace, cudaStream_t st) {
+  Params p{};
+  p.a = a;
+  p.G = a.Hq / a.Hkv;
+  LB2_CHECK_ARG(int64_t(p.G) * a.T < (1 << 20), "kv8_attend: too many query rows a KV head");
+  p.rows = p.G * a.T;
+  const Plan pl = plan(a.B, p.rows, a.Hkv, D, a.page, a.max_pages);
+  p.nrb = pl.nrb;
+  p.rpb = pl.rpb;
+  p.grid = pl.grid;
+  p.ws_ml = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + pl.ml);
+  p.ws_o = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + pl.o);
+  p.box = std::min(a.page, BK);
+  p.lpage = a.page == 16 ? 4 : a.page == 32 ? 5 : a.page == 64 ? 6 : 7;
+  p.wide_q = aligned16(a.q) && a.q_st[0] % 8 == 0 && a.q_st[1] % 8 == 0 && a.q_st[2] % 8 == 0;
+  p.scale_log2 = a.scale * 1.4426950408889634f;
+  const int64_t H = int64_t(a.Hkv) * p.nrb;
+  LB2_CHECK_ARG(std::min(a.B, MAX_B) * H * ((int64_t(a.max_pages) * a.page + BK - 1) / BK) < (int64_t(1) << 31),
+                "kv8_attend: too many key tiles a call");
+  CUtensorMap map;
+  {  // (D, page, K / V and head, page id), a box a page's rows, 128 (64) bytes wide
+    const uint64_t dims[4] = {uint64_t(D), uint64_t(a.page), uint64_t(2 * a.Hkv), uint64_t(a.num_pages)};
+    const uint64_t strides[3] = {uint64_t(D), uint64_t(a.page) * D, uint64_t(2 * a.Hkv) * a.page * D};
+    const uint32_t box[4] = {uint32_t(std::min(D, 128)), uint32_t(p.box), 1, 1};
+    const int rc = encode_tensor_map(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, a.pages, dims, strides, box,
+                                     D == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B);
+    if (rc) return rc;
+  }
+  const int item = 2;  // bytes a query value
+  for (int b0 = 0; b0 < a.B; b0 += MAX_B) {
+    Params c = p;
+    c.a.B = std::min(MAX_B, a.B - b0);
+    c.a.q = static_cast<const uint8_t*>(a.q) + b0 * a.q_st[0] * item;
+    c.a.o = static_cast<uint8_t*>(a.o) + b0 * a.o_st[0] * item;
+    c.a.table = a.table + b0 * a.table_st;
+    c.a.kv_len = a.kv_len + b0;
+    const int rc = dtype == LB2_BF16 ? launch<__nv_bfloat16>(map, c, D, st) : launch<__half>(map, c, D, st);
+    if (rc) return rc;
+  }
+  return LB2_OK;
+}
+
+}  // namespace kv8attn
+}  // namespace lb2
+
 extern "C" {
 
 size_t lb2_kv8_attend_workspace_size(int B, int Hq, int Hkv, int T, int D, int page, int max_pages) {
   if (B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || T <= 0 || D <= 0 || page <= 0 || max_pages <= 0) return 0;
-  return 256;
+  return kv8attn::plan(B, Hq / Hkv * T, Hkv, D, page, max_pages).total;
 }
 
 int lb2_kv8_attend(const void* q, const int64_t* q_st, const uint8_t* pages, const float* scales, const int32_t* table,
@@ -1600,9 +1715,6 @@ int lb2_kv8_attend(const void* q, const int64_t* q_st, const uint8_t* pages, con
   if (B == 0 || T == 0) return LB2_OK;
   LB2_CHECK_ARG(q && q_st && pages && scales && table && kv_len && o && o_st, "kv8_attend: missing argument");
   LB2_CHECK_ARG(aligned16(pages), "kv8_attend: pages must be 16-byte aligned");
-  LB2_CHECK_ARG(workspace != nullptr &&
-                    workspace_bytes >= lb2_kv8_attend_workspace_size(B, Hq, Hkv, T, D, page, max_pages),
-                "kv8_attend: workspace too small");
   arows::PagedParams p{};
   p.q = q;
   p.o = o;
@@ -1618,7 +1730,10 @@ int lb2_kv8_attend(const void* q, const int64_t* q_st, const uint8_t* pages, con
   p.scale = scale;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (dtype == LB2_F32) return paged_rows<float>(p, D, st);
-  return dtype == LB2_BF16 ? paged_rows<__nv_bfloat16>(p, D, st) : paged_rows<__half>(p, D, st);
+  LB2_CHECK_ARG(workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0 &&
+                    workspace_bytes >= lb2_kv8_attend_workspace_size(B, Hq, Hkv, T, D, page, max_pages),
+                "kv8_attend: workspace too small or not 256-byte aligned");
+  return kv8attn::run(p, D, dtype, workspace, st);
 }
 
 // ------------------------------------------------------------------------------------------------ packed prompts
