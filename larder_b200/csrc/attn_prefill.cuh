@@ -74,6 +74,13 @@ struct Params {
   const int32_t* tl;
   const int32_t* tn;
   int tl_ld;
+  // Packed prompts (the kernels' PK form; B = 1, causal within each prompt): the row blocks of all prompts, heaviest
+  // first, as (prompt's first row, its rows, block index m, key tiles it reads), *pk_n of them, listed by
+  // packed::plan_kernel; and q, k, v for the rows that are taken again (packed_row_exact).
+  const int4* pk;
+  const int32_t* pk_n;
+  const void* src[3];
+  int64_t src_st[3][2];  // H, T
 };
 
 // Applies a row's mask to its scores s of keys key0 .. key0 + HC - 1: -inf past lim (the causal limit) or N, and,
@@ -209,6 +216,34 @@ __device__ __forceinline__ float ex2_fma(float x) {
   return x < -125.f ? 0.f : r;
 }
 
+// The PK form's second look at a row whose output came out non-finite with a finite sum of weights: a value that is
+// infinite or NaN was multiplied by a weight, possibly the 0 of a key that the row does not see (a later row of its
+// prompt in the last tile, or the next prompt's rows behind it). Takes `cols` columns of the row again, reading only the
+// keys 0 .. row it sees. Rare; one thread a row.
+template <typename T, int D>
+__device__ __noinline__ void packed_row_exact(const Params& p, int base, int row, int h, int c0, int cols, T* out) {
+  const T* q = static_cast<const T*>(p.src[0]) + h * p.src_st[0][0] + int64_t(base + row) * p.src_st[0][1];
+  const T* k = static_cast<const T*>(p.src[1]) + (h / p.G) * p.src_st[1][0] + int64_t(base) * p.src_st[1][1];
+  const T* v = static_cast<const T*>(p.src[2]) + (h / p.G) * p.src_st[2][0] + int64_t(base) * p.src_st[2][1] + c0;
+  for (int c = 0; c < cols; c += 16) {
+    float o[16], m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[e] = 0.f;
+    for (int i = 0; i <= row; ++i) {
+      float s = 0.f;
+      for (int d = 0; d < D; ++d) s = fmaf(to_f<T>(q[d]), to_f<T>(k[i * p.src_st[1][1] + d]), s);
+      s *= p.scale_log2;
+      const float m1 = fmaxf(m, s), mu = m1 == -INFINITY ? 0.f : m1, f = exp2f(m - mu), w = exp2f(s - mu);
+      l = l * f + w;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[e] = fmaf(w, to_f<T>(v[i * p.src_st[2][1] + c + e]), o[e] * f);
+      m = m1;
+    }
+#pragma unroll
+    for (int e = 0; e < 16; ++e) out[c + e] = from_f<T>(o[e] / l);
+  }
+}
+
 // Number of BN-key tiles query tile mt reads.
 template <int D>
 __device__ __forceinline__ int kv_tiles(const Params& p, int mt) {
@@ -222,7 +257,8 @@ __device__ __forceinline__ int kv_tiles(const Params& p, int mt) {
   return last <= 0 ? 0 : (last + BN - 1) / BN;
 }
 
-template <typename T, int D>
+// PK: packed prompts, a block of the plan's list and a head a CTA; the grid is sized by the most blocks there can be.
+template <typename T, int D, bool PK = false>
 __global__ void __launch_bounds__(THREADS, 1) fmha_kernel(const __grid_constant__ CUtensorMap qmap,
                                                            const __grid_constant__ CUtensorMap kmap,
                                                            const __grid_constant__ CUtensorMap vmap,
@@ -237,10 +273,17 @@ __global__ void __launch_bounds__(THREADS, 1) fmha_kernel(const __grid_constant_
   // Heaviest query tiles first (causal tiles late in the sequence read the most keys); heads vary fastest so that
   // neighbouring CTAs share their KV head's tiles in L2.
   const int bh = blockIdx.x % (p.B * p.Hq);
-  const int mt = p.mtiles - 1 - int(blockIdx.x / (p.B * p.Hq));
+  int4 blk = make_int4(0, 0, 0, 0);
+  if constexpr (PK) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // the plan
+    const int e = int(blockIdx.x / p.Hq);
+    if (e >= *p.pk_n) return;
+    blk = p.pk[e];
+  }
+  const int mt = PK ? blk.z : p.mtiles - 1 - int(blockIdx.x / (p.B * p.Hq));
   const int b = bh / p.Hq, h = bh % p.Hq, hk = h / p.G;
   const int r0 = mt * BM;
-  const int ntiles = kv_tiles<D>(p, mt);
+  const int ntiles = PK ? blk.w : kv_tiles<D>(p, mt);
 
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -301,7 +344,7 @@ __global__ void __launch_bounds__(THREADS, 1) fmha_kernel(const __grid_constant_
         mbar_arrive_expect_tx(q_full, C::QBYTES);
 #pragma unroll
         for (int db = 0; db < D / 64; ++db)
-          tma_load_4d(sm + C::Q_OFF + db * BM * 128, &qmap, db * 64, r0, h, b, q_full);
+          tma_load_4d(sm + C::Q_OFF + db * BM * 128, &qmap, db * 64, blk.x + r0, h, b, q_full);
       } else {
         prefetch_tensormap(&vmap);
       }
@@ -320,7 +363,7 @@ __global__ void __launch_bounds__(THREADS, 1) fmha_kernel(const __grid_constant_
         mbar_arrive_expect_tx(&fullb[st], C::KBYTES);
 #pragma unroll
         for (int db = 0; db < D / 64; ++db)
-          tma_load_4d(sm + off + st * C::KBYTES + db * BN * 128, map, db * 64, key_tile(p, mt, j) * BN, hk, b,
+          tma_load_4d(sm + off + st * C::KBYTES + db * BN * 128, map, db * 64, blk.x + key_tile(p, mt, j) * BN, hk, b,
                       &fullb[st]);
         issued = j + 1;
       }
@@ -415,7 +458,8 @@ __global__ void __launch_bounds__(THREADS, 1) fmha_kernel(const __grid_constant_
     const uint32_t lane_base = tmem + (uint32_t(32 * (warp & 3)) << 16);
     const uint32_t pair_bar = 2 + (warp & 3);  // named barrier of warps w and w + 4 (ids 2..5)
     float* red = reinterpret_cast<float*>(sm + C::RED_OFF);
-    const int lim = p.mask_kind == LB2_MASK_CAUSAL ? p.N - p.T + row : p.N - 1;
+    const int lim = PK ? row : p.mask_kind == LB2_MASK_CAUSAL ? p.N - p.T + row : p.N - 1;
+    const int nkeys = PK ? 0x7fffffff : p.N;  // (packed: the horizon alone bounds a row's keys)
     const uint8_t* mrow = (p.mask_kind == LB2_MASK_ARRAY && row < p.T) ? p.mask + int64_t(row) * p.m_st[0] : nullptr;
     float m_run = -INFINITY, l_run = 0.f;
     bool ok = true;
@@ -442,13 +486,13 @@ __global__ void __launch_bounds__(THREADS, 1) fmha_kernel(const __grid_constant_
 
       const int kt = key_tile(p, mt, j);
       const int key0 = kt * BN + hf * HC;
-      const bool full_tile = kt * BN + BN - 1 <= lim && kt * BN + BN <= p.N && !mrow;
+      const bool full_tile = kt * BN + BN - 1 <= lim && kt * BN + BN <= nkeys && !mrow;
       float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
       if (full_tile) {
 #pragma unroll
         for (int c = 0; c < HC; ++c) mx4[c & 3] = fmaxf(mx4[c & 3], s[c]);
       } else {
-        mask_scores<HC>(s, mrow, p.m_st[1], key0, lim, p.N);
+        mask_scores<HC>(s, mrow, p.m_st[1], key0, lim, nkeys);
 #pragma unroll
         for (int c = 0; c < HC; ++c) mx4[c & 3] = fmaxf(mx4[c & 3], s[c]);
       }
@@ -526,12 +570,12 @@ __global__ void __launch_bounds__(THREADS, 1) fmha_kernel(const __grid_constant_
     asm volatile("bar.sync %0, 64;" ::"r"(pair_bar));
     const float l_tot = l_run + red[(1 - hf) * BM + r];
     const bool have_o = ntiles > 0 && ok;
-    const bool store = row < p.T;
-    T* orow = reinterpret_cast<T*>(p.o) + b * p.o_st[0] + int64_t(h) * p.o_st[1] + int64_t(row) * p.o_st[2] + hf * HD;
+    const bool store = row < (PK ? blk.y : p.T);
+    T* orow = reinterpret_cast<T*>(p.o) + b * p.o_st[0] + int64_t(h) * p.o_st[1] + int64_t(blk.x + row) * p.o_st[2] + hf * HD;
     const T* grow = p.gate ? reinterpret_cast<const T*>(p.gate) + b * p.g_st[0] + int64_t(h) * p.g_st[1] +
                                  int64_t(row) * p.g_st[2] + hf * HD
                            : nullptr;
-    const float inv = (have_o && l_tot > 0.f) ? 1.f / l_tot : 0.f;
+    const float inv = (have_o && (l_tot > 0.f || (PK && l_tot != l_tot))) ? 1.f / l_tot : 0.f;
 #pragma unroll 1
     for (int c = 0; c < HD; c += 32) {
       float ov[32];
@@ -543,6 +587,15 @@ __global__ void __launch_bounds__(THREADS, 1) fmha_kernel(const __grid_constant_
         for (int e = 0; e < 32; ++e) ov[e] = 0.f;
       }
       if (!store) continue;
+      if constexpr (PK) {
+        float sum = 0.f;  // (finite unless some value is not)
+#pragma unroll
+        for (int e = 0; e < 32; ++e) sum = fmaf(ov[e], 0.f, sum);
+        if (sum != sum && l_tot == l_tot) {
+          packed_row_exact<T, D>(p, blk.x, row, h, hf * HD + c, 32, orow + c);
+          continue;
+        }
+      }
 #pragma unroll
       for (int e = 0; e < 32; e += 8) {
         float x[8];

@@ -163,15 +163,30 @@ __device__ __forceinline__ int kv_tiles2(const Params& p, int mt2) {
 // Work item k of a pass, heaviest first; heads vary fastest so that neighbouring clusters share their KV head's
 // tiles in L2: the 256-row pair mt2 of (batch, query head) b, h. (A sequence-major order, one sequence's K and V at a
 // time, measured 5 % slower on 8 sequences of 8192 rows.)
+// In the PK form (packed prompts) r0 counts from the prompt's first row, `base`, and the prompt has n rows.
 struct Item {
-  int b, h, hk, r0, ntiles, mt2;
+  int b, h, hk, r0, ntiles, mt2, base, n;
 };
 
 __device__ __forceinline__ int item_mt2(const Params& p, int k) { return p.mtiles - 1 - k / (p.B * p.Hq); }
 
-template <int D>
+template <int D, bool PK>
 __device__ __forceinline__ Item item_of(const Params& p, int k, uint32_t rank) {
   Item it;
+  if constexpr (PK) {
+    const int4 blk = p.pk[k / p.Hq];
+    it.b = 0;
+    it.h = k % p.Hq;
+    it.hk = it.h / p.G;
+    it.r0 = blk.z * 2 * BM + int(rank) * BM;
+    it.ntiles = blk.w;
+    it.mt2 = blk.z;
+    it.base = blk.x;
+    it.n = blk.y;
+    return it;
+  }
+  it.base = 0;
+  it.n = p.T;
   const int bh = k % (p.B * p.Hq);
   const int mt2 = item_mt2(p, k);
   it.b = bh / p.Hq;
@@ -192,7 +207,7 @@ __device__ __forceinline__ int item_index(int r, int c, int nc) { return r * nc 
 // items. Two barriers hand resources from one item to the next: q_empty (the item's last score MMA has read Q, so
 // the next Q may land) and o_free (the epilogue has read O out of TMEM, so the next item's first PV may overwrite
 // it). Both count only items that have keys, so that no waiter can fall two phases behind.
-template <typename T, int D>
+template <typename T, int D, bool PK = false>
 __global__ void __launch_bounds__(THREADS, 1) fmha2_kernel(const __grid_constant__ CUtensorMap qmap,
                                                             const __grid_constant__ CUtensorMap kmap,
                                                             const __grid_constant__ CUtensorMap vmap,
@@ -207,7 +222,6 @@ __global__ void __launch_bounds__(THREADS, 1) fmha2_kernel(const __grid_constant
   const uint32_t rank = cluster_rank();
   const bool leader = rank == 0;
   const int cl = blockIdx.x >> 1, ncl = gridDim.x >> 1;
-  const int total = p.B * p.Hq * p.mtiles;
 
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -263,6 +277,8 @@ __global__ void __launch_bounds__(THREADS, 1) fmha2_kernel(const __grid_constant
   cluster_sync();  // both CTAs' barriers are initialised before any remote arrive or load completion
   prefill::tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  if constexpr (PK) asm volatile("griddepcontrol.wait;" ::: "memory");  // the plan
+  const int total = PK ? *p.pk_n * p.Hq : p.B * p.Hq * p.mtiles;
 
   if (warp == PRODUCER_WARP) {
     // ------------------------------------------------------------------------------------ TMA producers
@@ -282,7 +298,7 @@ __global__ void __launch_bounds__(THREADS, 1) fmha2_kernel(const __grid_constant
       for (int rr = 0; rr * ncl < total && !stop; ++rr) {
         const int kidx = item_index(rr, cl, ncl);
         if (kidx >= total) continue;
-        const Item itm = item_of<D>(p, kidx, rank);
+        const Item itm = item_of<D, PK>(p, kidx, rank);
         if (itm.ntiles == 0) continue;
         if (lane == 0) {  // Q of this item, once the previous item's score MMAs are done with the buffer
           if (qi > 0 && !mbar_wait(q_empty, (qi - 1) & 1, 45)) {
@@ -292,7 +308,7 @@ __global__ void __launch_bounds__(THREADS, 1) fmha2_kernel(const __grid_constant
           if (leader) mbar_arrive_expect_tx(q_full, 2 * C::QBYTES);
 #pragma unroll
           for (int db = 0; db < D / 64; ++db)
-            tma_load_4d_pair(sm + C::Q_OFF + db * BM * 128, &qmap, db * 64, itm.r0, itm.h, itm.b, q_full);
+            tma_load_4d_pair(sm + C::Q_OFF + db * BM * 128, &qmap, db * 64, itm.base + itm.r0, itm.h, itm.b, q_full);
           q_issued = qi;
         }
         for (int j = 0; j < itm.ntiles; ++j, ++jg) {
@@ -311,14 +327,14 @@ __global__ void __launch_bounds__(THREADS, 1) fmha2_kernel(const __grid_constant
             uint8_t* dst = sm + C::K_OFF + st * C::KHBYTES;
 #pragma unroll
             for (int db = 0; db < D / 64; ++db)
-              tma_load_4d_pair(dst + db * HN * 128, &kmap, db * 64, prefill::key_tile(p, itm.mt2, j) * BN + int(rank) * HN, itm.hk, itm.b,
-                               &fullb[st]);
+              tma_load_4d_pair(dst + db * HN * 128, &kmap, db * 64,
+                               itm.base + prefill::key_tile(p, itm.mt2, j) * BN + int(rank) * HN, itm.hk, itm.b, &fullb[st]);
           } else {  // keys [j BN, + BN), columns [rank HD, + HD): HD / 64 boxes of (64, BN)
             uint8_t* dst = sm + C::V_OFF + st * C::VHBYTES;
 #pragma unroll
             for (int db = 0; db < HD / 64; ++db)
-              tma_load_4d_pair(dst + db * BN * 128, &vmap, int(rank) * HD + db * 64, prefill::key_tile(p, itm.mt2, j) * BN, itm.hk, itm.b,
-                               &fullb[st]);
+              tma_load_4d_pair(dst + db * BN * 128, &vmap, int(rank) * HD + db * 64,
+                               itm.base + prefill::key_tile(p, itm.mt2, j) * BN, itm.hk, itm.b, &fullb[st]);
           }
         }
         ++qi;
@@ -366,7 +382,7 @@ __global__ void __launch_bounds__(THREADS, 1) fmha2_kernel(const __grid_constant
         for (int rr = 0; ok && rr * ncl < total; ++rr) {
           const int kidx = item_index(rr, cl, ncl);
           if (kidx >= total) continue;
-          const int nt = kv_tiles2<D>(p, item_mt2(p, kidx));
+          const int nt = PK ? p.pk[kidx / p.Hq].w : kv_tiles2<D>(p, item_mt2(p, kidx));
           if (nt == 0) continue;
           ok = mbar_wait(q_full, qi & 1, 51);
           bool o_ok = qi == 0;  // O may be overwritten by this item's first PV
@@ -443,10 +459,11 @@ __global__ void __launch_bounds__(THREADS, 1) fmha2_kernel(const __grid_constant
     for (int rr = 0; ok && rr * ncl < total; ++rr) {
       const int kidx = item_index(rr, cl, ncl);
       if (kidx >= total) continue;
-      const Item itm = item_of<D>(p, kidx, rank);
+      const Item itm = item_of<D, PK>(p, kidx, rank);
       const int ntiles = itm.ntiles;
       const int row = itm.r0 + r;
-      const int lim = p.mask_kind == LB2_MASK_CAUSAL ? p.N - p.T + row : p.N - 1;
+      const int lim = PK ? row : p.mask_kind == LB2_MASK_CAUSAL ? p.N - p.T + row : p.N - 1;
+      const int nkeys = PK ? 0x7fffffff : p.N;  // (packed: the horizon alone bounds a row's keys)
       const uint8_t* mrow =
           (p.mask_kind == LB2_MASK_ARRAY && row < p.T) ? p.mask + int64_t(row) * p.m_st[0] : nullptr;
       float m_run = -INFINITY, l_run = 0.f;
@@ -469,8 +486,8 @@ __global__ void __launch_bounds__(THREADS, 1) fmha2_kernel(const __grid_constant
         }
         const int kt = prefill::key_tile(p, itm.mt2, j);
         const int key0 = kt * BN + grp * HC;
-        const bool full_tile = kt * BN + BN - 1 <= lim && kt * BN + BN <= p.N && !mrow;
-        if (!full_tile) prefill::mask_scores<HC>(s, mrow, p.m_st[1], key0, lim, p.N);
+        const bool full_tile = kt * BN + BN - 1 <= lim && kt * BN + BN <= nkeys && !mrow;
+        if (!full_tile) prefill::mask_scores<HC>(s, mrow, p.m_st[1], key0, lim, nkeys);
         // P_j with the running max. The running max moves only when a row's tile max exceeds it by more than 2^8,
         // i.e. when some P of the row exceeds 2^8; P >= 0, so a thread whose P sum is at most 2^8 has no such
         // element and skips the max altogether. Otherwise (or before the row's first key) the exact check below
@@ -582,13 +599,15 @@ __global__ void __launch_bounds__(THREADS, 1) fmha2_kernel(const __grid_constant
         for (int g2 = 0; g2 < NG; ++g2) l_tot += red[g2 * BM + r];
       }
       const bool have_o = ntiles > 0 && ok;
-      const bool store = row < p.T;
-      T* orow = reinterpret_cast<T*>(p.o) + itm.b * p.o_st[0] + int64_t(itm.h) * p.o_st[1] + int64_t(row) * p.o_st[2] +
+      const bool store = row < itm.n;
+      T* orow = reinterpret_cast<T*>(p.o) + itm.b * p.o_st[0] + int64_t(itm.h) * p.o_st[1] +
+                int64_t(itm.base + row) * p.o_st[2] +
                 grp * DH;
       const T* grow = p.gate ? reinterpret_cast<const T*>(p.gate) + itm.b * p.g_st[0] + int64_t(itm.h) * p.g_st[1] +
                                    int64_t(row) * p.g_st[2] + grp * DH
                              : nullptr;
-      const float inv = (have_o && m_run != -INFINITY && l_tot > 0.f) ? 1.f / l_tot : 0.f;
+      const float inv =
+          (have_o && m_run != -INFINITY && (l_tot > 0.f || (PK && l_tot != l_tot))) ? 1.f / l_tot : 0.f;
 #pragma unroll 1
       for (int c = 0; c < DH; c += 32) {
         float ov[32];
@@ -600,6 +619,15 @@ __global__ void __launch_bounds__(THREADS, 1) fmha2_kernel(const __grid_constant
           for (int e = 0; e < 32; ++e) ov[e] = 0.f;
         }
         if (!store) continue;
+        if constexpr (PK) {
+          float sum = 0.f;  // (finite unless some value is not)
+#pragma unroll
+          for (int e = 0; e < 32; ++e) sum = fmaf(ov[e], 0.f, sum);
+          if (sum != sum && l_tot == l_tot) {
+            prefill::packed_row_exact<T, D>(p, itm.base, row, itm.h, grp * DH + c, 32, orow + c);
+            continue;
+          }
+        }
 #pragma unroll
         for (int e = 0; e < 32; e += 8) {
           float x[8];

@@ -20,6 +20,7 @@
 #include "peer_xch.cuh"
 #include "kv_runs.cuh"
 #include "attn_tiles.cuh"
+#include "attn_packed.cuh"
 #include "gdn_glue.cuh"
 #include "rope.cuh"
 #include "kv8.cuh"
@@ -1751,11 +1752,142 @@ static int packed_rows(const arows::PackedParams& p, int D, cudaStream_t st) {
   return LB2_OK;
 }
 
+namespace lb2 {
+namespace packed {
+
+struct Layout {
+  size_t cnt, at, out, total;
+};
+
+static Layout layout(int64_t S, int64_t T) {  // sized for the smaller blocks
+  Layout l;
+  l.cnt = 256;
+  l.at = l.cnt + align_up(size_t(T / prefill::BM + 2) * 4, 256);
+  l.out = l.at + align_up(size_t(S + 2) * 4, 256);
+  l.total = l.out + align_up(size_t(T / prefill::BM + S + 2) * sizeof(int4), 256);
+  return l;
+}
+
+template <typename T, int D>
+static int launch(bool pair, const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm,
+                  const prefill::Params& p, int64_t blocks, cudaStream_t st) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 2;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  int dev = 0;
+  LB2_CUDA(cudaGetDevice(&dev));
+  if constexpr (D >= 128) {
+    if (pair) {
+      auto kern = prefill2::fmha2_kernel<T, D, true>;
+      cfg.blockDim = dim3(prefill2::THREADS);
+      cfg.dynamicSmemBytes = prefill2::Cfg<D>::SMEM_BYTES;
+      static int attr_dev = -1, max_clusters = 0;
+      if (attr_dev != dev) {
+        LB2_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, prefill2::Cfg<D>::SMEM_BYTES));
+        cfg.gridDim = dim3(2);
+        cfg.attrs = attr + 1;
+        cfg.numAttrs = 1;
+        LB2_CUDA(cudaOccupancyMaxActiveClusters(&max_clusters, kern, &cfg));
+        if (max_clusters < 1) return fail(LB2_ECUDA, "attn_packed: no 2-CTA cluster of the pair kernel fits the device");
+        attr_dev = dev;
+      }
+      cfg.attrs = attr;
+      cfg.numAttrs = 2;
+      cfg.gridDim = dim3(unsigned(2 * std::min<int64_t>(blocks * p.Hq, max_clusters)));
+      LB2_CUDA(cudaLaunchKernelEx(&cfg, kern, qm, km, vm, p));
+      return LB2_OK;
+    }
+  }
+  auto kern = prefill::fmha_kernel<T, D, true>;
+  static int attr_dev = -1;
+  if (attr_dev != dev) {
+    LB2_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, prefill::Cfg<D>::SMEM_BYTES));
+    attr_dev = dev;
+  }
+  cfg.blockDim = dim3(prefill::THREADS);
+  cfg.dynamicSmemBytes = prefill::Cfg<D>::SMEM_BYTES;
+  cfg.numAttrs = 1;
+  LB2_CHECK_ARG(blocks * p.Hq < (int64_t(1) << 31), "attn_packed: too many row blocks");
+  cfg.gridDim = dim3(unsigned(blocks * p.Hq));
+  LB2_CUDA(cudaLaunchKernelEx(&cfg, kern, qm, km, vm, p));
+  return LB2_OK;
+}
+
+static int run(const arows::PackedParams& a, int D, int dtype, void* workspace, cudaStream_t st) {
+  const void* src[3] = {a.q, a.k, a.v};
+  const int64_t* sst[3] = {a.q_st, a.k_st, a.v_st};
+  for (int i = 0; i < 3; ++i)
+    LB2_CHECK_ARG(aligned16(src[i]) && sst[i][0] % 8 == 0 && sst[i][1] % 8 == 0,
+                  "attn_packed: q, k and v must be 16-byte aligned with strides that are multiples of 8 elements");
+  LB2_CHECK_ARG(aligned16(a.o) && a.o_st[0] % 8 == 0 && a.o_st[1] % 8 == 0,
+                "attn_packed: o must be 16-byte aligned with strides that are multiples of 8 elements");
+  // Pairs of CTAs on 256 rows halve the K / V bytes an SM takes a product; one CTA on 128 rows leaves less of a tile
+  // empty. The lengths are on the device, so the mean length decides.
+  const bool pair = D >= 128 && int64_t(a.T) > int64_t(128) * a.S;
+  const Layout l = layout(a.S, a.T);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  PlanParams pp{};
+  pp.cu = a.cu;
+  pp.n = reinterpret_cast<int32_t*>(ws);
+  pp.cnt = reinterpret_cast<int32_t*>(ws + l.cnt);
+  pp.at = reinterpret_cast<int32_t*>(ws + l.at);
+  pp.out = reinterpret_cast<int4*>(ws + l.out);
+  pp.S = a.S;
+  pp.T = a.T;
+  pp.rb = pair ? 2 * prefill::BM : prefill::BM;
+  pp.bn = !pair && D == 256 ? prefill::Cfg<256>::BN : 128;
+  plan_kernel<<<1, THREADS, 0, st>>>(pp);
+  LB2_CUDA(cudaGetLastError());
+  prefill::Params p{};
+  p.o = a.o;
+  p.o_st[1] = a.o_st[0];
+  p.o_st[2] = a.o_st[1];
+  p.B = 1;
+  p.Hq = a.Hq;
+  p.Hkv = a.Hkv;
+  p.T = p.N = a.T;
+  p.G = a.Hq / a.Hkv;
+  p.mask_kind = LB2_MASK_CAUSAL;
+  p.scale_log2 = a.scale * 1.4426950408889634f;
+  p.pk = pp.out;
+  p.pk_n = pp.n;
+  for (int i = 0; i < 3; ++i) {
+    p.src[i] = src[i];
+    p.src_st[i][0] = sst[i][0];
+    p.src_st[i][1] = sst[i][1];
+  }
+  CUtensorMap maps[3];
+  const int rows[3] = {prefill::BM, pair ? 64 : pp.bn, pair ? 128 : pp.bn};
+  for (int i = 0; i < 3; ++i) {
+    const int64_t st4[3] = {8, sst[i][0], sst[i][1]};  // (one batch: its stride is never used)
+    const int rc = prefill::map4(&maps[i], src[i], st4, 1, i ? a.Hkv : a.Hq, a.T, D, dtype, rows[i]);
+    if (rc) return rc;
+  }
+  const int64_t blocks = int64_t(a.T) / pp.rb + a.S + 1;
+#define LB2_PACKED(TT)                                                                               \
+  return D == 64 ? launch<TT, 64>(pair, maps[0], maps[1], maps[2], p, blocks, st)                    \
+         : D == 128 ? launch<TT, 128>(pair, maps[0], maps[1], maps[2], p, blocks, st)                \
+                    : launch<TT, 256>(pair, maps[0], maps[1], maps[2], p, blocks, st)
+  if (dtype == LB2_BF16) LB2_PACKED(__nv_bfloat16);
+  LB2_PACKED(__half);
+#undef LB2_PACKED
+}
+
+}  // namespace packed
+}  // namespace lb2
+
 extern "C" {
 
 size_t lb2_attn_packed_workspace_size(int S, int T) {
   if (S <= 0 || T <= 0) return 0;
-  return 256;
+  return packed::layout(S, T).total;
 }
 
 int lb2_attn_packed(const void* q, const int64_t* q_st, const void* k, const int64_t* k_st, const void* v,
@@ -1767,8 +1899,6 @@ int lb2_attn_packed(const void* q, const int64_t* q_st, const void* k, const int
   LB2_CHECK_ARG(dtype == LB2_F32 || dtype == LB2_BF16 || dtype == LB2_F16, "attn_packed: dtype");
   if (T == 0) return LB2_OK;
   LB2_CHECK_ARG(q && k && v && o && q_st && k_st && v_st && o_st && cu, "attn_packed: missing argument");
-  LB2_CHECK_ARG(workspace != nullptr && workspace_bytes >= lb2_attn_packed_workspace_size(S, T),
-                "attn_packed: workspace too small");
   arows::PackedParams p{};
   p.q = q, p.k = k, p.v = v, p.o = o;
   for (int i = 0; i < 2; ++i) p.q_st[i] = q_st[i], p.k_st[i] = k_st[i], p.v_st[i] = v_st[i], p.o_st[i] = o_st[i];
@@ -1777,7 +1907,10 @@ int lb2_attn_packed(const void* q, const int64_t* q_st, const void* k, const int
   p.scale = scale;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (dtype == LB2_F32) return packed_rows<float>(p, D, st);
-  return dtype == LB2_BF16 ? packed_rows<__nv_bfloat16>(p, D, st) : packed_rows<__half>(p, D, st);
+  LB2_CHECK_ARG(workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0 &&
+                    workspace_bytes >= lb2_attn_packed_workspace_size(S, T),
+                "attn_packed: workspace too small or not 256-byte aligned");
+  return packed::run(p, D, dtype, workspace, st);
 }
 
 }  // extern "C"
