@@ -67,6 +67,8 @@ struct AppendParams {
   const int32_t* cu;    // packed: rows [cu[b], cu[b + 1]) are b's, or nullptr
   const uint64_t* turns;
   int B, Hkv, T, D, R, page, num_pages, max_pages, touched;
+  int lpage, lupr;  // log2 of page and of a row's units (D / 16)
+  int hpb;          // heads a block takes in turn
   int interleaved;
   float amp;
 };
@@ -78,39 +80,97 @@ __device__ __forceinline__ float finite_abs(float x) {
   return a < INFINITY ? a : 0.f;
 }
 
-// One block a (page that a sequence's new tokens reach, head, K or V): the rows' largest magnitude after rotation, the
-// page's new scale, held codes rescaled where it grew, the new rows' codes. Rows are walked twice (the second time from
-// L1 / L2).
+// The sequence and page (b, j-th page that its new tokens reach) of block i. With T tokens each there are `touched` blocks
+// a sequence. Packed, sequence b's blocks start at cu[b] / page + 2 b, which leaves room for every page its tokens can
+// reach at any alignment (n tokens touch at most n / page + 2): a 32-way search, each warp for itself.
+__device__ __forceinline__ bool find_page(const AppendParams& p, int i, int& b, int& j) {
+  if (!p.cu) {
+    b = p.touched == 1 ? i : i / p.touched;
+    j = i - b * p.touched;
+    return true;
+  }
+  auto base = [&](int s) { return (min(max(p.cu[s], 0), p.T) >> p.lpage) + 2 * s; };
+  int lo = 0, hi = p.B;  // base(lo) <= i, and base(hi) > i or hi == B
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 31) / 32, s = lo + (threadIdx.x & 31) * step;
+    const uint32_t le = __ballot_sync(0xffffffffu, s < hi && (s == lo || base(s) <= i));
+    const int k = 31 - __clz(le);
+    lo += k * step;
+    hi = min(hi, lo + step);
+  }
+  b = lo;
+  j = i - base(lo);
+  return j >= 0;
+}
+
+// One block's work: a page of sequence b that its new tokens reach, K or V, of heads h on.
+struct Piece {
+  int b, h, kind;
+  int lo, hi;       // the page's new rows
+  int id;           // physical page, or out of range
+  int64_t base;     // position of the page's first token
+  int64_t row0;     // source row of page row lo
+  int64_t slot;     // (page, K / V, head) index of the scale
+};
+
+__device__ __forceinline__ bool piece_of(const AppendParams& p, Piece& w) {
+  w.kind = blockIdx.y & 1;
+  w.h = (blockIdx.y >> 1) * p.hpb;
+  int j;
+  if (!find_page(p, blockIdx.x, w.b, j)) return false;
+  const int n0 = p.start[w.b];
+  const int r0 = p.cu ? p.cu[w.b] : 0;
+  const int n = p.cu ? min(p.cu[w.b + 1], p.T) - r0 : p.lens ? min(p.lens[w.b], p.T) : p.T;
+  if (n <= 0 || n0 < 0 || r0 < 0) return false;
+  const int64_t pj = int64_t(n0 >> p.lpage) + j;  // the sequence's page
+  w.base = pj << p.lpage;
+  if (w.base >= int64_t(n0) + n) return false;
+  w.lo = int(max(int64_t(n0) - w.base, int64_t(0)));
+  w.hi = int(min(int64_t(n0) + n - w.base, int64_t(p.page)));
+  w.row0 = int64_t(r0) + (w.base + w.lo - n0);
+  w.id = pj < p.max_pages ? p.table[w.b * p.table_st + pj] : -1;
+  w.slot = (int64_t(w.id) * 2 + w.kind) * p.Hkv + w.h;
+  return true;
+}
+
+__device__ __forceinline__ bool bad_page(const AppendParams& p, const Piece& w) {
+  if (w.id >= 0 && w.id < p.num_pages) return false;
+  if (threadIdx.x == 0) report_bad_index(STATUS_APPEND);
+  return true;
+}
+
+// Rescales the page's held codes (rows before lo) where its scale grew from `was` to 1 / inv.
+template <int THREADS>
+__device__ __forceinline__ void rescale_held(uint8_t* dst, int bytes, float was, float now, float inv) {
+  if (now == was || !(was > 0.f)) return;
+  const float ratio = was * inv;
+  for (int i = threadIdx.x; i < bytes / 16; i += THREADS) {
+    uint4 w = reinterpret_cast<uint4*>(dst)[i];
+    uint32_t* u = reinterpret_cast<uint32_t*>(&w);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      uint32_t a, c;
+      dec4(u[e], a, c);
+      const float2 f = half2_f(a), g = half2_f(c);
+      u[e] = enc4(f.x * ratio, f.y * ratio, g.x * ratio, g.y * ratio);
+    }
+    reinterpret_cast<uint4*>(dst)[i] = w;
+  }
+}
+
+// Any strides, alignment and number of rotated dims: an element at a time, walked twice (the second time from L1 / L2).
 template <typename T>
-__global__ void __launch_bounds__(128) append_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(128) append_any_kernel(const AppendParams p) {
   __shared__ float red[4];
-  const int kind = blockIdx.y & 1, h = blockIdx.y >> 1;
-  int b, j;
-  {
-    b = blockIdx.x / p.touched;
-    j = blockIdx.x - b * p.touched;
-  }
-  const int n0 = p.start[b];
-  const int r0 = p.cu ? p.cu[b] : 0;
-  const int n = p.cu ? min(p.cu[b + 1], p.T) - r0 : p.lens ? min(p.lens[b], p.T) : p.T;
-  if (n <= 0 || n0 < 0 || r0 < 0) return;
-  const int64_t pj = int64_t(n0 / p.page) + j;  // the sequence's page
-  const int64_t base = pj * p.page;
-  if (base >= int64_t(n0) + n) return;
-  const int lo = int(max(int64_t(n0) - base, int64_t(0)));                      // first new row of the page
-  const int hi = int(min(int64_t(n0) + n - base, int64_t(p.page)));             // past the last
-  const int id = pj < p.max_pages ? p.table[b * p.table_st + pj] : -1;
-  if (id < 0 || id >= p.num_pages) {
-    if (threadIdx.x == 0) report_bad_index(STATUS_APPEND);
-    return;
-  }
-  const T* x = static_cast<const T*>(p.x[kind]) + (p.cu ? 0 : b * p.st[kind][0]) + h * p.st[kind][1];
-  const int64_t row0 = int64_t(r0) + (base + lo - n0);  // source row of page row lo
-  const int rot = kind == 0 ? p.R : 0, R2 = rot >> 1;
-  const int D = p.D, cnt = (hi - lo) * D;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  Piece w;
+  if (!piece_of(p, w) || bad_page(p, w)) return;
+  const T* x = static_cast<const T*>(p.x[w.kind]) + (p.cu ? 0 : w.b * p.st[w.kind][0]) + w.h * p.st[w.kind][1];
+  const int rot = w.kind == 0 ? p.R : 0, R2 = rot >> 1;
+  const int D = p.D, cnt = (w.hi - w.lo) * D;
   auto value = [&](int i) {
     const int r = i / D, d = i - r * D;
-    const T* xr = x + (row0 + r) * p.st[kind][2];
+    const T* xr = x + (w.row0 + r) * p.st[w.kind][2];
     const float v = to_f<T>(xr[d]);
     if (d >= rot) return v;
     int f, o;
@@ -120,7 +180,7 @@ __global__ void __launch_bounds__(128) append_kernel(const AppendParams p) {
     } else {
       f = d < R2 ? d : d - R2, o = d < R2 ? d + R2 : d - R2, sg = d < R2 ? -1.f : 1.f;
     }
-    const float2 z = rope::turn_cs(uint64_t(base + lo + r) * p.turns[f]);
+    const float2 z = rope::turn_cs(uint64_t(w.base + w.lo + r) * p.turns[f]);
     return p.amp * (v * z.x + sg * to_f<T>(xr[o]) * z.y);
   };
   float m = 0.f;
@@ -128,27 +188,147 @@ __global__ void __launch_bounds__(128) append_kernel(const AppendParams p) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
-  __syncthreads();
+  const float was = w.lo > 0 ? p.scales[w.slot] : 0.f;
+  __syncthreads();  // (every thread has read the old scale)
   m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  const int64_t slot = (int64_t(id) * 2 + kind) * p.Hkv + h;
-  const float was = lo > 0 ? p.scales[slot] : 0.f;
-  const float now = fmaxf(was, scale_of(m));
-  __syncthreads();  // every thread has read the old scale
-  if (threadIdx.x == 0) p.scales[slot] = now;
-  uint8_t* dst = p.pages + slot * int64_t(p.page) * D;
-  const float inv = scale_inv(now);
-  if (now != was && was > 0.f) {
-    const float ratio = was * inv;
-    for (int i = threadIdx.x; i < lo * D / 4; i += 128) {
-      uint32_t a, c;
-      dec4(reinterpret_cast<uint32_t*>(dst)[i], a, c);
-      const float2 f = half2_f(a), g = half2_f(c);
-      reinterpret_cast<uint32_t*>(dst)[i] = enc4(f.x * ratio, f.y * ratio, g.x * ratio, g.y * ratio);
+  const float now = fmaxf(was, scale_of(m)), inv = scale_inv(now);
+  if (threadIdx.x == 0) p.scales[w.slot] = now;
+  uint8_t* dst = p.pages + w.slot * int64_t(p.page) * D;
+  rescale_held<128>(dst, w.lo * D, was, now, inv);
+  for (int i = 4 * threadIdx.x; i < cnt; i += 4 * 128)
+    *reinterpret_cast<uint32_t*>(dst + w.lo * D + i) =
+        enc4(value(i) * inv, value(i + 1) * inv, value(i + 2) * inv, value(i + 3) * inv);
+}
+
+// (cos, sin) of frac 2^-32 turns by the multi-function unit: the angle is within pi 2^-23 of the fraction's, the unit
+// within 2^-21 of its sine and cosine; the code that the key becomes has 4 significant bits.
+__device__ __forceinline__ float2 turn_cs_fast(uint32_t frac) {
+  const float t = __uint_as_float(0x3f800000u | ((frac ^ 0x80000000u) >> 9)) - 1.5f;  // turns, in [-1/2, 1/2)
+  const float a = t * 6.2831853071795865f;
+  return make_float2(__cosf(a), __sinf(a));
+}
+
+// Rows of 16-byte groups: the page's new rows are held in registers, read once. A unit is two groups of 8 elements: in
+// the rotated half layout a group and its partners R / 2 on, elsewhere neighbours; a thread has one unit of K rows. The
+// block takes `hpb` heads in turn, the next one's loads in flight while it works: the angles of its rows serve them all.
+// Bound by HBM for long prompts (2 bytes read and 1 written a value), by the chain start -> table -> scale for single
+// tokens.
+template <typename T, int THREADS, int K>
+__global__ void __launch_bounds__(THREADS) append_kernel(const AppendParams p) {
+  constexpr int WARPS = THREADS / 32;
+  constexpr int V = 16 / int(sizeof(T)), N = 8 / V;  // values a load, loads a group
+  __shared__ float red[2][WARPS];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  Piece w;
+  if (!piece_of(p, w)) return;
+  const int D = p.D, u = threadIdx.x & ((1 << p.lupr) - 1), first = threadIdx.x >> p.lupr;
+  const int rpp = THREADS >> p.lupr, nrows = w.hi - w.lo;
+  const int rot = w.kind == 0 ? p.R : 0, R2 = rot >> 1;
+  const bool half = !p.interleaved && u * 8 < R2;
+  const int a = half ? u * 8 : u * 16, c = half ? a + R2 : a + 8;
+  const int64_t hst = p.st[w.kind][1], tst = p.st[w.kind][2];
+  const T* x = static_cast<const T*>(p.x[w.kind]) + (p.cu ? 0 : w.b * p.st[w.kind][0]) + w.h * hst +
+               (w.row0 + first) * tst;
+  const int nh = min(p.hpb, p.Hkv - w.h);
+  rope::Raw<T, V> ra[K][N], rc[K][N];
+  auto fetch = [&](const T* xr) {
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+      if (first + k * rpp < nrows)
+#pragma unroll
+        for (int g = 0; g < N; ++g) {
+          ra[k][g].load(xr + k * rpp * tst + a + g * V);
+          rc[k][g].load(xr + k * rpp * tst + c + g * V);
+        }
+  };
+  fetch(x);
+  if (bad_page(p, w)) return;  // (the same for every thread)
+  float was = w.lo > 0 ? p.scales[w.slot] : 0.f;
+  const bool turn = half || (p.interleaved && a < rot);  // (R is a multiple of 16: a unit is rotated whole or not at all)
+  float2 z[K][8];
+  if (turn) {
+    uint64_t f[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = p.turns[half ? a + e : (a >> 1) + e];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      if (first + k * rpp >= nrows) break;
+      const uint32_t pos = uint32_t(w.base + w.lo + first + k * rpp);  // (below 2^31)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        z[k][e] = turn_cs_fast(uint32_t((pos * f[e]) >> 32));
+        z[k][e].x *= p.amp, z[k][e].y *= p.amp;
+      }
     }
   }
-  for (int i = 4 * threadIdx.x; i < cnt; i += 4 * 128)
-    *reinterpret_cast<uint32_t*>(dst + lo * D + i) =
-        enc4(value(i) * inv, value(i + 1) * inv, value(i + 2) * inv, value(i + 3) * inv);
+  for (int i = 0; i < nh; ++i) {
+    float xa[K][8], xc[K][8], m = 0.f;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      if (first + k * rpp >= nrows) break;
+#pragma unroll
+      for (int g = 0; g < N; ++g) {
+        ra[k][g].get(xa[k] + g * V);
+        rc[k][g].get(xc[k] + g * V);
+      }
+      if (turn) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          float& x0 = half ? xa[k][e] : (e < 4 ? xa[k][(2 * e) & 7] : xc[k][(2 * e) & 7]);
+          float& x1 = half ? xc[k][e] : (e < 4 ? xa[k][(2 * e + 1) & 7] : xc[k][(2 * e + 1) & 7]);
+          const float y0 = x0 * z[k][e].x - x1 * z[k][e].y, y1 = x1 * z[k][e].x + x0 * z[k][e].y;
+          x0 = y0, x1 = y1;
+        }
+      }
+      float mk = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) mk = fmaxf(mk, fmaxf(fabsf(xa[k][e]), fabsf(xc[k][e])));  // (NaN is passed over)
+      if (mk == INFINITY) {  // rare: the largest of the finite
+        mk = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) mk = fmaxf(mk, fmaxf(finite_abs(xa[k][e]), finite_abs(xc[k][e])));
+      }
+      m = fmaxf(m, mk);
+    }
+    const int64_t slot = w.slot + i;
+    const float old = was;
+    if (i + 1 < nh) {
+      fetch(x + (i + 1) * hst);
+      if (w.lo > 0) was = p.scales[slot + 1];
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if constexpr (WARPS > 1) {
+      float* r = red[i & 1];  // (the other half may still be read by warps behind)
+      if ((threadIdx.x & 31) == 0) r[threadIdx.x >> 5] = m;
+      __syncthreads();  // (every thread has read the old scale)
+      for (int q = 0; q < WARPS; ++q) m = fmaxf(m, r[q]);
+    } else {
+      __syncwarp();
+    }
+    const float now = fmaxf(old, scale_of(m)), inv = scale_inv(now);
+    if (threadIdx.x == 0) p.scales[slot] = now;
+    uint8_t* dst = p.pages + slot * (int64_t(D) << p.lpage);
+    rescale_held<THREADS>(dst, w.lo * D, old, now, inv);
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int r = first + k * rpp;
+      if (r >= nrows) break;
+      uint8_t* d = dst + (w.lo + r) * D;
+      auto enc8 = [&](const float* f) {
+        return make_uint2(enc4(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv),
+                          enc4(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv));
+      };
+      const uint2 ya = enc8(xa[k]), yc = enc8(xc[k]);
+      if (half) {
+        *reinterpret_cast<uint2*>(d + a) = ya;
+        *reinterpret_cast<uint2*>(d + c) = yc;
+      } else {
+        *reinterpret_cast<uint4*>(d + a) = make_uint4(ya.x, ya.y, yc.x, yc.y);
+      }
+    }
+  }
 }
 
 }  // namespace kv8

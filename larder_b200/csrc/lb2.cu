@@ -1463,19 +1463,36 @@ int lb2_qsa_select(const void* q, const void* pooled, int64_t pool_bstride, int 
 
 namespace {
 
-template <typename T, int V>
+template <typename T, int V, int K>
 int rope_launch(const rope::Params& p0, cudaStream_t st) {
   rope::Params p = p0;
-  // A block takes about 1024 units (four a thread), whole tokens of as many heads as that allows; small calls are cut
-  // finer so that they fill the SMs.
   const int upr = p.D / (2 * V), rows = p.B * p.T;
-  p.hg = p.H;
-  p.tok = std::max(1, std::min(rows, 1024 / std::max(1, upr * p.H)));
-  const int smem = p.tok * (p.R / 2) * int(sizeof(float2));
-  const dim3 grid(unsigned((rows + p.tok - 1) / p.tok), unsigned((p.H + p.hg - 1) / p.hg));
-  rope::rope_kernel<T, V><<<grid, rope::THREADS, smem, st>>>(p);
-  LB2_CUDA(cudaGetLastError());
+  const int rpp = std::max(1, rope::THREADS / upr), per = rpp * K;  // (token, head) rows a pass, a block
+  p.hg = std::min(p.H, per);
+  p.ltok = 0;  // tokens that divide a pass's rows, so that a thread's rows are of one token; 8 bytes an angle
+  while (rpp % (2 << p.ltok) == 0 && (2 << p.ltok) * p.hg <= per && (2 << p.ltok) * p.R * 4 <= 32 * 1024) ++p.ltok;
+  const int tok = 1 << p.ltok;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned((rows + tok - 1) / tok), unsigned((p.H + p.hg - 1) / p.hg));
+  cfg.blockDim = dim3(rope::THREADS);
+  cfg.dynamicSmemBytes = size_t(tok) * (p.R / 2) * sizeof(float2);
+  cfg.stream = st;
+  LB2_CHECK_ARG(cfg.gridDim.y < 65536, "rope: too many heads");
+  cudaLaunchAttribute pdl[1];
+  pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  pdl[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = pdl;
+  cfg.numAttrs = 1;
+  LB2_CUDA(cudaLaunchKernelEx(&cfg, rope::rope_kernel<T, V, K>, p));
   return LB2_OK;
+}
+
+// Four rows a thread keep enough loads in flight to stream; a call too small to give every SM a block that way spreads
+// over more blocks of one row a thread.
+template <typename T, int V>
+int rope_rows(const rope::Params& p, cudaStream_t st) {
+  const int64_t units = int64_t(p.B) * p.T * p.H * (p.D / (2 * V));
+  return units >= int64_t(2) * 148 * 4 * rope::THREADS ? rope_launch<T, V, 4>(p, st) : rope_launch<T, V, 1>(p, st);
 }
 
 template <typename T>
@@ -1483,7 +1500,7 @@ int rope_run(const rope::Params& p, cudaStream_t st) {
   constexpr int V = 16 / int(sizeof(T));
   bool wide = p.D % (2 * V) == 0 && p.R % (2 * V) == 0 && aligned16(p.x) && aligned16(p.y);
   for (int i = 0; i < 3; ++i) wide = wide && p.x_st[i] % V == 0 && p.y_st[i] % V == 0;
-  return wide ? rope_launch<T, V>(p, st) : rope_launch<T, 1>(p, st);
+  return wide ? rope_rows<T, V>(p, st) : rope_launch<T, 1, 1>(p, st);
 }
 
 }  // namespace
@@ -1531,6 +1548,41 @@ static int kv8_shape(int B, int Hkv, int T, int D, int page, int num_pages, int 
   return LB2_OK;
 }
 
+}  // extern "C"
+
+template <typename T>
+static int kv8_append_run(kv8::AppendParams& p, bool wide, int64_t blocks, cudaStream_t st) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.stream = st;
+  cudaLaunchAttribute pdl[1];
+  pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  pdl[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = pdl;
+  cfg.numAttrs = 1;
+  auto go = [&](auto kern, int threads) {
+    cfg.blockDim = dim3(unsigned(threads));
+    cfg.gridDim = dim3(unsigned(blocks), unsigned(2 * ((p.Hkv + p.hpb - 1) / p.hpb)));
+    LB2_CUDA(cudaLaunchKernelEx(&cfg, kern, p));
+    return int(LB2_OK);
+  };
+  p.hpb = 1;
+  if (!wide) return go(kv8::append_any_kernel<T>, 128);
+  const int upr = p.D / 16;
+  if (!p.cu && int64_t(p.T) * upr <= 32) return go(kv8::append_kernel<T, 32, 1>, 32);  // a few tokens: a warp a piece
+  // heads a block: as many as leave every SM several blocks
+  while (p.hpb < 4 && blocks * 2 * p.Hkv >= int64_t(148) * 8 * 2 * p.hpb) p.hpb *= 2;
+  switch (p.page * upr) {  // a page's units over the threads, at most two a thread
+    case 64: return go(kv8::append_kernel<T, 64, 1>, 64);
+    case 128: return go(kv8::append_kernel<T, 128, 1>, 128);
+    case 256: return go(kv8::append_kernel<T, 128, 2>, 128);
+    case 512: return go(kv8::append_kernel<T, 256, 2>, 256);
+    case 1024: return go(kv8::append_kernel<T, 512, 2>, 512);
+    default: return go(kv8::append_kernel<T, 1024, 2>, 1024);
+  }
+}
+
+extern "C" {
+
 int lb2_kv8_append(uint8_t* pages, float* scales, const void* k, const int64_t* k_st, const void* v,
                    const int64_t* v_st, const int32_t* table, int64_t table_st, const int32_t* start,
                    const int32_t* lens, const int32_t* cu, const uint64_t* turns, int B, int Hkv, int T, int D, int R,
@@ -1559,16 +1611,20 @@ int lb2_kv8_append(uint8_t* pages, float* scales, const void* k, const int64_t* 
   p.B = B, p.Hkv = Hkv, p.T = T, p.D = D, p.R = R;
   p.page = page, p.num_pages = num_pages, p.max_pages = max_pages;
   p.touched = int((int64_t(T) + page - 2) / page) + 1;
+  p.lpage = page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : 7;
+  p.lupr = D == 64 ? 2 : D == 128 ? 3 : 4;
   p.interleaved = interleaved != 0;
   p.amp = amp;
-  LB2_CHECK_ARG(int64_t(B) * p.touched < (int64_t(1) << 31), "kv8_append: too many rows");
-  const dim3 grid(unsigned(B) * unsigned(p.touched), unsigned(2 * Hkv));
+  const int64_t blocks = cu ? int64_t(T) / page + 2 * int64_t(B) : int64_t(B) * p.touched;
+  LB2_CHECK_ARG(blocks < (int64_t(1) << 31), "kv8_append: too many rows");
+  // 16-byte groups where every row starts on one and a unit of two groups is rotated whole or not at all
+  const int item = dtype == LB2_F32 ? 4 : 2;
+  bool wide = R % 16 == 0 && aligned16(k) && aligned16(v);
+  for (int i = 0; i < 3; ++i) wide = wide && k_st[i] * item % 16 == 0 && v_st[i] * item % 16 == 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (dtype == LB2_F32) kv8::append_kernel<float><<<grid, 128, 0, st>>>(p);
-  else if (dtype == LB2_BF16) kv8::append_kernel<__nv_bfloat16><<<grid, 128, 0, st>>>(p);
-  else kv8::append_kernel<__half><<<grid, 128, 0, st>>>(p);
-  LB2_CUDA(cudaGetLastError());
-  return LB2_OK;
+  return dtype == LB2_F32    ? kv8_append_run<float>(p, wide, blocks, st)
+         : dtype == LB2_BF16 ? kv8_append_run<__nv_bfloat16>(p, wide, blocks, st)
+                             : kv8_append_run<__half>(p, wide, blocks, st);
 }
 
 }  // extern "C"
