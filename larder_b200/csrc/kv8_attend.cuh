@@ -41,13 +41,16 @@ constexpr int BK = 64;       // keys a tile
 constexpr int MAX_B = 1024;  // sequences a launch (the prefix table in shared memory); larger batches go in several
 constexpr int STATUS = 112;  // where (lb2_status): 112 page id, 113.. waits
 
-// NT: 8-row tiles of query rows a warp; RG: row groups (sets of four warps taking the same tile for other rows); KG: key
-// groups (sets of four warps taking alternate tiles).
-template <int D, int NT, int RG, int KG>
+// NT: 8-row tiles of query rows a warp; MK: 16-key blocks of a tile a warp (two give it two independent chains of
+// products); RG: row groups (sets of warps taking the same tile for other rows); KG: key groups (sets of warps taking
+// every KG-th tile).
+template <int D, int NT, int RG, int MK, int KG>
 struct Cfg {
   static constexpr int RP = 8 * NT * RG;  // rows of a block, padded
-  static constexpr int WARPS = 4 * RG * KG;
-  static constexpr int THREADS = (WARPS + 1) * 32;
+  static constexpr int SL = 4 / MK;       // key slices of a tile
+  static constexpr int WARPS = SL * RG * KG;
+  static constexpr int NP = D == 256 ? 2 : 4;  // producer warps: they take the tiles in turn
+  static constexpr int THREADS = (WARPS + NP) * 32;
   static constexpr int BW = D < 128 ? D : 128;  // bytes a box row
   static constexpr int TILE = BK * D;           // bytes of a K (or V) tile
   static constexpr int STAGE = 2 * TILE;
@@ -57,7 +60,10 @@ struct Cfg {
   static constexpr int PART = WARPS / 2 * PART_REGS * 32 * 16;  // half the warps' parts
   static constexpr int FIXED = QBYTES + PART + (2 * MAX_B + 1) * 4 + 1024 + 1024;
   static constexpr int FIT = (232448 - FIXED) / (STAGE + 48);
-  static constexpr int STAGES = (FIT > 10 ? 10 : FIT) / KG * KG;
+  // A multiple of both, so that a stage only ever serves one producer warp and one key group, whose waits on it then
+  // follow its phases in order (a wait two phases ahead would pass at once).
+  static constexpr int STEP = KG > NP ? KG : NP;
+  static constexpr int STAGES = (FIT > 16 ? 16 : FIT) / STEP * STEP;
   static constexpr int Q_OFF = STAGES * STAGE;
   static constexpr int PART_OFF = Q_OFF + QBYTES;
   static constexpr int SC_OFF = PART_OFF + PART;                 // [STAGES][4 slices][K, V] fp32
@@ -65,7 +71,7 @@ struct Cfg {
   static constexpr int LENS_OFF = PREFIX_OFF + (MAX_B + 1) * 4;  // [MAX_B]
   static constexpr int BAR_OFF = (LENS_OFF + MAX_B * 4 + 15) / 16 * 16;
   static constexpr int SMEM = BAR_OFF + 2 * STAGES * 8 + 16 + 1024;
-  static_assert(STAGES >= 2 && SMEM <= 232448, "shared memory budget");
+  static_assert(STEP % KG == 0 && STEP % NP == 0 && STAGES >= 2 * KG && SMEM <= 232448, "shared memory budget");
 };
 
 struct Params {
@@ -166,11 +172,11 @@ __device__ __forceinline__ int seq_len(const Params& p, int b) {
   return int(min(int64_t(max(p.a.kv_len[b], 0)), int64_t(p.a.max_pages) << p.lpage));
 }
 
-template <typename T, int D, int NT, int RG, int KG>
-__global__ void __launch_bounds__(Cfg<D, NT, RG, KG>::THREADS, 1)
+template <typename T, int D, int NT, int RG, int MK, int KG>
+__global__ void __launch_bounds__(Cfg<D, NT, RG, MK, KG>::THREADS, 1)
     attend_kernel(const __grid_constant__ CUtensorMap map, const Params p) {
-  using C = Cfg<D, NT, RG, KG>;
-  constexpr int STAGES = C::STAGES, WARPS = C::WARPS, SEG = D / 64;
+  using C = Cfg<D, NT, RG, MK, KG>;
+  constexpr int STAGES = C::STAGES, WARPS = C::WARPS, SL = C::SL, SEG = D / 64;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   int* prefix = reinterpret_cast<int*>(sm + C::PREFIX_OFF);
@@ -184,7 +190,7 @@ __global__ void __launch_bounds__(Cfg<D, NT, RG, KG>::THREADS, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < STAGES; ++i) {
       mbar_init(&full[i], 1);
-      mbar_init(&empty[i], 4 * RG);
+      mbar_init(&empty[i], SL * RG);
     }
     *abort_flag = 0;
     fence_barrier_init();
@@ -217,14 +223,21 @@ __global__ void __launch_bounds__(Cfg<D, NT, RG, KG>::THREADS, 1)
   Sched sched(p, prefix, lens);
   Item it;
 
-  if (warp == WARPS) {
-    // ------------------------------------------------------------------ producer warp
+  if (warp >= WARPS) {
+    // ------------------------------------------------------------------ producer warps
     // Page ids and scales come 32 pages at a time, a lane a page, the next 32 loaded while these are used. A tile's boxes
-    // (a page's rows, K or V, 128 bytes wide) are issued by a lane each.
+    // (a page's rows, K or V, 128 bytes wide) are issued by a lane each. One warp's chain of instructions for a tile
+    // (about 800 clocks) is slower than the tile's bytes arrive, so several warps take the tiles in turn.
     constexpr int NB = D / C::BW;  // boxes across a row
+    constexpr int NP = C::NP;
     const int sub = BK / p.box;    // boxes down a tile
     const int per = p.box < (1 << p.lpage) ? (1 << p.lpage) / p.box : 1;  // tiles a page (128-token pages: 2)
-    int gt = 0;
+    // lane = ((page in tile) NB + box) 2 + (K, V); lanes 0 .. 3 also write a slice of 16 keys' scales
+    const int kv = lane & 1, bx = (lane >> 1) % NB, pg = (lane >> 1) / NB;
+    const bool mine = pg < sub;
+    const int dst = kv * C::TILE + bx * (BK * C::BW) + pg * p.box * C::BW;
+    const int sp = (lane & 3) * 16 / p.box;
+    int gt = warp - WARPS, done = 0;  // this warp's next tile; tiles of the items before
     bool ok = true;
     while (ok && sched.next(it)) {
       const int hk = it.hb / p.nrb;
@@ -249,9 +262,11 @@ __global__ void __launch_bounds__(Cfg<D, NT, RG, KG>::THREADS, 1)
       float ks, vs, nks, nvs;
       fetch(j0 + lane, id, ks, vs);
       fetch(j0 + 32 + lane, nid, nks, nvs);
-      for (int i = it.i0; i < it.i1; ++i, ++gt) {
+      const int tiles = it.i1 - it.i0;
+      for (; gt - done < tiles; gt += NP) {
+        const int i = it.i0 + gt - done;
         const int j = (i * BK) >> p.lpage;  // first page of the tile
-        if (j - j0 >= 32) {                 // (a tile's pages never straddle: sub divides 32)
+        if (j - j0 >= 32) {                 // (a tile's pages never straddle: a tile has 1, 2 or 4; steps are below 32)
           j0 += 32;
           id = nid, ks = nks, vs = nvs;
           fetch(j0 + 32 + lane, nid, nks, nvs);
@@ -263,33 +278,29 @@ __global__ void __launch_bounds__(Cfg<D, NT, RG, KG>::THREADS, 1)
           ok = false;
           break;
         }
-        uint8_t* base = sm + st * C::STAGE;
-        // lane = ((page in tile) NB + box) 2 + (K, V)
-        const int kv = lane & 1, bx = (lane >> 1) % NB, pg = (lane >> 1) / NB;
-        const int pid = __shfl_sync(0xffffffffu, id, (j - j0 + (pg < sub ? pg : 0)) & 31);
-        const bool go = pg < sub && pid >= 0;
+        const int pid = __shfl_sync(0xffffffffu, id, j - j0 + (mine ? pg : 0));
+        const bool go = mine && pid >= 0;
         if (go)
-          tma_load_4d(base + kv * C::TILE + bx * (BK * C::BW) + pg * p.box * C::BW, &map, bx * C::BW,
-                      per > 1 ? (i & (per - 1)) * BK : 0, kv * p.a.Hkv + hk, pid, &full[st]);
-        // slice of 16 keys: its page's scales
-        const int sp = (lane & 3) * 16 >= p.box ? (lane & 3) * 16 / p.box : 0;
-        const float a = __shfl_sync(0xffffffffu, ks, (j - j0 + sp) & 31), c = __shfl_sync(0xffffffffu, vs, (j - j0 + sp) & 31);
+          tma_load_4d(sm + st * C::STAGE + dst, &map, bx * C::BW, per > 1 ? (i & (per - 1)) * BK : 0, kv * p.a.Hkv + hk,
+                      pid, &full[st]);
+        const float a = __shfl_sync(0xffffffffu, ks, j - j0 + sp), c = __shfl_sync(0xffffffffu, vs, j - j0 + sp);
         if (lane < 4) *reinterpret_cast<float2*>(scl + (st * 4 + lane) * 2) = make_float2(a, c);
         const uint32_t n = __popc(__ballot_sync(0xffffffffu, go));
         __syncwarp();  // the scales are written before lane 0's arrival
         if (lane == 0) mbar_arrive_expect_tx(&full[st], n * uint32_t(p.box * C::BW));
       }
+      done += tiles;
     }
     if (!ok && lane == 0) *abort_flag = 1;
-    // Drain: the last copies issued have landed before the CTA ends.
+    // Drain: the last copies this warp issued have landed before the CTA ends.
     if (lane == 0)
-      for (int g = max(0, gt - STAGES); g < gt; ++g) mbar_wait(&full[g % STAGES], (g / STAGES) & 1, STATUS + 2);
+      for (int g = gt - NP; g >= 0 && g > gt - NP - STAGES; g -= NP) mbar_wait(&full[g % STAGES], (g / STAGES) & 1, STATUS + 2);
     return;
   }
 
   // ------------------------------------------------------------------ consumer warps
   const int quad = lane >> 2, qid = lane & 3;
-  const int wq = warp & 3, rg = (warp >> 2) % RG, kg = (warp >> 2) / RG;
+  const int sl = warp % SL, rg = (warp / SL) % RG, kg = warp / (SL * RG);
   const int Tq = p.a.T;
   uint32_t qf[C::Q_REGS ? NT : 1][C::Q_REGS ? SEG : 1][8];  // this row's 16 dims of each 64-dim segment
   uint4* qsm = reinterpret_cast<uint4*>(sm + C::Q_OFF);     // [RG][NT][SEG][2][32 lanes]
@@ -337,7 +348,7 @@ __global__ void __launch_bounds__(Cfg<D, NT, RG, KG>::THREADS, 1)
         if constexpr (C::Q_REGS) {
 #pragma unroll
           for (int e = 0; e < 8; ++e) qf[nt][s][e] = w[e];
-        } else if (wq == 0 && kg == 0) {
+        } else if (sl == 0 && kg == 0) {
           uint4* d = qsm + ((rg * NT + nt) * SEG + s) * 64 + lane;
           d[0] = make_uint4(w[0], w[1], w[2], w[3]);
           d[32] = make_uint4(w[4], w[5], w[6], w[7]);
@@ -373,25 +384,29 @@ __global__ void __launch_bounds__(Cfg<D, NT, RG, KG>::THREADS, 1)
       }
       uint8_t* kt = sm + st * C::STAGE;
       uint8_t* vt = kt + C::TILE;
-      const int kbase = i * BK + wq * 16;
-      const int nvalid = min(16, max(0, it.len - kbase));
-      const float2 sc2 = *reinterpret_cast<const float2*>(scl + (st * 4 + wq) * 2);
-      if (nvalid < 16) {  // values past the length: zeros (rows by key, so that P = 0 meets no NaN code)
-        for (int e = lane; e < (16 - nvalid) * (D / 16); e += 32) {
-          const int r = wq * 16 + nvalid + e / (D / 16), c = e % (D / 16);
+      const int kbase = i * BK + sl * 16 * MK;  // the warp's first key
+      const int nvalid = min(16 * MK, max(0, it.len - kbase));
+      if (nvalid < 16 * MK) {  // values past the length: zeros, so that P = 0 meets no NaN code
+        for (int e = lane; e < (16 * MK - nvalid) * (D / 16); e += 32) {
+          const int r = sl * 16 * MK + nvalid + e / (D / 16), c = e % (D / 16);
           *reinterpret_cast<uint4*>(vt + at<D>(r, c)) = make_uint4(0, 0, 0, 0);
         }
         __syncwarp();
       }
-      float s[NT][4];
+      float s[MK][NT][4];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
-      const int kr = wq * 16 + key_of<D>(quad);
+      for (int mk = 0; mk < MK; ++mk)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) s[mk][nt][0] = s[mk][nt][1] = s[mk][nt][2] = s[mk][nt][3] = 0.f;
 #pragma unroll
       for (int sg = 0; sg < SEG; ++sg) {
-        const uint4 ka = *reinterpret_cast<const uint4*>(kt + at<D>(kr, 4 * sg + qid));
-        const uint4 kb = *reinterpret_cast<const uint4*>(kt + at<D>(kr + 8, 4 * sg + qid));
-        const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
+        uint4 ka[MK], kb[MK];
+#pragma unroll
+        for (int mk = 0; mk < MK; ++mk) {
+          const int kr = (sl * MK + mk) * 16 + key_of<D>(quad);
+          ka[mk] = *reinterpret_cast<const uint4*>(kt + at<D>(kr, 4 * sg + qid));
+          kb[mk] = *reinterpret_cast<const uint4*>(kt + at<D>(kr + 8, 4 * sg + qid));
+        }
         uint32_t qs[NT][8];
         if constexpr (!C::Q_REGS) {
 #pragma unroll
@@ -404,67 +419,98 @@ __global__ void __launch_bounds__(Cfg<D, NT, RG, KG>::THREADS, 1)
         }
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-          uint32_t a0, a1, a2, a3;
-          kv8::dec4(wa[w], a0, a2);
-          kv8::dec4(wb[w], a1, a3);
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            const uint32_t* q = C::Q_REGS ? qf[C::Q_REGS ? nt : 0][C::Q_REGS ? sg : 0] : qs[nt];
-            mma16816(s[nt], a0, a1, a2, a3, q[2 * w], q[2 * w + 1]);
+          for (int mk = 0; mk < MK; ++mk) {
+            uint32_t a0, a1, a2, a3;
+            kv8::dec4(w == 0 ? ka[mk].x : w == 1 ? ka[mk].y : w == 2 ? ka[mk].z : ka[mk].w, a0, a2);
+            kv8::dec4(w == 0 ? kb[mk].x : w == 1 ? kb[mk].y : w == 2 ? kb[mk].z : kb[mk].w, a1, a3);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              const uint32_t* q = C::Q_REGS ? qf[C::Q_REGS ? nt : 0][C::Q_REGS ? sg : 0] : qs[nt];
+              mma16816(s[mk][nt], a0, a1, a2, a3, q[2 * w], q[2 * w + 1]);
+            }
           }
         }
       }
       // the values' scale as a power of two: its logarithm (at least -100), what that leaves of it, its reciprocal
-      const float vs = sc2.y;
-      const float lv = fmaxf(log2f(vs), -100.f);
-      const float iv = ex2(-lv), rest = lv == -100.f ? vs * 0x1p100f : 1.f;
-      uint32_t pb[NT][2];
-      const int key0 = kbase + key_of<D>(quad), key1 = key0 + 8;
+      float ks[MK], lv[MK], iv[MK], rest[MK];
+#pragma unroll
+      for (int mk = 0; mk < MK; ++mk) {
+        const float2 sc = *reinterpret_cast<const float2*>(scl + (st * 4 + sl * MK + mk) * 2);
+        ks[mk] = sc.x;
+        lv[mk] = fmaxf(log2f(sc.y), -100.f);
+        iv[mk] = ex2(-lv[mk]);
+        rest[mk] = lv[mk] == -100.f ? sc.y * 0x1p100f : 1.f;
+      }
+      uint32_t pb[NT][MK][2];
+      float corr[NT][2];
+      bool moved = false;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float f = fac[nt][e] * sc2.x;
-          float x0 = key0 <= lim[nt][e] ? fmaf(s[nt][e], f, lv) : -INFINITY;
-          float x1 = key1 <= lim[nt][e] ? fmaf(s[nt][2 + e], f, lv) : -INFINITY;
-          float mx = fmaxf(x0, x1);
+          float mx = -INFINITY;
+#pragma unroll
+          for (int mk = 0; mk < MK; ++mk) {
+            const float f = fac[nt][e] * ks[mk];
+            const int key0 = kbase + 16 * mk + key_of<D>(quad);
+            s[mk][nt][e] = key0 <= lim[nt][e] ? fmaf(s[mk][nt][e], f, lv[mk]) : -INFINITY;
+            s[mk][nt][2 + e] = key0 + 8 <= lim[nt][e] ? fmaf(s[mk][nt][2 + e], f, lv[mk]) : -INFINITY;
+            mx = fmaxf(mx, fmaxf(s[mk][nt][e], s[mk][nt][2 + e]));
+          }
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-          const float mn = fmaxf(m_run[nt][e], mx);
-          const float mu = mn == -INFINITY ? 0.f : mn;
-          const float corr = ex2(m_run[nt][e] - mu);
+          const float mn = fmaxf(m_run[nt][e], mx), mu = mn == -INFINITY ? 0.f : mn;
+          moved = moved || mn > m_run[nt][e];
+          corr[nt][e] = ex2(m_run[nt][e] - mu);
           m_run[nt][e] = mn;
-          x0 = ex2(x0 - mu);
-          x1 = ex2(x1 - mu);
-          l_run[nt][e] = fmaf(x0 + x1, iv, l_run[nt][e] * corr);
-          s[nt][e] = x0 * rest;
-          s[nt][2 + e] = x1 * rest;
+          float l = 0.f;
+#pragma unroll
+          for (int mk = 0; mk < MK; ++mk) {
+            const float x0 = ex2(s[mk][nt][e] - mu), x1 = ex2(s[mk][nt][2 + e] - mu);
+            l = fmaf(x0 + x1, iv[mk], l);
+            s[mk][nt][e] = x0 * rest[mk];
+            s[mk][nt][2 + e] = x1 * rest[mk];
+          }
+          l_run[nt][e] = fmaf(l_run[nt][e], corr[nt][e], l);
+        }
+#pragma unroll
+        for (int mk = 0; mk < MK; ++mk) {
+          pb[nt][mk][0] = movm_t(pack2<__half>(s[mk][nt][0], s[mk][nt][1]));
+          pb[nt][mk][1] = movm_t(pack2<__half>(s[mk][nt][2], s[mk][nt][3]));
+        }
+      }
+      if (__any_sync(0xffffffffu, moved)) {  // (rare after a run's first tiles)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int j = 0; j < D / 16; ++j) {
-            acc[nt][j][e] *= corr;
-            acc[nt][j][2 + e] *= corr;
+            acc[nt][j][0] *= corr[nt][0];
+            acc[nt][j][1] *= corr[nt][1];
+            acc[nt][j][2] *= corr[nt][0];
+            acc[nt][j][3] *= corr[nt][1];
           }
-        }
-        pb[nt][0] = movm_t(pack2<__half>(s[nt][0], s[nt][1]));
-        pb[nt][1] = movm_t(pack2<__half>(s[nt][2], s[nt][3]));
       }
       const uint32_t vbase = smem_u32(vt);
 #pragma unroll
       for (int c = 0; c < D / 16; c += 2) {  // 32 dims: matrices (keys 0-7, 8-15) x (chunks c, c + 1)
-        uint32_t v[4];
-        const int r = wq * 16 + ((lane >> 3) & 1) * 8 + key_of<D>(lane & 7);
-        ldsm_x4_t(vbase + at<D>(r, c + (lane >> 4)), v);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t a0, a1, a2, a3;
-          kv8::dec4(__byte_perm(v[2 * h], 0, 0x3120), a0, a1);
-          kv8::dec4(__byte_perm(v[2 * h + 1], 0, 0x3120), a2, a3);
+        for (int mk = 0; mk < MK; ++mk) {
+          uint32_t v[4];
+          const int r = (sl * MK + mk) * 16 + ((lane >> 3) & 1) * 8 + key_of<D>(lane & 7);
+          ldsm_x4_t(vbase + at<D>(r, c + (lane >> 4)), v);
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma16816(acc[nt][c + h], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
+          for (int h = 0; h < 2; ++h) {
+            uint32_t a0, a1, a2, a3;
+            kv8::dec4(__byte_perm(v[2 * h], 0, 0x3120), a0, a1);
+            kv8::dec4(__byte_perm(v[2 * h + 1], 0, 0x3120), a2, a3);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma16816(acc[nt][c + h], a0, a1, a2, a3, pb[nt][mk][0], pb[nt][mk][1]);
+          }
         }
       }
-      if (nvalid < 16) fence_proxy_async_shared();  // the zeros precede the next copy into this stage
+      if (nvalid < 16 * MK) fence_proxy_async_shared();  // the zeros precede the next copy into this stage
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty[st]);
     }
@@ -490,9 +536,9 @@ __global__ void __launch_bounds__(Cfg<D, NT, RG, KG>::THREADS, 1)
       if (lane == 0) *abort_flag = 1;
       break;
     }
-    const int pi = kg * 4 + wq;
+    const int pi = kg * SL + sl;
 #pragma unroll
-    for (int half = 2 * KG; half > 0; half >>= 1) {
+    for (int half = SL * KG / 2; half > 0; half >>= 1) {
       if (pi >= half && pi < 2 * half) {
         float4* d = part + ((pi - half) * RG + rg) * C::PART_REGS * 32 + lane;
 #pragma unroll

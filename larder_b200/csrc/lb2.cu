@@ -1668,10 +1668,10 @@ static Plan plan(int B, int rows, int Hkv, int D, int page, int max_pages) {
   return pl;
 }
 
-template <typename T, int D, int NT, int RG, int KG>
+template <typename T, int D, int NT, int RG, int MK, int KG>
 static int launch_t(const CUtensorMap& map, const Params& p, cudaStream_t st) {
-  using C = Cfg<D, NT, RG, KG>;
-  auto kern = attend_kernel<T, D, NT, RG, KG>;
+  using C = Cfg<D, NT, RG, MK, KG>;
+  auto kern = attend_kernel<T, D, NT, RG, MK, KG>;
   static int attr_dev = -1;
   int dev = 0;
   LB2_CUDA(cudaGetDevice(&dev));
@@ -1699,9 +1699,9 @@ static int launch_t(const CUtensorMap& map, const Params& p, cudaStream_t st) {
 
 template <typename T, int D>
 static int launch_d(const CUtensorMap& map, const Params& p, cudaStream_t st) {
-  if (p.rpb <= 8) return launch_t<T, D, 1, 1, 2>(map, p, st);
-  if (p.rpb <= 16) return launch_t<T, D, 2, 1, 2>(map, p, st);
-  return launch_t<T, D, 2, 2, 1>(map, p, st);
+  if (p.rpb <= 8) return launch_t<T, D, 1, 1, 2, D == 256 ? 2 : 4>(map, p, st);
+  if (p.rpb <= 16) return launch_t<T, D, 2, 1, 2, D == 256 ? 2 : 4>(map, p, st);
+  return launch_t<T, D, 2, 2, 2, 2>(map, p, st);
 }
 
 template <typename T>

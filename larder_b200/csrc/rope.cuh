@@ -106,7 +106,7 @@ __device__ __forceinline__ void turn_pairs(float* f, const float2* z) {
 // apart, so that neighbouring lanes access neighbouring groups (V == 1, interleaved: the pair (2 u, 2 u + 1)).
 // A thread has one unit of K rows (token, head), all loaded before the block's angles are formed.
 template <typename T, int V, int K>
-__global__ void __launch_bounds__(THREADS) rope_kernel(const Params p) {
+__global__ void __launch_bounds__(THREADS, 3) rope_kernel(const Params p) {
   extern __shared__ __align__(16) float2 cs[];  // [tokens][R / 2]
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
