@@ -43,22 +43,28 @@ constexpr int STATUS = 112;  // where (lb2_status): 112 page id, 113.. waits
 
 // NT: 8-row tiles of query rows a warp; MK: 16-key blocks of a tile a warp (two give it two independent chains of
 // products); RG: row groups (sets of warps taking the same tile for other rows); KG: key groups (sets of warps taking
-// every KG-th tile).
+// every KG-th tile). At head dim 256 two warps share a warp's work (DS = 2), each with half the dims: O and the query's
+// fragments then fit the registers up to 24 rows, so that a key's conversion serves them all; the two add their halves of
+// the scores through shared memory.
 template <int D, int NT, int RG, int MK, int KG>
 struct Cfg {
+  static constexpr int DS = D == 256 ? 2 : 1;
+  static constexpr int DW = D / DS;             // dims a warp
   static constexpr int RP = 8 * NT * RG;  // rows of a block, padded
   static constexpr int SL = 4 / MK;       // key slices of a tile
-  static constexpr int WARPS = SL * RG * KG;
+  static constexpr int WARPS = DS * SL * RG * KG;
   static constexpr int NP = D == 256 ? 2 : 4;  // producer warps: they take the tiles in turn
   static constexpr int THREADS = (WARPS + NP) * 32;
   static constexpr int BW = D < 128 ? D : 128;  // bytes a box row
   static constexpr int TILE = BK * D;           // bytes of a K (or V) tile
   static constexpr int STAGE = 2 * TILE;
-  static constexpr bool Q_REGS = NT * D <= 256;
+  static constexpr bool Q_REGS = NT * DW <= 256;
   static constexpr int QBYTES = Q_REGS ? 0 : RG * NT * (D / 64) * 32 * 32;
-  static constexpr int PART_REGS = NT * (D / 16 + 1);           // float4 a lane: O and (m, l) of a warp's rows
+  static constexpr int PART_REGS = NT * (DW / 16 + 1);          // float4 a lane: O and (m, l) of a warp's rows
   static constexpr int PART = WARPS / 2 * PART_REGS * 32 * 16;  // half the warps' parts
-  static constexpr int FIXED = QBYTES + PART + (2 * MAX_B + 1) * 4 + 1024 + 1024;
+  static constexpr int XCH = DS > 1 ? 2 * WARPS * MK * NT * 32 * 16 : 0;  // two tiles' half scores of every warp
+  static constexpr int JOIN = PART > XCH ? PART : XCH;  // (one area: a barrier lies between the two uses)
+  static constexpr int FIXED = QBYTES + JOIN + (2 * MAX_B + 1) * 4 + 1024 + 1024;
   static constexpr int FIT = (232448 - FIXED) / (STAGE + 48);
   // A multiple of both, so that a stage only ever serves one producer warp and one key group, whose waits on it then
   // follow its phases in order (a wait two phases ahead would pass at once).
@@ -66,7 +72,7 @@ struct Cfg {
   static constexpr int STAGES = (FIT > 16 ? 16 : FIT) / STEP * STEP;
   static constexpr int Q_OFF = STAGES * STAGE;
   static constexpr int PART_OFF = Q_OFF + QBYTES;
-  static constexpr int SC_OFF = PART_OFF + PART;                 // [STAGES][4 slices][K, V] fp32
+  static constexpr int SC_OFF = PART_OFF + JOIN;                // [STAGES][4 slices][K, V] fp32
   static constexpr int PREFIX_OFF = SC_OFF + STAGES * 32;        // [MAX_B + 1]
   static constexpr int LENS_OFF = PREFIX_OFF + (MAX_B + 1) * 4;  // [MAX_B]
   static constexpr int BAR_OFF = (LENS_OFF + MAX_B * 4 + 15) / 16 * 16;
@@ -176,7 +182,7 @@ template <typename T, int D, int NT, int RG, int MK, int KG>
 __global__ void __launch_bounds__(Cfg<D, NT, RG, MK, KG>::THREADS, 1)
     attend_kernel(const __grid_constant__ CUtensorMap map, const Params p) {
   using C = Cfg<D, NT, RG, MK, KG>;
-  constexpr int STAGES = C::STAGES, WARPS = C::WARPS, SL = C::SL, SEG = D / 64;
+  constexpr int STAGES = C::STAGES, WARPS = C::WARPS, SL = C::SL, DS = C::DS, DW = C::DW, SEG = DW / 64;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   int* prefix = reinterpret_cast<int*>(sm + C::PREFIX_OFF);
@@ -190,7 +196,7 @@ __global__ void __launch_bounds__(Cfg<D, NT, RG, MK, KG>::THREADS, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < STAGES; ++i) {
       mbar_init(&full[i], 1);
-      mbar_init(&empty[i], SL * RG);
+      mbar_init(&empty[i], DS * SL * RG);
     }
     *abort_flag = 0;
     fence_barrier_init();
@@ -300,11 +306,13 @@ __global__ void __launch_bounds__(Cfg<D, NT, RG, MK, KG>::THREADS, 1)
 
   // ------------------------------------------------------------------ consumer warps
   const int quad = lane >> 2, qid = lane & 3;
-  const int sl = warp % SL, rg = (warp / SL) % RG, kg = warp / (SL * RG);
+  const int sl = warp % SL, rg = (warp / SL) % RG, kg = warp / (SL * RG) % KG, dh = warp / (SL * RG * KG);
   const int Tq = p.a.T;
   uint32_t qf[C::Q_REGS ? NT : 1][C::Q_REGS ? SEG : 1][8];  // this row's 16 dims of each 64-dim segment
   uint4* qsm = reinterpret_cast<uint4*>(sm + C::Q_OFF);     // [RG][NT][SEG][2][32 lanes]
-  int gt = 0;
+  float4* xch = reinterpret_cast<float4*>(sm + C::PART_OFF);  // [2 tiles][DS][WARPS / 2][MK NT][32 lanes]
+  const int pair = warp % (WARPS / 2);
+  int gt = 0, xpar = 0;
   bool ok = true;
   while (sched.next(it)) {
     const int hk = it.hb / p.nrb, rb = it.hb - hk * p.nrb;
@@ -315,25 +323,31 @@ __global__ void __launch_bounds__(Cfg<D, NT, RG, MK, KG>::THREADS, 1)
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int r = r0 + (rg * NT + nt) * 8 + quad;
-      float x[SEG][16], mx = 0.f;
+      float x[SEG][16], mx = 0.f;  // (the warp's dims; the largest value is the whole row's)
       const bool live = r < r1;
       const int g = live ? r / Tq : 0, t = live ? r - g * Tq : 0;
       const T* src = static_cast<const T*>(p.a.q) + it.b * p.a.q_st[0] + int64_t(hk * p.G + g) * p.a.q_st[1] +
                      t * p.a.q_st[2] + 16 * qid;
-#pragma unroll
-      for (int s = 0; s < SEG; ++s) {
+      auto load = [&](const T* from, float* y) {
         if (!live) {
 #pragma unroll
-          for (int e = 0; e < 16; ++e) x[s][e] = 0.f;
+          for (int e = 0; e < 16; ++e) y[e] = 0.f;
         } else if (p.wide_q) {
-          rope::ld_vec<T, 8>(src + 64 * s, x[s]);
-          rope::ld_vec<T, 8>(src + 64 * s + 8, x[s] + 8);
+          rope::ld_vec<T, 8>(from, y);
+          rope::ld_vec<T, 8>(from + 8, y + 8);
         } else {
 #pragma unroll
-          for (int e = 0; e < 16; ++e) x[s][e] = to_f<T>(src[64 * s + e]);
+          for (int e = 0; e < 16; ++e) y[e] = to_f<T>(from[e]);
         }
 #pragma unroll
-        for (int e = 0; e < 16; ++e) mx = fmaxf(mx, kv8::finite_abs(x[s][e]));
+        for (int e = 0; e < 16; ++e) mx = fmaxf(mx, kv8::finite_abs(y[e]));
+      };
+#pragma unroll
+      for (int s = 0; s < SEG; ++s) load(src + dh * DW + 64 * s, x[s]);
+      if constexpr (DS > 1) {
+        float y[16];
+#pragma unroll
+        for (int s = 0; s < SEG; ++s) load(src + (1 - dh) * DW + 64 * s, y);
       }
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
@@ -349,7 +363,7 @@ __global__ void __launch_bounds__(Cfg<D, NT, RG, MK, KG>::THREADS, 1)
 #pragma unroll
           for (int e = 0; e < 8; ++e) qf[nt][s][e] = w[e];
         } else if (sl == 0 && kg == 0) {
-          uint4* d = qsm + ((rg * NT + nt) * SEG + s) * 64 + lane;
+          uint4* d = qsm + ((rg * NT + nt) * (DS * SEG) + dh * SEG + s) * 64 + lane;
           d[0] = make_uint4(w[0], w[1], w[2], w[3]);
           d[32] = make_uint4(w[4], w[5], w[6], w[7]);
         }
@@ -366,29 +380,31 @@ __global__ void __launch_bounds__(Cfg<D, NT, RG, MK, KG>::THREADS, 1)
     }
     if constexpr (!C::Q_REGS) asm volatile("bar.sync 1, %0;" ::"n"(WARPS * 32) : "memory");
 
-    float m_run[NT][2], l_run[NT][2], acc[NT][D / 16][4];
+    float m_run[NT][2], l_run[NT][2], acc[NT][DW / 16][4];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       m_run[nt][0] = m_run[nt][1] = -INFINITY;
       l_run[nt][0] = l_run[nt][1] = 0.f;
 #pragma unroll
-      for (int j = 0; j < D / 16; ++j) acc[nt][j][0] = acc[nt][j][1] = acc[nt][j][2] = acc[nt][j][3] = 0.f;
+      for (int j = 0; j < DW / 16; ++j) acc[nt][j][0] = acc[nt][j][1] = acc[nt][j][2] = acc[nt][j][3] = 0.f;
     }
     for (int i = it.i0; i < it.i1; ++i, ++gt) {
       if (KG > 1 && gt % KG != kg) continue;
       const int st = gt % STAGES;
       if (!ok || *abort_flag || !mbar_wait(&full[st], (gt / STAGES) & 1, STATUS + 3)) {
         ok = false;
-        gt += it.i1 - i;
-        break;
+        if constexpr (DS == 1) {
+          gt += it.i1 - i;
+          break;
+        }  // (DS > 1: the pair leaves together, below)
       }
       uint8_t* kt = sm + st * C::STAGE;
       uint8_t* vt = kt + C::TILE;
       const int kbase = i * BK + sl * 16 * MK;  // the warp's first key
       const int nvalid = min(16 * MK, max(0, it.len - kbase));
       if (nvalid < 16 * MK) {  // values past the length: zeros, so that P = 0 meets no NaN code
-        for (int e = lane; e < (16 * MK - nvalid) * (D / 16); e += 32) {
-          const int r = sl * 16 * MK + nvalid + e / (D / 16), c = e % (D / 16);
+        for (int e = lane; e < (16 * MK - nvalid) * (DW / 16); e += 32) {
+          const int r = sl * 16 * MK + nvalid + e / (DW / 16), c = dh * (DW / 16) + e % (DW / 16);
           *reinterpret_cast<uint4*>(vt + at<D>(r, c)) = make_uint4(0, 0, 0, 0);
         }
         __syncwarp();
@@ -404,14 +420,14 @@ __global__ void __launch_bounds__(Cfg<D, NT, RG, MK, KG>::THREADS, 1)
 #pragma unroll
         for (int mk = 0; mk < MK; ++mk) {
           const int kr = (sl * MK + mk) * 16 + key_of<D>(quad);
-          ka[mk] = *reinterpret_cast<const uint4*>(kt + at<D>(kr, 4 * sg + qid));
-          kb[mk] = *reinterpret_cast<const uint4*>(kt + at<D>(kr + 8, 4 * sg + qid));
+          ka[mk] = *reinterpret_cast<const uint4*>(kt + at<D>(kr, dh * (DW / 16) + 4 * sg + qid));
+          kb[mk] = *reinterpret_cast<const uint4*>(kt + at<D>(kr + 8, dh * (DW / 16) + 4 * sg + qid));
         }
         uint32_t qs[NT][8];
         if constexpr (!C::Q_REGS) {
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            const uint4* d = qsm + ((rg * NT + nt) * SEG + sg) * 64 + lane;
+            const uint4* d = qsm + ((rg * NT + nt) * (DS * SEG) + dh * SEG + sg) * 64 + lane;
             const uint4 u = d[0], v = d[32];
             qs[nt][0] = u.x, qs[nt][1] = u.y, qs[nt][2] = u.z, qs[nt][3] = u.w;
             qs[nt][4] = v.x, qs[nt][5] = v.y, qs[nt][6] = v.z, qs[nt][7] = v.w;
@@ -431,6 +447,34 @@ __global__ void __launch_bounds__(Cfg<D, NT, RG, MK, KG>::THREADS, 1)
             }
           }
         }
+      }
+      if constexpr (DS > 1) {  // the pair's halves of the scores (buffers alternate, so one barrier a tile is enough)
+        constexpr int XW = MK * NT * 32;  // float4 a warp
+        float4* mine = xch + ((xpar * 2 + dh) * (C::WARPS / 2) + pair) * XW + lane;
+        const float4* other = xch + ((xpar * 2 + 1 - dh) * (C::WARPS / 2) + pair) * XW + lane;
+        xpar ^= 1;
+#pragma unroll
+        for (int mk = 0; mk < MK; ++mk)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+            mine[(mk * NT + nt) * 32] = make_float4(s[mk][nt][0], s[mk][nt][1], s[mk][nt][2], s[mk][nt][3]);
+        uint32_t both;  // the waits of both held: else both leave
+        asm volatile(
+            "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.and.pred q, %2, 64, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+            : "=r"(both)
+            : "r"(uint32_t(ok)), "r"(2 + pair)
+            : "memory");
+        if (!both) {
+          ok = false;
+          break;
+        }
+#pragma unroll
+        for (int mk = 0; mk < MK; ++mk)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            const float4 o = other[(mk * NT + nt) * 32];
+            s[mk][nt][0] += o.x, s[mk][nt][1] += o.y, s[mk][nt][2] += o.z, s[mk][nt][3] += o.w;
+          }
       }
       // the values' scale as a power of two: its logarithm (at least -100), what that leaves of it, its reciprocal
       float ks[MK], lv[MK], iv[MK], rest[MK];
@@ -485,7 +529,7 @@ __global__ void __launch_bounds__(Cfg<D, NT, RG, MK, KG>::THREADS, 1)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int j = 0; j < D / 16; ++j) {
+          for (int j = 0; j < DW / 16; ++j) {
             acc[nt][j][0] *= corr[nt][0];
             acc[nt][j][1] *= corr[nt][1];
             acc[nt][j][2] *= corr[nt][0];
@@ -494,12 +538,12 @@ __global__ void __launch_bounds__(Cfg<D, NT, RG, MK, KG>::THREADS, 1)
       }
       const uint32_t vbase = smem_u32(vt);
 #pragma unroll
-      for (int c = 0; c < D / 16; c += 2) {  // 32 dims: matrices (keys 0-7, 8-15) x (chunks c, c + 1)
+      for (int c = 0; c < DW / 16; c += 2) {  // 32 dims: matrices (keys 0-7, 8-15) x (chunks c, c + 1)
 #pragma unroll
         for (int mk = 0; mk < MK; ++mk) {
           uint32_t v[4];
           const int r = (sl * MK + mk) * 16 + ((lane >> 3) & 1) * 8 + key_of<D>(lane & 7);
-          ldsm_x4_t(vbase + at<D>(r, c + (lane >> 4)), v);
+          ldsm_x4_t(vbase + at<D>(r, dh * (DW / 16) + c + (lane >> 4)), v);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             uint32_t a0, a1, a2, a3;
@@ -540,18 +584,18 @@ __global__ void __launch_bounds__(Cfg<D, NT, RG, MK, KG>::THREADS, 1)
 #pragma unroll
     for (int half = SL * KG / 2; half > 0; half >>= 1) {
       if (pi >= half && pi < 2 * half) {
-        float4* d = part + ((pi - half) * RG + rg) * C::PART_REGS * 32 + lane;
+        float4* d = part + (((pi - half) * RG + rg) * DS + dh) * C::PART_REGS * 32 + lane;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           *d = make_float4(m_run[nt][0], m_run[nt][1], l_run[nt][0], l_run[nt][1]);
           d += 32;
 #pragma unroll
-          for (int j = 0; j < D / 16; ++j, d += 32) *d = make_float4(acc[nt][j][0], acc[nt][j][1], acc[nt][j][2], acc[nt][j][3]);
+          for (int j = 0; j < DW / 16; ++j, d += 32) *d = make_float4(acc[nt][j][0], acc[nt][j][1], acc[nt][j][2], acc[nt][j][3]);
         }
       }
       asm volatile("bar.sync 1, %0;" ::"n"(WARPS * 32) : "memory");
       if (pi < half) {
-        const float4* d = part + (pi * RG + rg) * C::PART_REGS * 32 + lane;
+        const float4* d = part + ((pi * RG + rg) * DS + dh) * C::PART_REGS * 32 + lane;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           const float4 x = *d;
@@ -567,7 +611,7 @@ __global__ void __launch_bounds__(Cfg<D, NT, RG, MK, KG>::THREADS, 1)
             l_run[nt][e] = l_run[nt][e] * f[e] + xl[e] * g[e];
           }
 #pragma unroll
-          for (int j = 0; j < D / 16; ++j, d += 32) {
+          for (int j = 0; j < DW / 16; ++j, d += 32) {
             const float4 o = *d;
             acc[nt][j][0] = acc[nt][j][0] * f[0] + o.x * g[0];
             acc[nt][j][1] = acc[nt][j][1] * f[1] + o.y * g[1];
@@ -576,7 +620,7 @@ __global__ void __launch_bounds__(Cfg<D, NT, RG, MK, KG>::THREADS, 1)
           }
         }
       }
-      if (half > 1) asm volatile("bar.sync 1, %0;" ::"n"(WARPS * 32) : "memory");
+      if (half > 1 || DS > 1) asm volatile("bar.sync 1, %0;" ::"n"(WARPS * 32) : "memory");
     }
     if (pi == 0) {
 #pragma unroll
@@ -586,17 +630,17 @@ __global__ void __launch_bounds__(Cfg<D, NT, RG, MK, KG>::THREADS, 1)
           const int r = (rg * NT + nt) * 8 + 2 * qid + e;
           if (r >= r1 - r0) continue;
           const size_t out = size_t(it.slot) * p.rpb + r;
-          if (quad == 0) *reinterpret_cast<float2*>(p.ws_ml + 2 * out) = make_float2(m_run[nt][e], l_run[nt][e]);
+          if (quad == 0 && dh == 0) *reinterpret_cast<float2*>(p.ws_ml + 2 * out) = make_float2(m_run[nt][e], l_run[nt][e]);
 #pragma unroll
-          for (int j = 0; j < D / 16; ++j)
-            *reinterpret_cast<float2*>(p.ws_o + out * D + 16 * j + 2 * quad) =
+          for (int j = 0; j < DW / 16; ++j)
+            *reinterpret_cast<float2*>(p.ws_o + out * D + dh * DW + 16 * j + 2 * quad) =
                 make_float2(acc[nt][j][e], acc[nt][j][2 + e]);
         }
     }
   }
 }
 
-// Merges the partials of each (b, KV head, row block): a block each, a warp a row. The pair's partials sit in consecutive
+// Merges the partials of each (b, KV head, row block): a block for eight rows of each, a warp a row. The pair's partials sit in consecutive
 // slots, found from its first and last tile.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) combine_kernel(const Params p) {
@@ -631,7 +675,7 @@ __global__ void __launch_bounds__(256) combine_kernel(const Params p) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int hk = hb / p.nrb, r0 = (hb - hk * p.nrb) * p.rpb, nrows = min(p.rows - r0, p.rpb);
-  for (int r = w; r < nrows; r += 8) {
+  for (int r = blockIdx.y * 8 + w; r < nrows; r += 8 * gridDim.y) {
     float x[E], M = -INFINITY, L = 0.f;
 #pragma unroll
     for (int e = 0; e < E; ++e) x[e] = 0.f;

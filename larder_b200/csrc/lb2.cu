@@ -1643,8 +1643,7 @@ static int paged_rows(const arows::PagedParams& p, int D, cudaStream_t st) {
 namespace lb2 {
 namespace kv8attn {
 
-// Rows a block and the kernel's shape: up to 8 and 16 rows by one set of four warps a tile and two sets on alternate
-// tiles, up to 32 by two sets sharing each tile; more rows take further passes over the codes (from L2 as far as it holds
+// Rows a block: up to 32 (24 at head dim 256); more rows take further passes over the codes (from L2 as far as it holds
 // them).
 struct Plan {
   int nrb, rpb, grid;
@@ -1656,7 +1655,8 @@ static Plan plan(int B, int rows, int Hkv, int D, int page, int max_pages) {
   Plan pl{};
   int dev = 0;
   cudaGetDevice(&dev);
-  pl.nrb = (rows + 31) / 32;
+  const int most = D == 256 ? 24 : 32;
+  pl.nrb = (rows + most - 1) / most;
   pl.rpb = ((rows + pl.nrb - 1) / pl.nrb + 7) / 8 * 8;
   const int nb = std::min(B, MAX_B);
   const int64_t H = int64_t(Hkv) * pl.nrb, tiles = int64_t(nb) * H * ((int64_t(max_pages) * page + BK - 1) / BK);
@@ -1690,7 +1690,7 @@ static int launch_t(const CUtensorMap& map, const Params& p, cudaStream_t st) {
   cfg.attrs = pdl;
   cfg.numAttrs = 1;
   LB2_CUDA(cudaLaunchKernelEx(&cfg, kern, map, p));
-  cfg.gridDim = dim3(unsigned(p.a.B * p.a.Hkv * p.nrb));
+  cfg.gridDim = dim3(unsigned(p.a.B * p.a.Hkv * p.nrb), unsigned((p.rpb + 7) / 8));
   cfg.blockDim = dim3(256);
   cfg.dynamicSmemBytes = 0;
   LB2_CUDA(cudaLaunchKernelEx(&cfg, combine_kernel<T, D>, p));
@@ -1699,9 +1699,11 @@ static int launch_t(const CUtensorMap& map, const Params& p, cudaStream_t st) {
 
 template <typename T, int D>
 static int launch_d(const CUtensorMap& map, const Params& p, cudaStream_t st) {
-  if (p.rpb <= 8) return launch_t<T, D, 1, 1, 2, D == 256 ? 2 : 4>(map, p, st);
-  if (p.rpb <= 16) return launch_t<T, D, 2, 1, 2, D == 256 ? 2 : 4>(map, p, st);
-  return launch_t<T, D, 2, 2, 2, 2>(map, p, st);
+  constexpr int KG = D == 256 ? 2 : 4;
+  if (p.rpb <= 8) return launch_t<T, D, 1, 1, 2, KG>(map, p, st);
+  if (p.rpb <= 16) return launch_t<T, D, 2, 1, 2, KG>(map, p, st);
+  if constexpr (D == 256) return launch_t<T, D, 3, 1, 1, 1>(map, p, st);
+  else return launch_t<T, D, 2, 2, 2, 2>(map, p, st);
 }
 
 template <typename T>
