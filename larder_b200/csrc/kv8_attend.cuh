@@ -53,7 +53,7 @@ struct Cfg {
   static constexpr int RP = 8 * NT * RG;  // rows of a block, padded
   static constexpr int SL = 4 / MK;       // key slices of a tile
   static constexpr int WARPS = DS * SL * RG * KG;
-  static constexpr int NP = D == 256 ? 2 : 4;  // producer warps: they take the tiles in turn
+  static constexpr int NP = 4;            // producer warps: they take the tiles in turn
   static constexpr int THREADS = (WARPS + NP) * 32;
   static constexpr int BW = D < 128 ? D : 128;  // bytes a box row
   static constexpr int TILE = BK * D;           // bytes of a K (or V) tile
@@ -96,6 +96,12 @@ struct Params {
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ float lg2(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 
@@ -310,55 +316,66 @@ __global__ void __launch_bounds__(Cfg<D, NT, RG, MK, KG>::THREADS, 1)
   const int Tq = p.a.T;
   uint32_t qf[C::Q_REGS ? NT : 1][C::Q_REGS ? SEG : 1][8];  // this row's 16 dims of each 64-dim segment
   uint4* qsm = reinterpret_cast<uint4*>(sm + C::Q_OFF);     // [RG][NT][SEG][2][32 lanes]
+  rope::Raw<T, 8> raw[NT][DS * SEG][2];  // the query rows' dims as they lie, the warp's own first
+  auto load_q = [&](const Item& w) {
+    const int hk = w.hb / p.nrb, r0 = (w.hb - hk * p.nrb) * p.rpb, r1 = min(p.rows, r0 + p.rpb);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int r = r0 + (rg * NT + nt) * 8 + quad;
+      const int g = Tq == 1 ? r : r / Tq, t = r - g * Tq;
+      const T* src = static_cast<const T*>(p.a.q) + w.b * p.a.q_st[0] + int64_t(hk * p.G + g) * p.a.q_st[1] +
+                     t * p.a.q_st[2] + 16 * qid;
+#pragma unroll
+      for (int s = 0; s < DS * SEG; ++s) {
+        const T* from = src + (s < SEG ? dh : 1 - dh) * DW + 64 * (s % SEG);
+        if (r >= r1) {
+          raw[nt][s][0].u = raw[nt][s][1].u = make_uint4(0, 0, 0, 0);
+        } else if (p.wide_q) {
+          raw[nt][s][0].load(from);
+          raw[nt][s][1].load(from + 8);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) reinterpret_cast<T*>(&raw[nt][s][e >> 3].u)[e & 7] = from[e];
+        }
+      }
+    }
+  };
+  constexpr bool AHEAD = NT * D <= 256;  // the next item's rows are loaded while this one's parts are merged
+  bool have_q = false;
   float4* xch = reinterpret_cast<float4*>(sm + C::PART_OFF);  // [2 tiles][DS][WARPS / 2][MK NT][32 lanes]
   const int pair = warp % (WARPS / 2);
   int gt = 0, xpar = 0;
   bool ok = true;
   while (sched.next(it)) {
-    const int hk = it.hb / p.nrb, rb = it.hb - hk * p.nrb;
-    const int r0 = rb * p.rpb, r1 = min(p.rows, r0 + p.rpb);  // the block's rows
+    const int hk = it.hb / p.nrb, r0 = (it.hb - hk * p.nrb) * p.rpb, r1 = min(p.rows, r0 + p.rpb);  // the block's rows
     // Query fragments: lane (quad, qid) holds dims 64 s + 16 qid .. + 15 of row quad of each row tile.
+    if (!have_q) load_q(it);
     float fac[NT][2];
     int lim[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int r = r0 + (rg * NT + nt) * 8 + quad;
-      float x[SEG][16], mx = 0.f;  // (the warp's dims; the largest value is the whole row's)
-      const bool live = r < r1;
-      const int g = live ? r / Tq : 0, t = live ? r - g * Tq : 0;
-      const T* src = static_cast<const T*>(p.a.q) + it.b * p.a.q_st[0] + int64_t(hk * p.G + g) * p.a.q_st[1] +
-                     t * p.a.q_st[2] + 16 * qid;
-      auto load = [&](const T* from, float* y) {
-        if (!live) {
+      float mx = 0.f;  // the row's largest value: of all its dims
 #pragma unroll
-          for (int e = 0; e < 16; ++e) y[e] = 0.f;
-        } else if (p.wide_q) {
-          rope::ld_vec<T, 8>(from, y);
-          rope::ld_vec<T, 8>(from + 8, y + 8);
-        } else {
+      for (int s = 0; s < DS * SEG; ++s) {
+        float x[16];
+        raw[nt][s][0].get(x);
+        raw[nt][s][1].get(x + 8);
 #pragma unroll
-          for (int e = 0; e < 16; ++e) y[e] = to_f<T>(from[e]);
-        }
-#pragma unroll
-        for (int e = 0; e < 16; ++e) mx = fmaxf(mx, kv8::finite_abs(y[e]));
-      };
-#pragma unroll
-      for (int s = 0; s < SEG; ++s) load(src + dh * DW + 64 * s, x[s]);
-      if constexpr (DS > 1) {
-        float y[16];
-#pragma unroll
-        for (int s = 0; s < SEG; ++s) load(src + (1 - dh) * DW + 64 * s, y);
+        for (int e = 0; e < 16; ++e) mx = fmaxf(mx, kv8::finite_abs(x[e]));
       }
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-      // multiply by 2^(14 - floor(log2 mx)), in two factors where that leaves fp32's range of exponents
+      // multiply by 2^(14 - floor(log2 mx))
       const int ex = mx > 0.f ? min(max(int(__float_as_uint(mx) >> 23) - 127, -112), 127) : 14;
       const float up = __uint_as_float(uint32_t(127 + 14 - ex) << 23);  // 14 - ex in [-113, 126]
 #pragma unroll
-      for (int s = 0; s < SEG; ++s) {
+      for (int s = 0; s < SEG; ++s) {  // (raw holds the warp's own dims first)
+        float x[16];
+        raw[nt][s][0].get(x);
+        raw[nt][s][1].get(x + 8);
         uint32_t w[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) w[e] = pack2<__half>(x[s][2 * e] * up, x[s][2 * e + 1] * up);
+        for (int e = 0; e < 8; ++e) w[e] = pack2<__half>(x[2 * e] * up, x[2 * e + 1] * up);
         if constexpr (C::Q_REGS) {
 #pragma unroll
           for (int e = 0; e < 8; ++e) qf[nt][s][e] = w[e];
@@ -374,10 +391,12 @@ __global__ void __launch_bounds__(Cfg<D, NT, RG, MK, KG>::THREADS, 1)
         // scale 2^(ex - 14), the two powers apart so that neither leaves fp32's range
         fac[nt][e] = p.scale_log2 * __uint_as_float(uint32_t(127 + (exr - 14) / 2) << 23) *
                      __uint_as_float(uint32_t(127 + (exr - 14) - (exr - 14) / 2) << 23);
+        // the row's last key (rows past the block's are zeros that see what the others see; nothing of them is kept)
         const int rr = r0 + (rg * NT + nt) * 8 + 2 * qid + e;
-        lim[nt][e] = rr >= r1 ? -1 : p.a.causal ? it.len - Tq + rr % Tq : it.len - 1;
+        lim[nt][e] = p.a.causal && Tq > 1 ? it.len - Tq + rr % Tq : it.len - 1;
       }
     }
+    const int all_see = p.a.causal ? it.len - Tq : it.len - 1;  // the last key that every row sees
     if constexpr (!C::Q_REGS) asm volatile("bar.sync 1, %0;" ::"n"(WARPS * 32) : "memory");
 
     float m_run[NT][2], l_run[NT][2], acc[NT][DW / 16][4];
@@ -482,59 +501,60 @@ __global__ void __launch_bounds__(Cfg<D, NT, RG, MK, KG>::THREADS, 1)
       for (int mk = 0; mk < MK; ++mk) {
         const float2 sc = *reinterpret_cast<const float2*>(scl + (st * 4 + sl * MK + mk) * 2);
         ks[mk] = sc.x;
-        lv[mk] = fmaxf(log2f(sc.y), -100.f);
+        lv[mk] = fmaxf(lg2(sc.y), -100.f);
         iv[mk] = ex2(-lv[mk]);
         rest[mk] = lv[mk] == -100.f ? sc.y * 0x1p100f : 1.f;
       }
-      uint32_t pb[NT][MK][2];
-      float corr[NT][2];
-      bool moved = false;
+      // Scores in base 2 with the values' scale. The maximum a row is taken against moves only when one of its scores
+      // passes it by more than 8: weights up to 2^8 lose nothing in f16, and most tiles need no exchange between lanes.
+      bool over = false;
+      const bool whole = kbase + 16 * MK - 1 <= all_see;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float mx = -INFINITY;
-#pragma unroll
-          for (int mk = 0; mk < MK; ++mk) {
-            const float f = fac[nt][e] * ks[mk];
-            const int key0 = kbase + 16 * mk + key_of<D>(quad);
-            s[mk][nt][e] = key0 <= lim[nt][e] ? fmaf(s[mk][nt][e], f, lv[mk]) : -INFINITY;
-            s[mk][nt][2 + e] = key0 + 8 <= lim[nt][e] ? fmaf(s[mk][nt][2 + e], f, lv[mk]) : -INFINITY;
-            mx = fmaxf(mx, fmaxf(s[mk][nt][e], s[mk][nt][2 + e]));
-          }
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-          const float mn = fmaxf(m_run[nt][e], mx), mu = mn == -INFINITY ? 0.f : mn;
-          moved = moved || mn > m_run[nt][e];
-          corr[nt][e] = ex2(m_run[nt][e] - mu);
-          m_run[nt][e] = mn;
-          float l = 0.f;
-#pragma unroll
-          for (int mk = 0; mk < MK; ++mk) {
-            const float x0 = ex2(s[mk][nt][e] - mu), x1 = ex2(s[mk][nt][2 + e] - mu);
-            l = fmaf(x0 + x1, iv[mk], l);
-            s[mk][nt][e] = x0 * rest[mk];
-            s[mk][nt][2 + e] = x1 * rest[mk];
-          }
-          l_run[nt][e] = fmaf(l_run[nt][e], corr[nt][e], l);
-        }
-#pragma unroll
-        for (int mk = 0; mk < MK; ++mk) {
-          pb[nt][mk][0] = movm_t(pack2<__half>(s[mk][nt][0], s[mk][nt][1]));
-          pb[nt][mk][1] = movm_t(pack2<__half>(s[mk][nt][2], s[mk][nt][3]));
-        }
-      }
-      if (__any_sync(0xffffffffu, moved)) {  // (rare after a run's first tiles)
+      for (int mk = 0; mk < MK; ++mk)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int j = 0; j < DW / 16; ++j) {
-            acc[nt][j][0] *= corr[nt][0];
-            acc[nt][j][1] *= corr[nt][1];
-            acc[nt][j][2] *= corr[nt][0];
-            acc[nt][j][3] *= corr[nt][1];
+          for (int e = 0; e < 4; ++e) {
+            float x = fmaf(s[mk][nt][e], fac[nt][e & 1] * ks[mk], lv[mk]);
+            if (!whole && kbase + 16 * mk + key_of<D>(quad) + 8 * (e >> 1) > lim[nt][e & 1]) x = -INFINITY;
+            over = over || x > m_run[nt][e & 1] + 8.f;
+            s[mk][nt][e] = x;
           }
+      if (__any_sync(0xffffffffu, over)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float mx = m_run[nt][e];
+#pragma unroll
+            for (int mk = 0; mk < MK; ++mk) mx = fmaxf(mx, fmaxf(s[mk][nt][e], s[mk][nt][2 + e]));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+            const float corr = ex2(m_run[nt][e] - (mx == -INFINITY ? 0.f : mx));
+            m_run[nt][e] = mx;
+            l_run[nt][e] *= corr;
+#pragma unroll
+            for (int j = 0; j < DW / 16; ++j) {
+              acc[nt][j][e] *= corr;
+              acc[nt][j][2 + e] *= corr;
+            }
+          }
+      }
+      uint32_t pb[NT][MK][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const float mu[2] = {m_run[nt][0] == -INFINITY ? 0.f : m_run[nt][0], m_run[nt][1] == -INFINITY ? 0.f : m_run[nt][1]};
+#pragma unroll
+        for (int mk = 0; mk < MK; ++mk) {
+          float x[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[e] = ex2(s[mk][nt][e] - mu[e & 1]);
+          l_run[nt][0] = fmaf(x[0] + x[2], iv[mk], l_run[nt][0]);
+          l_run[nt][1] = fmaf(x[1] + x[3], iv[mk], l_run[nt][1]);
+          pb[nt][mk][0] = movm_t(pack2<__half>(x[0] * rest[mk], x[1] * rest[mk]));
+          pb[nt][mk][1] = movm_t(pack2<__half>(x[2] * rest[mk], x[3] * rest[mk]));
+        }
       }
       const uint32_t vbase = smem_u32(vt);
 #pragma unroll
@@ -562,6 +582,10 @@ __global__ void __launch_bounds__(Cfg<D, NT, RG, MK, KG>::THREADS, 1)
     // ------------------------------------------------------------------ the item's partial
     // The parts of a row (one a key slice and key group) meet in a tree through shared memory, each warp's registers as
     // they lie (a lane's counterpart is the same lane); the warps of part 0 write the merged partial.
+    Sched ahead = sched;
+    Item nx;
+    have_q = AHEAD && ahead.next(nx);
+    if (have_q) load_q(nx);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll

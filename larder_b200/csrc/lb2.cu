@@ -1660,7 +1660,7 @@ static Plan plan(int B, int rows, int Hkv, int D, int page, int max_pages) {
   pl.rpb = ((rows + pl.nrb - 1) / pl.nrb + 7) / 8 * 8;
   const int nb = std::min(B, MAX_B);
   const int64_t H = int64_t(Hkv) * pl.nrb, tiles = int64_t(nb) * H * ((int64_t(max_pages) * page + BK - 1) / BK);
-  pl.grid = int(std::max<int64_t>(1, std::min<int64_t>(sm_count(dev), tiles / 2)));
+  pl.grid = int(std::max<int64_t>(1, std::min<int64_t>(sm_count(dev), tiles)));
   pl.slots = pl.grid + nb * H;
   pl.ml = 0;
   pl.o = align_up(size_t(pl.slots) * pl.rpb * 2 * sizeof(float), 256);
