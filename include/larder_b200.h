@@ -393,10 +393,10 @@ int lb2_kv8_attend(const void* q, const int64_t* q_st, const uint8_t* pages, con
  * [S + 1] on the device, rising from 0 to T; empty prompts allowed), and row i of a prompt sees its rows 0 .. i.
  *   q, o [Hq, T, D], k, v [Hkv, T, D]: strides [0..1] for H, T; unit on D; dtype LB2_BF16 / F16 (row strides multiples
  *   of 8 elements, 16-byte aligned bases) or LB2_F32 (exact CUDA-core kernel); D in {64, 128, 256}.
- *   workspace: lb2_attn_packed_workspace_size(S, T) bytes, 256-byte aligned, any contents.
+ *   workspace: lb2_attn_packed_workspace_size() bytes, 256-byte aligned, any contents.
  * Rows of no prompt (cu[S] < T) give zeros. No value of one prompt reaches another's rows, infinities and NaN among
  * them, nor a later row's an earlier row. */
-size_t lb2_attn_packed_workspace_size(int S, int T);
+size_t lb2_attn_packed_workspace_size(int S, int Hq, int Hkv, int T, int D);
 int lb2_attn_packed(const void* q, const int64_t* q_st, const void* k, const int64_t* k_st, const void* v,
                     const int64_t* v_st, void* o, const int64_t* o_st, const int32_t* cu, int S, int Hq, int Hkv, int T,
                     int D, int dtype, float scale, void* workspace, size_t workspace_bytes, void* stream);

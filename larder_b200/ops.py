@@ -651,11 +651,13 @@ def attn_packed(q, k, v, scale, cu, out=None):
         raise ValueError("attn_packed: cu must be int32 [S + 1], S >= 1")
     S = cu.numel() - 1
     _int32(cu, (S + 1,), dev, "attn_packed: cu")
+    if Hkv == 0 or Hq % Hkv:
+        raise ValueError("attn_packed: Hq must be a multiple of Hkv")
     if out is None:
         out = torch.empty((1, Hq, T, D), dtype=q.dtype, device=dev)
     elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or out.stride(-1) != 1:
         raise ValueError("attn_packed: out must match q")
-    ws = _stream_workspace(q, lib().lb2_attn_packed_workspace_size(S, T), "attn_packed")
+    ws = _stream_workspace(q, lib().lb2_attn_packed_workspace_size(S, Hq, Hkv, T, D), "attn_packed")
     rc = lib().lb2_attn_packed(q.data_ptr(), i64(*q.stride()[1:3]), k.data_ptr(), i64(*k.stride()[1:3]), v.data_ptr(),
                                i64(*v.stride()[1:3]), out.data_ptr(), i64(*out.stride()[1:3]), cu.data_ptr(), S, Hq,
                                Hkv, T, D, dtype_code(q), scale, ws.data_ptr(), ws.numel(), _stream(q))
