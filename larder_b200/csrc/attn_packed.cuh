@@ -1,6 +1,6 @@
-// Packed prompts: the list of row blocks that the prefill kernels' PK forms take (attn_prefill.cuh, attn_prefill2.cuh).
+// Packed prompts: the list of row blocks that the kernels take (attn_short.cuh, attn_prefill2.cuh's PK form).
 //
-// Prompt s is rows [cu[s], cu[s + 1]) of one row axis; its blocks of RB rows (RB = 256 on CTA pairs, 128 on one CTA) read
+// Prompt s is rows [cu[s], cu[s + 1]) of one row axis; its blocks of RB rows (256 on CTA pairs, 128 over the folded heads on one CTA) read
 // its key tiles from the first up to the block's last row. The lengths are known on the device only, so the list is made
 // there, by one block of threads: blocks in falling order of their index m in their prompt (the work of block m grows with
 // m, so this is heaviest first but for prompts' last, partial blocks), prompts in order within an m. Each warp takes the
@@ -26,7 +26,11 @@ struct PlanParams {
 };
 
 __global__ void __launch_bounds__(THREADS) plan_kernel(const PlanParams p) {
-  __shared__ int s_w[32], s_max;
+  constexpr int HELD = 2048;  // bounds and counts up to so many stay in shared memory
+  __shared__ int s_w[32], s_max, s_at[HELD], s_cnt[HELD];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // (the attention kernel waits for this one's end)
+  int* const at = p.S + 2 <= HELD ? s_at : p.at;
+  int* const cnt = p.T / p.rb + 2 <= HELD ? s_cnt : p.cnt;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (tid == 0) s_max = 0;
   __syncthreads();
@@ -47,14 +51,14 @@ __global__ void __launch_bounds__(THREADS) plan_kernel(const PlanParams p) {
       if (w < warp) pre = max(pre, s_w[w]);
       all = max(all, s_w[w]);
     }
-    if (s <= p.S) p.at[s] = max(x, pre);
+    if (s <= p.S) at[s] = max(x, pre);
     carry = all;
     __syncthreads();
   }
-  if (tid == 0) p.at[p.S + 1] = p.T;
+  if (tid == 0) at[p.S + 1] = p.T;
   __syncthreads();
   int mx = 0;
-  for (int s = tid; s <= p.S; s += THREADS) mx = max(mx, (p.at[s + 1] - p.at[s] + p.rb - 1) / p.rb);
+  for (int s = tid; s <= p.S; s += THREADS) mx = max(mx, (at[s + 1] - at[s] + p.rb - 1) / p.rb);
   atomicMax(&s_max, mx);
   __syncthreads();
   const int M = s_max;  // m runs over 0 .. M - 1
@@ -62,16 +66,16 @@ __global__ void __launch_bounds__(THREADS) plan_kernel(const PlanParams p) {
     int c = 0;
     for (int s0 = 0; s0 <= p.S; s0 += 32) {
       const int s = s0 + lane;
-      c += __popc(__ballot_sync(0xffffffffu, s <= p.S && p.at[s + 1] - p.at[s] > m * p.rb));
+      c += __popc(__ballot_sync(0xffffffffu, s <= p.S && at[s + 1] - at[s] > m * p.rb));
     }
-    if (lane == 0) p.cnt[m] = c;
+    if (lane == 0) cnt[m] = c;
   }
   __syncthreads();
   // where m's blocks begin: the blocks of all larger m come first
   int run = 0;
   for (int b0 = 0; b0 < M; b0 += THREADS) {
     const int m = M - 1 - b0 - tid;
-    const int own = m >= 0 ? p.cnt[m] : 0;
+    const int own = m >= 0 ? cnt[m] : 0;
     int x = own;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -85,15 +89,15 @@ __global__ void __launch_bounds__(THREADS) plan_kernel(const PlanParams p) {
       if (w < warp) pre += s_w[w];
       all += s_w[w];
     }
-    if (m >= 0) p.cnt[m] = pre + x - own;
+    if (m >= 0) cnt[m] = pre + x - own;
     run = all;
     __syncthreads();
   }
   for (int m = warp; m < M; m += 32) {
-    int c = p.cnt[m];
+    int c = cnt[m];
     for (int s0 = 0; s0 <= p.S; s0 += 32) {
       const int s = s0 + lane;
-      const int a = s <= p.S ? p.at[s] : 0, n = s <= p.S ? p.at[s + 1] - a : 0;
+      const int a = s <= p.S ? at[s] : 0, n = s <= p.S ? at[s + 1] - a : 0;
       const uint32_t has = __ballot_sync(0xffffffffu, n > m * p.rb);
       if (n > m * p.rb)
         p.out[c + __popc(has & ((1u << lane) - 1))] =

@@ -34,18 +34,14 @@ constexpr int PRODUCER_WARP = 8;
 constexpr int MMA_WARP = 9;
 constexpr int TMEM_COLS = 512;
 
-// SHORT: packed short prompts (head dims 64, 128): half the tensor memory and shared memory, so that two CTAs share an SM
-// and one's set-up, loads and epilogue run under the other's products (a short prompt's block has one to four tiles).
-template <int D, bool SHORT = false>
+template <int D>
 struct Cfg {
-  static constexpr int BN = D == 256 || (SHORT && D == 128) ? 64 : 128;
+  static constexpr int BN = D == 256 ? 64 : 128;
   static constexpr int QBYTES = BM * D * 2;
   static constexpr int KBYTES = BN * D * 2;  // one K tile; a V tile is the same size
-  static constexpr int KSTAGES = SHORT ? 2 : 3;  // K_{j+3} loads while S_j.. S_{j+2} are still ahead of it
+  static constexpr int KSTAGES = 3;  // K_{j+3} loads while S_j.. S_{j+2} are still ahead of it
   static constexpr int VSTAGES = 2;
-  static constexpr int SBUF = SHORT ? 1 : 2;  // S buffers in TMEM (fp32), and P buffers (16-bit, BN / 2 columns each)
-  static constexpr int TCOLS = SHORT ? 256 : TMEM_COLS;
-  static constexpr int CTAS = SHORT ? 2 : 1;
+  static constexpr int SBUF = 2;  // S buffers in TMEM (fp32), and as many P buffers (16-bit, BN / 2 columns each)
   static constexpr int Q_OFF = 0;
   static constexpr int K_OFF = Q_OFF + QBYTES;
   static constexpr int V_OFF = K_OFF + KSTAGES * KBYTES;
@@ -53,11 +49,11 @@ struct Cfg {
   // at least ~120 KB so that one CTA holds an SM (its TMEM allocation is all 512 columns)
   static constexpr int RED_OFF = BAR_OFF + 256;  // [2 halves][128 rows] fp32: a row's partial max / sum
   static constexpr int SMEM_RAW = RED_OFF + 2 * BM * 4;
-  static constexpr int SMEM_BYTES = (SMEM_RAW < 120 * 1024 && !SHORT ? 120 * 1024 : SMEM_RAW) + 1024;
+  static constexpr int SMEM_BYTES = (SMEM_RAW < 120 * 1024 ? 120 * 1024 : SMEM_RAW) + 1024;
   static constexpr int S_COL = 0;                // S buffers at columns [b BN, (b + 1) BN)
   static constexpr int P_COL = SBUF * BN;        // P buffers at [P_COL + b BN / 2, ...)
   static constexpr int O_COL = P_COL + SBUF * BN / 2;  // O at [3 BN, 3 BN + D)
-  static_assert(O_COL + D <= TCOLS, "TMEM budget");
+  static_assert(O_COL + D <= TMEM_COLS, "TMEM budget");
   static_assert(SMEM_BYTES <= 232448, "shared memory budget");
 };
 
@@ -78,12 +74,13 @@ struct Params {
   const int32_t* tl;
   const int32_t* tn;
   int tl_ld;
-  // Packed prompts (the kernels' PK form; B = 1, causal within each prompt): the row blocks of all prompts, heaviest
+  // Packed prompts (attn_short.cuh, the pair kernel's PK form; causal within each prompt): the row blocks, heaviest
   // first, as (prompt's first row, its rows, block index m, key tiles it reads), *pk_n of them, listed by
   // packed::plan_kernel; and q, k, v for the rows that are taken again (packed_row_exact).
   const int4* pk;
   const int32_t* pk_n;
-  int tpb;  // SHORT: tokens a block, all G query heads of a KV head side by side (row = token G + head)
+  int fold, tpb;  // attn_short.cuh: query heads side by side in a block, and its tokens (row = token fold + head)
+  int wide_o;     // its output rows may be written 32 bytes at a time
   const void* src[3];
   int64_t src_st[3][2];  // H, T
 };
@@ -221,7 +218,7 @@ __device__ __forceinline__ float ex2_fma(float x) {
   return x < -125.f ? 0.f : r;
 }
 
-// The PK form's second look at a row whose output came out non-finite with a finite sum of weights: a value that is
+// Packed prompts' second look at a row whose output came out non-finite with a finite sum of weights: a value that is
 // infinite or NaN was multiplied by a weight, possibly the 0 of a key that the row does not see (a later row of its
 // prompt in the last tile, or the next prompt's rows behind it). Takes `cols` columns of the row again, reading only the
 // keys 0 .. row it sees. Rare; one thread a row.
@@ -262,14 +259,12 @@ __device__ __forceinline__ int kv_tiles(const Params& p, int mt) {
   return last <= 0 ? 0 : (last + BN - 1) / BN;
 }
 
-// PK: packed prompts, a block of the plan's list and a head a CTA; the grid is sized by the most blocks there can be.
-// SHORT: a KV head a CTA, a block being tpb tokens of its G query heads.
-template <typename T, int D, bool PK = false, bool SHORT = false>
-__global__ void __launch_bounds__(THREADS, Cfg<D, SHORT>::CTAS) fmha_kernel(const __grid_constant__ CUtensorMap qmap,
+template <typename T, int D>
+__global__ void __launch_bounds__(THREADS, 1) fmha_kernel(const __grid_constant__ CUtensorMap qmap,
                                                            const __grid_constant__ CUtensorMap kmap,
                                                            const __grid_constant__ CUtensorMap vmap,
                                                            const Params p) {
-  using C = Cfg<D, SHORT>;
+  using C = Cfg<D>;
   constexpr int BN = C::BN;
   constexpr int KS = C::KSTAGES, VS = C::VSTAGES, SB = C::SBUF;
   constexpr int AB = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
@@ -278,19 +273,11 @@ __global__ void __launch_bounds__(THREADS, Cfg<D, SHORT>::CTAS) fmha_kernel(cons
 
   // Heaviest query tiles first (causal tiles late in the sequence read the most keys); heads vary fastest so that
   // neighbouring CTAs share their KV head's tiles in L2.
-  const int heads = SHORT ? p.Hkv : p.B * p.Hq;
-  const int bh = blockIdx.x % heads;
-  int4 blk = make_int4(0, 0, 0, 0);
-  if constexpr (PK) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");  // the plan
-    const int e = int(blockIdx.x / heads);
-    if (e >= *p.pk_n) return;
-    blk = p.pk[e];
-  }
-  const int mt = PK ? blk.z : p.mtiles - 1 - int(blockIdx.x / (p.B * p.Hq));
-  const int b = SHORT ? 0 : bh / p.Hq, h = SHORT ? bh * p.G : bh % p.Hq, hk = SHORT ? bh : h / p.G;
-  const int r0 = mt * (SHORT ? p.tpb : BM);
-  const int ntiles = PK ? blk.w : kv_tiles<D>(p, mt);
+  const int bh = blockIdx.x % (p.B * p.Hq);
+  const int mt = p.mtiles - 1 - int(blockIdx.x / (p.B * p.Hq));
+  const int b = bh / p.Hq, h = bh % p.Hq, hk = h / p.G;
+  const int r0 = mt * BM;
+  const int ntiles = kv_tiles<D>(p, mt);
 
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -332,7 +319,7 @@ __global__ void __launch_bounds__(THREADS, Cfg<D, SHORT>::CTAS) fmha_kernel(cons
   }
   if (warp == MMA_WARP) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
-                 "r"(C::TCOLS));
+                 "r"(TMEM_COLS));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
   tc_fence_before();
@@ -348,14 +335,10 @@ __global__ void __launch_bounds__(THREADS, Cfg<D, SHORT>::CTAS) fmha_kernel(cons
       if (lane == 0) {
         prefetch_tensormap(&qmap);
         prefetch_tensormap(&kmap);
-        mbar_arrive_expect_tx(q_full, SHORT ? p.tpb * p.G * D * 2 : C::QBYTES);
+        mbar_arrive_expect_tx(q_full, C::QBYTES);
 #pragma unroll
-        for (int db = 0; db < D / 64; ++db) {
-          if constexpr (SHORT)  // (64, G heads, tpb tokens) boxes: a row a (token, head)
-            tma_load_4d(sm + C::Q_OFF + db * BM * 128, &qmap, db * 64, h, blk.x + r0, 0, q_full);
-          else
-            tma_load_4d(sm + C::Q_OFF + db * BM * 128, &qmap, db * 64, blk.x + r0, h, b, q_full);
-        }
+        for (int db = 0; db < D / 64; ++db)
+          tma_load_4d(sm + C::Q_OFF + db * BM * 128, &qmap, db * 64, r0, h, b, q_full);
       } else {
         prefetch_tensormap(&vmap);
       }
@@ -374,7 +357,7 @@ __global__ void __launch_bounds__(THREADS, Cfg<D, SHORT>::CTAS) fmha_kernel(cons
         mbar_arrive_expect_tx(&fullb[st], C::KBYTES);
 #pragma unroll
         for (int db = 0; db < D / 64; ++db)
-          tma_load_4d(sm + off + st * C::KBYTES + db * BN * 128, map, db * 64, blk.x + key_tile(p, mt, j) * BN, hk, b,
+          tma_load_4d(sm + off + st * C::KBYTES + db * BN * 128, map, db * 64, key_tile(p, mt, j) * BN, hk, b,
                       &fullb[st]);
         issued = j + 1;
       }
@@ -465,12 +448,11 @@ __global__ void __launch_bounds__(THREADS, Cfg<D, SHORT>::CTAS) fmha_kernel(cons
     constexpr int HD = D / 2;   // O columns a thread owns
     const int r = 32 * (warp & 3) + lane;  // row in the tile == TMEM lane
     const int hf = warp >> 2;              // which half of the columns
-    const int row = r0 + (SHORT ? r / p.G : r), hr = h + (SHORT ? r % p.G : 0);  // the thread's row (token) and head
+    const int row = r0 + r;
     const uint32_t lane_base = tmem + (uint32_t(32 * (warp & 3)) << 16);
     const uint32_t pair_bar = 2 + (warp & 3);  // named barrier of warps w and w + 4 (ids 2..5)
     float* red = reinterpret_cast<float*>(sm + C::RED_OFF);
-    const int lim = PK ? row : p.mask_kind == LB2_MASK_CAUSAL ? p.N - p.T + row : p.N - 1;
-    const int nkeys = PK ? 0x7fffffff : p.N;  // (packed: the horizon alone bounds a row's keys)
+    const int lim = p.mask_kind == LB2_MASK_CAUSAL ? p.N - p.T + row : p.N - 1;
     const uint8_t* mrow = (p.mask_kind == LB2_MASK_ARRAY && row < p.T) ? p.mask + int64_t(row) * p.m_st[0] : nullptr;
     float m_run = -INFINITY, l_run = 0.f;
     bool ok = true;
@@ -497,13 +479,13 @@ __global__ void __launch_bounds__(THREADS, Cfg<D, SHORT>::CTAS) fmha_kernel(cons
 
       const int kt = key_tile(p, mt, j);
       const int key0 = kt * BN + hf * HC;
-      const bool full_tile = kt * BN + BN - 1 <= lim && kt * BN + BN <= nkeys && !mrow;
+      const bool full_tile = kt * BN + BN - 1 <= lim && kt * BN + BN <= p.N && !mrow;
       float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
       if (full_tile) {
 #pragma unroll
         for (int c = 0; c < HC; ++c) mx4[c & 3] = fmaxf(mx4[c & 3], s[c]);
       } else {
-        mask_scores<HC>(s, mrow, p.m_st[1], key0, lim, nkeys);
+        mask_scores<HC>(s, mrow, p.m_st[1], key0, lim, p.N);
 #pragma unroll
         for (int c = 0; c < HC; ++c) mx4[c & 3] = fmaxf(mx4[c & 3], s[c]);
       }
@@ -581,12 +563,12 @@ __global__ void __launch_bounds__(THREADS, Cfg<D, SHORT>::CTAS) fmha_kernel(cons
     asm volatile("bar.sync %0, 64;" ::"r"(pair_bar));
     const float l_tot = l_run + red[(1 - hf) * BM + r];
     const bool have_o = ntiles > 0 && ok;
-    const bool store = row < (PK ? blk.y : p.T) && (!SHORT || r < p.tpb * p.G);
-    T* orow = reinterpret_cast<T*>(p.o) + b * p.o_st[0] + int64_t(hr) * p.o_st[1] + int64_t(blk.x + row) * p.o_st[2] + hf * HD;
+    const bool store = row < p.T;
+    T* orow = reinterpret_cast<T*>(p.o) + b * p.o_st[0] + int64_t(h) * p.o_st[1] + int64_t(row) * p.o_st[2] + hf * HD;
     const T* grow = p.gate ? reinterpret_cast<const T*>(p.gate) + b * p.g_st[0] + int64_t(h) * p.g_st[1] +
                                  int64_t(row) * p.g_st[2] + hf * HD
                            : nullptr;
-    const float inv = (have_o && (l_tot > 0.f || (PK && l_tot != l_tot))) ? 1.f / l_tot : 0.f;
+    const float inv = (have_o && l_tot > 0.f) ? 1.f / l_tot : 0.f;
 #pragma unroll 1
     for (int c = 0; c < HD; c += 32) {
       float ov[32];
@@ -598,15 +580,6 @@ __global__ void __launch_bounds__(THREADS, Cfg<D, SHORT>::CTAS) fmha_kernel(cons
         for (int e = 0; e < 32; ++e) ov[e] = 0.f;
       }
       if (!store) continue;
-      if constexpr (PK) {
-        float sum = 0.f;  // (finite unless some value is not)
-#pragma unroll
-        for (int e = 0; e < 32; ++e) sum = fmaf(ov[e], 0.f, sum);
-        if (sum != sum && l_tot == l_tot) {
-          packed_row_exact<T, D>(p, blk.x, row, hr, hf * HD + c, 32, orow + c);
-          continue;
-        }
-      }
 #pragma unroll
       for (int e = 0; e < 32; e += 8) {
         float x[8];
@@ -635,7 +608,7 @@ __global__ void __launch_bounds__(THREADS, Cfg<D, SHORT>::CTAS) fmha_kernel(cons
   __syncthreads();
   if (warp == MMA_WARP) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::TCOLS));
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS));
   }
 }
 

@@ -21,6 +21,7 @@
 #include "kv_runs.cuh"
 #include "attn_tiles.cuh"
 #include "attn_packed.cuh"
+#include "attn_short.cuh"
 #include "gdn_glue.cuh"
 #include "rope.cuh"
 #include "kv8.cuh"
@@ -1813,23 +1814,17 @@ static int packed_rows(const arows::PackedParams& p, int D, cudaStream_t st) {
 namespace lb2 {
 namespace packed {
 
+constexpr int SHORT_MEAN = 128;
+
 struct Layout {
   size_t cnt, at, out, total;
 };
 
-// The form a call takes. Pairs of CTAs on 256 rows of a head halve the K / V bytes an SM takes a product; for short prompts
-// a block of 128 rows holds all G query heads of a KV head (128 / G tokens), two CTAs an SM. The lengths are on the
-// device, so the mean length decides.
-enum Form { SHORT, SINGLE, PAIR };
-
-static Form form_of(int64_t S, int64_t T, int G, int D) {
-  if (D >= 128 && T > 128 * S) return PAIR;
-  return D <= 128 && G <= 64 ? SHORT : SINGLE;
-}
-
-static int block_rows(Form f, int G) {
-  return f == PAIR ? 2 * prefill::BM : f == SHORT ? prefill::BM / G : prefill::BM;
-}
+// Pairs of CTAs on 256 rows of a head halve the K / V bytes an SM takes a product; for short prompts a block of 128 rows
+// holds all query heads of a KV head (attn_short.cuh). The lengths are on the device, so the mean length decides.
+static bool pair_form(int64_t S, int64_t T, int D) { return D >= 128 && T > SHORT_MEAN * S; }
+static int fold_of(int G) { return G <= 64 ? G : 1; }
+static int block_rows(bool pair, int G) { return pair ? 2 * prefill::BM : prefill::BM / fold_of(G); }
 
 static Layout layout(int64_t S, int64_t T, int rb) {
   Layout l;
@@ -1841,7 +1836,7 @@ static Layout layout(int64_t S, int64_t T, int rb) {
 }
 
 template <typename T, int D>
-static int launch(Form form, const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm,
+static int launch(bool pair, const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm,
                   const prefill::Params& p, int64_t blocks, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
   cfg.stream = st;
@@ -1856,7 +1851,7 @@ static int launch(Form form, const CUtensorMap& qm, const CUtensorMap& km, const
   int dev = 0;
   LB2_CUDA(cudaGetDevice(&dev));
   if constexpr (D >= 128) {
-    if (form == PAIR) {
+    if (pair) {
       auto kern = prefill2::fmha2_kernel<T, D, true>;
       cfg.blockDim = dim3(prefill2::THREADS);
       cfg.dynamicSmemBytes = prefill2::Cfg<D>::SMEM_BYTES;
@@ -1877,24 +1872,19 @@ static int launch(Form form, const CUtensorMap& qm, const CUtensorMap& km, const
       return LB2_OK;
     }
   }
-  auto single = [&](auto kern, int smem, int heads) -> int {
-    static int attr_dev = -1;  // (one a kernel: the lambda is instantiated for each)
-    if (attr_dev != dev) {
-      LB2_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-      attr_dev = dev;
-    }
-    cfg.blockDim = dim3(prefill::THREADS);
-    cfg.dynamicSmemBytes = size_t(smem);
-    cfg.numAttrs = 1;
-    LB2_CHECK_ARG(blocks * heads < (int64_t(1) << 31), "attn_packed: too many row blocks");
-    cfg.gridDim = dim3(unsigned(blocks * heads));
-    LB2_CUDA(cudaLaunchKernelEx(&cfg, kern, qm, km, vm, p));
-    return LB2_OK;
-  };
-  if constexpr (D <= 128)
-    if (form == SHORT)
-      return single(prefill::fmha_kernel<T, D, true, true>, prefill::Cfg<D, true>::SMEM_BYTES, p.Hkv);
-  return single(prefill::fmha_kernel<T, D, true>, prefill::Cfg<D>::SMEM_BYTES, p.Hq);
+  auto kern = shortp::short_kernel<T, D>;
+  static int attr_dev = -1;
+  if (attr_dev != dev) {
+    LB2_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, shortp::Cfg<D>::SMEM_BYTES));
+    attr_dev = dev;
+  }
+  cfg.blockDim = dim3(shortp::THREADS);
+  cfg.dynamicSmemBytes = shortp::Cfg<D>::SMEM_BYTES;
+  cfg.numAttrs = 1;
+  LB2_CHECK_ARG(blocks * (p.Hq / p.fold) < (int64_t(1) << 31), "attn_packed: too many row blocks");
+  cfg.gridDim = dim3(unsigned(std::min<int64_t>(blocks * (p.Hq / p.fold), int64_t(sm_count(dev)) * shortp::Cfg<D>::CTAS)));
+  LB2_CUDA(cudaLaunchKernelEx(&cfg, kern, qm, km, vm, p));
+  return LB2_OK;
 }
 
 static int run(const arows::PackedParams& a, int D, int dtype, void* workspace, cudaStream_t st) {
@@ -1906,8 +1896,8 @@ static int run(const arows::PackedParams& a, int D, int dtype, void* workspace, 
   LB2_CHECK_ARG(aligned16(a.o) && a.o_st[0] % 8 == 0 && a.o_st[1] % 8 == 0,
                 "attn_packed: o must be 16-byte aligned with strides that are multiples of 8 elements");
   const int G = a.Hq / a.Hkv;
-  const Form form = form_of(a.S, a.T, G, D);
-  const int rb = block_rows(form, G);
+  const bool pair = pair_form(a.S, a.T, D);
+  const int rb = block_rows(pair, G), fold = fold_of(G);
   const Layout l = layout(a.S, a.T, rb);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   PlanParams pp{};
@@ -1919,9 +1909,7 @@ static int run(const arows::PackedParams& a, int D, int dtype, void* workspace, 
   pp.S = a.S;
   pp.T = a.T;
   pp.rb = rb;
-  pp.bn = form == SHORT ? (D == 128 ? prefill::Cfg<128, true>::BN : prefill::Cfg<64, true>::BN)
-          : form == SINGLE && D == 256 ? prefill::Cfg<256>::BN
-                                       : 128;
+  pp.bn = pair ? prefill2::Cfg<128>::BN : shortp::Cfg<128>::BN;
   plan_kernel<<<1, THREADS, 0, st>>>(pp);
   LB2_CUDA(cudaGetLastError());
   prefill::Params p{};
@@ -1933,7 +1921,9 @@ static int run(const arows::PackedParams& a, int D, int dtype, void* workspace, 
   p.Hkv = a.Hkv;
   p.T = p.N = a.T;
   p.G = G;
+  p.fold = fold;
   p.tpb = rb;
+  p.wide_o = (reinterpret_cast<uintptr_t>(a.o) & 31) == 0 && a.o_st[0] % 16 == 0 && a.o_st[1] % 16 == 0;
   p.mask_kind = LB2_MASK_CAUSAL;
   p.scale_log2 = a.scale * 1.4426950408889634f;
   p.pk = pp.out;
@@ -1944,14 +1934,14 @@ static int run(const arows::PackedParams& a, int D, int dtype, void* workspace, 
     p.src_st[i][1] = sst[i][1];
   }
   CUtensorMap maps[3];
-  const int rows[3] = {prefill::BM, form == PAIR ? 64 : pp.bn, pp.bn};
+  const int rows[3] = {prefill::BM, pair ? prefill2::Cfg<128>::HN : pp.bn, pp.bn};
   for (int i = 0; i < 3; ++i) {
     const int64_t st4[3] = {8, sst[i][0], sst[i][1]};  // (one batch: its stride is never used)
     int rc;
-    if (form == SHORT && i == 0) {  // (D, heads, rows): a box of all heads of a KV head and the block's tokens
+    if (!pair && i == 0) {  // (D, heads, rows): a box of the block's heads and tokens
       const uint64_t dims[4] = {uint64_t(D), uint64_t(a.Hq), uint64_t(a.T), 1};
       const uint64_t strides[3] = {uint64_t(a.q_st[0]) * 2, uint64_t(a.q_st[1]) * 2, 16};
-      const uint32_t box[4] = {64, uint32_t(G), uint32_t(rb), 1};
+      const uint32_t box[4] = {64, uint32_t(fold), uint32_t(rb), 1};
       rc = encode_tensor_map(&maps[0], dtype == LB2_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
                              4, a.q, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
     } else {
@@ -1961,9 +1951,9 @@ static int run(const arows::PackedParams& a, int D, int dtype, void* workspace, 
   }
   const int64_t blocks = int64_t(a.T) / rb + a.S + 1;
 #define LB2_PACKED(TT)                                                                               \
-  return D == 64 ? launch<TT, 64>(form, maps[0], maps[1], maps[2], p, blocks, st)                    \
-         : D == 128 ? launch<TT, 128>(form, maps[0], maps[1], maps[2], p, blocks, st)                \
-                    : launch<TT, 256>(form, maps[0], maps[1], maps[2], p, blocks, st)
+  return D == 64 ? launch<TT, 64>(pair, maps[0], maps[1], maps[2], p, blocks, st)                    \
+         : D == 128 ? launch<TT, 128>(pair, maps[0], maps[1], maps[2], p, blocks, st)                \
+                    : launch<TT, 256>(pair, maps[0], maps[1], maps[2], p, blocks, st)
   if (dtype == LB2_BF16) LB2_PACKED(__nv_bfloat16);
   LB2_PACKED(__half);
 #undef LB2_PACKED
@@ -1977,7 +1967,7 @@ extern "C" {
 size_t lb2_attn_packed_workspace_size(int S, int Hq, int Hkv, int T, int D) {
   if (S <= 0 || T <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv) return 0;
   const int G = Hq / Hkv;
-  return packed::layout(S, T, packed::block_rows(packed::form_of(S, T, G, D), G)).total;
+  return packed::layout(S, T, packed::block_rows(packed::pair_form(S, T, D), G)).total;
 }
 
 int lb2_attn_packed(const void* q, const int64_t* q_st, const void* k, const int64_t* k_st, const void* v,
