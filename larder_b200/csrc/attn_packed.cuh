@@ -1,4 +1,4 @@
-// Packed prompts: the list of row blocks that the kernels take (attn_short.cuh, attn_prefill2.cuh's PK form).
+// Packed prompts: the list of row blocks that the kernels take (attn_pfold.cuh, attn_prefill2.cuh's PK form).
 //
 // Prompt s is rows [cu[s], cu[s + 1]) of one row axis; its blocks of RB rows (256 on CTA pairs, 128 over the folded heads on one CTA) read
 // its key tiles from the first up to the block's last row. The lengths are known on the device only, so the list is made

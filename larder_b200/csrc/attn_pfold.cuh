@@ -1,12 +1,13 @@
-// Packed short prompts on one CTA (tcgen05): blocks of 128 rows, a row being a (token, query head) of one KV head, so that
-// the F = G query heads that share K and V fill a block with 128 / F tokens (F = 1 for more than 64 heads a KV head). A
-// short prompt then leaves little of its last block empty, and a block reads few key tiles past its own tokens.
+// Packed prompts on one CTA (tcgen05): blocks of 128 rows, a row being a (token, query head) of one KV head, so that the
+// F = G query heads that share K and V fill a block with 128 / F tokens (F = 1 for more than 64 heads a KV head). A short
+// prompt then leaves little of its last block empty, and a block reads few key tiles past its own tokens.
 //
-// A block has one to a few key tiles: what bounds it is not the products (32 KB of Q and O, a few microseconds of latency
-// a block) but the chain load -> S -> softmax -> P V -> epilogue. So the kernel is persistent, each CTA walking the plan's
-// blocks (heaviest first) in rounds, with Q, K and V of the next block on their way and its first S computed while this
-// one's O is written; and at head dims 64 and 128 a CTA takes half an SM's tensor memory and shared memory, so that two
-// share the SM.
+// What bounds a block is the chain load -> S -> softmax -> P V (-> epilogue) and the softmax's instructions, not the
+// products. So the kernel is persistent, each CTA walking the plan's blocks (heaviest first) in rounds, with Q, K and V of
+// the next block on their way and its first S computed while this one's O is written; and at head dims 64 and 128 a CTA
+// takes half an SM's tensor memory and shared memory, so that two share the SM, one's products under the other's softmax.
+// Measured (bf16, 32 / 8 heads x 128): 33 prompts of 8 to 441 rows, 4001 in all, 35.6 us (128 us with a CTA a block of one
+// head, 55 us not persistent); 982 TFLOP/s at prompts of 4096 rows.
 //
 // Roles (320 threads): warps 0-7 softmax and epilogue (warp w: TMEM lanes of quarter w % 4, key / O column half w / 4),
 // warp 8 TMA (lane 0 Q and K, lane 1 V), warp 9 issues the MMAs. S_j = Q K_j^T and O += P_j V_j as in attn_prefill.cuh;
@@ -18,7 +19,7 @@
 #include "attn_prefill2.cuh"
 
 namespace lb2 {
-namespace shortp {
+namespace pfold {
 
 using prefill::BM;
 using prefill::Params;
@@ -57,7 +58,7 @@ __device__ __forceinline__ void st_global32(void* p, const uint32_t* w) {
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(THREADS, Cfg<D>::CTAS) short_kernel(const __grid_constant__ CUtensorMap qmap,
+__global__ void __launch_bounds__(THREADS, Cfg<D>::CTAS) pfold_kernel(const __grid_constant__ CUtensorMap qmap,
                                                                       const __grid_constant__ CUtensorMap kmap,
                                                                       const __grid_constant__ CUtensorMap vmap,
                                                                       const Params p) {
@@ -427,5 +428,5 @@ __global__ void __launch_bounds__(THREADS, Cfg<D>::CTAS) short_kernel(const __gr
   }
 }
 
-}  // namespace shortp
+}  // namespace pfold
 }  // namespace lb2

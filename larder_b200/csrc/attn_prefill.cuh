@@ -74,12 +74,12 @@ struct Params {
   const int32_t* tl;
   const int32_t* tn;
   int tl_ld;
-  // Packed prompts (attn_short.cuh, the pair kernel's PK form; causal within each prompt): the row blocks, heaviest
+  // Packed prompts (attn_pfold.cuh, the pair kernel's PK form; causal within each prompt): the row blocks, heaviest
   // first, as (prompt's first row, its rows, block index m, key tiles it reads), *pk_n of them, listed by
   // packed::plan_kernel; and q, k, v for the rows that are taken again (packed_row_exact).
   const int4* pk;
   const int32_t* pk_n;
-  int fold, tpb;  // attn_short.cuh: query heads side by side in a block, and its tokens (row = token fold + head)
+  int fold, tpb;  // attn_pfold.cuh: query heads side by side in a block, and its tokens (row = token fold + head)
   int wide_o;     // its output rows may be written 32 bytes at a time
   const void* src[3];
   int64_t src_st[3][2];  // H, T

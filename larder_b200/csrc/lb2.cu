@@ -21,7 +21,7 @@
 #include "kv_runs.cuh"
 #include "attn_tiles.cuh"
 #include "attn_packed.cuh"
-#include "attn_short.cuh"
+#include "attn_pfold.cuh"
 #include "gdn_glue.cuh"
 #include "rope.cuh"
 #include "kv8.cuh"
@@ -1814,15 +1814,18 @@ static int packed_rows(const arows::PackedParams& p, int D, cudaStream_t st) {
 namespace lb2 {
 namespace packed {
 
-constexpr int SHORT_MEAN = 128;
+constexpr int PAIR_MEAN = 3000;
 
 struct Layout {
   size_t cnt, at, out, total;
 };
 
-// Pairs of CTAs on 256 rows of a head halve the K / V bytes an SM takes a product; for short prompts a block of 128 rows
-// holds all query heads of a KV head (attn_short.cuh). The lengths are on the device, so the mean length decides.
-static bool pair_form(int64_t S, int64_t T, int D) { return D >= 128 && T > SHORT_MEAN * S; }
+// Blocks of 128 rows over the folded heads (attn_pfold.cuh) at head dims 64 and 128, whatever the length: two CTAs share an
+// SM and hide each other's softmax (32 / 8 heads x 128: 316 against the pairs' 128 TFLOP/s at prompts of 256, 868 against
+// 540 at 2048, 982 against 698 at 4096). At head dim 256 one CTA fills an SM's tensor memory, and from some thousand rows
+// on pairs of CTAs, which halve the K / V bytes an SM takes a product, are faster (16 / 2 heads: 900 folded against 819 at
+// 2048, 1009 against 1087 at 4096). The lengths are on the device, so the mean length decides.
+static bool pair_form(int64_t S, int64_t T, int D) { return D == 256 && T > PAIR_MEAN * S; }
 static int fold_of(int G) { return G <= 64 ? G : 1; }
 static int block_rows(bool pair, int G) { return pair ? 2 * prefill::BM : prefill::BM / fold_of(G); }
 
@@ -1850,7 +1853,7 @@ static int launch(bool pair, const CUtensorMap& qm, const CUtensorMap& km, const
   cfg.attrs = attr;
   int dev = 0;
   LB2_CUDA(cudaGetDevice(&dev));
-  if constexpr (D >= 128) {
+  if constexpr (D == 256) {
     if (pair) {
       auto kern = prefill2::fmha2_kernel<T, D, true>;
       cfg.blockDim = dim3(prefill2::THREADS);
@@ -1872,17 +1875,17 @@ static int launch(bool pair, const CUtensorMap& qm, const CUtensorMap& km, const
       return LB2_OK;
     }
   }
-  auto kern = shortp::short_kernel<T, D>;
+  auto kern = pfold::pfold_kernel<T, D>;
   static int attr_dev = -1;
   if (attr_dev != dev) {
-    LB2_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, shortp::Cfg<D>::SMEM_BYTES));
+    LB2_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, pfold::Cfg<D>::SMEM_BYTES));
     attr_dev = dev;
   }
-  cfg.blockDim = dim3(shortp::THREADS);
-  cfg.dynamicSmemBytes = shortp::Cfg<D>::SMEM_BYTES;
+  cfg.blockDim = dim3(pfold::THREADS);
+  cfg.dynamicSmemBytes = pfold::Cfg<D>::SMEM_BYTES;
   cfg.numAttrs = 1;
   LB2_CHECK_ARG(blocks * (p.Hq / p.fold) < (int64_t(1) << 31), "attn_packed: too many row blocks");
-  cfg.gridDim = dim3(unsigned(std::min<int64_t>(blocks * (p.Hq / p.fold), int64_t(sm_count(dev)) * shortp::Cfg<D>::CTAS)));
+  cfg.gridDim = dim3(unsigned(std::min<int64_t>(blocks * (p.Hq / p.fold), int64_t(sm_count(dev)) * pfold::Cfg<D>::CTAS)));
   LB2_CUDA(cudaLaunchKernelEx(&cfg, kern, qm, km, vm, p));
   return LB2_OK;
 }
@@ -1909,7 +1912,7 @@ static int run(const arows::PackedParams& a, int D, int dtype, void* workspace, 
   pp.S = a.S;
   pp.T = a.T;
   pp.rb = rb;
-  pp.bn = pair ? prefill2::Cfg<128>::BN : shortp::Cfg<128>::BN;
+  pp.bn = pair ? prefill2::Cfg<128>::BN : pfold::Cfg<128>::BN;
   plan_kernel<<<1, THREADS, 0, st>>>(pp);
   LB2_CUDA(cudaGetLastError());
   prefill::Params p{};
