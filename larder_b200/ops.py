@@ -39,6 +39,11 @@ def _stream(t):
     return torch.cuda.current_stream(t.device).cuda_stream
 
 
+def _stream_of(dev):
+    """The same for a device index."""
+    return _raw_stream(dev) if _raw_stream is not None else torch.cuda.current_stream(dev).cuda_stream
+
+
 def _ptr(t):
     """A tensor's device address as the C ABI's void* (None for NULL); the argtypes convert plain ints."""
     return None if t is None else t.data_ptr()
@@ -494,7 +499,11 @@ def gdn_norm_gate(x, z, weight, eps):
 
 # ---------------------------------------------------------------------------------------------------- paged 8-bit cache
 
+# These calls are a few microseconds on the device, as much as Python needs for a dozen attribute reads: each reads what it
+# checks once and looks for the reason of a refusal only when there is one.
+
 _LAYOUTS = {"half": 0, "interleaved": 1}
+_E4M3, _I32, _I64, _FP32 = torch.float8_e4m3fn, torch.int32, torch.int64, torch.float32
 
 
 def _interleaved(layout, what):
@@ -505,17 +514,31 @@ def _interleaved(layout, what):
 
 
 def _int32(t, shape, dev, what):
-    if t.dtype != torch.int32 or tuple(t.shape) != shape or t.device != dev or not t.is_contiguous():
+    if t.dtype is not _I32 or t.shape != shape or t.get_device() != dev or not t.is_contiguous():
         raise ValueError(f"{what} must be contiguous int32 {list(shape)} on the same device")
 
 
 def _turns(turns, D, dev, what):
-    if turns.dtype != torch.int64 or turns.dim() != 1 or turns.device != dev or not turns.is_contiguous():
-        raise ValueError(f"{what}: turns must be contiguous int64 [R / 2] on the same device")
     R = 2 * turns.numel()
+    if turns.dtype is not _I64 or turns.dim() != 1 or turns.get_device() != dev or not turns.is_contiguous():
+        raise ValueError(f"{what}: turns must be contiguous int64 [R / 2] on the same device")
     if not 2 <= R <= D:
         raise ValueError(f"{what}: turns for 2 to {D} rotated dims (one a pair), got {R}")
     return R
+
+
+def _stream_workspace(dev, stream, nbytes, tag):
+    """A workspace of the stream's own (the current one): calls on different streams may run at once, and a buffer that has
+    become too small goes back to the allocator of the stream that used it."""
+    ws = _WS.get((dev, (tag, stream)))
+    if ws is None or ws.numel() < nbytes:
+        ws = workspace(torch.device("cuda", dev), nbytes, (tag, stream))
+    return ws
+
+
+def _out_like(out, x, what):
+    if out.shape != x.shape or out.dtype is not x.dtype or out.get_device() != x.get_device() or out.stride(-1) != 1:
+        raise ValueError(f"{what}: out must have the result's shape, dtype and device, and a unit last stride")
 
 
 def rope(x, positions, turns, layout="half", amp=1.0, inverse=False, out=None):
@@ -523,43 +546,46 @@ def rope(x, positions, turns, layout="half", amp=1.0, inverse=False, out=None):
 
     positions int32 [B, T] or [T]; turns int64 [R / 2] (larder_b200.rope.Rope(...).turns); layout "half" (pairs i,
     i + R / 2) or "interleaved" (2 i, 2 i + 1); inverse=True is the gradient. out may be x."""
-    _cuda(x, positions, turns, out)
-    if x.dim() != 4:
-        raise ValueError("rope: x must be [B, H, T, D]")
-    _unit_last(x, "x")
+    dev, st = x.get_device(), x.stride()
+    if dev < 0:
+        _cuda(x)
+    if len(st) != 4 or st[3] != 1:
+        raise ValueError("rope: x must be [B, H, T, D] with a unit last stride")
     B, H, T, D = x.shape
-    code, dev = dtype_code(x), x.device
     R = _turns(turns, D, dev, "rope")
-    if positions.dim() == 1:
-        _int32(positions, (T,), dev, "rope: positions")
-        pst = 0
-    else:
-        _int32(positions, (B, T), dev, "rope: positions")
-        pst = T
+    ps = positions.shape
+    _int32(positions, (T,) if len(ps) == 1 else (B, T), dev, "rope: positions")
     if out is None:
         out = torch.empty_like(x)
-        if out.stride(-1) != 1:
-            out = torch.empty((B, H, T, D), dtype=x.dtype, device=dev)
-    elif out.shape != x.shape or out.dtype != x.dtype or out.device != dev or out.stride(-1) != 1:
-        raise ValueError("rope: out must match x")
-    elif out.data_ptr() == x.data_ptr() and out.stride() != x.stride():
-        raise ValueError("rope: out over x must have x's strides")
-    rc = lib().lb2_rope(x.data_ptr(), i64(*x.stride()[:3]), out.data_ptr(), i64(*out.stride()[:3]),
-                        positions.data_ptr(), pst, turns.data_ptr(), B, H, T, D, R, code,
-                        _interleaved(layout, "rope"), 1 if inverse else 0, amp, _stream(x))
-    check(rc, "rope")
+        ost = out.stride()
+        if ost[3] != 1:
+            out = torch.empty((B, H, T, D), dtype=x.dtype, device=x.device)
+            ost = out.stride()
+    else:
+        _out_like(out, x, "rope")
+        ost = out.stride()
+        if out.data_ptr() == x.data_ptr() and ost != st:
+            raise ValueError("rope: out over x must have x's strides")
+    rc = lib().lb2_rope(x.data_ptr(), i64(*st[:3]), out.data_ptr(), i64(*ost[:3]), positions.data_ptr(),
+                        0 if len(ps) == 1 else T, turns.data_ptr(), B, H, T, D, R, dtype_code(x),
+                        _interleaved(layout, "rope"), 1 if inverse else 0, amp, _stream_of(dev))
+    if rc:
+        check(rc, "rope")
     return out
 
 
 def _kv8_pool(pages, scales, table, what):
-    if pages.dim() != 5 or pages.shape[1] != 2 or pages.dtype != torch.float8_e4m3fn or not pages.is_contiguous():
+    """(pages' shape, table's shape, device index) of a checked pool."""
+    ps, ts, dev = pages.shape, table.shape, pages.get_device()
+    if dev < 0:
+        _cuda(pages)
+    if len(ps) != 5 or ps[1] != 2 or pages.dtype is not _E4M3 or not pages.is_contiguous():
         raise ValueError(f"{what}: pages must be contiguous float8_e4m3fn [num_pages, 2, Hkv, page, D]")
-    if scales.dtype != torch.float32 or scales.shape != pages.shape[:3] or not scales.is_contiguous():
-        raise ValueError(f"{what}: scales must be contiguous fp32 [num_pages, 2, Hkv]")
-    if table.dtype != torch.int32 or table.dim() != 2 or table.stride(1) != 1:
-        raise ValueError(f"{what}: table must be int32 [B, max_pages] with a unit last stride")
-    if scales.device != pages.device or table.device != pages.device:
-        raise ValueError(f"{what}: pages, scales and table must share a device")
+    if scales.dtype is not _FP32 or scales.shape != ps[:3] or scales.get_device() != dev or not scales.is_contiguous():
+        raise ValueError(f"{what}: scales must be contiguous fp32 [num_pages, 2, Hkv] on the pages' device")
+    if table.dtype is not _I32 or len(ts) != 2 or table.get_device() != dev or table.stride(1) != 1:
+        raise ValueError(f"{what}: table must be int32 [B, max_pages] with a unit last stride on the pages' device")
+    return ps, ts, dev
 
 
 def kv8_append(pages, scales, k, v, table, start, lens=None, cu=None, turns=None, layout="half", amp=1.0):
@@ -567,17 +593,13 @@ def kv8_append(pages, scales, k, v, table, start, lens=None, cu=None, turns=None
     positions start[b] onwards (start int32 [B]), keys rotated by them when turns is given. lens int32 [B]: only the
     first lens[b] tokens of each. cu int32 [B + 1]: k / v are [1, Hkv, T, D] and sequence b's tokens are rows cu[b] to
     cu[b + 1] - 1."""
-    _cuda(pages, scales, k, v, table, start, lens, cu, turns)
-    _kv8_pool(pages, scales, table, "kv8_append")
-    num_pages, _, Hkv, page, D = pages.shape
-    B, max_pages = table.shape
-    dev = pages.device
-    if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.device != dev or v.device != dev:
-        raise ValueError("kv8_append: k and v must share shape, dtype and the cache's device")
-    _unit_last(k, "k")
-    _unit_last(v, "v")
-    T = k.shape[2]
-    if tuple(k.shape) != (1 if cu is not None else B, Hkv, T, D):
+    (num_pages, _, Hkv, page, D), (B, max_pages), dev = _kv8_pool(pages, scales, table, "kv8_append")
+    ks, kst, vst = k.shape, k.stride(), v.stride()
+    if (len(ks) != 4 or ks != v.shape or k.dtype is not v.dtype or k.get_device() != dev or v.get_device() != dev
+            or kst[3] != 1 or vst[3] != 1):
+        raise ValueError("kv8_append: k and v must share shape, dtype and the cache's device, with unit last strides")
+    T = ks[2]
+    if ks[0] != (B if cu is None else 1) or ks[1] != Hkv or ks[3] != D:
         raise ValueError("kv8_append: k / v must be [B, Hkv, T, D] for the table's B and the cache's Hkv and D "
                          "([1, Hkv, T, D] with cu)")
     _int32(start, (B,), dev, "kv8_append: start")
@@ -586,17 +608,12 @@ def kv8_append(pages, scales, k, v, table, start, lens=None, cu=None, turns=None
     if cu is not None:
         _int32(cu, (B + 1,), dev, "kv8_append: cu")
     R = 0 if turns is None else _turns(turns, D, dev, "kv8_append")
-    rc = lib().lb2_kv8_append(pages.data_ptr(), scales.data_ptr(), k.data_ptr(), i64(*k.stride()[:3]), v.data_ptr(),
-                              i64(*v.stride()[:3]), table.data_ptr(), table.stride(0), start.data_ptr(), _ptr(lens),
-                              _ptr(cu), _ptr(turns), B, Hkv, T, D, R, page, num_pages, max_pages, dtype_code(k),
-                              _interleaved(layout, "kv8_append"), amp, _stream(pages))
-    check(rc, "kv8_append")
-
-
-def _stream_workspace(t, nbytes, tag):
-    """A workspace of the current stream's own: calls on different streams may run at once, and a buffer that has become
-    too small goes back to the allocator of the stream that used it."""
-    return workspace(t.device, nbytes, (tag, _stream(t)))
+    rc = lib().lb2_kv8_append(pages.data_ptr(), scales.data_ptr(), k.data_ptr(), i64(*kst[:3]), v.data_ptr(),
+                              i64(*vst[:3]), table.data_ptr(), table.stride(0), start.data_ptr(), _ptr(lens), _ptr(cu),
+                              _ptr(turns), B, Hkv, T, D, R, page, num_pages, max_pages, dtype_code(k),
+                              _interleaved(layout, "kv8_append"), amp, _stream_of(dev))
+    if rc:
+        check(rc, "kv8_append")
 
 
 _KV8_WS = {}  # (B, Hq, Hkv, T, D, page, max_pages, device index) -> workspace bytes
@@ -605,61 +622,66 @@ _KV8_WS = {}  # (B, Hq, Hkv, T, D, page, max_pages, device index) -> workspace b
 def kv8_attend(q, pages, scales, table, kv_len, scale, causal=True, out=None):
     """Attention of q [B, Hq, T, D] over each sequence's first kv_len[b] cached tokens (lb2_kv8_attend); kv_len int32
     [B] counts the call's own tokens, which are already appended. causal: row t sees keys 0 .. kv_len - T + t."""
-    _cuda(q, pages, scales, table, kv_len, out)
-    _kv8_pool(pages, scales, table, "kv8_attend")
-    num_pages, _, Hkv, page, D = pages.shape
-    max_pages, dev = table.shape[1], pages.device
-    if q.dim() != 4 or q.shape[0] != table.shape[0] or q.shape[3] != D or q.device != dev:
-        raise ValueError("kv8_attend: q must be [B, Hq, T, D] for the table's B and the cache's D and device")
-    _unit_last(q, "q")
-    B, Hq, T, _ = q.shape
+    (num_pages, _, Hkv, page, D), (B, max_pages), dev = _kv8_pool(pages, scales, table, "kv8_attend")
+    qs, qst = q.shape, q.stride()
+    if len(qs) != 4 or qs[0] != B or qs[3] != D or q.get_device() != dev or qst[3] != 1:
+        raise ValueError("kv8_attend: q must be [B, Hq, T, D] for the table's B and the cache's D and device, with a unit "
+                         "last stride")
+    Hq, T = qs[1], qs[2]
     if Hq == 0 or Hq % Hkv:
         raise ValueError("kv8_attend: Hq must be a multiple of the cache's Hkv")
     _int32(kv_len, (B,), dev, "kv8_attend: kv_len")
     if out is None:
-        out = torch.empty((B, Hq, T, D), dtype=q.dtype, device=dev)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or out.stride(-1) != 1:
-        raise ValueError("kv8_attend: out must match q")
-    key = (B, Hq, Hkv, T, D, page, max_pages, dev.index)
+        out = torch.empty_like(q)
+    else:
+        _out_like(out, q, "kv8_attend")
+    key = (B, Hq, Hkv, T, D, page, max_pages, dev)
     n = _KV8_WS.get(key)
     if n is None:
         n = _KV8_WS[key] = lib().lb2_kv8_attend_workspace_size(*key[:7])
-    ws = _stream_workspace(q, n, "kv8_attend")
-    rc = lib().lb2_kv8_attend(q.data_ptr(), i64(*q.stride()[:3]), pages.data_ptr(), scales.data_ptr(), table.data_ptr(),
+    stream = _stream_of(dev)
+    ws = _stream_workspace(dev, stream, n, "kv8_attend")
+    rc = lib().lb2_kv8_attend(q.data_ptr(), i64(*qst[:3]), pages.data_ptr(), scales.data_ptr(), table.data_ptr(),
                               table.stride(0), kv_len.data_ptr(), out.data_ptr(), i64(*out.stride()[:3]), B, Hq, Hkv, T,
                               D, page, num_pages, max_pages, dtype_code(q), scale, 1 if causal else 0, ws.data_ptr(),
-                              ws.numel(), _stream(q))
-    check(rc, "kv8_attend")
+                              ws.numel(), stream)
+    if rc:
+        check(rc, "kv8_attend")
     return out
 
 
 def attn_packed(q, k, v, scale, cu, out=None):
     """Causal attention over prompts packed on one row axis (lb2_attn_packed): q [1, Hq, T, D], k / v [1, Hkv, T, D],
     cu int32 [S + 1] on the device, prompt s being rows cu[s] .. cu[s + 1] - 1."""
-    _cuda(q, k, v, cu, out)
-    if q.dim() != 4 or k.dim() != 4 or q.shape[0] != 1 or k.shape[0] != 1 or k.shape != v.shape:
+    dev, qs, ks = q.get_device(), q.shape, k.shape
+    qst, kst, vst = q.stride(), k.stride(), v.stride()
+    if dev < 0:
+        _cuda(q)
+    if len(qs) != 4 or len(ks) != 4 or qs[0] != 1 or ks[0] != 1 or ks != v.shape:
         raise ValueError("attn_packed: q must be [1, Hq, T, D], k and v [1, Hkv, T, D]")
-    for t, n in ((q, "q"), (k, "k"), (v, "v")):
-        _unit_last(t, n)
-    _, Hq, T, D = q.shape
-    Hkv, dev = k.shape[1], q.device
-    if k.shape[2] != T or k.shape[3] != D or k.dtype != q.dtype or v.dtype != q.dtype:
+    if qst[3] != 1 or kst[3] != 1 or vst[3] != 1:
+        raise ValueError("attn_packed: the last axis must have unit stride")
+    _, Hq, T, D = qs
+    Hkv = ks[1]
+    if ks[2] != T or ks[3] != D or k.dtype is not q.dtype or v.dtype is not q.dtype:
         raise ValueError("attn_packed: q, k and v must share rows, head dim and dtype")
-    if k.device != dev or v.device != dev:
+    if k.get_device() != dev or v.get_device() != dev:
         raise ValueError("attn_packed: q, k and v must share a device")
-    if cu.dim() != 1 or cu.numel() < 2:
-        raise ValueError("attn_packed: cu must be int32 [S + 1], S >= 1")
     S = cu.numel() - 1
+    if S < 1:
+        raise ValueError("attn_packed: cu must be int32 [S + 1], S >= 1")
     _int32(cu, (S + 1,), dev, "attn_packed: cu")
-    if Hkv == 0 or Hq % Hkv:
+    if Hkv == 0 or Hq == 0 or Hq % Hkv:
         raise ValueError("attn_packed: Hq must be a multiple of Hkv")
     if out is None:
-        out = torch.empty((1, Hq, T, D), dtype=q.dtype, device=dev)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or out.stride(-1) != 1:
-        raise ValueError("attn_packed: out must match q")
-    ws = _stream_workspace(q, lib().lb2_attn_packed_workspace_size(S, Hq, Hkv, T, D), "attn_packed")
-    rc = lib().lb2_attn_packed(q.data_ptr(), i64(*q.stride()[1:3]), k.data_ptr(), i64(*k.stride()[1:3]), v.data_ptr(),
-                               i64(*v.stride()[1:3]), out.data_ptr(), i64(*out.stride()[1:3]), cu.data_ptr(), S, Hq,
-                               Hkv, T, D, dtype_code(q), scale, ws.data_ptr(), ws.numel(), _stream(q))
-    check(rc, "attn_packed")
+        out = torch.empty_like(q)
+    else:
+        _out_like(out, q, "attn_packed")
+    stream = _stream_of(dev)
+    ws = _stream_workspace(dev, stream, lib().lb2_attn_packed_workspace_size(S, Hq, Hkv, T, D), "attn_packed")
+    rc = lib().lb2_attn_packed(q.data_ptr(), i64(*qst[1:3]), k.data_ptr(), i64(*kst[1:3]), v.data_ptr(),
+                               i64(*vst[1:3]), out.data_ptr(), i64(*out.stride()[1:3]), cu.data_ptr(), S, Hq, Hkv, T,
+                               D, dtype_code(q), scale, ws.data_ptr(), ws.numel(), stream)
+    if rc:
+        check(rc, "attn_packed")
     return out
