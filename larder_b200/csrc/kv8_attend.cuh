@@ -18,8 +18,8 @@
 //    read different halves of the 128-byte lines (no bank conflicts).
 //  - O^T += V^T P^T: ldmatrix.trans on 16-bit units gives a lane two dims of two keys; one byte permute and two
 //    conversions make them the operand pairs of two dims (rows quad and quad + 8 of the MMA are dims 2 quad, 2 quad + 1).
-// Query rows go to f16 exactly: a row is shifted by a power of two (its largest value to [2^14, 2^15)), which the score's
-// factor undoes; bf16's 8 bits fit f16's 11 down to 2^-28 of the row's largest value.
+// bf16 query rows go to f16 exactly: a row is shifted by a power of two (its largest value to [2^14, 2^15)), which the
+// score's factor undoes; bf16's 8 bits fit f16's 11 down to 2^-28 of the row's largest value.
 //
 // Softmax in base 2, fp32. The weights carry the values' scale: p'_n = 2^(s_n + log2 s_v - m), m the running maximum of
 // s_n + log2 s_v, and l = sum p'_n / s_v, so that o = sum p'_n code_n / l; the weights of pages with scales far apart thus
@@ -64,7 +64,7 @@ struct Cfg {
   static constexpr int PART = WARPS / 2 * PART_REGS * 32 * 16;  // half the warps' parts
   static constexpr int XCH = DS > 1 ? 2 * WARPS * MK * NT * 32 * 16 : 0;  // two tiles' half scores of every warp
   static constexpr int JOIN = PART > XCH ? PART : XCH;  // (one area: a barrier lies between the two uses)
-  static constexpr int FIXED = QBYTES + JOIN + (2 * MAX_B + 1) * 4 + 1024 + 1024;
+  static constexpr int FIXED = QBYTES + JOIN + 2 * WARPS * 8 * NT * 4 + (2 * MAX_B + 1) * 4 + 1024 + 1024;
   static constexpr int FIT = (232448 - FIXED) / (STAGE + 48);
   // A multiple of both, so that a stage only ever serves one producer warp and one key group, whose waits on it then
   // follow its phases in order (a wait two phases ahead would pass at once).
@@ -72,7 +72,9 @@ struct Cfg {
   static constexpr int STAGES = (FIT > 16 ? 16 : FIT) / STEP * STEP;
   static constexpr int Q_OFF = STAGES * STAGE;
   static constexpr int PART_OFF = Q_OFF + QBYTES;
-  static constexpr int SC_OFF = PART_OFF + JOIN;                // [STAGES][4 slices][K, V] fp32
+  static constexpr int QMAX = DS > 1 ? 2 * WARPS * 8 * NT * 4 : 0;  // two items' largest query values by half
+  static constexpr int QMAX_OFF = PART_OFF + JOIN;
+  static constexpr int SC_OFF = QMAX_OFF + QMAX;                // [STAGES][4 slices][K, V] fp32
   static constexpr int PREFIX_OFF = SC_OFF + STAGES * 32;        // [MAX_B + 1]
   static constexpr int LENS_OFF = PREFIX_OFF + (MAX_B + 1) * 4;  // [MAX_B]
   static constexpr int BAR_OFF = (LENS_OFF + MAX_B * 4 + 15) / 16 * 16;
@@ -316,7 +318,7 @@ __global__ void __launch_bounds__(Cfg<D, NT, RG, MK, KG>::THREADS, 1)
   const int Tq = p.a.T;
   uint32_t qf[C::Q_REGS ? NT : 1][C::Q_REGS ? SEG : 1][8];  // this row's 16 dims of each 64-dim segment
   uint4* qsm = reinterpret_cast<uint4*>(sm + C::Q_OFF);     // [RG][NT][SEG][2][32 lanes]
-  rope::Raw<T, 8> raw[NT][DS * SEG][2];  // the query rows' dims as they lie, the warp's own first
+  rope::Raw<T, 8> raw[NT][SEG][2];  // the warp's dims of the query rows as they lie
   auto load_q = [&](const Item& w) {
     const int hk = w.hb / p.nrb, r0 = (w.hb - hk * p.nrb) * p.rpb, r1 = min(p.rows, r0 + p.rpb);
 #pragma unroll
@@ -324,10 +326,10 @@ __global__ void __launch_bounds__(Cfg<D, NT, RG, MK, KG>::THREADS, 1)
       const int r = r0 + (rg * NT + nt) * 8 + quad;
       const int g = Tq == 1 ? r : r / Tq, t = r - g * Tq;
       const T* src = static_cast<const T*>(p.a.q) + w.b * p.a.q_st[0] + int64_t(hk * p.G + g) * p.a.q_st[1] +
-                     t * p.a.q_st[2] + 16 * qid;
+                     t * p.a.q_st[2] + dh * DW + 16 * qid;
 #pragma unroll
-      for (int s = 0; s < DS * SEG; ++s) {
-        const T* from = src + (s < SEG ? dh : 1 - dh) * DW + 64 * (s % SEG);
+      for (int s = 0; s < SEG; ++s) {
+        const T* from = src + 64 * s;
         if (r >= r1) {
           raw[nt][s][0].u = raw[nt][s][1].u = make_uint4(0, 0, 0, 0);
         } else if (p.wide_q) {
@@ -340,42 +342,69 @@ __global__ void __launch_bounds__(Cfg<D, NT, RG, MK, KG>::THREADS, 1)
       }
     }
   };
-  constexpr bool AHEAD = NT * D <= 256;  // the next item's rows are loaded while this one's parts are merged
+  constexpr bool AHEAD = NT == 1 && DS == 1;  // where registers allow, the next item's rows are loaded while this one's parts are merged
   bool have_q = false;
   float4* xch = reinterpret_cast<float4*>(sm + C::PART_OFF);  // [2 tiles][DS][WARPS / 2][MK NT][32 lanes]
+  float* qmax = reinterpret_cast<float*>(sm + C::QMAX_OFF);  // [2 items][DS][WARPS / 2][8 NT]
   const int pair = warp % (WARPS / 2);
-  int gt = 0, xpar = 0;
+  int gt = 0, xpar = 0, qpar = 0;
   bool ok = true;
   while (sched.next(it)) {
     const int hk = it.hb / p.nrb, r0 = (it.hb - hk * p.nrb) * p.rpb, r1 = min(p.rows, r0 + p.rpb);  // the block's rows
     // Query fragments: lane (quad, qid) holds dims 64 s + 16 qid .. + 15 of row quad of each row tile.
     if (!have_q) load_q(it);
     float fac[NT][2];
-    int lim[NT][2];
+    int lim[NT][2], ex[NT];
+    constexpr bool SHIFT = !std::is_same<T, __half>::value;
+    if constexpr (SHIFT) {  // the exponent of each row's largest value
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float mx = 0.f;
+#pragma unroll
+        for (int s = 0; s < SEG; ++s) {
+          __nv_bfloat162 m = __floats2bfloat162_rn(0.f, 0.f);
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&raw[nt][s][g].u);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) m = __hmax2(m, __habs2(h[e]));  // (NaN is passed over)
+          }
+          mx = fmaxf(mx, fmaxf(__low2float(m), __high2float(m)));
+        }
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        if constexpr (DS > 1) {  // of both halves of the dims
+          if (qid == 0) qmax[((qpar * 2 + dh) * (WARPS / 2) + pair) * 8 * NT + nt * 8 + quad] = mx;
+        }
+        ex[nt] = __float_as_int(mx);
+      }
+      if constexpr (DS > 1) {
+        asm volatile("bar.sync %0, 64;" ::"r"(2 + pair) : "memory");
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+          ex[nt] = __float_as_int(fmaxf(__int_as_float(ex[nt]), qmax[((qpar * 2 + 1 - dh) * (WARPS / 2) + pair) * 8 * NT + nt * 8 + quad]));
+        qpar ^= 1;
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) ex[nt] = ex[nt] > 0 ? min(max((ex[nt] >> 23) - 127, -112), 127) : 14;
+    }
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      float mx = 0.f;  // the row's largest value: of all its dims
+      // bf16: times 2^(14 - ex), 14 - ex in [-113, 126]; f16 goes as it is
+      const float up = SHIFT ? __uint_as_float(uint32_t(127 + 14 - ex[nt]) << 23) : 1.f;
 #pragma unroll
-      for (int s = 0; s < DS * SEG; ++s) {
-        float x[16];
-        raw[nt][s][0].get(x);
-        raw[nt][s][1].get(x + 8);
-#pragma unroll
-        for (int e = 0; e < 16; ++e) mx = fmaxf(mx, kv8::finite_abs(x[e]));
-      }
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-      // multiply by 2^(14 - floor(log2 mx))
-      const int ex = mx > 0.f ? min(max(int(__float_as_uint(mx) >> 23) - 127, -112), 127) : 14;
-      const float up = __uint_as_float(uint32_t(127 + 14 - ex) << 23);  // 14 - ex in [-113, 126]
-#pragma unroll
-      for (int s = 0; s < SEG; ++s) {  // (raw holds the warp's own dims first)
-        float x[16];
-        raw[nt][s][0].get(x);
-        raw[nt][s][1].get(x + 8);
+      for (int s = 0; s < SEG; ++s) {
         uint32_t w[8];
+        if constexpr (SHIFT) {
+          float x[16];
+          raw[nt][s][0].get(x);
+          raw[nt][s][1].get(x + 8);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) w[e] = pack2<__half>(x[2 * e] * up, x[2 * e + 1] * up);
+          for (int e = 0; e < 8; ++e) w[e] = pack2<__half>(x[2 * e] * up, x[2 * e + 1] * up);
+        } else {
+          const uint4 a = raw[nt][s][0].u, b = raw[nt][s][1].u;
+          w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w, w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
+        }
         if constexpr (C::Q_REGS) {
 #pragma unroll
           for (int e = 0; e < 8; ++e) qf[nt][s][e] = w[e];
@@ -387,10 +416,11 @@ __global__ void __launch_bounds__(Cfg<D, NT, RG, MK, KG>::THREADS, 1)
       }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {  // for columns 2 qid + e: the row whose fragments quad 2 qid + e holds
-        const int exr = __shfl_sync(0xffffffffu, ex, (2 * qid + e) * 4);
-        // scale 2^(ex - 14), the two powers apart so that neither leaves fp32's range
-        fac[nt][e] = p.scale_log2 * __uint_as_float(uint32_t(127 + (exr - 14) / 2) << 23) *
-                     __uint_as_float(uint32_t(127 + (exr - 14) - (exr - 14) / 2) << 23);
+        fac[nt][e] = p.scale_log2;
+        if constexpr (SHIFT) {  // times 2^(ex - 14), as two powers so that neither leaves fp32's range
+          const int d = __shfl_sync(0xffffffffu, ex[nt], (2 * qid + e) * 4) - 14;
+          fac[nt][e] = fac[nt][e] * __uint_as_float(uint32_t(127 + d / 2) << 23) * __uint_as_float(uint32_t(127 + d - d / 2) << 23);
+        }
         // the row's last key (rows past the block's are zeros that see what the others see; nothing of them is kept)
         const int rr = r0 + (rg * NT + nt) * 8 + 2 * qid + e;
         lim[nt][e] = p.a.causal && Tq > 1 ? it.len - Tq + rr % Tq : it.len - 1;
@@ -605,7 +635,7 @@ __global__ void __launch_bounds__(Cfg<D, NT, RG, MK, KG>::THREADS, 1)
       break;
     }
     const int pi = kg * SL + sl;
-#pragma unroll
+#pragma unroll 1  // (one copy of the code: at an item's end it is fetched cold)
     for (int half = SL * KG / 2; half > 0; half >>= 1) {
       if (pi >= half && pi < 2 * half) {
         float4* d = part + (((pi - half) * RG + rg) * DS + dh) * C::PART_REGS * 32 + lane;
@@ -710,11 +740,16 @@ __global__ void __launch_bounds__(256) combine_kernel(const Params p) {
       for (int k = 0; k < HELD; ++k) {
         const size_t at = size_t(first + min(k0 + k, nparts - 1)) * p.rpb + r;
         ml[k] = *reinterpret_cast<const float2*>(p.ws_ml + 2 * at);
-        const float2* src = reinterpret_cast<const float2*>(p.ws_o + at * D + lane * E);
+        const float* src = p.ws_o + at * D + lane * E;
+        if constexpr (E == 2) {
+          const float2 v = *reinterpret_cast<const float2*>(src);
+          y[k][0] = v.x, y[k][1] = v.y;
+        } else {
 #pragma unroll
-        for (int e = 0; e < E; e += 2) {
-          const float2 v = src[e / 2];
-          y[k][e] = v.x, y[k][e + 1] = v.y;
+          for (int e = 0; e < E; e += 4) {
+            const float4 v = *reinterpret_cast<const float4*>(src + e);
+            y[k][e] = v.x, y[k][e + 1] = v.y, y[k][e + 2] = v.z, y[k][e + 3] = v.w;
+          }
         }
       }
       float m1 = M;
