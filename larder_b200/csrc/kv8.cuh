@@ -10,6 +10,8 @@
 // Infinities are held as +-448 s, NaN as NaN; neither sets the scale.
 #pragma once
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "rope.cuh"
 
@@ -114,10 +116,12 @@ struct Piece {
 };
 
 __device__ __forceinline__ bool piece_of(const AppendParams& p, Piece& w) {
-  w.kind = blockIdx.y & 1;
-  w.h = (blockIdx.y >> 1) * p.hpb;
+  // K / V and the head groups vary fastest, so that the blocks that run together read whole token rows
+  const int groups = (p.Hkv + p.hpb - 1) / p.hpb, i = blockIdx.x / (2 * groups), g = blockIdx.x - i * 2 * groups;
+  w.kind = g >= groups;
+  w.h = (g - w.kind * groups) * p.hpb;
   int j;
-  if (!find_page(p, blockIdx.x, w.b, j)) return false;
+  if (!find_page(p, i, w.b, j)) return false;
   const int n0 = p.start[w.b];
   const int r0 = p.cu ? p.cu[w.b] : 0;
   const int n = p.cu ? min(p.cu[w.b + 1], p.T) - r0 : p.lens ? min(p.lens[w.b], p.T) : p.T;
@@ -208,6 +212,40 @@ __device__ __forceinline__ float2 turn_cs_fast(uint32_t frac) {
   return make_float2(__cosf(a), __sinf(a));
 }
 
+__device__ __forceinline__ void turn2(float& x0, float& x1, float2 z) {
+  const float y0 = x0 * z.x - x1 * z.y, y1 = x1 * z.x + x0 * z.y;
+  x0 = y0, x1 = y1;
+}
+
+// Two 16-bit values a word: the larger magnitudes, and four codes of two words scaled by a power of two.
+template <typename T>
+struct Pair;
+template <>
+struct Pair<__half> {
+  using V2 = __half2;
+  // f16 codes come from f16 pairs: x 2^k is exact in f16 (|x 2^k| <= 448; what falls under 2^-14 rounds to code 0 either
+  // way), unless 2^k itself leaves f16's range
+  static __device__ __forceinline__ bool direct(float inv) { return inv >= 0x1p-14f && inv <= 0x1p15f; }
+  static __device__ __forceinline__ uint32_t enc4(uint32_t a, uint32_t b, float inv) {
+    const __half2 k = __float2half2_rn(inv);
+    const __half2 x = __hmul2(*reinterpret_cast<const __half2*>(&a), k), y = __hmul2(*reinterpret_cast<const __half2*>(&b), k);
+    uint32_t r;
+    asm("{\n\t.reg .b16 lo, hi;\n\t"
+        "cvt.rn.satfinite.e4m3x2.f16x2 lo, %1;\n\t"
+        "cvt.rn.satfinite.e4m3x2.f16x2 hi, %2;\n\t"
+        "mov.b32 %0, {lo, hi};\n\t}"
+        : "=r"(r)
+        : "r"(*reinterpret_cast<const uint32_t*>(&x)), "r"(*reinterpret_cast<const uint32_t*>(&y)));
+    return r;
+  }
+};
+template <>
+struct Pair<__nv_bfloat16> {
+  using V2 = __nv_bfloat162;
+  static __device__ __forceinline__ bool direct(float) { return false; }
+  static __device__ __forceinline__ uint32_t enc4(uint32_t, uint32_t, float) { return 0; }
+};
+
 // Rows of 16-byte groups: the page's new rows are held in registers, read once. A unit is two groups of 8 elements: in
 // the rotated half layout a group and its partners R / 2 on, elsewhere neighbours; a thread has one unit of K rows. The
 // block takes `hpb` heads in turn, the next one's loads in flight while it works: the angles of its rows serve them all.
@@ -217,7 +255,7 @@ template <typename T, int THREADS, int K>
 __global__ void __launch_bounds__(THREADS) append_kernel(const AppendParams p) {
   constexpr int WARPS = THREADS / 32;
   constexpr int V = 16 / int(sizeof(T)), N = 8 / V;  // values a load, loads a group
-  __shared__ float red[2][WARPS];
+  __shared__ __align__(16) uint32_t red[2][WARPS < 4 ? 4 : WARPS];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   Piece w;
@@ -229,20 +267,21 @@ __global__ void __launch_bounds__(THREADS) append_kernel(const AppendParams p) {
   const int a = half ? u * 8 : u * 16, c = half ? a + R2 : a + 8;
   const int64_t hst = p.st[w.kind][1], tst = p.st[w.kind][2];
   const T* x = static_cast<const T*>(p.x[w.kind]) + (p.cu ? 0 : w.b * p.st[w.kind][0]) + w.h * hst +
-               (w.row0 + first) * tst;
+               (w.row0 + first) * tst + a;  // this thread's first row
+  const int64_t kst = rpp * tst;
   const int nh = min(p.hpb, p.Hkv - w.h);
   rope::Raw<T, V> ra[K][N], rc[K][N];
-  auto fetch = [&](const T* xr) {
+  auto fetch = [&] {
 #pragma unroll
     for (int k = 0; k < K; ++k)
       if (first + k * rpp < nrows)
 #pragma unroll
         for (int g = 0; g < N; ++g) {
-          ra[k][g].load(xr + k * rpp * tst + a + g * V);
-          rc[k][g].load(xr + k * rpp * tst + c + g * V);
+          ra[k][g].load(x + k * kst + g * V);
+          rc[k][g].load(x + k * kst + (c - a) + g * V);
         }
   };
-  fetch(x);
+  fetch();
   if (bad_page(p, w)) return;  // (the same for every thread)
   float was = w.lo > 0 ? p.scales[w.slot] : 0.f;
   const bool turn = half || (p.interleaved && a < rot);  // (R is a multiple of 16: a unit is rotated whole or not at all)
@@ -262,8 +301,11 @@ __global__ void __launch_bounds__(THREADS) append_kernel(const AppendParams p) {
       }
     }
   }
-  for (int i = 0; i < nh; ++i) {
-    float xa[K][8], xc[K][8], m = 0.f;
+  uint8_t* page = p.pages + w.slot * (int64_t(D) << p.lpage);
+  const int out = (w.lo + first) * D + a;  // of this thread's first row in a head's page
+  for (int i = 0; i < nh; ++i, page += D << p.lpage) {
+    float xa[K][8], xc[K][8];
+    uint32_t m = 0;  // the largest finite magnitude, as the bits of a float
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       if (first + k * rpp >= nrows) break;
@@ -272,60 +314,88 @@ __global__ void __launch_bounds__(THREADS) append_kernel(const AppendParams p) {
         ra[k][g].get(xa[k] + g * V);
         rc[k][g].get(xc[k] + g * V);
       }
-      if (turn) {
+      float mk = 0.f;
+      if (half) {  // (two branches: one with the operands chosen inside would select every register twice)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          float& x0 = half ? xa[k][e] : (e < 4 ? xa[k][(2 * e) & 7] : xc[k][(2 * e) & 7]);
-          float& x1 = half ? xc[k][e] : (e < 4 ? xa[k][(2 * e + 1) & 7] : xc[k][(2 * e + 1) & 7]);
-          const float y0 = x0 * z[k][e].x - x1 * z[k][e].y, y1 = x1 * z[k][e].x + x0 * z[k][e].y;
-          x0 = y0, x1 = y1;
+        for (int e = 0; e < 8; ++e) turn2(xa[k][e], xc[k][e], z[k][e]);
+      } else if (turn) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          turn2(xa[k][2 * e], xa[k][2 * e + 1], z[k][e]);
+          turn2(xc[k][2 * e], xc[k][2 * e + 1], z[k][e + 4]);
         }
       }
-      float mk = 0.f;
+      if (sizeof(T) == 4 || turn) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) mk = fmaxf(mk, fmaxf(fabsf(xa[k][e]), fabsf(xc[k][e])));  // (NaN is passed over)
+        for (int e = 0; e < 8; ++e) mk = fmaxf(mk, fmaxf(fabsf(xa[k][e]), fabsf(xc[k][e])));  // (NaN is passed over)
+      } else if constexpr (sizeof(T) == 2) {
+        using V2 = typename Pair<T>::V2;
+        const V2 *pa = reinterpret_cast<const V2*>(&ra[k][0].u), *pc = reinterpret_cast<const V2*>(&rc[k][0].u);
+        V2 m2 = __hmax2(__habs2(pa[0]), __habs2(pc[0]));
+#pragma unroll
+        for (int e = 1; e < 4; ++e) m2 = __hmax2(m2, __hmax2(__habs2(pa[e]), __habs2(pc[e])));
+        mk = fmaxf(fmaxf(to_f<T>(m2.x), to_f<T>(m2.y)), 0.f);
+      }
       if (mk == INFINITY) {  // rare: the largest of the finite
         mk = 0.f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) mk = fmaxf(mk, fmaxf(finite_abs(xa[k][e]), finite_abs(xc[k][e])));
       }
-      m = fmaxf(m, mk);
+      m = max(m, __float_as_uint(mk));
     }
+    m = __reduce_max_sync(0xffffffffu, m);
     const int64_t slot = w.slot + i;
     const float old = was;
+    uint4 keep_a[sizeof(T) == 2 ? K : 1], keep_c[sizeof(T) == 2 ? K : 1];  // the 16-bit words, for Pair<T>::enc4
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) keep_a[k] = ra[k][0].u, keep_c[k] = rc[k][0].u;
+    }
     if (i + 1 < nh) {
-      fetch(x + (i + 1) * hst);
+      x += hst;
+      fetch();
       if (w.lo > 0) was = p.scales[slot + 1];
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     if constexpr (WARPS > 1) {
-      float* r = red[i & 1];  // (the other half may still be read by warps behind)
+      uint32_t* r = red[i & 1];  // (the other half may still be read by warps behind)
       if ((threadIdx.x & 31) == 0) r[threadIdx.x >> 5] = m;
       __syncthreads();  // (every thread has read the old scale)
-      for (int q = 0; q < WARPS; ++q) m = fmaxf(m, r[q]);
+      if constexpr (WARPS == 2) {
+        m = max(r[0], r[1]);
+      } else {
+#pragma unroll
+        for (int q = 0; q < WARPS; q += 4) {
+          const uint4 v = *reinterpret_cast<const uint4*>(r + q);
+          m = max(max(m, max(v.x, v.y)), max(v.z, v.w));
+        }
+      }
     } else {
       __syncwarp();
     }
-    const float now = fmaxf(old, scale_of(m)), inv = scale_inv(now);
+    const float now = fmaxf(old, scale_of(__uint_as_float(m))), inv = scale_inv(now);
     if (threadIdx.x == 0) p.scales[slot] = now;
-    uint8_t* dst = p.pages + slot * (int64_t(D) << p.lpage);
-    rescale_held<THREADS>(dst, w.lo * D, old, now, inv);
+    rescale_held<THREADS>(page, w.lo * D, old, now, inv);
+    uint8_t* d = page + out;
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int r = first + k * rpp;
-      if (r >= nrows) break;
-      uint8_t* d = dst + (w.lo + r) * D;
-      auto enc8 = [&](const float* f) {
-        return make_uint2(enc4(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv),
-                          enc4(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv));
-      };
-      const uint2 ya = enc8(xa[k]), yc = enc8(xc[k]);
-      if (half) {
-        *reinterpret_cast<uint2*>(d + a) = ya;
-        *reinterpret_cast<uint2*>(d + c) = yc;
+    for (int k = 0; k < K; ++k, d += rpp * D) {
+      if (first + k * rpp >= nrows) break;
+      uint2 ya, yc;
+      if (sizeof(T) == 2 && !turn && Pair<typename std::conditional<sizeof(T) == 2, T, __half>::type>::direct(inv)) {
+        using P = Pair<typename std::conditional<sizeof(T) == 2, T, __half>::type>;
+        ya = make_uint2(P::enc4(keep_a[k].x, keep_a[k].y, inv), P::enc4(keep_a[k].z, keep_a[k].w, inv));
+        yc = make_uint2(P::enc4(keep_c[k].x, keep_c[k].y, inv), P::enc4(keep_c[k].z, keep_c[k].w, inv));
       } else {
-        *reinterpret_cast<uint4*>(d + a) = make_uint4(ya.x, ya.y, yc.x, yc.y);
+        auto enc8 = [&](const float* f) {
+          return make_uint2(enc4(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv),
+                            enc4(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv));
+        };
+        ya = enc8(xa[k]), yc = enc8(xc[k]);
+      }
+      if (half) {
+        *reinterpret_cast<uint2*>(d) = ya;
+        *reinterpret_cast<uint2*>(d + (c - a)) = yc;
+      } else {
+        *reinterpret_cast<uint4*>(d) = make_uint4(ya.x, ya.y, yc.x, yc.y);
       }
     }
   }

@@ -1562,7 +1562,9 @@ static int kv8_append_run(kv8::AppendParams& p, bool wide, int64_t blocks, cudaS
   cfg.numAttrs = 1;
   auto go = [&](auto kern, int threads) {
     cfg.blockDim = dim3(unsigned(threads));
-    cfg.gridDim = dim3(unsigned(blocks), unsigned(2 * ((p.Hkv + p.hpb - 1) / p.hpb)));
+    const int64_t grid = blocks * 2 * ((p.Hkv + p.hpb - 1) / p.hpb);
+    LB2_CHECK_ARG(grid < (int64_t(1) << 31), "kv8_append: too many rows and heads");
+    cfg.gridDim = dim3(static_cast<unsigned>(grid));
     LB2_CUDA(cudaLaunchKernelEx(&cfg, kern, p));
     return int(LB2_OK);
   };
