@@ -105,6 +105,7 @@ __global__ void __launch_bounds__(128) paged_kernel(const PagedParams p) {
   const T* q = static_cast<const T*>(p.q) + b * p.q_st[0] + h * p.q_st[1] + t * p.q_st[2] + d0;
   T* o = static_cast<T*>(p.o) + b * p.o_st[0] + h * p.o_st[1] + t * p.o_st[2] + d0;
   const int len = int(min(int64_t(max(p.kv_len[b], 0)), int64_t(p.max_pages) * p.page));
+  if (len != p.kv_len[b] && d0 == 0) report_bad_index(111);
   PagedKeys<E> keys{p.pages, p.scales, p.table + b * p.table_st, p.Hkv, h / (p.Hq / p.Hkv), p.page, p.num_pages, d0};
   float x[E];
 #pragma unroll

@@ -39,7 +39,7 @@ namespace kv8attn {
 
 constexpr int BK = 64;       // keys a tile
 constexpr int MAX_B = 1024;  // sequences a launch (the prefix table in shared memory); larger batches go in several
-constexpr int STATUS = 112;  // where (lb2_status): 112 page id, 113.. waits
+constexpr int STATUS = 112;  // where (lb2_status): 112 a page id or length, 113.. waits
 
 // NT: 8-row tiles of query rows a warp; MK: 16-key blocks of a tile a warp (two give it two independent chains of
 // products); RG: row groups (sets of warps taking the same tile for other rows); KG: key groups (sets of warps taking
@@ -214,6 +214,7 @@ __global__ void __launch_bounds__(Cfg<D, NT, RG, MK, KG>::THREADS, 1)
   asm volatile("griddepcontrol.wait;" ::: "memory");
   for (int b = threadIdx.x; b < p.a.B; b += C::THREADS) {
     const int len = seq_len(p, b);
+    if (len != p.a.kv_len[b] && blockIdx.x == 0) report_bad_index(STATUS);
     lens[b] = len;
     prefix[b + 1] = (len + BK - 1) / BK;
   }

@@ -1,6 +1,7 @@
 // larder_b200: the C-ABI library. One translation unit (so the device status word is one symbol) that includes
 // every kernel header and implements the entry points declared in include/larder_b200.h.
 #include <algorithm>
+#include <cmath>
 #include <cstring>
 #include <initializer_list>
 #include <mutex>
@@ -1773,6 +1774,7 @@ int lb2_kv8_attend(const void* q, const int64_t* q_st, const uint8_t* pages, con
   const int rc = kv8_shape(B, Hkv, T, D, page, num_pages, max_pages, "kv8_attend");
   if (rc) return rc;
   LB2_CHECK_ARG(Hq > 0 && Hq % Hkv == 0, "kv8_attend: Hq must be a multiple of Hkv");
+  LB2_CHECK_ARG(std::isfinite(scale), "kv8_attend: the scale must be finite");
   LB2_CHECK_ARG(dtype == LB2_F32 || dtype == LB2_BF16 || dtype == LB2_F16, "kv8_attend: dtype");
   if (B == 0 || T == 0) return LB2_OK;
   LB2_CHECK_ARG(q && q_st && pages && scales && table && kv_len && o && o_st, "kv8_attend: missing argument");
@@ -1981,6 +1983,7 @@ int lb2_attn_packed(const void* q, const int64_t* q_st, const void* k, const int
   LB2_CHECK_ARG(S >= 1 && Hq > 0 && Hkv > 0 && T >= 0, "attn_packed: shape");
   LB2_CHECK_ARG(Hq % Hkv == 0, "attn_packed: Hq must be a multiple of Hkv");
   LB2_CHECK_ARG(D == 64 || D == 128 || D == 256, "attn_packed: head dim must be 64, 128 or 256");
+  LB2_CHECK_ARG(scale > 0.f && scale < INFINITY, "attn_packed: the scale must be positive and finite");
   LB2_CHECK_ARG(dtype == LB2_F32 || dtype == LB2_BF16 || dtype == LB2_F16, "attn_packed: dtype");
   if (T == 0) return LB2_OK;
   LB2_CHECK_ARG(q && k && v && o && q_st && k_st && v_st && o_st && cu, "attn_packed: missing argument");

@@ -340,6 +340,30 @@ def test_attend_bad_page_is_reported():
     assert ops.status() != 0 and ops.status() == 0
 
 
+def test_attend_lengths_out_of_range_are_reported():
+    pages, scales, table = filled([50, 30], 1, 16, 64)
+    for dt in (BF, F):
+        q = torch.randn(2, 2, 1, 64, generator=torch.Generator().manual_seed(1)).to(dt).cuda()
+        o = ops.kv8_attend(q, pages, scales, table, i32([50, -3]), 0.1)
+        assert ops.status() != 0 and ops.status() == 0
+        assert (o[1] == 0).all()
+        ops.kv8_attend(q, pages, scales, table[:1].repeat(2, 1), i32([50, 65]), 0.1)
+        assert ops.status() != 0
+        check_attend(ops.kv8_attend(q, pages, scales, table, i32([50, 30]), 0.1), q, pages, scales, table, [50, 30], 0.1)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.07])
+def test_attend_any_scale(scale):
+    pages, scales, table = filled([90], 1, 16, 128)
+    q = torch.randn(1, 4, 2, 128, generator=torch.Generator().manual_seed(1)).to(BF).cuda()
+    check_attend(ops.kv8_attend(q, pages, scales, table, i32([90]), scale), q, pages, scales, table, [90], scale)
+
+
+def test_attend_more_sequences_than_a_launch_takes():
+    lens = [(i * 7) % 19 for i in range(1500)]
+    run_attend(lens, 2, 1, 1, 16, 64, BF)
+
+
 def test_attend_on_two_streams():
     pages, scales, table = filled([3000, 2000], 2, 16, 128)
     q = torch.randn(2, 8, 1, 128, device="cuda").to(BF)
@@ -386,7 +410,7 @@ def test_refused():
                 lambda: at(q, pages[:, :, :, :8], scales, table, n, 0.1), lambda: at(q, pages, scales, table.long(), n, 0.1),
                 lambda: at(q, pages, scales, table, n[:1], 0.1), lambda: at(q.cpu(), pages, scales, table, n, 0.1),
                 lambda: at(q, pages[:, :, :, :8].contiguous(), scales, table, n, 0.1),
-                lambda: at(q.double(), pages, scales, table, n, 0.1),
+                lambda: at(q.double(), pages, scales, table, n, 0.1), lambda: at(q, pages, scales, table, n, float("nan")),
                 lambda: ap(pages, scales, k, k[:, :1], table, n), lambda: ap(pages, scales, k, k.half(), table, n),
                 lambda: ap(pages, scales, k, k, table[:1], n), lambda: ap(pages, scales, k, k, table, n.long()),
                 lambda: ap(pages, scales, k, k, table, n, lens=n, cu=i32([0, 1, 2])),

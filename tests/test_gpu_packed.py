@@ -46,7 +46,7 @@ LENS = [[1], [5, 1, 3], [128], [129, 127], [256, 256], [257], [0, 40, 0, 0, 300,
 
 
 @pytest.mark.parametrize("dtype", [BF, HF, F])
-@pytest.mark.parametrize("D,Hq,Hkv", [(64, 4, 4), (128, 8, 2), (256, 6, 2)])
+@pytest.mark.parametrize("D,Hq,Hkv", [(64, 4, 4), (128, 8, 2), (256, 6, 2), (128, 7, 1), (64, 65, 1), (256, 16, 1)])
 @pytest.mark.parametrize("lens", LENS, ids=str)
 def test_packed(dtype, D, Hq, Hkv, lens):
     q, k, v = inputs(lens, Hq, Hkv, D, dtype)
@@ -59,6 +59,38 @@ def test_many_prompts(D):
     lens = [(i * 37) % 61 for i in range(200)]
     q, k, v = inputs(lens, 2, 1, D, BF)
     check(ops.attn_packed(q, k, v, 0.3, cu_of(lens)), q, k, v, lens, 0.3)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("D,Hq,Hkv", [(128, 2, 1), (256, 2, 1), (256, 3, 3)])
+def test_long_prompts(D, Hq, Hkv, dtype):
+    """Prompts long enough on average for every form of the kernels, short ones among them."""
+    lens = [4001, 7, 0, 9000, 130]
+    q, k, v = inputs(lens, Hq, Hkv, D, dtype)
+    check(ops.attn_packed(q, k, v, D ** -0.5, cu_of(lens)), q, k, v, lens, D ** -0.5)
+    lens = [6500, 0, 200, 5400]
+    q, k, v = inputs(lens, Hq, Hkv, D, dtype, seed=1, pad=300)
+    out = torch.full_like(q, 9.0)
+    check(ops.attn_packed(q, k, v, D ** -0.5, cu_of(lens), out=out), q, k, v, lens, D ** -0.5)
+    assert (out[:, :, 12100:] == 0).all()
+    v[0, 0, 6500 + 111, 3] = float("nan")  # reaches the later rows of its own prompt
+    o = ops.attn_packed(q, k, v, D ** -0.5, cu_of(lens))
+    bad = torch.zeros_like(o, dtype=torch.bool)
+    bad[0, :Hq // Hkv, 6500 + 111:6700, 3] = True
+    assert torch.equal(torch.isnan(o), bad)
+    assert ((o - out).abs()[~bad].double() <= 6 * ref.UNIT[dtype] * v.nan_to_num(0).abs().max()).all()
+
+
+def test_wrong_bounds_stay_inside():
+    """Bounds that fall or leave the rows are clamped: nothing outside the tensors is touched, whatever comes out."""
+    q, k, v = inputs([300], 4, 2, 128, BF)
+    wide = torch.full((1, 310, 4, 128), 5.0, dtype=BF, device="cuda")
+    out = wide[:, 5:305].transpose(1, 2)
+    for cu in ([0, 200, 100, 300], [-50, 20, 5000], [300, 0], [0, 1 << 30]):
+        for f, a in ((BF, (q, k, v)), (F, (q.float(), k.float(), v.float()))):
+            o = ops.attn_packed(*a, 0.1, torch.tensor(cu, dtype=torch.int32).cuda(), out=out if f is BF else None)
+            torch.cuda.synchronize()
+    assert (wide[:, :5] == 5).all() and (wide[:, 305:] == 5).all() and ops.status() == 0
 
 
 @pytest.mark.parametrize("dtype", [BF, F])
@@ -135,6 +167,7 @@ def test_refused():
                 lambda: f(q, k, v, 1.0, cu.long()), lambda: f(q, k, v, 1.0, cu[:1]), lambda: f(q[0], k, v, 1.0, cu),
                 lambda: f(q[..., :96], k[..., :96], v[..., :96], 1.0, cu), lambda: f(q[:, :, :4], k, v, 1.0, cu),
                 lambda: f(q.cpu(), k, v, 1.0, cu), lambda: f(q, k, v, 1.0, cu, out=torch.empty(1, 4, 8, 64, device="cuda")),
+                lambda: f(q, k, v, 0.0, cu), lambda: f(q, k, v, -1.0, cu), lambda: f(q, k, v, float("nan"), cu),
                 lambda: f(q.transpose(2, 3), k, v, 1.0, cu), lambda: f(q.double(), k.double(), v.double(), 1.0, cu)):
         with pytest.raises(ValueError):
             bad()
