@@ -14,7 +14,7 @@
 namespace lb2 {
 namespace packed {
 
-constexpr int THREADS = 1024;
+constexpr int THREADS = 256;
 
 struct PlanParams {
   const int32_t* cu;
@@ -47,7 +47,7 @@ __global__ void __launch_bounds__(THREADS) plan_kernel(const PlanParams p) {
     if (lane == 31) s_w[warp] = x;
     __syncthreads();
     int pre = carry, all = carry;
-    for (int w = 0; w < 32; ++w) {
+    for (int w = 0; w < THREADS / 32; ++w) {
       if (w < warp) pre = max(pre, s_w[w]);
       all = max(all, s_w[w]);
     }
@@ -62,7 +62,7 @@ __global__ void __launch_bounds__(THREADS) plan_kernel(const PlanParams p) {
   atomicMax(&s_max, mx);
   __syncthreads();
   const int M = s_max;  // m runs over 0 .. M - 1
-  for (int m = warp; m < M; m += 32) {
+  for (int m = warp; m < M; m += THREADS / 32) {
     int c = 0;
     for (int s0 = 0; s0 <= p.S; s0 += 32) {
       const int s = s0 + lane;
@@ -85,7 +85,7 @@ __global__ void __launch_bounds__(THREADS) plan_kernel(const PlanParams p) {
     if (lane == 31) s_w[warp] = x;
     __syncthreads();
     int pre = run, all = run;
-    for (int w = 0; w < 32; ++w) {
+    for (int w = 0; w < THREADS / 32; ++w) {
       if (w < warp) pre += s_w[w];
       all += s_w[w];
     }
@@ -93,7 +93,7 @@ __global__ void __launch_bounds__(THREADS) plan_kernel(const PlanParams p) {
     run = all;
     __syncthreads();
   }
-  for (int m = warp; m < M; m += 32) {
+  for (int m = warp; m < M; m += THREADS / 32) {
     int c = cnt[m];
     for (int s0 = 0; s0 <= p.S; s0 += 32) {
       const int s = s0 + lane;

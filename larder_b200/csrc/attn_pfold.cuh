@@ -57,6 +57,12 @@ __device__ __forceinline__ void st_global32(void* p, const uint32_t* w) {
                : "memory");
 }
 
+// Item (block, heads) r of CTA c of n: the heaviest-first list dealt in a snake, so that the CTAs' totals even out.
+__device__ __forceinline__ int item_at(int r) {
+  const int n = gridDim.x, c = blockIdx.x;
+  return r * n + ((r & 1) ? n - 1 - c : c);
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(THREADS, Cfg<D>::CTAS) pfold_kernel(const __grid_constant__ CUtensorMap qmap,
                                                                       const __grid_constant__ CUtensorMap kmap,
@@ -133,7 +139,8 @@ __global__ void __launch_bounds__(THREADS, Cfg<D>::CTAS) pfold_kernel(const __gr
       const int off = lane == 0 ? C::K_OFF : C::V_OFF;
       int jg = 0, qi = 0, q_issued = -1;
       bool stop = false;
-      for (int it = blockIdx.x; it < total && !stop; it += gridDim.x) {
+      for (int r = 0, it; r * int(gridDim.x) < total && !stop; ++r) {
+        if ((it = item_at(r)) >= total) continue;
         const int4 blk = p.pk[it / heads];
         const int h = it % heads * F, hk = h / p.G;
         if (blk.w == 0) continue;
@@ -172,7 +179,8 @@ __global__ void __launch_bounds__(THREADS, Cfg<D>::CTAS) pfold_kernel(const __gr
       const uint32_t q_addr = smem_u32(sm + C::Q_OFF);
       bool ok = true;
       int js_g = 0, jp_g = 0, qi = 0;  // S and PV tiles issued; blocks with keys so far
-      for (int it = blockIdx.x; ok && it < total; it += gridDim.x) {
+      for (int r = 0, it; ok && r * int(gridDim.x) < total; ++r) {
+        if ((it = item_at(r)) >= total) continue;
         const int nt = p.pk[it / heads].w;
         if (nt == 0) continue;
         ok = mbar_wait(q_full, qi & 1, 126);
@@ -252,7 +260,8 @@ __global__ void __launch_bounds__(THREADS, Cfg<D>::CTAS) pfold_kernel(const __gr
     const int tok = r / F, head = r - tok * F;  // the row's token in the block, and head
     bool ok = true;
     int jg = 0;
-    for (int it = blockIdx.x; ok && it < total; it += gridDim.x) {
+    for (int rr = 0, it; ok && rr * int(gridDim.x) < total; ++rr) {
+      if ((it = item_at(rr)) >= total) continue;
       const int4 blk = p.pk[it / heads];
       const int h = it % heads * F + head, nt = blk.w;
       const int row = blk.z * tpb + tok;  // in its prompt
