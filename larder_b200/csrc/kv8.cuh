@@ -212,19 +212,68 @@ __device__ __forceinline__ float2 turn_cs_fast(uint32_t frac) {
   return make_float2(__cosf(a), __sinf(a));
 }
 
-__device__ __forceinline__ void turn2(float& x0, float& x1, float2 z) {
-  const float y0 = x0 * z.x - x1 * z.y, y1 = x1 * z.x + x0 * z.y;
-  x0 = y0, x1 = y1;
+// Two fp32 products, or products and sums, in one instruction.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\tfma.rn.f32x2 w, x, y, z;\n\t"
+      "mov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
 }
 
-// Two 16-bit values a word: the larger magnitudes, and four codes of two words scaled by a power of two.
+// The largest magnitude of three (NaN is passed over).
+__device__ __forceinline__ float max3_abs(float a, float b, float c) {
+  float r;
+  asm("max.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// The largest finite magnitude of M loads of V values.
+template <typename T, int V, int M>
+__device__ __forceinline__ float max_raw(const rope::Raw<T, V>* r) {
+  float mk = 0.f;
+  if constexpr (sizeof(T) == 2) {  // two values an instruction (NaN is passed over)
+    using V2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+    const V2* h = reinterpret_cast<const V2*>(r);
+    V2 m2 = __habs2(h[0]);
+#pragma unroll
+    for (int e = 1; e < 4 * M; ++e) m2 = __hmax2(m2, __habs2(h[e]));
+    mk = fmaxf(fmaxf(to_f<T>(m2.x), to_f<T>(m2.y)), 0.f);
+  } else {
+    const float* f = reinterpret_cast<const float*>(r);
+#pragma unroll
+    for (int e = 0; e < V * M; e += 2) mk = max3_abs(mk, f[e], f[e + 1]);
+  }
+  if (mk == INFINITY) {  // rare
+    mk = 0.f;
+#pragma unroll
+    for (int g = 0; g < M; ++g) {
+      float f[V];
+      r[g].get(f);
+#pragma unroll
+      for (int e = 0; e < V; ++e) mk = fmaxf(mk, finite_abs(f[e]));
+    }
+  }
+  return mk;
+}
+
+// Four codes straight from two words of 16-bit pairs. f16: x 2^k is exact in f16 (|x 2^k| <= 448; what falls under 2^-14
+// rounds to code 0 either way) unless 2^k itself leaves f16's range.
 template <typename T>
-struct Pair;
+struct Pair {
+  static __device__ __forceinline__ bool direct(float) { return false; }
+  static __device__ __forceinline__ uint32_t enc4(uint32_t, uint32_t, float) { return 0; }
+};
 template <>
 struct Pair<__half> {
-  using V2 = __half2;
-  // f16 codes come from f16 pairs: x 2^k is exact in f16 (|x 2^k| <= 448; what falls under 2^-14 rounds to code 0 either
-  // way), unless 2^k itself leaves f16's range
   static __device__ __forceinline__ bool direct(float inv) { return inv >= 0x1p-14f && inv <= 0x1p15f; }
   static __device__ __forceinline__ uint32_t enc4(uint32_t a, uint32_t b, float inv) {
     const __half2 k = __float2half2_rn(inv);
@@ -239,123 +288,118 @@ struct Pair<__half> {
     return r;
   }
 };
-template <>
-struct Pair<__nv_bfloat16> {
-  using V2 = __nv_bfloat162;
-  static __device__ __forceinline__ bool direct(float) { return false; }
-  static __device__ __forceinline__ uint32_t enc4(uint32_t, uint32_t, float) { return 0; }
-};
 
 // Rows of 16-byte groups: the page's new rows are held in registers, read once. A unit is two groups of 8 elements: in
 // the rotated half layout a group and its partners R / 2 on, elsewhere neighbours; a thread has one unit of K rows. The
-// block takes `hpb` heads in turn, the next one's loads in flight while it works: the angles of its rows serve them all.
-// Bound by HBM for long prompts (2 bytes read and 1 written a value), by the chain start -> table -> scale for single
-// tokens.
-template <typename T, int THREADS, int K>
-__global__ void __launch_bounds__(THREADS) append_kernel(const AppendParams p) {
+// block takes `hpb` heads in turn, the next one's loads in flight while it works: the angles of its rows serve them all
+// (in shared memory, each thread its own).
+// Bound for long prompts by instruction issue and HBM alike: 2 x 16384 tokens of 8 heads x 128 (f16) take 47 us, 4250 GB/s of
+// the 2 bytes read and 1 written a value; the same loads and stores without rotation and conversion take 35 us. Two
+// products an instruction (f32x2) and word-wise maxima keep a value of V at about 4 instructions, one of K at 7. Single
+// tokens are bound by the chain start -> table -> scale (64 sequences: 3 us).
+template <typename T, int THREADS, int K, int OCC = THREADS == 256 ? 3 : 1>
+__global__ void __launch_bounds__(THREADS, OCC) append_kernel(const AppendParams p) {
   constexpr int WARPS = THREADS / 32;
   constexpr int V = 16 / int(sizeof(T)), N = 8 / V;  // values a load, loads a group
+  extern __shared__ __align__(16) float4 zsm[];  // [4 K][THREADS]: each thread's angles, two cosines and their sines a word
   __shared__ __align__(16) uint32_t red[2][WARPS < 4 ? 4 : WARPS];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   Piece w;
   if (!piece_of(p, w)) return;
   const int D = p.D, u = threadIdx.x & ((1 << p.lupr) - 1), first = threadIdx.x >> p.lupr;
-  const int rpp = THREADS >> p.lupr, nrows = w.hi - w.lo;
+  const int rpp = THREADS >> p.lupr;
+  const int mine = (w.hi - w.lo - first + rpp - 1) / rpp;  // rows of this thread (a unit each; <= 0 for none)
   const int rot = w.kind == 0 ? p.R : 0, R2 = rot >> 1;
   const bool half = !p.interleaved && u * 8 < R2;
   const int a = half ? u * 8 : u * 16, c = half ? a + R2 : a + 8;
+  const bool turn = half || (p.interleaved && a < rot);  // (R is a multiple of 16: a unit is rotated whole or not at all)
   const int64_t hst = p.st[w.kind][1], tst = p.st[w.kind][2];
   const T* x = static_cast<const T*>(p.x[w.kind]) + (p.cu ? 0 : w.b * p.st[w.kind][0]) + w.h * hst +
                (w.row0 + first) * tst + a;  // this thread's first row
   const int64_t kst = rpp * tst;
   const int nh = min(p.hpb, p.Hkv - w.h);
-  rope::Raw<T, V> ra[K][N], rc[K][N];
+  rope::Raw<T, V> next[K][2 * N];
   auto fetch = [&] {
 #pragma unroll
     for (int k = 0; k < K; ++k)
-      if (first + k * rpp < nrows)
+      if (k < mine)
 #pragma unroll
         for (int g = 0; g < N; ++g) {
-          ra[k][g].load(x + k * kst + g * V);
-          rc[k][g].load(x + k * kst + (c - a) + g * V);
+          next[k][g].load(x + k * kst + g * V);
+          next[k][N + g].load(x + k * kst + (c - a) + g * V);
         }
   };
   fetch();
   if (bad_page(p, w)) return;  // (the same for every thread)
   float was = w.lo > 0 ? p.scales[w.slot] : 0.f;
-  const bool turn = half || (p.interleaved && a < rot);  // (R is a multiple of 16: a unit is rotated whole or not at all)
-  float2 z[K][8];
+  float4* zt = zsm + threadIdx.x;
   if (turn) {
     uint64_t f[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) f[e] = p.turns[half ? a + e : (a >> 1) + e];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      if (first + k * rpp >= nrows) break;
+      if (k >= mine) break;
       const uint32_t pos = uint32_t(w.base + w.lo + first + k * rpp);  // (below 2^31)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        z[k][e] = turn_cs_fast(uint32_t((pos * f[e]) >> 32));
-        z[k][e].x *= p.amp, z[k][e].y *= p.amp;
+      for (int e = 0; e < 4; ++e) {
+        const float2 a = turn_cs_fast(uint32_t((pos * f[2 * e]) >> 32)), b = turn_cs_fast(uint32_t((pos * f[2 * e + 1]) >> 32));
+        zt[(k * 4 + e) * THREADS] = make_float4(a.x * p.amp, b.x * p.amp, a.y * p.amp, b.y * p.amp);
       }
     }
   }
   uint8_t* page = p.pages + w.slot * (int64_t(D) << p.lpage);
-  const int out = (w.lo + first) * D + a;  // of this thread's first row in a head's page
-  for (int i = 0; i < nh; ++i, page += D << p.lpage) {
-    float xa[K][8], xc[K][8];
-    uint32_t m = 0;  // the largest finite magnitude, as the bits of a float
+  uint8_t* out = page + (w.lo + first) * D + a;  // this thread's first row
+  const int page_bytes = D << p.lpage, held = w.lo * D;
+  for (int i = 0; i < nh; ++i, page += page_bytes, out += page_bytes) {
+    rope::Raw<T, V> raw[K][2 * N];  // the rows as they lie: what a unit that is not rotated is encoded from
+    float2 y[K][8];                 // or rotated: the unit's two groups, two values a word
+    uint32_t m = 0;                 // the largest finite magnitude, as the bits of a float
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      if (first + k * rpp >= nrows) break;
+      if (k >= mine) break;
 #pragma unroll
-      for (int g = 0; g < N; ++g) {
-        ra[k][g].get(xa[k] + g * V);
-        rc[k][g].get(xc[k] + g * V);
-      }
+      for (int g = 0; g < 2 * N; ++g) raw[k][g] = next[k][g];
       float mk = 0.f;
-      if (half) {  // (two branches: one with the operands chosen inside would select every register twice)
+      if (turn) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) turn2(xa[k][e], xc[k][e], z[k][e]);
-      } else if (turn) {
+        for (int g = 0; g < 2 * N; ++g) raw[k][g].get(reinterpret_cast<float*>(y[k]) + g * V);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          turn2(xa[k][2 * e], xa[k][2 * e + 1], z[k][e]);
-          turn2(xc[k][2 * e], xc[k][2 * e + 1], z[k][e + 4]);
+          const float4 z = zt[(k * 4 + e) * THREADS];
+          const float2 co = make_float2(z.x, z.y), si = make_float2(z.z, z.w), ns = make_float2(-z.z, -z.w);
+          if (half) {  // partners in two words
+            const float2 x0 = y[k][e], x1 = y[k][4 + e];
+            y[k][e] = fma2(x1, ns, mul2(x0, co));
+            y[k][4 + e] = fma2(x0, si, mul2(x1, co));
+          } else {  // a pair a word: two words a step
+            const float2 p0 = y[k][2 * e], p1 = y[k][2 * e + 1];
+            const float2 x0 = make_float2(p0.x, p1.x), x1 = make_float2(p0.y, p1.y);
+            const float2 y0 = fma2(x1, ns, mul2(x0, co)), y1 = fma2(x0, si, mul2(x1, co));
+            y[k][2 * e] = make_float2(y0.x, y1.x);
+            y[k][2 * e + 1] = make_float2(y0.y, y1.y);
+          }
         }
-      }
-      if (sizeof(T) == 4 || turn) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) mk = fmaxf(mk, fmaxf(fabsf(xa[k][e]), fabsf(xc[k][e])));  // (NaN is passed over)
-      } else if constexpr (sizeof(T) == 2) {
-        using V2 = typename Pair<T>::V2;
-        const V2 *pa = reinterpret_cast<const V2*>(&ra[k][0].u), *pc = reinterpret_cast<const V2*>(&rc[k][0].u);
-        V2 m2 = __hmax2(__habs2(pa[0]), __habs2(pc[0]));
+        for (int e = 0; e < 8; ++e) mk = max3_abs(mk, y[k][e].x, y[k][e].y);
+        if (mk == INFINITY) {  // rare: the largest of the finite
+          mk = 0.f;
 #pragma unroll
-        for (int e = 1; e < 4; ++e) m2 = __hmax2(m2, __hmax2(__habs2(pa[e]), __habs2(pc[e])));
-        mk = fmaxf(fmaxf(to_f<T>(m2.x), to_f<T>(m2.y)), 0.f);
-      }
-      if (mk == INFINITY) {  // rare: the largest of the finite
-        mk = 0.f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) mk = fmaxf(mk, fmaxf(finite_abs(xa[k][e]), finite_abs(xc[k][e])));
+          for (int e = 0; e < 8; ++e) mk = fmaxf(mk, fmaxf(finite_abs(y[k][e].x), finite_abs(y[k][e].y)));
+        }
+      } else {
+        mk = max_raw<T, V, 2 * N>(raw[k]);
       }
       m = max(m, __float_as_uint(mk));
     }
-    m = __reduce_max_sync(0xffffffffu, m);
-    const int64_t slot = w.slot + i;
     const float old = was;
-    uint4 keep_a[sizeof(T) == 2 ? K : 1], keep_c[sizeof(T) == 2 ? K : 1];  // the 16-bit words, for Pair<T>::enc4
-    if constexpr (sizeof(T) == 2) {
-#pragma unroll
-      for (int k = 0; k < K; ++k) keep_a[k] = ra[k][0].u, keep_c[k] = rc[k][0].u;
-    }
     if (i + 1 < nh) {
       x += hst;
       fetch();
-      if (w.lo > 0) was = p.scales[slot + 1];
+      if (w.lo > 0) was = p.scales[w.slot + i + 1];
     }
+    m = __reduce_max_sync(0xffffffffu, m);
     if constexpr (WARPS > 1) {
       uint32_t* r = red[i & 1];  // (the other half may still be read by warps behind)
       if ((threadIdx.x & 31) == 0) r[threadIdx.x >> 5] = m;
@@ -373,29 +417,37 @@ __global__ void __launch_bounds__(THREADS) append_kernel(const AppendParams p) {
       __syncwarp();
     }
     const float now = fmaxf(old, scale_of(__uint_as_float(m))), inv = scale_inv(now);
-    if (threadIdx.x == 0) p.scales[slot] = now;
-    rescale_held<THREADS>(page, w.lo * D, old, now, inv);
-    uint8_t* d = page + out;
+    if (threadIdx.x == 0) p.scales[w.slot + i] = now;
+    if (held) rescale_held<THREADS>(page, held, old, now, inv);
+    const float2 i2 = make_float2(inv, inv);
+    const bool words = sizeof(T) == 2 && !turn && Pair<T>::direct(inv);
 #pragma unroll
-    for (int k = 0; k < K; ++k, d += rpp * D) {
-      if (first + k * rpp >= nrows) break;
-      uint2 ya, yc;
-      if (sizeof(T) == 2 && !turn && Pair<typename std::conditional<sizeof(T) == 2, T, __half>::type>::direct(inv)) {
-        using P = Pair<typename std::conditional<sizeof(T) == 2, T, __half>::type>;
-        ya = make_uint2(P::enc4(keep_a[k].x, keep_a[k].y, inv), P::enc4(keep_a[k].z, keep_a[k].w, inv));
-        yc = make_uint2(P::enc4(keep_c[k].x, keep_c[k].y, inv), P::enc4(keep_c[k].z, keep_c[k].w, inv));
+    for (int k = 0; k < K; ++k) {
+      if (k >= mine) break;
+      uint32_t code[4];
+      if (words) {
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          const uint4 v = raw[k][g * N].u;
+          code[2 * g] = Pair<T>::enc4(v.x, v.y, inv);
+          code[2 * g + 1] = Pair<T>::enc4(v.z, v.w, inv);
+        }
       } else {
-        auto enc8 = [&](const float* f) {
-          return make_uint2(enc4(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv),
-                            enc4(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv));
-        };
-        ya = enc8(xa[k]), yc = enc8(xc[k]);
+        if (!turn)
+#pragma unroll
+          for (int g = 0; g < 2 * N; ++g) raw[k][g].get(reinterpret_cast<float*>(y[k]) + g * V);
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const float2 s = mul2(y[k][2 * g], i2), t = mul2(y[k][2 * g + 1], i2);
+          code[g] = enc4(s.x, s.y, t.x, t.y);
+        }
       }
+      uint8_t* d = out + k * rpp * D;
       if (half) {
-        *reinterpret_cast<uint2*>(d) = ya;
-        *reinterpret_cast<uint2*>(d + (c - a)) = yc;
+        *reinterpret_cast<uint2*>(d) = make_uint2(code[0], code[1]);
+        *reinterpret_cast<uint2*>(d + (c - a)) = make_uint2(code[2], code[3]);
       } else {
-        *reinterpret_cast<uint4*>(d) = make_uint4(ya.x, ya.y, yc.x, yc.y);
+        *reinterpret_cast<uint4*>(d) = make_uint4(code[0], code[1], code[2], code[3]);
       }
     }
   }
