@@ -6,7 +6,9 @@ the reference's module surface so its callers pick them up as a drop-in:
   chunkattn  -- chunked / wide-cut causal prefill attention and the patched scaled_dot_product_attention
   foldattn   -- folded GQA multi-row (verify) attention on the split-KV decode kernel
   gdn_cuda   -- the Gated-DeltaNet recurrence (chunked prefill and recurrent decode) and gated_delta_update
-  ops        -- the torch-level wrappers of every C-ABI entry point
+  rope       -- rotary positions: frequencies, long-context scalings, both pair layouts, the gradient
+  kv8        -- a paged 8-bit KV cache: pages handed out to sequences, append, attention
+  ops        -- the torch-level wrappers of every C-ABI entry point (attn_packed: prompts packed on one row axis)
   sharded    -- multi-GPU: sequence-sharded prefill, KV-range-sharded decode merged over NCCL
 """
 from . import _lib, ops  # noqa: F401

@@ -204,14 +204,6 @@ __global__ void __launch_bounds__(128) append_any_kernel(const AppendParams p) {
         enc4(value(i) * inv, value(i + 1) * inv, value(i + 2) * inv, value(i + 3) * inv);
 }
 
-// (cos, sin) of frac 2^-32 turns by the multi-function unit: the angle is within pi 2^-23 of the fraction's, the unit
-// within 2^-21 of its sine and cosine; the code that the key becomes has 4 significant bits.
-__device__ __forceinline__ float2 turn_cs_fast(uint32_t frac) {
-  const float t = __uint_as_float(0x3f800000u | ((frac ^ 0x80000000u) >> 9)) - 1.5f;  // turns, in [-1/2, 1/2)
-  const float a = t * 6.2831853071795865f;
-  return make_float2(__cosf(a), __sinf(a));
-}
-
 // Two fp32 products, or products and sums, in one instruction.
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
   float2 r;
@@ -293,7 +285,7 @@ struct Pair<__half> {
 // the rotated half layout a group and its partners R / 2 on, elsewhere neighbours; a thread has one unit of K rows. The
 // block takes `hpb` heads in turn, the next one's loads in flight while it works: the angles of its rows serve them all
 // (in shared memory, each thread its own).
-// Bound for long prompts by instruction issue and HBM alike: 2 x 16384 tokens of 8 heads x 128 (f16) take 47 us, 4250 GB/s of
+// Bound for long prompts by instruction issue and HBM alike: 2 x 16384 tokens of 8 heads x 128 (f16) take 50 us, 4050 GB/s of
 // the 2 bytes read and 1 written a value; the same loads and stores without rotation and conversion take 35 us. Two
 // products an instruction (f32x2) and word-wise maxima keep a value of V at about 4 instructions, one of K at 7. Single
 // tokens are bound by the chain start -> table -> scale (64 sequences: 3 us).
@@ -341,10 +333,10 @@ __global__ void __launch_bounds__(THREADS, OCC) append_kernel(const AppendParams
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       if (k >= mine) break;
-      const uint32_t pos = uint32_t(w.base + w.lo + first + k * rpp);  // (below 2^31)
+      const uint64_t pos = uint64_t(w.base + w.lo + first + k * rpp);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float2 a = turn_cs_fast(uint32_t((pos * f[2 * e]) >> 32)), b = turn_cs_fast(uint32_t((pos * f[2 * e + 1]) >> 32));
+        const float2 a = rope::turn_cs(pos * f[2 * e]), b = rope::turn_cs(pos * f[2 * e + 1]);
         zt[(k * 4 + e) * THREADS] = make_float4(a.x * p.amp, b.x * p.amp, a.y * p.amp, b.y * p.amp);
       }
     }

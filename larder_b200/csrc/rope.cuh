@@ -9,7 +9,9 @@
 // read. sincospi takes the reduced angle. Every scaling for long contexts is a choice of F_i and amp by the host.
 //
 // HBM-bound: a row is read once and written once. A block takes a few tokens and a group of their heads; it forms each
-// token's R / 2 (cos, sin) pairs once, in shared memory, while the rows' first loads are in flight.
+// token's R / 2 (cos, sin) pairs once, in shared memory, while its rows' loads are in flight. 8192 tokens of 32 heads x 128
+// (f16) take 26 us, 5130 GB/s (66 us with four fp32 rows a thread held unpacked, at two blocks an SM; 39 us with the
+// angles read from shared memory for every row); one token for each of 16 sequences takes 2.4 us behind another kernel.
 #pragma once
 
 #include "common.cuh"

@@ -58,7 +58,7 @@ def frequencies(dims, base=10000.0, scaling=None):
     hi = min(math.ceil(pair_of(float(scaling.get("beta_slow", 1.0)))), dims - 1)
     hi = hi if hi > lo else lo + 0.001
     ramp = [min(max((i - lo) / (hi - lo), 0.0), 1.0) for i in range(half)]
-    return [x * (1 - r) + x / f * r for x, r in zip(w, ramp)], 0.1 * math.log(f) + 1.0
+    return [x + (x / f - x) * r for x, r in zip(w, ramp)], 0.1 * math.log(f) + 1.0
 
 
 def turns_of(w, device=None):
