@@ -528,6 +528,7 @@ __global__ void __launch_bounds__(Cfg<D, NT, RG, MK, KG>::THREADS, 1)
       }
       // the values' scale as a power of two: its logarithm (at least -100), what that leaves of it, its reciprocal
       float ks[MK], lv[MK], iv[MK], rest[MK];
+      bool odd = false;  // (uniform in the warp)
 #pragma unroll
       for (int mk = 0; mk < MK; ++mk) {
         const float2 sc = *reinterpret_cast<const float2*>(scl + (st * 4 + sl * MK + mk) * 2);
@@ -535,30 +536,46 @@ __global__ void __launch_bounds__(Cfg<D, NT, RG, MK, KG>::THREADS, 1)
         lv[mk] = fmaxf(lg2(sc.y), -100.f);
         iv[mk] = ex2(-lv[mk]);
         rest[mk] = lv[mk] == -100.f ? sc.y * 0x1p100f : 1.f;
+        odd = odd || rest[mk] != 1.f;
       }
-      // Scores in base 2 with the values' scale. The maximum a row is taken against moves only when one of its scores
-      // passes it by more than 8: weights up to 2^8 lose nothing in f16, and most tiles need no exchange between lanes.
-      bool over = false;
+      // Scores in base 2 with the values' scale, against the row's running maximum. It moves only when a score passes it
+      // by more than 8 (weights up to 2^8 lose nothing in f16), so most tiles need no exchange between lanes; before a
+      // row's first key it is -inf, which every score passes.
       const bool whole = kbase + 16 * MK - 1 <= all_see;
+      float t[MK][NT][4];
+      auto against = [&] {  // t = score - maximum; the lane's largest
+        float top = -INFINITY;
 #pragma unroll
-      for (int mk = 0; mk < MK; ++mk)
+        for (int mk = 0; mk < MK; ++mk)
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+          for (int nt = 0; nt < NT; ++nt) {
+            const float f0 = fac[nt][0] * ks[mk], f1 = fac[nt][1] * ks[mk];
+            const float b0 = lv[mk] - m_run[nt][0], b1 = lv[mk] - m_run[nt][1];
+            float* x = t[mk][nt];
+            const float* y = s[mk][nt];
+            x[0] = fmaf(y[0], f0, b0), x[1] = fmaf(y[1], f1, b1), x[2] = fmaf(y[2], f0, b0), x[3] = fmaf(y[3], f1, b1);
+            if (!whole) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float x = fmaf(s[mk][nt][e], fac[nt][e & 1] * ks[mk], lv[mk]);
-            if (!whole && kbase + 16 * mk + key_of<D>(quad) + 8 * (e >> 1) > lim[nt][e & 1]) x = -INFINITY;
-            over = over || x > m_run[nt][e & 1] + 8.f;
-            s[mk][nt][e] = x;
+              for (int e = 0; e < 4; ++e)
+                if (kbase + 16 * mk + key_of<D>(quad) + 8 * (e >> 1) > lim[nt][e & 1]) x[e] = -INFINITY;
+            }
+            top = fmaxf(fmaxf(top, fmaxf(x[0], x[1])), fmaxf(x[2], x[3]));
           }
-      if (__any_sync(0xffffffffu, over)) {
+        return top;
+      };
+      if (__any_sync(0xffffffffu, against() > 8.f)) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             float mx = m_run[nt][e];
 #pragma unroll
-            for (int mk = 0; mk < MK; ++mk) mx = fmaxf(mx, fmaxf(s[mk][nt][e], s[mk][nt][2 + e]));
+            for (int mk = 0; mk < MK; ++mk)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const float x = fmaf(s[mk][nt][2 * h + e], fac[nt][e] * ks[mk], lv[mk]);
+                if (kbase + 16 * mk + key_of<D>(quad) + 8 * h <= lim[nt][e]) mx = fmaxf(mx, x);
+              }
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
@@ -571,20 +588,24 @@ __global__ void __launch_bounds__(Cfg<D, NT, RG, MK, KG>::THREADS, 1)
               acc[nt][j][2 + e] *= corr;
             }
           }
+        against();
       }
       uint32_t pb[NT][MK][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        const float mu[2] = {m_run[nt][0] == -INFINITY ? 0.f : m_run[nt][0], m_run[nt][1] == -INFINITY ? 0.f : m_run[nt][1]};
 #pragma unroll
         for (int mk = 0; mk < MK; ++mk) {
           float x[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) x[e] = ex2(s[mk][nt][e] - mu[e & 1]);
+          for (int e = 0; e < 4; ++e) x[e] = ex2(t[mk][nt][e]);
           l_run[nt][0] = fmaf(x[0] + x[2], iv[mk], l_run[nt][0]);
           l_run[nt][1] = fmaf(x[1] + x[3], iv[mk], l_run[nt][1]);
-          pb[nt][mk][0] = movm_t(pack2<__half>(x[0] * rest[mk], x[1] * rest[mk]));
-          pb[nt][mk][1] = movm_t(pack2<__half>(x[2] * rest[mk], x[3] * rest[mk]));
+          if (odd) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] *= rest[mk];
+          }
+          pb[nt][mk][0] = movm_t(pack2<__half>(x[0], x[1]));
+          pb[nt][mk][1] = movm_t(pack2<__half>(x[2], x[3]));
         }
       }
       const uint32_t vbase = smem_u32(vt);
