@@ -65,7 +65,7 @@ struct Cfg {
   static constexpr int XCH = DS > 1 ? 2 * WARPS * MK * NT * 32 * 16 : 0;  // two tiles' half scores of every warp
   static constexpr int JOIN = PART > XCH ? PART : XCH;  // (one area: a barrier lies between the two uses)
   static constexpr int FIXED = QBYTES + JOIN + 2 * WARPS * 8 * NT * 4 + (2 * MAX_B + 1) * 4 + 1024 + 1024;
-  static constexpr int FIT = (232448 - FIXED) / (STAGE + 48);
+  static constexpr int FIT = (232448 - FIXED) / (STAGE + 80);
   // A multiple of both, so that a stage only ever serves one producer warp and one key group, whose waits on it then
   // follow its phases in order (a wait two phases ahead would pass at once).
   static constexpr int STEP = KG > NP ? KG : NP;
@@ -74,8 +74,8 @@ struct Cfg {
   static constexpr int PART_OFF = Q_OFF + QBYTES;
   static constexpr int QMAX = DS > 1 ? 2 * WARPS * 8 * NT * 4 : 0;  // two items' largest query values by half
   static constexpr int QMAX_OFF = PART_OFF + JOIN;
-  static constexpr int SC_OFF = QMAX_OFF + QMAX;                // [STAGES][4 slices][K, V] fp32
-  static constexpr int PREFIX_OFF = SC_OFF + STAGES * 32;        // [MAX_B + 1]
+  static constexpr int SC_OFF = QMAX_OFF + QMAX;                // [STAGES][4 slices of 16 keys] Slice
+  static constexpr int PREFIX_OFF = SC_OFF + STAGES * 64;        // [MAX_B + 1]
   static constexpr int LENS_OFF = PREFIX_OFF + (MAX_B + 1) * 4;  // [MAX_B]
   static constexpr int BAR_OFF = (LENS_OFF + MAX_B * 4 + 15) / 16 * 16;
   static constexpr int SMEM = BAR_OFF + 2 * STAGES * 8 + 16 + 1024;
@@ -195,7 +195,7 @@ __global__ void __launch_bounds__(Cfg<D, NT, RG, MK, KG>::THREADS, 1)
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   int* prefix = reinterpret_cast<int*>(sm + C::PREFIX_OFF);
   int* lens = reinterpret_cast<int*>(sm + C::LENS_OFF);
-  float* scl = reinterpret_cast<float*>(sm + C::SC_OFF);
+  float4* scl = reinterpret_cast<float4*>(sm + C::SC_OFF);
   float4* part = reinterpret_cast<float4*>(sm + C::PART_OFF);  // [WARPS / 2][PART_REGS][32 lanes]
   uint64_t* full = reinterpret_cast<uint64_t*>(sm + C::BAR_OFF);
   uint64_t* empty = full + STAGES;
@@ -253,6 +253,7 @@ __global__ void __launch_bounds__(Cfg<D, NT, RG, MK, KG>::THREADS, 1)
     const int dst = kv * C::TILE + bx * (BK * C::BW) + pg * p.box * C::BW;
     const int sp = (lane & 3) * 16 / p.box;
     int gt = warp - WARPS, done = 0;  // this warp's next tile; tiles of the items before
+    int st = gt, phase = 1;           // its stage; parity of the stage's use before (1 at first: passes at once)
     bool ok = true;
     while (ok && sched.next(it)) {
       const int hk = it.hb / p.nrb;
@@ -286,9 +287,8 @@ __global__ void __launch_bounds__(Cfg<D, NT, RG, MK, KG>::THREADS, 1)
           id = nid, ks = nks, vs = nvs;
           fetch(j0 + 32 + lane, nid, nks, nvs);
         }
-        const int st = gt % STAGES;
         bool w = true;
-        if (lane == 0 && gt >= STAGES) w = !*abort_flag && mbar_wait(&empty[st], ((gt / STAGES) - 1) & 1, STATUS + 1);
+        if (lane == 0 && !mbar_try_wait(&empty[st], phase)) w = !*abort_flag && mbar_wait(&empty[st], phase, STATUS + 1);
         if (!__shfl_sync(0xffffffffu, w, 0)) {
           ok = false;
           break;
@@ -299,10 +299,15 @@ __global__ void __launch_bounds__(Cfg<D, NT, RG, MK, KG>::THREADS, 1)
           tma_load_4d(sm + st * C::STAGE + dst, &map, bx * C::BW, per > 1 ? (i & (per - 1)) * BK : 0, kv * p.a.Hkv + hk,
                       pid, &full[st]);
         const float a = __shfl_sync(0xffffffffu, ks, j - j0 + sp), c = __shfl_sync(0xffffffffu, vs, j - j0 + sp);
-        if (lane < 4) *reinterpret_cast<float2*>(scl + (st * 4 + lane) * 2) = make_float2(a, c);
+        // the slice's K scale; its V scale's logarithm (at least -100), the reciprocal of that power, what it leaves out
+        if (lane < 4) {
+          const float lv = fmaxf(lg2(c), -100.f);
+          scl[st * 4 + lane] = make_float4(a, lv, ex2(-lv), lv == -100.f ? c * 0x1p100f : 1.f);
+        }
         const uint32_t n = __popc(__ballot_sync(0xffffffffu, go));
         __syncwarp();  // the scales are written before lane 0's arrival
         if (lane == 0) mbar_arrive_expect_tx(&full[st], n * uint32_t(p.box * C::BW));
+        if ((st += NP) >= STAGES) st -= STAGES, phase ^= 1;
       }
       done += tiles;
     }
@@ -348,7 +353,8 @@ __global__ void __launch_bounds__(Cfg<D, NT, RG, MK, KG>::THREADS, 1)
   float4* xch = reinterpret_cast<float4*>(sm + C::PART_OFF);  // [2 tiles][DS][WARPS / 2][MK NT][32 lanes]
   float* qmax = reinterpret_cast<float*>(sm + C::QMAX_OFF);  // [2 items][DS][WARPS / 2][8 NT]
   const int pair = warp % (WARPS / 2);
-  int gt = 0, xpar = 0, qpar = 0;
+  int seen = 0, st = kg, phase = 0;  // tiles of the items before; this key group's next stage and its parity
+  int xpar = 0, qpar = 0;
   bool ok = true;
   while (sched.next(it)) {
     const int hk = it.hb / p.nrb, r0 = (it.hb - hk * p.nrb) * p.rpb, r1 = min(p.rows, r0 + p.rpb);  // the block's rows
@@ -438,15 +444,12 @@ __global__ void __launch_bounds__(Cfg<D, NT, RG, MK, KG>::THREADS, 1)
 #pragma unroll
       for (int j = 0; j < DW / 16; ++j) acc[nt][j][0] = acc[nt][j][1] = acc[nt][j][2] = acc[nt][j][3] = 0.f;
     }
-    for (int i = it.i0; i < it.i1; ++i, ++gt) {
-      if (KG > 1 && gt % KG != kg) continue;
-      const int st = gt % STAGES;
-      if (!ok || *abort_flag || !mbar_wait(&full[st], (gt / STAGES) & 1, STATUS + 3)) {
+    const int i0 = it.i0 + ((kg - seen) & (KG - 1));  // this key group's first tile
+    seen += it.i1 - it.i0;
+    for (int i = i0; i < it.i1; i += KG) {
+      if (!mbar_try_wait(&full[st], phase) && (*abort_flag || !mbar_wait(&full[st], phase, STATUS + 3))) {
         ok = false;
-        if constexpr (DS == 1) {
-          gt += it.i1 - i;
-          break;
-        }  // (DS > 1: the pair leaves together, below)
+        if constexpr (DS == 1) break;  // (DS > 1: the pair leaves together, below)
       }
       uint8_t* kt = sm + st * C::STAGE;
       uint8_t* vt = kt + C::TILE;
@@ -459,11 +462,16 @@ __global__ void __launch_bounds__(Cfg<D, NT, RG, MK, KG>::THREADS, 1)
         }
         __syncwarp();
       }
-      float s[MK][NT][4];
+      // (with few independent products the k-steps alternate between two accumulators: shorter chains)
+      constexpr int KSP = MK * NT <= 2 ? 2 : 1;
+      float s[MK][NT][4], s2[KSP > 1 ? MK : 1][KSP > 1 ? NT : 1][4];
 #pragma unroll
       for (int mk = 0; mk < MK; ++mk)
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) s[mk][nt][0] = s[mk][nt][1] = s[mk][nt][2] = s[mk][nt][3] = 0.f;
+        for (int nt = 0; nt < NT; ++nt) {
+          s[mk][nt][0] = s[mk][nt][1] = s[mk][nt][2] = s[mk][nt][3] = 0.f;
+          if constexpr (KSP > 1) s2[mk][nt][0] = s2[mk][nt][1] = s2[mk][nt][2] = s2[mk][nt][3] = 0.f;
+        }
 #pragma unroll
       for (int sg = 0; sg < SEG; ++sg) {
         uint4 ka[MK], kb[MK];
@@ -493,10 +501,21 @@ __global__ void __launch_bounds__(Cfg<D, NT, RG, MK, KG>::THREADS, 1)
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
               const uint32_t* q = C::Q_REGS ? qf[C::Q_REGS ? nt : 0][C::Q_REGS ? sg : 0] : qs[nt];
-              mma16816(s[mk][nt], a0, a1, a2, a3, q[2 * w], q[2 * w + 1]);
+              if (KSP > 1 && (w & 1))
+                mma16816(s2[KSP > 1 ? mk : 0][KSP > 1 ? nt : 0], a0, a1, a2, a3, q[2 * w], q[2 * w + 1]);
+              else
+                mma16816(s[mk][nt], a0, a1, a2, a3, q[2 * w], q[2 * w + 1]);
             }
           }
         }
+      }
+      if constexpr (KSP > 1) {
+#pragma unroll
+        for (int mk = 0; mk < MK; ++mk)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[mk][nt][e] += s2[mk][nt][e];
       }
       if constexpr (DS > 1) {  // the pair's halves of the scores (buffers alternate, so one barrier a tile is enough)
         constexpr int XW = MK * NT * 32;  // float4 a warp
@@ -526,16 +545,12 @@ __global__ void __launch_bounds__(Cfg<D, NT, RG, MK, KG>::THREADS, 1)
             s[mk][nt][0] += o.x, s[mk][nt][1] += o.y, s[mk][nt][2] += o.z, s[mk][nt][3] += o.w;
           }
       }
-      // the values' scale as a power of two: its logarithm (at least -100), what that leaves of it, its reciprocal
       float ks[MK], lv[MK], iv[MK], rest[MK];
       bool odd = false;  // (uniform in the warp)
 #pragma unroll
       for (int mk = 0; mk < MK; ++mk) {
-        const float2 sc = *reinterpret_cast<const float2*>(scl + (st * 4 + sl * MK + mk) * 2);
-        ks[mk] = sc.x;
-        lv[mk] = fmaxf(lg2(sc.y), -100.f);
-        iv[mk] = ex2(-lv[mk]);
-        rest[mk] = lv[mk] == -100.f ? sc.y * 0x1p100f : 1.f;
+        const float4 sc = scl[st * 4 + sl * MK + mk];
+        ks[mk] = sc.x, lv[mk] = sc.y, iv[mk] = sc.z, rest[mk] = sc.w;
         odd = odd || rest[mk] != 1.f;
       }
       // Scores in base 2 with the values' scale, against the row's running maximum. It moves only when a score passes it
@@ -629,6 +644,7 @@ __global__ void __launch_bounds__(Cfg<D, NT, RG, MK, KG>::THREADS, 1)
       if (nvalid < 16 * MK) fence_proxy_async_shared();  // the zeros precede the next copy into this stage
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty[st]);
+      if ((st += KG) >= STAGES) st -= STAGES, phase ^= 1;
     }
 
     // ------------------------------------------------------------------ the item's partial
