@@ -1,8 +1,9 @@
 """The paged 8-bit KV cache on the GPU: what append leaves in the pages, and attention over them, in 64 bits.
 
 Append. The scale is a power of two fixed by the rotated values' largest magnitude; a held value is the nearest e4m3
-code: |held - x| <= half a code step, plus, for rotated keys, the error of the rotated value in fp32 with the hardware's
-sine and cosine (2^-21 absolute, an argument rounding of pi 2^-23, three fp32 roundings: under 2^-18 (|x0| + |x1|)).
+code: |held - x| <= half a code step, plus, for rotated keys, the error of the rotated value in fp32, whatever forms the sine
+and cosine (the multi-function unit's are off by 2^-21, its argument by pi 2^-23, three fp32 roundings: under 2^-18 (|x0| +
+|x1|)).
 Values and held codes that are rescaled take no such error: they must be the nearest codes exactly.
 
 Attention. Codes are exact in f16. Queries go to f16 exactly (bf16 has fewer bits, the range is shifted); scores are
