@@ -274,18 +274,19 @@ __global__ void __launch_bounds__(Cfg<D, NT, RG, MK, KG>::THREADS, 1)
         }
       };
       int j0 = (it.i0 * BK) >> p.lpage;  // first page of the current 32
-      int id, nid;
-      float ks, vs, nks, nvs;
+      int id, nid = -1;
+      float ks, vs, nks = 0.f, nvs = 0.f;
       fetch(j0 + lane, id, ks, vs);
-      fetch(j0 + 32 + lane, nid, nks, nvs);
+      bool ahead = false;  // the next 32 are on their way (asked for once a tile has been issued: a load is waited for)
       const int tiles = it.i1 - it.i0;
       for (; gt - done < tiles; gt += NP) {
         const int i = it.i0 + gt - done;
         const int j = (i * BK) >> p.lpage;  // first page of the tile
         if (j - j0 >= 32) {                 // (a tile's pages never straddle: a tile has 1, 2 or 4; steps are below 32)
           j0 += 32;
+          if (!ahead) fetch(j0 + lane, nid, nks, nvs);
           id = nid, ks = nks, vs = nvs;
-          fetch(j0 + 32 + lane, nid, nks, nvs);
+          ahead = false;
         }
         bool w = true;
         if (lane == 0 && !mbar_try_wait(&empty[st], phase)) w = !*abort_flag && mbar_wait(&empty[st], phase, STATUS + 1);
@@ -308,6 +309,10 @@ __global__ void __launch_bounds__(Cfg<D, NT, RG, MK, KG>::THREADS, 1)
         __syncwarp();  // the scales are written before lane 0's arrival
         if (lane == 0) mbar_arrive_expect_tx(&full[st], n * uint32_t(p.box * C::BW));
         if ((st += NP) >= STAGES) st -= STAGES, phase ^= 1;
+        if (!ahead) {
+          ahead = true;
+          fetch(j0 + 32 + lane, nid, nks, nvs);
+        }
       }
       done += tiles;
     }
@@ -444,7 +449,8 @@ __global__ void __launch_bounds__(Cfg<D, NT, RG, MK, KG>::THREADS, 1)
 #pragma unroll
       for (int j = 0; j < DW / 16; ++j) acc[nt][j][0] = acc[nt][j][1] = acc[nt][j][2] = acc[nt][j][3] = 0.f;
     }
-    const int i0 = it.i0 + ((kg - seen) & (KG - 1));  // this key group's first tile
+    const int turn = (kg - seen) & (KG - 1);  // this key group takes the item's tiles turn, turn + KG, ...
+    const int i0 = it.i0 + turn, parts = SL * min(KG, it.i1 - it.i0);  // parts of a row that hold something
     seen += it.i1 - it.i0;
     for (int i = i0; i < it.i1; i += KG) {
       if (!mbar_try_wait(&full[st], phase) && (*abort_flag || !mbar_wait(&full[st], phase, STATUS + 3))) {
@@ -672,9 +678,10 @@ __global__ void __launch_bounds__(Cfg<D, NT, RG, MK, KG>::THREADS, 1)
       if (lane == 0) *abort_flag = 1;
       break;
     }
-    const int pi = kg * SL + sl;
+    const int pi = turn * SL + sl;
 #pragma unroll 1  // (one copy of the code: at an item's end it is fetched cold)
     for (int half = SL * KG / 2; half > 0; half >>= 1) {
+      if (half >= parts) continue;  // (the same for every warp)
       if (pi >= half && pi < 2 * half) {
         float4* d = part + (((pi - half) * RG + rg) * DS + dh) * C::PART_REGS * 32 + lane;
 #pragma unroll
