@@ -3,10 +3,11 @@
 // Persistent kernel: one CTA per SM walks its share of the call's work items, an item being (sequence b, KV head hk,
 // a key range of b). The G*T query rows sharing KV head hk are folded into 16-row tiles (the fold of
 // foldattn.py:230-259), so every K/V byte is read from HBM once per call. Two schedules:
-//  - balanced (split = 0): the call's 64-key tiles, ordered (b, hk, tile), are cut into gridDim.x equal runs and CTA c
-//    takes run c, cut again where a (b, hk) pair ends. Every CTA streams the same number of tiles whatever the
-//    per-sequence lengths, and CTA c's item of pair p writes partial slot c + p: unique (a later CTA starts at or
-//    after an earlier CTA's last pair) and contiguous per pair, so the combine finds a pair's partials by arithmetic;
+//  - balanced (split = 0): the call's 64-key tiles, ordered (b, hk, tile), are cut into equal runs, one a CTA but none
+//    without a tile (the grid is sized by the capacity, the lengths are read on the device), and CTA c takes run c, cut
+//    again where a (b, hk) pair ends. Every CTA streams the same number of tiles whatever the per-sequence lengths, and
+//    CTA c's item of pair p writes partial slot c + p: unique (a later CTA starts at or after an earlier CTA's last
+//    pair), contiguous per pair and all written, so the combine finds a pair's partials by arithmetic;
 //  - split (split > 0): equal `split`-key units (b, s, hk) dealt round-robin, partial slot (b Hkv + hk) nsplit + s.
 // A producer warp streams, item after item without a pause, the item's folded Q tile (a 2-slot ring) and its 64-key
 // K and V tiles (a STAGES-deep ring), all with TMA into 128-byte swizzled boxes of 64 head-dim elements; four
@@ -166,6 +167,10 @@ __device__ __forceinline__ uint32_t movm_t(uint32_t x) {
   return y;
 }
 
+// How many runs the balanced schedule cuts the call's tiles into: with an empty run a slot between a pair's first and last
+// would be one that no CTA writes.
+__device__ __forceinline__ int64_t runs_of(int grid, int64_t total) { return min(int64_t(grid), total); }
+
 // One work item: KV head hk of sequence b (length len), keys [n0, n1), partial slot `slot`.
 struct Item {
   int b, hk, n0, n1, len, slot;
@@ -183,8 +188,9 @@ struct Sched {
       : prefix(prefix_), lens(lens_), B(p.B), Hkv(p.Hkv), split(p.split), nsplit(p.nsplit), balanced(p.balanced) {
     const int total = prefix[p.B] * p.Hkv;  // units or tiles of the call
     if (balanced) {
-      cur = int(int64_t(blockIdx.x) * total / gridDim.x);
-      end = int(int64_t(blockIdx.x + 1) * total / gridDim.x);
+      const int64_t runs = runs_of(int(gridDim.x), total), c = blockIdx.x;
+      cur = c < runs ? int(c * total / runs) : 0;
+      end = c < runs ? int((c + 1) * total / runs) : 0;
       step = 0;
     } else {
       cur = blockIdx.x;
@@ -736,9 +742,10 @@ __global__ void __launch_bounds__(256) split_combine_kernel(const Params p) {
     if (nt == 0) {
       first = 0;
       nparts = 0;
-    } else {  // CTA of tile t: the largest c with floor(c total / grid) <= t, i.e. ((t + 1) grid - 1) / total
+    } else {  // CTA of tile t: the largest c with floor(c total / runs) <= t, i.e. ((t + 1) runs - 1) / total
       const int64_t tt = int64_t(total) * p.Hkv, t0 = int64_t(before) * p.Hkv + int64_t(hk) * nt;
-      const int c0 = int(((t0 + 1) * p.grid - 1) / tt), c1 = int(((t0 + nt) * p.grid - 1) / tt);
+      const int64_t runs = runs_of(p.grid, tt);
+      const int c0 = int(((t0 + 1) * runs - 1) / tt), c1 = int(((t0 + nt) * runs - 1) / tt);
       first = c0 + bh;
       nparts = c1 - c0 + 1;
     }
