@@ -508,10 +508,12 @@ __global__ void __launch_bounds__(THREADS, 1) fmha_kernel(const __grid_constant_
       const float tmax2 = tmax * p.scale_log2;  // base-2 units
       // The running max moves only when it grew by more than 2^8 (fp32 O and the 16-bit P absorb the rest); O is
       // rescaled in TMEM then, after PV_{j-1} has completed. tcgen05.ld / st are warp-collective, so a warp rescales
-      // when any of its rows must (factor 1 for the others); both warps of a row pair decide alike.
+      // when any of its rows must (factor 1 for the others). Whether a row has weights in O yet is asked of the maximum,
+      // which the warps of a row share, and not of l_run: that sums this warp's share of the keys alone, and is 0 where
+      // they all lie 2^126 below the maximum.
       const bool move = tmax2 > m_run + 8.f;
       const float factor = move ? ex2f(m_run - tmax2) : 1.f;
-      if (__any_sync(0xffffffffu, move && j > 0 && l_run > 0.f)) {
+      if (__any_sync(0xffffffffu, move && m_run != -INFINITY)) {
         if (!mbar_wait(&o_done[(j - 1) % SB], ((j - 1) / SB) & 1, 32)) ok = false;
         tc_fence_after();
 #pragma unroll 1

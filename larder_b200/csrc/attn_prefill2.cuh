@@ -535,7 +535,8 @@ __global__ void __launch_bounds__(THREADS, 1) fmha2_kernel(const __grid_constant
           const float tmax2 = tmax * p.scale_log2;
           const bool move = tmax2 > m_run + 8.f;
           const float factor = move ? prefill::ex2f(m_run - tmax2) : 1.f;
-          if (__any_sync(0xffffffffu, move && j > 0 && l_run > 0.f)) {
+          // (the maximum is the row's; l_run, this group's share of the sum, may be 0 where O is not)
+          if (__any_sync(0xffffffffu, move && m_run != -INFINITY)) {
             if (!mbar_wait(&o_done[(g - 1) % C::PB], ((g - 1) / C::PB) & 1, 62)) ok = false;
             prefill::tc_fence_after();
 #pragma unroll 1
