@@ -395,7 +395,7 @@ int lb2_kv8_attend(const void* q, const int64_t* q_st, const uint8_t* pages, con
  *   q, o [Hq, T, D], k, v [Hkv, T, D]: strides [0..1] for H, T; unit on D; dtype LB2_BF16 / F16 (row strides multiples
  *   of 8 elements, 16-byte aligned bases) or LB2_F32 (exact CUDA-core kernel); D in {64, 128, 256}; scale > 0.
  *   workspace: lb2_attn_packed_workspace_size() bytes, 256-byte aligned, any contents.
- * Rows of no prompt (cu[S] < T) give zeros. No value of one prompt reaches another's rows, infinities and NaN among
+ * Rows of no prompt (before cu[0], from cu[S] on) give zeros. No value of one prompt reaches another's rows, infinities and NaN among
  * them, nor a later row's an earlier row. */
 size_t lb2_attn_packed_workspace_size(int S, int Hq, int Hkv, int T, int D);
 int lb2_attn_packed(const void* q, const int64_t* q_st, const void* k, const int64_t* k_st, const void* v,

@@ -1840,7 +1840,7 @@ static Layout layout(int64_t S, int64_t T, int rb) {
   Layout l;
   l.cnt = 256;
   l.at = l.cnt + align_up(size_t(T / rb + 2) * 4, 256);
-  l.out = l.at + align_up(size_t(S + 2) * 4, 256);
+  l.out = l.at + align_up(size_t(S + 3) * 4, 256);
   l.total = l.out + align_up(size_t(T / rb + S + 2) * sizeof(int4), 256);
   return l;
 }
@@ -1959,7 +1959,7 @@ static int run(const arows::PackedParams& a, int D, int dtype, void* workspace, 
     }
     if (rc) return rc;
   }
-  const int64_t blocks = int64_t(a.T) / rb + a.S + 1;
+  const int64_t blocks = int64_t(a.T) / rb + a.S + 2;  // (S + 2 ranges, a partial block each at most)
 #define LB2_PACKED(TT)                                                                               \
   return D == 64 ? launch<TT, 64>(pair, maps[0], maps[1], maps[2], p, blocks, st)                    \
          : D == 128 ? launch<TT, 128>(pair, maps[0], maps[1], maps[2], p, blocks, st)                \
