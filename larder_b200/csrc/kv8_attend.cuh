@@ -21,9 +21,12 @@
 // bf16 query rows go to f16 exactly: a row is shifted by a power of two (its largest value to [2^14, 2^15)), which the
 // score's factor undoes; bf16's 8 bits fit f16's 11 down to 2^-28 of the row's largest value.
 //
-// Softmax in base 2, fp32. The weights carry the values' scale: p'_n = 2^(s_n + log2 s_v - m), m the running maximum of
-// s_n + log2 s_v, and l = sum p'_n / s_v, so that o = sum p'_n code_n / l; the weights of pages with scales far apart thus
-// never leave f16's range, where p' is rounded (2^-11 relative; the sums are fp32).
+// Softmax in base 2, fp32. The weights carry the values' scale: p'_n = 2^(s_n + log2 s_v - m + 7), m the running maximum of
+// s_n + log2 s_v, and l = sum p'_n / s_v, so that o = sum p'_n code_n / l, with pages' scales far apart too. Only the
+// products' weights are rounded, to f16; the sums are fp32. The maximum lags by up to 2^8 (below), so a row's largest
+// p' lies between 2^7 and 2^15, the upper end of f16's range: weights down to 2^-21 of it at least keep f16's 11 bits, smaller
+// ones lose one a power of two and are 0 below 2^-32 of it, which is what a key that dominates the sum with a value of 0
+// leaves the others.
 //
 // A NaN code under a weight of 0 would spread to rows that do not see it: values past the length are zeroed in shared
 // memory; with several rows of different horizons, combine_kernel takes a row that came out NaN again, key by key
@@ -39,6 +42,7 @@ namespace kv8attn {
 
 constexpr int BK = 64;       // keys a tile
 constexpr int MAX_B = 1024;  // sequences a launch (the prefix table in shared memory); larger batches go in several
+constexpr float TOP = 7.f;   // a weight at the running maximum is 2^TOP
 constexpr int STATUS = 112;  // where (lb2_status): 112 a page id or length, 113.. waits
 
 // NT: 8-row tiles of query rows a warp; MK: 16-key blocks of a tile a warp (two give it two independent chains of
@@ -559,12 +563,12 @@ __global__ void __launch_bounds__(Cfg<D, NT, RG, MK, KG>::THREADS, 1)
         ks[mk] = sc.x, lv[mk] = sc.y, iv[mk] = sc.z, rest[mk] = sc.w;
         odd = odd || rest[mk] != 1.f;
       }
-      // Scores in base 2 with the values' scale, against the row's running maximum. It moves only when a score passes it
-      // by more than 8 (weights up to 2^8 lose nothing in f16), so most tiles need no exchange between lanes; before a
-      // row's first key it is -inf, which every score passes.
+      // Scores in base 2 with the values' scale, against the row's running maximum less TOP (what m_run holds). It moves
+      // only when a score passes the maximum by more than 8 (weights up to 2^15 lose nothing in f16), so most tiles need no
+      // exchange between lanes; before a row's first key it is -inf, which every score passes.
       const bool whole = kbase + 16 * MK - 1 <= all_see;
       float t[MK][NT][4];
-      auto against = [&] {  // t = score - maximum; the lane's largest
+      auto against = [&] {  // t = score - (maximum - TOP); the lane's largest
         float top = -INFINITY;
 #pragma unroll
         for (int mk = 0; mk < MK; ++mk)
@@ -584,12 +588,12 @@ __global__ void __launch_bounds__(Cfg<D, NT, RG, MK, KG>::THREADS, 1)
           }
         return top;
       };
-      if (__any_sync(0xffffffffu, against() > 8.f)) {
+      if (__any_sync(0xffffffffu, against() > TOP + 8.f)) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float mx = m_run[nt][e];
+            float mx = m_run[nt][e] + TOP;
 #pragma unroll
             for (int mk = 0; mk < MK; ++mk)
 #pragma unroll
@@ -600,6 +604,7 @@ __global__ void __launch_bounds__(Cfg<D, NT, RG, MK, KG>::THREADS, 1)
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+            mx -= TOP;
             const float corr = ex2(m_run[nt][e] - (mx == -INFINITY ? 0.f : mx));
             m_run[nt][e] = mx;
             l_run[nt][e] *= corr;
