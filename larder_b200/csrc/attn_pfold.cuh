@@ -253,6 +253,7 @@ __global__ void __launch_bounds__(THREADS, Cfg<D>::CTAS) pfold_kernel(const __gr
     // ------------------------------------------------------------------------------------ softmax warps
     constexpr int HC = BN / 2;  // S columns (keys) a thread owns
     constexpr int HD = D / 2;   // O columns a thread owns
+    constexpr float TOP = prefill::packed_top<T>();
     const int r = 32 * (warp & 3) + lane, half = warp >> 2;
     const uint32_t lane_base = tmem + (uint32_t(32 * (warp & 3)) << 16);
     const uint32_t pair_bar = 2 + (warp & 3);  // named barrier of the two warps of a lane quarter
@@ -290,9 +291,9 @@ __global__ void __launch_bounds__(THREADS, Cfg<D>::CTAS) pfold_kernel(const __gr
           for (int c = 0; c < HC; ++c)
             if (key0 + c > last) s[c] = -INFINITY;
         }
-        // P with the running maximum, which moves only when a weight would pass 2^8 (or at the row's first key): one
+        // P with the running maximum, which moves only when a weight would pass 2^(TOP + 8) (or at the row's first key): one
         // barrier of the two warps asks whether any of their rows wants that (or a wait failed).
-        float nm = m_run == -INFINITY ? 0.f : -m_run;
+        float nm = m_run == -INFINITY ? 0.f : TOP - m_run;
         float ls[4] = {0.f, 0.f, 0.f, 0.f};
         uint32_t pk[HC / 2];
         auto weights = [&] {
@@ -355,7 +356,7 @@ __global__ void __launch_bounds__(THREADS, Cfg<D>::CTAS) pfold_kernel(const __gr
           if (move) {
             l_run *= factor;
             m_run = tmax2;
-            nm = -m_run;
+            nm = TOP - m_run;
             weights();
           }
         }

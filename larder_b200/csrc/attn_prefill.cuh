@@ -218,6 +218,14 @@ __device__ __forceinline__ float ex2_fma(float x) {
   return x < -125.f ? 0.f : r;
 }
 
+// Packed prompts: a weight at the row's running maximum is 2^top. The maximum lags by up to 2^8, so f16 weights reach 2^15,
+// the upper end of the type, and keep their 11 bits down to 2^-21 of the largest (against 1 they were subnormal from 2^-14
+// on: under a dominating key whose value is 0 the others' weights were off by up to a tenth). bf16 has fp32's range.
+template <typename T>
+__device__ __host__ constexpr float packed_top() {
+  return std::is_same<T, __half>::value ? 7.f : 0.f;
+}
+
 // Packed prompts' second look at a row whose output came out non-finite with a finite sum of weights: a value that is
 // infinite or NaN was multiplied by a weight, possibly the 0 of a key that the row does not see (a later row of its
 // prompt in the last tile, or the next prompt's rows behind it). Takes `cols` columns of the row again, reading only the

@@ -447,6 +447,7 @@ __global__ void __launch_bounds__(THREADS, 1) fmha2_kernel(const __grid_constant
     constexpr int HC = BN / NG;  // S columns (keys) a thread owns
     constexpr int DH = D / NG;   // O columns a thread owns
     static_assert(HC == 32, "a softmax thread loads 32 S columns");
+    constexpr float TOP = PK ? prefill::packed_top<T>() : 0.f;  // P is relative to 2^TOP
     const int r = 32 * (warp & 3) + lane;
     const int grp = warp >> 2;
     const uint32_t lane_base = tmem + (uint32_t(32 * (warp & 3)) << 16);
@@ -492,7 +493,7 @@ __global__ void __launch_bounds__(THREADS, 1) fmha2_kernel(const __grid_constant
         // i.e. when some P of the row exceeds 2^8; P >= 0, so a thread whose P sum is at most 2^8 has no such
         // element and skips the max altogether. Otherwise (or before the row's first key) the exact check below
         // runs, and the rows that move recompute their P.
-        float nm = m_run == -INFINITY ? 0.f : -m_run;
+        float nm = m_run == -INFINITY ? 0.f : TOP - m_run;
         float ls4[4] = {0.f, 0.f, 0.f, 0.f};
         uint32_t pk[HC / 2];
 #pragma unroll
@@ -504,7 +505,7 @@ __global__ void __launch_bounds__(THREADS, 1) fmha2_kernel(const __grid_constant
           pk[c / 2] = pack2<T>(e0, e1);
         }
         // one barrier of the quarter's NG warps: does any of their rows want to move its max (or did a wait fail)?
-        const bool want = !okj || m_run == -INFINITY || !((ls4[0] + ls4[1]) + (ls4[2] + ls4[3]) <= 256.f);
+        const bool want = !okj || m_run == -INFINITY || !((ls4[0] + ls4[1]) + (ls4[2] + ls4[3]) <= 256.f * float(1 << int(TOP)));
         uint32_t any_want;
         asm volatile(
             "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\t"
@@ -553,7 +554,7 @@ __global__ void __launch_bounds__(THREADS, 1) fmha2_kernel(const __grid_constant
           if (move) {  // this row's P with its new max
             l_run *= factor;
             m_run = tmax2;
-            nm = -m_run;
+            nm = TOP - m_run;
 #pragma unroll
             for (int c = 0; c < 4; ++c) ls4[c] = 0.f;
 #pragma unroll
