@@ -7,7 +7,7 @@
 // little better, but e4m3 keeps its relative precision down to 2^-15 of the top), and when a later token raises the page's
 // scale the held codes are divided by a power of two: exact but for codes that reach e4m3's subnormals (below 2^-15 of the
 // page's largest value). The result does not depend on how the tokens are cut into calls, but for those.
-// Infinities are held as +-448 s, NaN as NaN; neither sets the scale.
+// Infinities are held as +-448 s (of the call that brings them, or the first scale but 0), NaN as NaN; neither sets the scale.
 #pragma once
 
 #include <type_traits>
@@ -52,9 +52,10 @@ __device__ __forceinline__ float scale_of(float m) {
   const int e = int(u >> 23) - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);  // 448 = 1.75 * 2^8
   return __uint_as_float(uint32_t(max(e, 1)) << 23);
 }
-// 1 / s of a scale (a power of two between 2^-126 and 2^121); 0 for 0.
+// What values are multiplied by before they are rounded to codes: 1 / s of a scale (a power of two between 2^-126 and
+// 2^121). For 0, where every finite value is 0, it is 1: infinities then saturate as anywhere else (times 0 they were NaN).
 __device__ __forceinline__ float scale_inv(float s) {
-  return s > 0.f ? __uint_as_float((254u << 23) - __float_as_uint(s)) : 0.f;
+  return s > 0.f ? __uint_as_float((254u << 23) - __float_as_uint(s)) : 1.f;
 }
 
 struct AppendParams {
