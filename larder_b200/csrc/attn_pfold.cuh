@@ -90,7 +90,8 @@ __global__ void __launch_bounds__(THREADS, Cfg<D>::CTAS) pfold_kernel(const __gr
   uint64_t* drain = o_free + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  static_assert((4 * ST + 8) * 8 + 8 <= 256, "barrier area");
+  volatile int* again = abort_flag + 1;  // some row came out non-finite with a finite sum of weights
+  static_assert((4 * ST + 8) * 8 + 12 <= 256, "barrier area");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -109,6 +110,7 @@ __global__ void __launch_bounds__(THREADS, Cfg<D>::CTAS) pfold_kernel(const __gr
     mbar_init(o_free, SOFTMAX_WARPS);
     mbar_init(drain, 1);
     *abort_flag = 0;
+    *again = 0;
     fence_barrier_init();
   }
   if (warp == MMA_WARP) {
@@ -410,10 +412,7 @@ __global__ void __launch_bounds__(THREADS, Cfg<D>::CTAS) pfold_kernel(const __gr
         float sum = 0.f;  // (finite unless some value is not)
 #pragma unroll
         for (int e = 0; e < 32; ++e) sum = fmaf(ov[e], 0.f, sum);
-        if (sum != sum && l_tot == l_tot) {
-          prefill::packed_row_exact<T, D>(p, blk.x, row, h, half * HD + c, 32, orow + c);
-          continue;
-        }
+        if (sum != sum && l_tot == l_tot) *again = 1;
         uint32_t w[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) w[e] = pack2<T>(ov[2 * e] * inv, ov[2 * e + 1] * inv);
@@ -436,6 +435,16 @@ __global__ void __launch_bounds__(THREADS, Cfg<D>::CTAS) pfold_kernel(const __gr
   if (warp == MMA_WARP) {
     prefill::tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::TCOLS));
+  }
+  // The second look (rare), when nothing waits for this CTA any more: its items' rows again, a warp a row.
+  if (*again && !*abort_flag) {
+    for (int r = 0, it; r * int(gridDim.x) < total; ++r) {
+      if ((it = item_at(r)) >= total) continue;
+      const int4 blk = p.pk[it / heads];
+      const int first = blk.z * tpb, rows = min(tpb, blk.y - first) * F, end = min(blk.w * BN, p.T - blk.x);
+      for (int x = warp; x < rows; x += THREADS / 32)
+        prefill::packed_row_again<T, D>(p, blk.x, first + x / F, end, it % heads * F + x % F);
+    }
   }
 }
 

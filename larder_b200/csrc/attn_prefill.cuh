@@ -76,7 +76,7 @@ struct Params {
   int tl_ld;
   // Packed prompts (attn_pfold.cuh, the pair kernel's PK form; causal within each prompt): the row blocks, heaviest
   // first, as (prompt's first row, its rows, block index m, key tiles it reads), *pk_n of them, listed by
-  // packed::plan_kernel; and q, k, v for the rows that are taken again (packed_row_exact).
+  // packed::plan_kernel; and q, k, v for the rows that are taken again (packed_row_again).
   const int4* pk;
   const int32_t* pk_n;
   int fold, tpb;  // attn_pfold.cuh: query heads side by side in a block, and its tokens (row = token fold + head)
@@ -226,32 +226,73 @@ __device__ __host__ constexpr float packed_top() {
   return std::is_same<T, __half>::value ? 7.f : 0.f;
 }
 
-// Packed prompts' second look at a row whose output came out non-finite with a finite sum of weights: a value that is
-// infinite or NaN was multiplied by a weight, possibly the 0 of a key that the row does not see (a later row of its
-// prompt in the last tile, or the next prompt's rows behind it). Takes `cols` columns of the row again, reading only the
-// keys 0 .. row it sees. Rare; one thread a row.
+// Packed prompts' second look, by one warp, at row `row` of the prompt whose rows begin at `base`, query head h. A block's
+// products reach keys behind the row (later rows of its prompt, the next prompt's: all below `end`) with weights of 0, and 0
+// times an infinity or NaN is NaN. Where a column of the row came out non-finite and one of those keys is non-finite in it,
+// the row is taken again, reading only the keys 0 .. row that it sees; a row that is non-finite by what it sees stays.
+// 32 keys at a time: a lane a key for the scores, then the lanes share the dims.
 template <typename T, int D>
-__device__ __noinline__ void packed_row_exact(const Params& p, int base, int row, int h, int c0, int cols, T* out) {
+__device__ __noinline__ void packed_row_again(const Params& p, int base, int row, int end, int h) {
+  constexpr int E = D / 32;
+  struct alignas(E * 2) Dims {
+    T x[E];
+  };
+  const int lane = threadIdx.x & 31;
+  const int64_t kst = p.src_st[1][1], vst = p.src_st[2][1];
   const T* q = static_cast<const T*>(p.src[0]) + h * p.src_st[0][0] + int64_t(base + row) * p.src_st[0][1];
-  const T* k = static_cast<const T*>(p.src[1]) + (h / p.G) * p.src_st[1][0] + int64_t(base) * p.src_st[1][1];
-  const T* v = static_cast<const T*>(p.src[2]) + (h / p.G) * p.src_st[2][0] + int64_t(base) * p.src_st[2][1] + c0;
-  for (int c = 0; c < cols; c += 16) {
-    float o[16], m = -INFINITY, l = 0.f;
+  const T* k = static_cast<const T*>(p.src[1]) + (h / p.G) * p.src_st[1][0] + int64_t(base) * kst;
+  const T* v = static_cast<const T*>(p.src[2]) + (h / p.G) * p.src_st[2][0] + int64_t(base) * vst + lane * E;
+  T* out = static_cast<T*>(p.o) + h * p.o_st[1] + int64_t(base + row) * p.o_st[2] + lane * E;
+  const Dims was = *reinterpret_cast<const Dims*>(out);
+  bool bad[E], any = false;
 #pragma unroll
-    for (int e = 0; e < 16; ++e) o[e] = 0.f;
-    for (int i = 0; i <= row; ++i) {
-      float s = 0.f;
-      for (int d = 0; d < D; ++d) s = fmaf(to_f<T>(q[d]), to_f<T>(k[i * p.src_st[1][1] + d]), s);
-      s *= p.scale_log2;
-      const float m1 = fmaxf(m, s), mu = m1 == -INFINITY ? 0.f : m1, f = exp2f(m - mu), w = exp2f(s - mu);
-      l = l * f + w;
+  for (int e = 0; e < E; ++e) any |= bad[e] = !isfinite(to_f<T>(was.x[e]));
+  if (!__any_sync(0xffffffffu, any)) return;
+  any = false;
+  for (int i = row + 1; i < end; ++i) {
+    const Dims w = *reinterpret_cast<const Dims*>(v + i * vst);
 #pragma unroll
-      for (int e = 0; e < 16; ++e) o[e] = fmaf(w, to_f<T>(v[i * p.src_st[2][1] + c + e]), o[e] * f);
-      m = m1;
-    }
-#pragma unroll
-    for (int e = 0; e < 16; ++e) out[c + e] = from_f<T>(o[e] / l);
+    for (int e = 0; e < E; ++e) any |= bad[e] && !isfinite(to_f<T>(w.x[e]));
   }
+  if (!__any_sync(0xffffffffu, any)) return;
+  float o[E], m = -INFINITY, l = 0.f;
+#pragma unroll
+  for (int e = 0; e < E; ++e) o[e] = 0.f;
+  for (int i0 = 0; i0 <= row; i0 += 32) {
+    float s = -INFINITY;
+    if (i0 + lane <= row) {
+      const T* kr = k + (i0 + lane) * kst;
+      s = 0.f;
+      for (int d = 0; d < D; d += 8) {
+        const uint4 a = *reinterpret_cast<const uint4*>(q + d), b = *reinterpret_cast<const uint4*>(kr + d);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          s = fmaf(to_f<T>(reinterpret_cast<const T*>(&a)[e]), to_f<T>(reinterpret_cast<const T*>(&b)[e]), s);
+      }
+      s *= p.scale_log2;
+    }
+    float m1 = fmaxf(m, s);  // (a NaN score stays out of m and reaches l and o through w)
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, x));
+    const float mu = m1 == -INFINITY ? 0.f : m1, f = exp2f(m - mu), w = exp2f(s - mu);
+    m = m1;
+    l = l * f + w;
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] *= f;
+    for (int i = i0; i <= min(i0 + 31, row); ++i) {
+      const float wi = __shfl_sync(0xffffffffu, w, i - i0);
+      const Dims x = *reinterpret_cast<const Dims*>(v + i * vst);
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[e] = fmaf(wi, to_f<T>(x.x[e]), o[e]);
+    }
+  }
+#pragma unroll
+  for (int x = 16; x > 0; x >>= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
+  const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+  Dims y;
+#pragma unroll
+  for (int e = 0; e < E; ++e) y.x[e] = from_f<T>(o[e] * inv);
+  *reinterpret_cast<Dims*>(out) = y;
 }
 
 // Number of BN-key tiles query tile mt reads.

@@ -240,6 +240,7 @@ __global__ void __launch_bounds__(THREADS, 1) fmha2_kernel(const __grid_constant
   uint64_t* drain = o_free + 1;       // [1]  leader
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(drain + 2);
+  [[maybe_unused]] volatile int* again = abort_flag + 1;  // (PK) some row came out non-finite with a finite sum of weights
   static_assert((2 + 2 * KS + 2 * VS + 2 * C::SB + 2 * C::PB + 2) * 8 + 16 <= 256, "barrier area");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -265,6 +266,7 @@ __global__ void __launch_bounds__(THREADS, 1) fmha2_kernel(const __grid_constant
     mbar_init(o_free, 2 * SOFTMAX_WARPS);
     mbar_init(drain, 1);
     *abort_flag = 0;
+    if constexpr (PK) *again = 0;
     fence_barrier_init();
   }
   if (warp == MMA_WARP) {
@@ -625,10 +627,7 @@ __global__ void __launch_bounds__(THREADS, 1) fmha2_kernel(const __grid_constant
           float sum = 0.f;  // (finite unless some value is not)
 #pragma unroll
           for (int e = 0; e < 32; ++e) sum = fmaf(ov[e], 0.f, sum);
-          if (sum != sum && l_tot == l_tot) {
-            prefill::packed_row_exact<T, D>(p, itm.base, row, itm.h, grp * DH + c, 32, orow + c);
-            continue;
-          }
+          if (sum != sum && l_tot == l_tot) *again = 1;
         }
 #pragma unroll
         for (int e = 0; e < 32; e += 8) {
@@ -669,6 +668,18 @@ __global__ void __launch_bounds__(THREADS, 1) fmha2_kernel(const __grid_constant
   if (warp == MMA_WARP) {
     prefill::tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS));
+  }
+  if constexpr (PK) {  // the second look (rare), when nothing waits for this CTA any more: its items' rows again, a warp a row
+    if (*again && !*abort_flag) {
+      for (int rr = 0; rr * ncl < total; ++rr) {
+        const int kidx = item_index(rr, cl, ncl);
+        if (kidx >= total) continue;
+        const Item itm = item_of<D, PK>(p, kidx, rank);
+        const int rows = min(BM, itm.n - itm.r0), end = min(itm.ntiles * BN, p.T - itm.base);
+        for (int x = warp; x < rows; x += THREADS / 32)
+          prefill::packed_row_again<T, D>(p, itm.base, itm.r0 + x, end, itm.h);
+      }
+    }
   }
 }
 
