@@ -70,10 +70,19 @@ int encode_tensor_map(CUtensorMap* map, CUtensorMapDataType dtype, int rank, con
   for (int i = 0; i < rank - 1; ++i)
     if (strides_bytes[i] % 16) return fail(LB2_EINVAL, "TMA stride is not a multiple of 16 bytes");
   cuuint32_t estr[5] = {1, 1, 1, 1, 1};
-  CUresult r = fn(map, dtype, cuuint32_t(rank), const_cast<void*>(base), reinterpret_cast<const cuuint64_t*>(dims),
-                  reinterpret_cast<const cuuint64_t*>(strides_bytes), reinterpret_cast<const cuuint32_t*>(box), estr,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  auto encode = [&] {
+    return fn(map, dtype, cuuint32_t(rank), const_cast<void*>(base), reinterpret_cast<const cuuint64_t*>(dims),
+              reinterpret_cast<const cuuint64_t*>(strides_bytes), reinterpret_cast<const cuuint32_t*>(box), estr,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult r = encode();
+  if (r == CUDA_ERROR_INVALID_CONTEXT) {  // a host thread that has not called the runtime yet has no context bound
+    int dev = 0;
+    LB2_CUDA(cudaGetDevice(&dev));
+    LB2_CUDA(cudaSetDevice(dev));
+    r = encode();
+  }
   if (r != CUDA_SUCCESS) return fail(LB2_EINVAL, "cuTensorMapEncodeTiled failed (code " + std::to_string(r) + ")");
   return LB2_OK;
 }
