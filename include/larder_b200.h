@@ -380,7 +380,7 @@ int lb2_kv8_append(uint8_t* pages, float* scales, const void* k, const int64_t* 
  *   kernel); pages, scales, table as lb2_kv8_append. causal: row t sees keys 0 .. kv_len[b] - T + t, else all; a row
  *   that sees none gives zeros. D in {64, 128, 256}, page in {16, 32, 64, 128}, any Hq / Hkv and T.
  *   workspace: lb2_kv8_attend_workspace_size() bytes, 256-byte aligned, any contents. Calls that share a workspace must
- *   be ordered on one stream.
+ *   be ordered on one stream and made one after the other (a call is two launches, which another thread's may not part).
  * Codes past kv_len are never used, whatever they hold. A kv_len below 0 or past the table's tokens is taken as the nearest
  * of them, and a page id outside [0, num_pages) is not read (the sequence's output is then unspecified): lb2_status
  * reports LB2_EINVAL for both. */
@@ -394,9 +394,9 @@ int lb2_kv8_attend(const void* q, const int64_t* q_st, const uint8_t* pages, con
  * [S + 1] on the device, rising from 0 to T; empty prompts allowed), and row i of a prompt sees its rows 0 .. i.
  *   q, o [Hq, T, D], k, v [Hkv, T, D]: strides [0..1] for H, T; unit on D; dtype LB2_BF16 / F16 (row strides multiples
  *   of 8 elements, 16-byte aligned bases) or LB2_F32 (exact CUDA-core kernel); D in {64, 128, 256}; scale > 0.
- *   workspace: lb2_attn_packed_workspace_size() bytes, 256-byte aligned, any contents.
- * Rows of no prompt (before cu[0], from cu[S] on) give zeros. No value of one prompt reaches another's rows, infinities and NaN among
- * them, nor a later row's an earlier row. */
+ *   workspace: lb2_attn_packed_workspace_size() bytes, 256-byte aligned, any contents; shared as lb2_kv8_attend's.
+ * Rows of no prompt (before cu[0], from cu[S] on) give zeros. No value of one prompt reaches another's rows, infinities
+ * and NaN among them, nor a later row's an earlier row. */
 size_t lb2_attn_packed_workspace_size(int S, int Hq, int Hkv, int T, int D);
 int lb2_attn_packed(const void* q, const int64_t* q_st, const void* k, const int64_t* k_st, const void* v,
                     const int64_t* v_st, void* o, const int64_t* o_st, const int32_t* cu, int S, int Hq, int Hkv, int T,

@@ -44,6 +44,19 @@ def _stream_of(dev):
     return _raw_stream(dev) if _raw_stream is not None else torch.cuda.current_stream(dev).cuda_stream
 
 
+# Scratch of one call, from the caching allocator and given back as soon as the call's kernels are queued: whoever gets the
+# memory next on the stream comes after them. Nothing holds its address for a later call, so that a captured graph owns
+# what it captured and calls of several threads or streams may run at once. (Addresses, not tensors: 0.5 us against 1.5.)
+_scratch = getattr(torch._C, "_cuda_cudaCachingAllocator_raw_alloc", None)
+_scratch_done = getattr(torch._C, "_cuda_cudaCachingAllocator_raw_delete", None)
+if _scratch is None or _scratch_done is None:
+    def _scratch(nbytes, stream):
+        return torch.cuda.caching_allocator_alloc(nbytes, stream=stream)
+
+    def _scratch_done(ptr):
+        torch.cuda.caching_allocator_delete(ptr)
+
+
 def _ptr(t):
     """A tensor's device address as the C ABI's void* (None for NULL); the argtypes convert plain ints."""
     return None if t is None else t.data_ptr()
@@ -527,15 +540,6 @@ def _turns(turns, D, dev, what):
     return R
 
 
-def _stream_workspace(dev, stream, nbytes, tag):
-    """A workspace of the stream's own (the current one): calls on different streams may run at once, and a buffer that has
-    become too small goes back to the allocator of the stream that used it."""
-    ws = _WS.get((dev, (tag, stream)))
-    if ws is None or ws.numel() < nbytes:
-        ws = workspace(torch.device("cuda", dev), nbytes, (tag, stream))
-    return ws
-
-
 def _out_like(out, x, what):
     if out.shape != x.shape or out.dtype is not x.dtype or out.get_device() != x.get_device() or out.stride(-1) != 1:
         raise ValueError(f"{what}: out must have the result's shape, dtype and device, and a unit last stride")
@@ -640,11 +644,13 @@ def kv8_attend(q, pages, scales, table, kv_len, scale, causal=True, out=None):
     if n is None:
         n = _KV8_WS[key] = lib().lb2_kv8_attend_workspace_size(*key[:7])
     stream = _stream_of(dev)
-    ws = _stream_workspace(dev, stream, n, "kv8_attend")
-    rc = lib().lb2_kv8_attend(q.data_ptr(), i64(*qst[:3]), pages.data_ptr(), scales.data_ptr(), table.data_ptr(),
-                              table.stride(0), kv_len.data_ptr(), out.data_ptr(), i64(*out.stride()[:3]), B, Hq, Hkv, T,
-                              D, page, num_pages, max_pages, dtype_code(q), scale, 1 if causal else 0, ws.data_ptr(),
-                              ws.numel(), stream)
+    ws = _scratch(n or 1, stream)
+    try:
+        rc = lib().lb2_kv8_attend(q.data_ptr(), i64(*qst[:3]), pages.data_ptr(), scales.data_ptr(), table.data_ptr(),
+                                  table.stride(0), kv_len.data_ptr(), out.data_ptr(), i64(*out.stride()[:3]), B, Hq, Hkv,
+                                  T, D, page, num_pages, max_pages, dtype_code(q), scale, 1 if causal else 0, ws, n, stream)
+    finally:
+        _scratch_done(ws)
     if rc:
         check(rc, "kv8_attend")
     return out
@@ -677,11 +683,15 @@ def attn_packed(q, k, v, scale, cu, out=None):
         out = torch.empty_like(q)
     else:
         _out_like(out, q, "attn_packed")
+    n = lib().lb2_attn_packed_workspace_size(S, Hq, Hkv, T, D)
     stream = _stream_of(dev)
-    ws = _stream_workspace(dev, stream, lib().lb2_attn_packed_workspace_size(S, Hq, Hkv, T, D), "attn_packed")
-    rc = lib().lb2_attn_packed(q.data_ptr(), i64(*qst[1:3]), k.data_ptr(), i64(*kst[1:3]), v.data_ptr(),
-                               i64(*vst[1:3]), out.data_ptr(), i64(*out.stride()[1:3]), cu.data_ptr(), S, Hq, Hkv, T,
-                               D, dtype_code(q), scale, ws.data_ptr(), ws.numel(), stream)
+    ws = _scratch(n or 1, stream)
+    try:
+        rc = lib().lb2_attn_packed(q.data_ptr(), i64(*qst[1:3]), k.data_ptr(), i64(*kst[1:3]), v.data_ptr(),
+                                   i64(*vst[1:3]), out.data_ptr(), i64(*out.stride()[1:3]), cu.data_ptr(), S, Hq, Hkv,
+                                   T, D, dtype_code(q), scale, ws, n, stream)
+    finally:
+        _scratch_done(ws)
     if rc:
         check(rc, "attn_packed")
     return out
