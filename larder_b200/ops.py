@@ -68,8 +68,8 @@ def _unit_last(t, name):
 
 
 def workspace(device, nbytes, tag):
-    """A 256-byte aligned uint8 buffer of at least nbytes on device, kept per (device, tag) and reused by later
-    calls on the same stream."""
+    """A 256-byte aligned uint8 buffer of at least nbytes on device, kept per (device, tag): for attn_decode_host, whose
+    staging slots outlive a call, and which waits for the copies in flight before it takes a larger one."""
     key = (device.index if device.index is not None else torch.cuda.current_device(), tag)
     ws = _WS.get(key)
     if ws is None or ws.numel() < nbytes:
@@ -146,11 +146,16 @@ def attn_prefill_tiled(q, k, v, scale, mask, gate=None, out=None):
             raise ValueError("gate must be [B, Hq, T, D] in q's dtype")
         _unit_last(gate, "gate")
         gst = i64(*gate.stride()[:3])
-    ws = workspace(q.device, lib().lb2_attn_prefill_tiled_workspace_size(T, N, D), "prefill_tiled")
-    rc = lib().lb2_attn_prefill_tiled(_ptr(q), i64(*q.stride()[:3]), _ptr(k), i64(*k.stride()[:3]), _ptr(v),
-                                      i64(*v.stride()[:3]), _ptr(out), i64(*out.stride()[:3]), _ptr(gate), gst,
-                                      _ptr(m), i64(m.stride(0), m.stride(1)), B, Hq, Hkv, T, N, D, dtype_code(q),
-                                      float(scale), _ptr(ws), ws.numel(), _stream(q))
+    n = lib().lb2_attn_prefill_tiled_workspace_size(T, N, D)
+    stream = _stream(q)
+    ws = _scratch(n or 1, stream)
+    try:
+        rc = lib().lb2_attn_prefill_tiled(_ptr(q), i64(*q.stride()[:3]), _ptr(k), i64(*k.stride()[:3]), _ptr(v),
+                                          i64(*v.stride()[:3]), _ptr(out), i64(*out.stride()[:3]), _ptr(gate), gst,
+                                          _ptr(m), i64(m.stride(0), m.stride(1)), B, Hq, Hkv, T, N, D, dtype_code(q),
+                                          float(scale), ws, n, stream)
+    finally:
+        _scratch_done(ws)
     check(rc, "attn_prefill_tiled")
     return out
 
@@ -181,13 +186,17 @@ def attn_decode(q, k, v, scale, causal=False, kv_len=None, split=0, out=None):
     Hkv, N = k.shape[1], k.shape[2]
     if out is None:
         out = torch.empty((B, Hq, T, D), dtype=q.dtype, device=q.device)
-    ws = workspace(q.device, _decode_ws_bytes(B, Hq, Hkv, T, N, D, split, q.device.index), "decode")
     if kv_len is not None and (kv_len.dtype != torch.int32 or kv_len.numel() != B):
         raise ValueError("kv_len must be int32 [B]")
-    rc = lib().lb2_attn_decode(_ptr(q), i64(*q.stride()[:3]), _ptr(k), i64(*k.stride()[:3]), _ptr(v),
-                               i64(*v.stride()[:3]), _ptr(out), i64(*out.stride()[:3]), _ptr(kv_len), B, Hq, Hkv, T,
-                               N, D, dtype_code(q), float(scale), int(bool(causal)), int(split), _ptr(ws), ws.numel(),
-                               _stream(q))
+    n = _decode_ws_bytes(B, Hq, Hkv, T, N, D, split, q.device.index)
+    stream = _stream(q)
+    ws = _scratch(n or 1, stream)
+    try:
+        rc = lib().lb2_attn_decode(_ptr(q), i64(*q.stride()[:3]), _ptr(k), i64(*k.stride()[:3]), _ptr(v),
+                                   i64(*v.stride()[:3]), _ptr(out), i64(*out.stride()[:3]), _ptr(kv_len), B, Hq, Hkv, T,
+                                   N, D, dtype_code(q), float(scale), int(bool(causal)), int(split), ws, n, stream)
+    finally:
+        _scratch_done(ws)
     check(rc, "attn_decode")
     return out
 
@@ -251,11 +260,15 @@ def decode_partial_into(q, k, v, scale, kv_len, split, part_o_ptr, part_lse_ptr)
     a peer-exchange buffer, which no tensor wraps."""
     B, Hq, T, D = q.shape
     Hkv, N = k.shape[1], k.shape[2]
-    ws = workspace(q.device, _decode_ws_bytes(B, Hq, Hkv, T, N, D, split, q.device.index), "decode_partial")
-    rc = lib().lb2_attn_decode_partial(_ptr(q), i64(*q.stride()[:3]), _ptr(k), i64(*k.stride()[:3]), _ptr(v),
-                                       i64(*v.stride()[:3]), part_o_ptr, part_lse_ptr, _ptr(kv_len), B, Hq, Hkv,
-                                       T, N, D, dtype_code(q), float(scale), int(split), _ptr(ws), ws.numel(),
-                                       _stream(q))
+    n = _decode_ws_bytes(B, Hq, Hkv, T, N, D, split, q.device.index)
+    stream = _stream(q)
+    ws = _scratch(n or 1, stream)
+    try:
+        rc = lib().lb2_attn_decode_partial(_ptr(q), i64(*q.stride()[:3]), _ptr(k), i64(*k.stride()[:3]), _ptr(v),
+                                           i64(*v.stride()[:3]), part_o_ptr, part_lse_ptr, _ptr(kv_len), B, Hq, Hkv,
+                                           T, N, D, dtype_code(q), float(scale), int(split), ws, n, stream)
+    finally:
+        _scratch_done(ws)
     check(rc, "attn_decode_partial")
 
 
@@ -264,11 +277,15 @@ def decode_push(q, k, v, scale, kv_len, split, bufs, R, rank, epoch):
     (bufs: a ctypes uint64 array of the R buffers as mapped here), lb2_attn_decode_push."""
     B, Hq, T, D = q.shape
     Hkv, N = k.shape[1], k.shape[2]
-    ws = workspace(q.device, _decode_ws_bytes(B, Hq, Hkv, T, N, D, split, q.device.index), "decode_partial")
-    rc = lib().lb2_attn_decode_push(_ptr(q), i64(*q.stride()[:3]), _ptr(k), i64(*k.stride()[:3]), _ptr(v),
-                                    i64(*v.stride()[:3]), _ptr(kv_len), B, Hq, Hkv, T, N, D, dtype_code(q),
-                                    float(scale), int(split), _ptr(ws), ws.numel(), bufs, int(R), int(rank),
-                                    int(epoch), _stream(q))
+    n = _decode_ws_bytes(B, Hq, Hkv, T, N, D, split, q.device.index)
+    stream = _stream(q)
+    ws = _scratch(n or 1, stream)
+    try:
+        rc = lib().lb2_attn_decode_push(_ptr(q), i64(*q.stride()[:3]), _ptr(k), i64(*k.stride()[:3]), _ptr(v),
+                                        i64(*v.stride()[:3]), _ptr(kv_len), B, Hq, Hkv, T, N, D, dtype_code(q),
+                                        float(scale), int(split), ws, n, bufs, int(R), int(rank), int(epoch), stream)
+    finally:
+        _scratch_done(ws)
     check(rc, "attn_decode_push")
 
 
@@ -347,10 +364,14 @@ def gdn_chunked(q, k, v, g, beta, state=None):
     y = torch.empty((B, T, Hv, Dv), dtype=q.dtype, device=q.device)
     s_out = torch.empty_like(state)
     nbytes = lib().lb2_gdn_chunked_workspace_size(B, T, Hk, Hv, Dk, Dv)
-    ws = workspace(q.device, nbytes, "gdn_chunked")
-    rc = lib().lb2_gdn_chunked(_ptr(q), _ptr(k), dtype_code(q), _ptr(v), dtype_code(v), _ptr(g), dtype_code(g),
-                               _ptr(beta), dtype_code(beta), _ptr(state), _ptr(s_out), _ptr(y), B, T, Hk, Dk, Hv, Dv,
-                               _ptr(ws), ws.numel(), _stream(q))
+    stream = _stream(q)
+    ws = _scratch(nbytes or 1, stream)
+    try:
+        rc = lib().lb2_gdn_chunked(_ptr(q), _ptr(k), dtype_code(q), _ptr(v), dtype_code(v), _ptr(g), dtype_code(g),
+                                   _ptr(beta), dtype_code(beta), _ptr(state), _ptr(s_out), _ptr(y), B, T, Hk, Dk, Hv,
+                                   Dv, ws, nbytes, stream)
+    finally:
+        _scratch_done(ws)
     check(rc, "gdn_chunked")
     return y, s_out
 
@@ -399,11 +420,15 @@ def qsa_decode(q, k, v, tb, cr, scale, n=None, out=None):
         out = torch.empty_like(q)
     nsel = tb.numel()
     L = lib()
-    ws = workspace(q.device, L.lb2_qsa_decode_workspace_size(nsel, int(cr), n, Hq, Hk, D), "decode")
-    # (the views as [1, Hk, n, D]: a batch stride of Hk heads, for the tensor maps the kernel is given)
-    rc = L.lb2_qsa_decode(_ptr(q), i64(*q.stride()[:3]), _ptr(k), i64(Hk * k.stride(0), *k.stride()[:2]), _ptr(v),
-                          i64(Hk * v.stride(0), *v.stride()[:2]), _ptr(out), i64(*out.stride()[:3]), _ptr(tb), nsel,
-                          int(cr), n, Hq, Hk, D, dtype_code(q), float(scale), _ptr(ws), ws.numel(), _stream(q))
+    nbytes = L.lb2_qsa_decode_workspace_size(nsel, int(cr), n, Hq, Hk, D)
+    stream = _stream(q)
+    ws = _scratch(nbytes or 1, stream)
+    try:  # (the views as [1, Hk, n, D]: a batch stride of Hk heads, for the tensor maps the kernel is given)
+        rc = L.lb2_qsa_decode(_ptr(q), i64(*q.stride()[:3]), _ptr(k), i64(Hk * k.stride(0), *k.stride()[:2]), _ptr(v),
+                              i64(Hk * v.stride(0), *v.stride()[:2]), _ptr(out), i64(*out.stride()[:3]), _ptr(tb), nsel,
+                              int(cr), n, Hq, Hk, D, dtype_code(q), float(scale), ws, nbytes, stream)
+    finally:
+        _scratch_done(ws)
     check(rc, "qsa_decode")
     return out
 

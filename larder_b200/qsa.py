@@ -35,13 +35,19 @@ def qsa_select(q, pooled, offset, cr, k, n_blocks=None, div=None, scores_out=Fal
     q = q.contiguous()
     div = math.sqrt(D) if div is None else float(div)
     top = torch.empty((B, S, k), dtype=torch.int32, device=q.device)
-    ws = ops.workspace(q.device, lib().lb2_qsa_select_workspace_size(B, S, n_blocks), "qsa_select")
-    rc = lib().lb2_qsa_select(ops._ptr(q), ops._ptr(pooled), pooled.stride(0), B, S, H, D, n_blocks, int(offset),
-                              int(cr), int(k), div, ops._ptr(ws), ws.numel(), ops._ptr(top), ops._stream(q))
+    nbytes = lib().lb2_qsa_select_workspace_size(B, S, n_blocks)
+    stream = ops._stream(q)
+    held = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if scores_out else None
+    ws = ops._ptr(held) if scores_out else ops._scratch(nbytes or 1, stream)
+    try:
+        rc = lib().lb2_qsa_select(ops._ptr(q), ops._ptr(pooled), pooled.stride(0), B, S, H, D, n_blocks, int(offset),
+                                  int(cr), int(k), div, ws, nbytes, ops._ptr(top), stream)
+    finally:
+        if held is None:
+            ops._scratch_done(ws)
     check(rc, "qsa_select")
     if scores_out:
-        scores = ws[:B * S * n_blocks * 4].view(torch.float32).view(B, S, n_blocks).clone()
-        return top, scores
+        return top, held[:B * S * n_blocks * 4].view(torch.float32).view(B, S, n_blocks)
     return top
 
 

@@ -1,4 +1,4 @@
-"""Workspaces of the serving calls: a captured graph keeps what it captured whatever is called afterwards, and threads that
+"""Workspaces of the calls: a captured graph keeps what it captured whatever is called afterwards, and threads that
 share a stream keep apart.
 
 Outputs are compared with the same call's made alone, bit for bit: the kernels' results do not depend on what runs beside."""
@@ -38,6 +38,34 @@ def packed(lens, seed=0):
     return lambda: ops.attn_packed(q, k, v, 0.1, cu)
 
 
+def decode(B, n, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    q, k, v = (torch.randn(B, h, t, 128, generator=g).to(BF).cuda() for h, t in ((8, 1), (2, n), (2, n)))
+    lens = i32([n - 11 * b for b in range(B)])
+    return lambda: ops.attn_decode(q, k, v, 0.1, kv_len=lens)
+
+
+def partial(B, n):
+    g = torch.Generator().manual_seed(n)
+    q, k, v = (torch.randn(B, h, t, 128, generator=g).to(BF).cuda() for h, t in ((8, 1), (2, n), (2, n)))
+    return lambda: ops.attn_decode_partial(q, k, v, 0.1)[0]
+
+
+def tiled(T, N):
+    g = torch.Generator().manual_seed(N)
+    q, k, v = (torch.randn(1, h, t, 128, generator=g).to(BF).cuda() for h, t in ((4, T), (2, N), (2, N)))
+    m = (torch.rand(T, N, generator=g) < 0.3).cuda()
+    m[:, 64:512] = False
+    return lambda: ops.attn_prefill_tiled(q, k, v, 0.1, m)
+
+
+def gdn(T):
+    g = torch.Generator().manual_seed(T)
+    q, k, v = (torch.randn(1, T, 2, 128, generator=g).to(BF).cuda() * 0.1 for _ in range(3))
+    a, b = torch.rand(1, T, 2, generator=g).cuda(), torch.rand(1, T, 2, generator=g).cuda()
+    return lambda: ops.gdn_chunked(q, k, v, a, b)[0]
+
+
 def replay_after(small, large):
     """small captured; large called eagerly on the same stream; memory taken and filled; small replayed."""
     want = small().clone()
@@ -68,8 +96,15 @@ def test_replay_after_more_prompts():
     replay_after(packed([40, 300]), packed([30] * 2500))
 
 
+@pytest.mark.parametrize("make,small,large", [(decode, (2, 500), (24, 6000)), (partial, (1, 900), (16, 5000)),
+                                              (tiled, (200, 700), (1500, 4000)), (gdn, (100,), (3000,))])
+def test_replay_after_a_larger_call(make, small, large):
+    replay_after(make(*small), make(*large))
+
+
 def test_threads_on_one_stream():
-    calls = [attend(3, 700 + 100 * i, seed=i) for i in range(4)] + [packed([50 + 90 * i, 20, 333], seed=i) for i in range(4)]
+    calls = [decode(2, 600 + 150 * i, seed=i) for i in range(3)]
+    calls += [attend(3, 700 + 100 * i, seed=i) for i in range(4)] + [packed([50 + 90 * i, 20, 333], seed=i) for i in range(4)]
     want = [f().clone() for f in calls]
     torch.cuda.synchronize()
     got = [[] for _ in calls]
