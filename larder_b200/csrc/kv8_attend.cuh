@@ -33,6 +33,8 @@
 // (attn_rows.cuh), which reads only what the row sees.
 #pragma once
 
+#include <cfloat>
+
 #include "attn_rows.cuh"
 #include "common.cuh"
 #include "kv8.cuh"
@@ -448,7 +450,7 @@ __global__ void __launch_bounds__(Cfg<D, NT, RG, MK, KG>::THREADS, 1)
     float m_run[NT][2], l_run[NT][2], acc[NT][DW / 16][4];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      m_run[nt][0] = m_run[nt][1] = -INFINITY;
+      m_run[nt][0] = m_run[nt][1] = -FLT_MAX;
       l_run[nt][0] = l_run[nt][1] = 0.f;
 #pragma unroll
       for (int j = 0; j < DW / 16; ++j) acc[nt][j][0] = acc[nt][j][1] = acc[nt][j][2] = acc[nt][j][3] = 0.f;
@@ -565,7 +567,8 @@ __global__ void __launch_bounds__(Cfg<D, NT, RG, MK, KG>::THREADS, 1)
       }
       // Scores in base 2 with the values' scale, against the row's running maximum less TOP (what m_run holds). It moves
       // only when a score passes the maximum by more than 8 (weights up to 2^15 lose nothing in f16), so most tiles need no
-      // exchange between lanes; before a row's first key it is -inf, which every score passes.
+      // exchange between lanes; before a row's first key it is the least finite number, which every score but -inf passes
+      // (-inf itself would make keys whose scores are all -inf NaN).
       const bool whole = kbase + 16 * MK - 1 <= all_see;
       float t[MK][NT][4];
       auto against = [&] {  // t = score - (maximum - TOP); the lane's largest
@@ -605,7 +608,7 @@ __global__ void __launch_bounds__(Cfg<D, NT, RG, MK, KG>::THREADS, 1)
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
             mx -= TOP;
-            const float corr = ex2(m_run[nt][e] - (mx == -INFINITY ? 0.f : mx));
+            const float corr = ex2(m_run[nt][e] - mx);
             m_run[nt][e] = mx;
             l_run[nt][e] *= corr;
 #pragma unroll
@@ -708,9 +711,9 @@ __global__ void __launch_bounds__(Cfg<D, NT, RG, MK, KG>::THREADS, 1)
           float f[2], g[2];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const float mn = fmaxf(m_run[nt][e], xm[e]), mu = mn == -INFINITY ? 0.f : mn;
-            f[e] = ex2(m_run[nt][e] - mu);
-            g[e] = ex2(xm[e] - mu);
+            const float mn = fmaxf(m_run[nt][e], xm[e]);
+            f[e] = ex2(m_run[nt][e] - mn);
+            g[e] = ex2(xm[e] - mn);
             m_run[nt][e] = mn;
             l_run[nt][e] = l_run[nt][e] * f[e] + xl[e] * g[e];
           }
