@@ -568,6 +568,8 @@ __global__ void __launch_bounds__(THREADS, 1) fmha2_kernel(const __grid_constant
               pk[c / 2] = pack2<T>(e0, e1);
             }
           }
+          // a NaN score that ex2_fma made FLT_MAX (its weight is infinite in 16 bits, and every column with it)
+          if (!((ls4[0] + ls4[1]) + (ls4[2] + ls4[3]) <= 1e30f)) ls4[0] = NAN;
         }
         // P_j into P buffer g % PB (last read by PV_{g-PB}): this group's HC keys at columns grp HC / 2 ...
         const int pbuf = g % C::PB;
