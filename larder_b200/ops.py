@@ -565,6 +565,17 @@ def _turns(turns, D, dev, what):
     return R
 
 
+def _new_like(x):
+    """An uninitialised tensor like x [B, H, T, D] with a unit last stride, and its strides. (empty_like follows the order of
+    x's strides, which for rows that overlap in memory may put D elsewhere.)"""
+    out = torch.empty_like(x)
+    st = out.stride()
+    if st[3] != 1:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        st = out.stride()
+    return out, st
+
+
 def _out_like(out, x, what):
     if out.shape != x.shape or out.dtype is not x.dtype or out.get_device() != x.get_device() or out.stride(-1) != 1:
         raise ValueError(f"{what}: out must have the result's shape, dtype and device, and a unit last stride")
@@ -585,11 +596,7 @@ def rope(x, positions, turns, layout="half", amp=1.0, inverse=False, out=None):
     ps = positions.shape
     _int32(positions, (T,) if len(ps) == 1 else (B, T), dev, "rope: positions")
     if out is None:
-        out = torch.empty_like(x)
-        ost = out.stride()
-        if ost[3] != 1:
-            out = torch.empty((B, H, T, D), dtype=x.dtype, device=x.device)
-            ost = out.stride()
+        out, ost = _new_like(x)
     else:
         _out_like(out, x, "rope")
         ost = out.stride()
@@ -661,9 +668,10 @@ def kv8_attend(q, pages, scales, table, kv_len, scale, causal=True, out=None):
         raise ValueError("kv8_attend: Hq must be a multiple of the cache's Hkv")
     _int32(kv_len, (B,), dev, "kv8_attend: kv_len")
     if out is None:
-        out = torch.empty_like(q)
+        out, ost = _new_like(q)
     else:
         _out_like(out, q, "kv8_attend")
+        ost = out.stride()
     key = (B, Hq, Hkv, T, D, page, max_pages, dev)
     n = _KV8_WS.get(key)
     if n is None:
@@ -672,7 +680,7 @@ def kv8_attend(q, pages, scales, table, kv_len, scale, causal=True, out=None):
     ws = _scratch(n or 1, stream)
     try:
         rc = lib().lb2_kv8_attend(q.data_ptr(), i64(*qst[:3]), pages.data_ptr(), scales.data_ptr(), table.data_ptr(),
-                                  table.stride(0), kv_len.data_ptr(), out.data_ptr(), i64(*out.stride()[:3]), B, Hq, Hkv,
+                                  table.stride(0), kv_len.data_ptr(), out.data_ptr(), i64(*ost[:3]), B, Hq, Hkv,
                                   T, D, page, num_pages, max_pages, dtype_code(q), scale, 1 if causal else 0, ws, n, stream)
     finally:
         _scratch_done(ws)
@@ -705,15 +713,16 @@ def attn_packed(q, k, v, scale, cu, out=None):
     if Hkv == 0 or Hq == 0 or Hq % Hkv:
         raise ValueError("attn_packed: Hq must be a multiple of Hkv")
     if out is None:
-        out = torch.empty_like(q)
+        out, ost = _new_like(q)
     else:
         _out_like(out, q, "attn_packed")
+        ost = out.stride()
     n = lib().lb2_attn_packed_workspace_size(S, Hq, Hkv, T, D)
     stream = _stream_of(dev)
     ws = _scratch(n or 1, stream)
     try:
         rc = lib().lb2_attn_packed(q.data_ptr(), i64(*qst[1:3]), k.data_ptr(), i64(*kst[1:3]), v.data_ptr(),
-                                   i64(*vst[1:3]), out.data_ptr(), i64(*out.stride()[1:3]), cu.data_ptr(), S, Hq, Hkv,
+                                   i64(*vst[1:3]), out.data_ptr(), i64(*ost[1:3]), cu.data_ptr(), S, Hq, Hkv,
                                    T, D, dtype_code(q), scale, ws, n, stream)
     finally:
         _scratch_done(ws)
