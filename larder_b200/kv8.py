@@ -22,9 +22,10 @@ class Step:
     cu int32 [B + 1] (row offsets of the new tokens packed), positions int32 (of the new tokens: [B, T] where every
     sequence has T, else packed [rows])."""
 
-    def __init__(self, table, start, kv_len, cu, positions, counts):
+    def __init__(self, table, start, kv_len, cu, positions, counts, spans=()):
         self.table, self.start, self.kv_len, self.cu = table, start, kv_len, cu
         self.positions, self.counts = positions, counts
+        self.spans = spans  # (handle, tokens before the call, new tokens) of each sequence, on the host
 
 
 class Cache:
@@ -37,6 +38,7 @@ class Cache:
         self.scales = torch.zeros((num_pages, 2, hk), dtype=torch.float32, device=device)
         self._free = list(range(num_pages - 1, -1, -1))
         self._seqs = {}  # handle -> [page ids, tokens]
+        self._missing = {}  # handle -> first positions of the steps whose append was refused
         self._next = 0
 
     @property
@@ -53,6 +55,7 @@ class Cache:
     def drop(self, handle):
         """Ends a sequence; its pages may be handed out again."""
         self._free.extend(reversed(self._seqs.pop(handle)[0]))
+        self._missing.pop(handle, None)
 
     def length(self, handle):
         return self._seqs[handle][1]
@@ -66,6 +69,14 @@ class Cache:
         self._free.extend(reversed(ids[keep:]))
         del ids[keep:]
         self._seqs[handle][1] = n
+        for s in [s for s in self._missing.get(handle, ()) if s >= n]:
+            self._found(handle, s)
+
+    def _found(self, handle, start):
+        starts = self._missing.get(handle, set())
+        starts.discard(start)
+        if not starts:
+            self._missing.pop(handle, None)
 
     def step(self, handles, counts):
         """Reserves room for counts[i] new tokens of handles[i] and returns the call's Step. Nothing is reserved, and a
@@ -93,22 +104,38 @@ class Cache:
         t = torch.tensor(flat, dtype=torch.int32).to(self.device)
         table, start_t, len_t, cu_t, pos = t.split([B * width, B, B, B + 1, len(positions)])
         same = B and all(c == counts[0] for c in counts)
-        return Step(table.view(B, width), start_t, len_t, cu_t, pos.view(B, counts[0]) if same else pos, list(counts))
+        return Step(table.view(B, width), start_t, len_t, cu_t, pos.view(B, counts[0]) if same else pos, list(counts),
+                    list(zip(handles, start, counts)))
 
     def append(self, step, k, v, rope=None, packed=False):
         """The step's new tokens: k / v [B, hk, T, d] where every sequence has T of them, or, packed, [1, hk, rows, d].
-        Keys are rotated by their positions when a Rope is given."""
-        kw = {} if rope is None else {"turns": rope.turns, "layout": rope.layout, "amp": rope.amp}
-        if packed:
-            if k.shape[2] != sum(step.counts):
-                raise ValueError(f"kv8: {sum(step.counts)} packed rows expected, got {k.shape[2]}")
-            kw["cu"] = step.cu
-        elif any(c != k.shape[2] for c in step.counts):
-            raise ValueError("kv8: sequences with different counts go in packed")
-        ops.kv8_append(self.pages, self.scales, k, v, step.table, step.start, **kw)
+        Keys are rotated by their positions when a Rope is given. After a refused append the step's tokens still count:
+        append them again, or trim them away; attend refuses sequences that lack them."""
+        try:
+            kw = {} if rope is None else {"turns": rope.turns, "layout": rope.layout, "amp": rope.amp}
+            if packed:
+                if k.shape[2] != sum(step.counts):
+                    raise ValueError(f"kv8: {sum(step.counts)} packed rows expected, got {k.shape[2]}")
+                kw["cu"] = step.cu
+            elif any(c != k.shape[2] for c in step.counts):
+                raise ValueError("kv8: sequences with different counts go in packed")
+            ops.kv8_append(self.pages, self.scales, k, v, step.table, step.start, **kw)
+        except Exception:  # the step's tokens count, but the pages do not hold them
+            for h, s, n in step.spans:
+                if n and h in self._seqs:
+                    self._missing.setdefault(h, set()).add(s)
+            raise
+        if self._missing:
+            for h, s, n in step.spans:
+                if n:
+                    self._found(h, s)
 
     def attend(self, step, q, scale, causal=True, out=None):
         """q [B, hq, T, d], the queries of each sequence's last T tokens, over everything cached."""
+        if self._missing:
+            for h, s, n in step.spans:
+                if any(x < s + n for x in self._missing.get(h, ())):
+                    raise ValueError(f"kv8: sequence {h} has tokens that were not appended (their append was refused)")
         return ops.kv8_attend(q, self.pages, self.scales, step.table, step.kv_len, scale, causal, out)
 
 
