@@ -585,7 +585,12 @@ def rope(x, positions, turns, layout="half", amp=1.0, inverse=False, out=None):
     """x [B, H, T, D] with the first 2 * len(turns) dims of each head rotated by the rows' positions (lb2_rope).
 
     positions int32 [B, T] or [T]; turns int64 [R / 2] (larder_b200.rope.Rope(...).turns); layout "half" (pairs i,
-    i + R / 2) or "interleaved" (2 i, 2 i + 1); inverse=True is the gradient. out may be x."""
+    i + R / 2) or "interleaved" (2 i, 2 i + 1); inverse=True is the gradient, which autograd takes where x asks for one.
+    out may be x."""
+    if x.requires_grad and torch.is_grad_enabled():
+        if out is not None:
+            raise ValueError("rope: out= does not take part in a graph; x requires a gradient")
+        return _Rope.apply(x, positions, turns, layout, amp, inverse)
     dev, st = x.get_device(), x.stride()
     if dev < 0:
         _cuda(x)
@@ -608,6 +613,23 @@ def rope(x, positions, turns, layout="half", amp=1.0, inverse=False, out=None):
     if rc:
         check(rc, "rope")
     return out
+
+
+class _Rope(torch.autograd.Function):
+    """rope in autograd's graph: the gradient is the transposed map, the inverse rotation with the same amp."""
+
+    @staticmethod
+    def forward(ctx, x, positions, turns, layout, amp, inverse):
+        ctx.save_for_backward(positions, turns)
+        ctx.how = layout, amp, inverse
+        return rope(x, positions, turns, layout, amp, inverse)
+
+    @staticmethod
+    def backward(ctx, dy):
+        layout, amp, inverse = ctx.how
+        if dy.stride(-1) != 1:
+            dy = dy.contiguous()
+        return rope(dy, *ctx.saved_tensors, layout, amp, not inverse), None, None, None, None, None
 
 
 def _kv8_pool(pages, scales, table, what):
@@ -657,7 +679,8 @@ _KV8_WS = {}  # (B, Hq, Hkv, T, D, page, max_pages, device index) -> workspace b
 
 def kv8_attend(q, pages, scales, table, kv_len, scale, causal=True, out=None):
     """Attention of q [B, Hq, T, D] over each sequence's first kv_len[b] cached tokens (lb2_kv8_attend); kv_len int32
-    [B] counts the call's own tokens, which are already appended. causal: row t sees keys 0 .. kv_len - T + t."""
+    [B] counts the call's own tokens, which are already appended. causal: row t sees keys 0 .. kv_len - T + t. For
+    inference: the result is in no autograd graph."""
     (num_pages, _, Hkv, page, D), (B, max_pages), dev = _kv8_pool(pages, scales, table, "kv8_attend")
     qs, qst = q.shape, q.stride()
     if len(qs) != 4 or qs[0] != B or qs[3] != D or q.get_device() != dev or qst[3] != 1:
@@ -691,7 +714,8 @@ def kv8_attend(q, pages, scales, table, kv_len, scale, causal=True, out=None):
 
 def attn_packed(q, k, v, scale, cu, out=None):
     """Causal attention over prompts packed on one row axis (lb2_attn_packed): q [1, Hq, T, D], k / v [1, Hkv, T, D],
-    cu int32 [S + 1] on the device, prompt s being rows cu[s] .. cu[s + 1] - 1."""
+    cu int32 [S + 1] on the device, prompt s being rows cu[s] .. cu[s + 1] - 1. For inference: the result is in no autograd
+    graph."""
     dev, qs, ks = q.get_device(), q.shape, k.shape
     qst, kst, vst = q.stride(), k.stride(), v.stride()
     if dev < 0:

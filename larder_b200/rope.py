@@ -75,7 +75,8 @@ class Rope:
         self.turns = turns_of(self.w, device)
 
     def apply(self, x, positions, inverse=False, out=None):
-        """x [B, H, T, D] rotated by positions int32 [B, T] or [T]; inverse=True gives the gradient."""
+        """x [B, H, T, D] rotated by positions int32 [B, T] or [T], in autograd's graph where x requires a gradient;
+        inverse=True is the gradient by hand."""
         return ops.rope(x, positions, self.turns, self.layout, self.amp, inverse, out)
 
 
