@@ -251,11 +251,22 @@ __device__ __noinline__ void packed_row_again(const Params& p, int base, int row
 #pragma unroll
   for (int e = 0; e < E; ++e) any |= bad[e] = !isfinite(to_f<T>(was.x[e]));
   if (!__any_sync(0xffffffffu, any)) return;
-  any = false;
-  for (int i = row + 1; i < end; ++i) {
-    const Dims w = *reinterpret_cast<const Dims*>(v + i * vst);
+  // (rows of values come eight at a time, which hides most of their latency)
+  auto values = [&](int i, int last, Dims* x) {
 #pragma unroll
-    for (int e = 0; e < E; ++e) any |= bad[e] && !isfinite(to_f<T>(w.x[e]));
+    for (int u = 0; u < 8; ++u) {
+      if (i + u <= last) x[u] = *reinterpret_cast<const Dims*>(v + (i + u) * vst);
+      else memset(&x[u], 0, sizeof(Dims));
+    }
+  };
+  any = false;
+  for (int i = row + 1; i < end; i += 8) {
+    Dims x[8];
+    values(i, end - 1, x);
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+#pragma unroll
+      for (int e = 0; e < E; ++e) any |= bad[e] && !isfinite(to_f<T>(x[u].x[e]));
   }
   if (!__any_sync(0xffffffffu, any)) return;
   float o[E], m = -INFINITY, l = 0.f;
@@ -266,6 +277,7 @@ __device__ __noinline__ void packed_row_again(const Params& p, int base, int row
     if (i0 + lane <= row) {
       const T* kr = k + (i0 + lane) * kst;
       s = 0.f;
+#pragma unroll 4
       for (int d = 0; d < D; d += 8) {
         const uint4 a = *reinterpret_cast<const uint4*>(q + d), b = *reinterpret_cast<const uint4*>(kr + d);
 #pragma unroll
@@ -282,11 +294,15 @@ __device__ __noinline__ void packed_row_again(const Params& p, int base, int row
     l = l * f + w;
 #pragma unroll
     for (int e = 0; e < E; ++e) o[e] *= f;
-    for (int i = i0; i <= min(i0 + 31, row); ++i) {
-      const float wi = __shfl_sync(0xffffffffu, w, i - i0);
-      const Dims x = *reinterpret_cast<const Dims*>(v + i * vst);
+    for (int i = i0; i <= min(i0 + 31, row); i += 8) {
+      Dims x[8];
+      values(i, row, x);
 #pragma unroll
-      for (int e = 0; e < E; ++e) o[e] = fmaf(wi, to_f<T>(x.x[e]), o[e]);
+      for (int u = 0; u < 8; ++u) {
+        const float wi = __shfl_sync(0xffffffffu, w, i - i0 + u);  // (0 past the row)
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] = fmaf(wi, to_f<T>(x[u].x[e]), o[e]);
+      }
     }
   }
 #pragma unroll
