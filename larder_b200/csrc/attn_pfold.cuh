@@ -6,8 +6,13 @@
 // products. So the kernel is persistent, each CTA walking the plan's blocks (heaviest first) in rounds, with Q, K and V of
 // the next block on their way and its first S computed while this one's O is written; and at head dims 64 and 128 a CTA
 // takes half an SM's tensor memory and shared memory, so that two share the SM, one's products under the other's softmax.
-// Measured (bf16, 32 / 8 heads x 128): 33 prompts of 8 to 441 rows, 4001 in all, 35.6 us (128 us with a CTA a block of one
-// head, 55 us not persistent); 982 TFLOP/s at prompts of 4096 rows.
+// Measured (bf16, 32 / 8 heads x 128): 33 prompts of 8 to 441 rows, 4001 in all, 34 us on the device with the plan's launch
+// (128 us with a CTA a block of one head, 55 us not persistent); 982 TFLOP/s at prompts of 4096 rows.
+//
+// A value that is infinite or NaN spoils the rows before it that share its tiles (0 times NaN): the epilogue only notes that
+// a row came out non-finite, and at its end, when no warp waits for another any more, the CTA looks at its rows again
+// (packed_row_again). That costs calls without such values nothing. One prompt of 4096 rows takes 0.15 ms; 0.33 ms with an
+// infinity in its first row, which all rows see; 7.7 ms with a NaN in its last, where a block's rows are taken again.
 //
 // Roles (320 threads): warps 0-7 softmax and epilogue (warp w: TMEM lanes of quarter w % 4, key / O column half w / 4),
 // warp 8 TMA (lane 0 Q and K, lane 1 V), warp 9 issues the MMAs. S_j = Q K_j^T and O += P_j V_j as in attn_prefill.cuh;

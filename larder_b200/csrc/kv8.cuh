@@ -286,10 +286,14 @@ struct Pair<__half> {
 // the rotated half layout a group and its partners R / 2 on, elsewhere neighbours; a thread has one unit of K rows. The
 // block takes `hpb` heads in turn, the next one's loads in flight while it works: the angles of its rows serve them all
 // (in shared memory, each thread its own).
-// Bound for long prompts by instruction issue and HBM alike: 2 x 16384 tokens of 8 heads x 128 (f16) take 50 us, 4050 GB/s of
-// the 2 bytes read and 1 written a value; the same loads and stores without rotation and conversion take 35 us. Two
+// Bound for long prompts by latency: 2 x 16384 tokens of 8 heads x 128 (f16) take 50 us, 4050 GB/s of the 2 bytes read and 1
+// written a value, with half the issue slots used (49 %), no pipe above 35 % and 31 % of the warps resident, which wait for
+// loads and at each head's barrier; the same loads and stores without rotation and conversion take 35 us. Two
 // products an instruction (f32x2) and word-wise maxima keep a value of V at about 4 instructions, one of K at 7. Single
 // tokens are bound by the chain start -> table -> scale (64 sequences: 3 us).
+// Pages of 128 tokens at head dim 256 take 1024 threads of 64 registers, which spill (bytes stored / loaded: bf16 168 / 124,
+// f16 168 / 156, fp32 480 / 348): 2 x 8192 tokens of 4 heads take 47 us in bf16 (2130 GB/s), 88 us in fp32 (1910). The 256
+// threads of three blocks an SM have 80 and spill a little (32 / 36, 32 / 56, 252 / 176); the other forms spill nothing.
 template <typename T, int THREADS, int K, int OCC = THREADS == 256 ? 3 : 1>
 __global__ void __launch_bounds__(THREADS, OCC) append_kernel(const AppendParams p) {
   constexpr int WARPS = THREADS / 32;

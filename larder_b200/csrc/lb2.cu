@@ -1584,8 +1584,10 @@ static int kv8_append_run(kv8::AppendParams& p, bool wide, int64_t blocks, cudaS
   if (!wide) return go(kv8::append_any_kernel<T>, 128, 0);
   const int upr = p.D / 16;
   if (!p.cu && int64_t(p.T) * upr <= 32) return go(kv8::append_kernel<T, 32, 1>, 32, 32 * 1 * 64);  // a few tokens: a warp a piece
-  // Heads a block, up to four where that leaves every SM two blocks: they share the angles and the block's start (2 x 16384
-  // tokens of 8 heads: 77 us with one, 59 with two, 50 with four or eight).
+  // Heads a block, up to four where that leaves every SM two blocks: they share the angles and the block's start, which is
+  // worth more than the warps that small pages' blocks leave idle. With one, two and four heads a block, 2 x 16384 tokens of
+  // 8 heads x 128 take 80, 58 and 50 us (f16, pages of 64), 139, 96 and 75 us (bf16, pages of 16, 64 threads a block); 4100
+  // packed tokens of 4 heads 10.4, 7.8 and 6.3 us; 2 x 8192 of fp32 66, 61 and 61 us.
   while (p.hpb < 4 && blocks * 2 * p.Hkv >= int64_t(148) * 2 * 2 * p.hpb) p.hpb *= 2;
   switch (p.page * upr) {  // a page's units over the threads, at most two a thread
     case 64: return go(kv8::append_kernel<T, 64, 1>, 64, 64 * 1 * 64);
@@ -1839,8 +1841,10 @@ struct Layout {
 // Blocks of 128 rows over the folded heads (attn_pfold.cuh) at head dims 64 and 128, whatever the length: two CTAs share an
 // SM and hide each other's softmax (32 / 8 heads x 128: 316 against the pairs' 128 TFLOP/s at prompts of 256, 868 against
 // 540 at 2048, 982 against 698 at 4096). At head dim 256 one CTA fills an SM's tensor memory, and from some thousand rows
-// on pairs of CTAs, which halve the K / V bytes an SM takes a product, are faster (16 / 2 heads: 900 folded against 819 at
-// 2048, 1009 against 1087 at 4096). The lengths are on the device, so the mean length decides.
+// on pairs of CTAs, which halve the K / V bytes an SM takes a product, are faster. The lengths are on the device, so the mean
+// length decides. TFLOP/s folded / by pairs of 16 query heads x 256 at 2048, 3000, 4096 and 8192 rows: 984 / 840, 1040 / 958,
+// 1101 / 1098, 1170 / 1273 with 2 KV heads (4 are alike), 760 / 777, 833 / 859, 930 / 975, 1060 / 1163 with 16, where no
+// heads fold. The crossing lies near 4100 rows with folded heads and near 1900 without; 3000 is between the two.
 static bool pair_form(int64_t S, int64_t T, int D) { return D == 256 && T > PAIR_MEAN * S; }
 static int fold_of(int G) { return G <= 64 ? G : 1; }
 static int block_rows(bool pair, int G) { return pair ? 2 * prefill::BM : prefill::BM / fold_of(G); }
