@@ -378,7 +378,7 @@ int lb2_kv8_append(uint8_t* pages, float* scales, const void* k, const int64_t* 
  * [B]; this call's own among them).
  *   q, o [B, Hq, T, D], strides q_st / o_st for B, H, T; unit on D; dtype LB2_BF16 / F16, or LB2_F32 (exact CUDA-core
  *   kernel); pages, scales, table as lb2_kv8_append. causal: row t sees keys 0 .. kv_len[b] - T + t, else all; a row
- *   that sees none gives zeros. D in {64, 128, 256}, page in {16, 32, 64, 128}, any Hq / Hkv and T.
+ *   that sees none gives zeros. D in {64, 128, 256}, page in {16, 32, 64, 128}, any Hq / Hkv and T with Hq / Hkv T < 2^20.
  *   workspace: lb2_kv8_attend_workspace_size() bytes, 256-byte aligned, any contents. Calls that share a workspace must
  *   be ordered on one stream and made one after the other (a call is two launches, which another thread's may not part).
  * Codes past kv_len are never used, whatever they hold. A kv_len below 0 or past the table's tokens is taken as the nearest
