@@ -390,6 +390,47 @@ int lb2_kv8_attend(const void* q, const int64_t* q_st, const uint8_t* pages, con
                    int D, int page, int num_pages, int max_pages, int dtype, float scale, int causal, void* workspace,
                    size_t workspace_bytes, void* stream);
 
+/* Attention of packed chunks of new tokens over the paged 8-bit cache: sequence b's new tokens are rows cu[b] ..
+ * cu[b + 1] - 1 (int32 [B + 1] on the device, rising within 0 .. T; empty sequences allowed), the last ones of its
+ * kv_len[b] cached tokens (int32 [B]; already appended). o = softmax(scale q K^T) V; causal: row i of n sees keys
+ * 0 .. kv_len[b] - n + i, else all kv_len[b]; a row that sees none gives zeros, as do rows of no sequence (before cu[0],
+ * from cu[B] on).
+ *   q, o [Hq, T, D], strides [0..1] for H, T; unit on D; dtype LB2_BF16 / F16, or LB2_F32 (exact CUDA-core kernel);
+ *   pages, scales, table as lb2_kv8_append; page, D as lb2_kv8_attend; T Hq < 2^30; any finite scale.
+ *   workspace: lb2_kv8_attend_packed_workspace_size() bytes, 256-byte aligned, any contents; shared as lb2_kv8_attend's.
+ * Codes past kv_len are never used, nor does a later token's value reach a row that does not see it, NaN codes among them.
+ * lb2_status reports LB2_EINVAL for a kv_len or cu out of range (the nearest value in range is taken) and for page ids
+ * outside [0, num_pages), which are not read: such a page counts as zeros. */
+size_t lb2_kv8_attend_packed_workspace_size(int B, int Hq, int Hkv, int T, int D);
+int lb2_kv8_attend_packed(const void* q, const int64_t* q_st, const uint8_t* pages, const float* scales,
+                          const int32_t* table, int64_t table_st, const int32_t* kv_len, const int32_t* cu, void* o,
+                          const int64_t* o_st, int B, int Hq, int Hkv, int T, int D, int page, int num_pages,
+                          int max_pages, int dtype, float scale, int causal, void* workspace, size_t workspace_bytes,
+                          void* stream);
+
+/* Copy n pages, codes and scales: page dst[i] of the pool `to` becomes page src[i] of the pool `from` (int32 [n] on the
+ * device; the pools may be one, and share Hkv, page and D). Both pools 16-byte aligned. No page may be in dst twice, and in
+ * one pool none in both dst and src but at the same i: such pages' contents are unspecified. A pair with an id out of range
+ * is skipped and lb2_status reports LB2_EINVAL. */
+int lb2_kv8_copy(const uint8_t* from_pages, const float* from_scales, int from_num, uint8_t* to_pages, float* to_scales,
+                 int to_num, const int32_t* src, const int32_t* dst, int n, int Hkv, int page, int D, void* stream);
+
+/* Compact sequences of the paged 8-bit cache: the held tokens at positions keep[cu[b]] .. keep[cu[b + 1] - 1] of sequence b
+ * become its positions start[b], start[b] + 1, .. in other pages.
+ *   table int32 [B, max_pages] (row stride table_st): the sequences as they are; to int32 [B, max_to] (row stride to_st):
+ *   the compacted sequences' pages, position p in pages[to[b][p / page]]; start int32 [B], each a page's beginning;
+ *   keep int32 [T], cu int32 [B + 1] rising within 0 .. T: any positions in any order, also the same one twice.
+ *   turns as lb2_rope with R dims: keys are turned by (new - old position) * turns; or R = 0.
+ * The codes are those that lb2_kv8_append would leave in fresh pages for the held values (keys: turned, in fp32): a scale for
+ * each page and head, the least power of two s with max |x| <= 448 s; NaN stays NaN. What lies past the last token of a page
+ * is left as it is. No page may be written twice or both read and written: such pages' contents are unspecified. A page id
+ * or position out of range, or a start inside a page, is skipped (a token that cannot be read counts as zeros) and lb2_status
+ * reports LB2_EINVAL. */
+int lb2_kv8_compact(uint8_t* pages, float* scales, const int32_t* table, int64_t table_st, const int32_t* keep,
+                    const int32_t* cu, const int32_t* to, int64_t to_st, const int32_t* start, const uint64_t* turns,
+                    int B, int Hkv, int T, int D, int R, int page, int num_pages, int max_pages, int max_to,
+                    int interleaved, void* stream);
+
 /* Causal attention over S whole prompts packed on one row axis: prompt s is rows cu[s] .. cu[s + 1] - 1 (int32
  * [S + 1] on the device, rising from 0 to T; empty prompts allowed), and row i of a prompt sees its rows 0 .. i.
  *   q, o [Hq, T, D], k, v [Hkv, T, D]: strides [0..1] for H, T; unit on D; dtype LB2_BF16 / F16 (row strides multiples

@@ -75,6 +75,12 @@ SIGNATURES = {
     "lb2_kv8_attend_workspace_size": ([_i, _i, _i, _i, _i, _i, _i], _sz),
     "lb2_kv8_attend": ([_p, _i64p, _p, _p, _p, ctypes.c_int64, _p, _p, _i64p, _i, _i, _i, _i, _i, _i, _i, _i, _i, _f, _i,
                         _p, _sz, _p], _i),
+    "lb2_kv8_attend_packed_workspace_size": ([_i, _i, _i, _i, _i], _sz),
+    "lb2_kv8_attend_packed": ([_p, _i64p, _p, _p, _p, ctypes.c_int64, _p, _p, _p, _i64p, _i, _i, _i, _i, _i, _i, _i, _i, _i,
+                               _f, _i, _p, _sz, _p], _i),
+    "lb2_kv8_copy": ([_p, _p, _i, _p, _p, _i, _p, _p, _i, _i, _i, _i, _p], _i),
+    "lb2_kv8_compact": ([_p, _p, _p, ctypes.c_int64, _p, _p, _p, ctypes.c_int64, _p, _p, _i, _i, _i, _i, _i, _i, _i, _i, _i,
+                         _i, _p], _i),
     "lb2_attn_packed_workspace_size": ([_i, _i, _i, _i, _i], _sz),
     "lb2_attn_packed": ([_p, _i64p, _p, _i64p, _p, _i64p, _p, _i64p, _p, _i, _i, _i, _i, _i, _i, _f, _p, _sz, _p], _i),
 }

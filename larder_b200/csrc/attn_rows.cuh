@@ -115,6 +115,57 @@ __global__ void __launch_bounds__(128) paged_kernel(const PagedParams p) {
   for (int e = 0; e < E; ++e) o[e] = from_f<T>(x[e]);
 }
 
+struct ChunkParams {
+  PagedParams a;  // (B, T: rows of the packed axis; strides [1..2])
+  const int32_t* cu;
+};
+
+// A sequence's rows [lo, hi) of T and its cached tokens, from cu and kv_len taken into range (`report`: say so).
+struct ChunkRange {
+  int lo, hi, len;
+};
+__device__ __forceinline__ ChunkRange chunk_range(const ChunkParams& p, int b, int where, bool report) {
+  const int c0 = p.cu[b], c1 = p.cu[b + 1], n = p.a.kv_len[b];
+  ChunkRange r;
+  r.lo = min(max(c0, 0), p.a.T);
+  r.hi = min(max(c1, r.lo), p.a.T);
+  r.len = int(min(int64_t(max(n, 0)), int64_t(p.a.max_pages) * p.a.page));
+  if (report && (r.lo != c0 || r.hi != c1 || r.len != n)) report_bad_index(where);
+  return r;
+}
+
+// The keys that row `row` of a sequence's range sees: the first so many.
+__device__ __forceinline__ int chunk_seen(const ChunkParams& p, const ChunkRange& r, int row) {
+  return p.a.causal ? max(r.len - (r.hi - 1 - row), 0) : r.len;
+}
+
+constexpr int STATUS_CHUNK = 140;  // lb2_status: kv8_attend_packed's lengths and bounds
+
+template <typename T, int D>
+__global__ void __launch_bounds__(128) chunk_kernel(const ChunkParams p) {
+  constexpr int E = D / 32;
+  const PagedParams& a = p.a;
+  const int64_t w = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 5);
+  if (w >= int64_t(a.Hq) * a.T) return;
+  const int d0 = (threadIdx.x & 31) * E;
+  const int row = int(w / a.Hq), h = int(w % a.Hq);
+  int lo = 0, hi = a.B;  // the last b with cu[b] <= row
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (p.cu[mid] <= row) lo = mid; else hi = mid;
+  }
+  const ChunkRange r = chunk_range(p, lo, STATUS_CHUNK, d0 == 0);
+  const T* q = static_cast<const T*>(a.q) + h * a.q_st[1] + row * a.q_st[2] + d0;
+  T* o = static_cast<T*>(a.o) + h * a.o_st[1] + row * a.o_st[2] + d0;
+  PagedKeys<E> keys{a.pages, a.scales, a.table + lo * a.table_st, a.Hkv, h / (a.Hq / a.Hkv), a.page, a.num_pages, d0};
+  float x[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) x[e] = to_f<T>(q[e]);
+  attend_row<E>(keys, row >= r.lo && row < r.hi ? chunk_seen(p, r, row) : 0, a.scale, x);
+#pragma unroll
+  for (int e = 0; e < E; ++e) o[e] = from_f<T>(x[e]);
+}
+
 struct PackedParams {
   const void* q;
   const void* k;

@@ -26,6 +26,7 @@
 #include "gdn_glue.cuh"
 #include "rope.cuh"
 #include "kv8.cuh"
+#include "kv8_pages.cuh"
 #include "attn_rows.cuh"
 #include "kv8_attend.cuh"
 
@@ -1812,6 +1813,107 @@ int lb2_kv8_attend(const void* q, const int64_t* q_st, const uint8_t* pages, con
                     workspace_bytes >= lb2_kv8_attend_workspace_size(B, Hq, Hkv, T, D, page, max_pages),
                 "kv8_attend: workspace too small or not 256-byte aligned");
   return kv8attn::run(p, D, dtype, workspace, st);
+}
+
+}  // extern "C"
+
+template <typename T>
+static int chunk_rows(const arows::ChunkParams& p, int D, cudaStream_t st) {
+  const int64_t blocks = (int64_t(p.a.Hq) * p.a.T + 3) / 4;
+  if (D == 64) arows::chunk_kernel<T, 64><<<unsigned(blocks), 128, 0, st>>>(p);
+  else if (D == 128) arows::chunk_kernel<T, 128><<<unsigned(blocks), 128, 0, st>>>(p);
+  else arows::chunk_kernel<T, 256><<<unsigned(blocks), 128, 0, st>>>(p);
+  LB2_CUDA(cudaGetLastError());
+  return LB2_OK;
+}
+
+extern "C" {
+
+size_t lb2_kv8_attend_packed_workspace_size(int B, int Hq, int Hkv, int T, int D) {
+  return 0;
+}
+
+int lb2_kv8_attend_packed(const void* q, const int64_t* q_st, const uint8_t* pages, const float* scales,
+                          const int32_t* table, int64_t table_st, const int32_t* kv_len, const int32_t* cu, void* o,
+                          const int64_t* o_st, int B, int Hq, int Hkv, int T, int D, int page, int num_pages,
+                          int max_pages, int dtype, float scale, int causal, void* workspace, size_t workspace_bytes,
+                          void* stream) {
+  const int rc = kv8_shape(B, Hkv, T, D, page, num_pages, max_pages, "kv8_attend_packed");
+  if (rc) return rc;
+  LB2_CHECK_ARG(B >= 1, "kv8_attend_packed: at least one sequence");
+  LB2_CHECK_ARG(Hq > 0 && Hq % Hkv == 0, "kv8_attend_packed: Hq must be a multiple of Hkv");
+  LB2_CHECK_ARG(std::isfinite(scale), "kv8_attend_packed: the scale must be finite");
+  LB2_CHECK_ARG(dtype == LB2_F32 || dtype == LB2_BF16 || dtype == LB2_F16, "kv8_attend_packed: dtype");
+  LB2_CHECK_ARG(int64_t(T) * Hq < (1 << 30), "kv8_attend_packed: too many rows");
+  if (T == 0) return LB2_OK;
+  LB2_CHECK_ARG(q && q_st && pages && scales && table && kv_len && cu && o && o_st, "kv8_attend_packed: missing argument");
+  LB2_CHECK_ARG(aligned16(pages), "kv8_attend_packed: pages must be 16-byte aligned");
+  arows::ChunkParams p{};
+  p.a.q = q;
+  p.a.o = o;
+  for (int i = 0; i < 2; ++i) p.a.q_st[i + 1] = q_st[i], p.a.o_st[i + 1] = o_st[i];
+  p.a.pages = pages;
+  p.a.scales = scales;
+  p.a.table = table;
+  p.a.table_st = table_st;
+  p.a.kv_len = kv_len;
+  p.a.B = B, p.a.Hq = Hq, p.a.Hkv = Hkv, p.a.T = T;
+  p.a.page = page, p.a.num_pages = num_pages, p.a.max_pages = max_pages;
+  p.a.causal = causal != 0;
+  p.a.scale = scale;
+  p.cu = cu;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return dtype == LB2_F32 ? chunk_rows<float>(p, D, st) : dtype == LB2_BF16 ? chunk_rows<__nv_bfloat16>(p, D, st) : chunk_rows<__half>(p, D, st);
+}
+
+// ------------------------------------------------------------------------------------------------ pages moved about
+
+int lb2_kv8_copy(const uint8_t* from_pages, const float* from_scales, int from_num, uint8_t* to_pages, float* to_scales,
+                 int to_num, const int32_t* src, const int32_t* dst, int n, int Hkv, int page, int D, void* stream) {
+  int rc = kv8_shape(0, Hkv, 0, D, page, from_num, 1, "kv8_copy");
+  if (!rc) rc = kv8_shape(0, Hkv, 0, D, page, to_num, 1, "kv8_copy");
+  if (rc) return rc;
+  LB2_CHECK_ARG(n >= 0, "kv8_copy: a number of pages");
+  LB2_CHECK_ARG(Hkv < 32768, "kv8_copy: too many heads");
+  if (n == 0) return LB2_OK;
+  LB2_CHECK_ARG(from_pages && from_scales && to_pages && to_scales && src && dst, "kv8_copy: missing argument");
+  LB2_CHECK_ARG(aligned16(from_pages) && aligned16(to_pages), "kv8_copy: pages must be 16-byte aligned");
+  kv8::CopyParams p{from_pages, from_scales, to_pages, to_scales, src, dst, n, from_num, to_num, 2 * Hkv,
+                    int64_t(2) * Hkv * page * D};
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  for (int i = 0; i < n; i += 65535) {
+    kv8::CopyParams c = p;
+    c.src += i, c.dst += i;
+    kv8::copy_kernel<<<dim3(8, unsigned(std::min(n - i, 65535))), kv8::COPY_THREADS, 0, st>>>(c);
+    LB2_CUDA(cudaGetLastError());
+  }
+  return LB2_OK;
+}
+
+int lb2_kv8_compact(uint8_t* pages, float* scales, const int32_t* table, int64_t table_st, const int32_t* keep,
+                    const int32_t* cu, const int32_t* to, int64_t to_st, const int32_t* start, const uint64_t* turns,
+                    int B, int Hkv, int T, int D, int R, int page, int num_pages, int max_pages, int max_to,
+                    int interleaved, void* stream) {
+  int rc = kv8_shape(B, Hkv, T, D, page, num_pages, max_pages, "kv8_compact");
+  if (!rc) rc = kv8_shape(B, Hkv, T, D, page, num_pages, max_to, "kv8_compact");
+  if (rc) return rc;
+  LB2_CHECK_ARG(R >= 0 && R <= D && R % 2 == 0, "kv8_compact: an even number of rotated dims, at most the head dim");
+  LB2_CHECK_ARG(R == 0 || turns != nullptr, "kv8_compact: rotated dims need their turns");
+  LB2_CHECK_ARG(Hkv < 32768, "kv8_compact: too many heads");
+  if (B == 0 || T == 0) return LB2_OK;
+  LB2_CHECK_ARG(pages && scales && table && keep && cu && to && start, "kv8_compact: missing argument");
+  LB2_CHECK_ARG(aligned16(pages), "kv8_compact: pages must be 16-byte aligned");
+  kv8::CompactParams p{};
+  p.pages = pages, p.scales = scales, p.table = table, p.keep = keep, p.cu = cu, p.to = to, p.start = start, p.turns = turns;
+  p.table_st = table_st, p.to_st = to_st;
+  p.B = B, p.Hkv = Hkv, p.T = T, p.D = D, p.R = R, p.num_pages = num_pages, p.max_pages = max_pages, p.max_to = max_to;
+  p.lpage = page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : 7;
+  p.interleaved = interleaved != 0;
+  const int64_t pieces = int64_t(T) / page + B;
+  LB2_CHECK_ARG(pieces < (int64_t(1) << 31), "kv8_compact: too many tokens");
+  kv8::compact_any_kernel<<<dim3(unsigned(pieces), unsigned(2 * Hkv)), 128, 0, static_cast<cudaStream_t>(stream)>>>(p);
+  LB2_CUDA(cudaGetLastError());
+  return LB2_OK;
 }
 
 // ------------------------------------------------------------------------------------------------ packed prompts

@@ -712,6 +712,85 @@ def kv8_attend(q, pages, scales, table, kv_len, scale, causal=True, out=None):
     return out
 
 
+def kv8_attend_packed(q, pages, scales, table, kv_len, cu, scale, causal=True, out=None):
+    """Attention of packed chunks of new tokens over the paged 8-bit cache (lb2_kv8_attend_packed): q [1, Hq, T, D], sequence
+    b's rows cu[b] .. cu[b + 1] - 1 (cu int32 [B + 1]) being the last of its kv_len[b] cached tokens (int32 [B], the call's
+    own among them, already appended). causal: each row sees the tokens up to its own. For inference: the result is in no
+    autograd graph."""
+    (num_pages, _, Hkv, page, D), (B, max_pages), dev = _kv8_pool(pages, scales, table, "kv8_attend_packed")
+    qs, qst = q.shape, q.stride()
+    if len(qs) != 4 or qs[0] != 1 or qs[3] != D or q.get_device() != dev or qst[3] != 1:
+        raise ValueError("kv8_attend_packed: q must be [1, Hq, T, D] for the cache's D and device, with a unit last stride")
+    Hq, T = qs[1], qs[2]
+    if Hq == 0 or Hq % Hkv:
+        raise ValueError("kv8_attend_packed: Hq must be a multiple of the cache's Hkv")
+    _int32(kv_len, (B,), dev, "kv8_attend_packed: kv_len")
+    _int32(cu, (B + 1,), dev, "kv8_attend_packed: cu")
+    if out is None:
+        out, ost = _new_like(q)
+    else:
+        _out_like(out, q, "kv8_attend_packed")
+        ost = out.stride()
+    n = lib().lb2_kv8_attend_packed_workspace_size(B, Hq, Hkv, T, D)
+    stream = _stream_of(dev)
+    ws = _scratch(n or 1, stream)
+    try:
+        rc = lib().lb2_kv8_attend_packed(q.data_ptr(), i64(*qst[1:3]), pages.data_ptr(), scales.data_ptr(),
+                                         table.data_ptr(), table.stride(0), kv_len.data_ptr(), cu.data_ptr(),
+                                         out.data_ptr(), i64(*ost[1:3]), B, Hq, Hkv, T, D, page, num_pages, max_pages,
+                                         dtype_code(q), scale, 1 if causal else 0, ws, n, stream)
+    finally:
+        _scratch_done(ws)
+    if rc:
+        check(rc, "kv8_attend_packed")
+    return out
+
+
+def kv8_copy(pages, scales, src, dst, into=None):
+    """Copies pages, codes and scales, in place: page dst[i] becomes page src[i] (int32 [n] on the device; lb2_kv8_copy).
+    into: (pages, scales) of another pool of the same heads, page and D, whose pages dst names. No page may be in dst
+    twice, nor, within one pool, in both src and dst."""
+    ps, dev = pages.shape, pages.get_device()
+    to, to_scales = (pages, scales) if into is None else into
+    for p, s in ((pages, scales), (to, to_scales)) if into is not None else ((pages, scales),):
+        if p.get_device() < 0:
+            _cuda(p)
+        if len(p.shape) != 5 or p.shape[1:] != ps[1:] or ps[1] != 2 or p.dtype is not _E4M3 or not p.is_contiguous():
+            raise ValueError("kv8_copy: pools must be contiguous float8_e4m3fn [num_pages, 2, Hkv, page, D], of one Hkv, page "
+                             "and D")
+        if s.dtype is not _FP32 or s.shape != p.shape[:3] or not s.is_contiguous():
+            raise ValueError("kv8_copy: scales must be contiguous fp32 [num_pages, 2, Hkv]")
+        if p.get_device() != dev or s.get_device() != dev:
+            raise ValueError("kv8_copy: the pools must be on one device")
+    n = src.numel()
+    _int32(src, (n,), dev, "kv8_copy: src")
+    _int32(dst, (n,), dev, "kv8_copy: dst")
+    rc = lib().lb2_kv8_copy(pages.data_ptr(), scales.data_ptr(), ps[0], to.data_ptr(), to_scales.data_ptr(), to.shape[0],
+                            src.data_ptr(), dst.data_ptr(), n, ps[2], ps[3], ps[4], _stream_of(dev))
+    if rc:
+        check(rc, "kv8_copy")
+
+
+def kv8_compact(pages, scales, table, keep, cu, to, start, turns=None, layout="half"):
+    """Moves kept tokens of paged sequences together, in place (lb2_kv8_compact): the tokens at positions keep[cu[b]] ..
+    keep[cu[b + 1] - 1] of sequence b (keep int32 [T], cu int32 [B + 1]) become its positions start[b] onwards (start int32
+    [B], page beginnings) in the pages to[b] (int32 [B, max_to], entry j for positions j * page and on), keys turned by the
+    difference of the positions when turns is given. No page may be written twice, or both read and written."""
+    (num_pages, _, Hkv, page, D), (B, max_pages), dev = _kv8_pool(pages, scales, table, "kv8_compact")
+    T, ts = keep.numel(), to.shape
+    _int32(keep, (T,), dev, "kv8_compact: keep")
+    _int32(cu, (B + 1,), dev, "kv8_compact: cu")
+    _int32(start, (B,), dev, "kv8_compact: start")
+    if to.dtype is not _I32 or len(ts) != 2 or ts[0] != B or to.get_device() != dev or to.stride(1) != 1:
+        raise ValueError("kv8_compact: to must be int32 [B, max_to] with a unit last stride on the pages' device")
+    R = 0 if turns is None else _turns(turns, D, dev, "kv8_compact")
+    rc = lib().lb2_kv8_compact(pages.data_ptr(), scales.data_ptr(), table.data_ptr(), table.stride(0), keep.data_ptr(),
+                               cu.data_ptr(), to.data_ptr(), to.stride(0), start.data_ptr(), _ptr(turns), B, Hkv, T, D, R,
+                               page, num_pages, max_pages, ts[1], _interleaved(layout, "kv8_compact"), _stream_of(dev))
+    if rc:
+        check(rc, "kv8_compact")
+
+
 def attn_packed(q, k, v, scale, cu, out=None):
     """Causal attention over prompts packed on one row axis (lb2_attn_packed): q [1, Hq, T, D], k / v [1, Hkv, T, D],
     cu int32 [S + 1] on the device, prompt s being rows cu[s] .. cu[s + 1] - 1. For inference: the result is in no autograd
