@@ -1,0 +1,958 @@
+// Attention of packed chunks of new tokens over the paged 8-bit KV cache (kv8.cuh) on tcgen05.
+//
+//   o = softmax(scale q (code_k s_k)^T) (code_v s_v)
+//
+// A row is a (token, query head) of one KV head, the G heads of a token side by side, so that all rows that share K and V
+// share the passes over them: an item is a block of 256 rows (128 at head dim 256) of one sequence and KV head, over 128-key
+// tiles up to its last row's horizon. The codes are read from the pages into registers, turned into f16 (every e4m3 value is
+// one) and stored as the swizzled operand tiles of both products: once for a block's 256 rows, and no raw tile passes
+// through shared memory, whose bandwidth is the products' too.
+//
+// The tensor pipe works on units, (row tile of 128, key tile) pairs, two S buffers in turn: S_i = Q K^T into buffer i % 2,
+// warpgroup i % 2 turns it into P_i (in its place), O += P_i V, S_{i+2}. So one warpgroup's softmax runs under the other's
+// products.
+//  - more than 128 rows, head dim 64 and 128: unit i is row tile i % 2 of key tile i / 2; each warpgroup has its own rows.
+//  - up to 128 rows there: unit i is key tile i of the one row tile; each warpgroup has its own maximum, sum and O over its
+//    half of the keys, joined at the end.
+//  - head dim 256 (O takes half the tensor memory): unit i is key tile i; the warpgroups share the rows' maximum, handed on
+//    from unit to unit, and O; each sums its own units' weights.
+//
+// Work is cut evenly whatever the lengths: the call's units in order, cut into equal runs, one a CTA (one CTA an SM). An item
+// that a cut parts is merged from fp32 partials by combine_kernel, launched behind as a programmatic dependent; its parts
+// are known from the units alone, so every sum is formed in the same order in every run of a call.
+//
+// Softmax in base 2, fp32, one thread a row. As in kv8_attend.cuh the weights carry the values' scale, p' = 2^(s + log2 s_v -
+// m), m the running maximum of s + log2 s_v less 7, l = sum p' / s_v, o = sum p' code_v / l; the maximum moves when it is
+// passed by more than 8, so p' reaches 2^15, the upper end of f16, and keeps f16's 11 bits down to 2^-21 of the largest. bf16 queries go to f16 exactly, a row shifted by a power of two that the score's factor undoes.
+//
+// A NaN code under a weight of 0 would spread to rows that do not see it. Keys past an item's horizon are stored as zeros; a
+// row that comes out NaN is looked at again at the end (row_again), and where a value that it does not see is to blame, taken
+// again reading only what it sees.
+//
+// Roles (512 threads): warps 0-3, 4-7 softmax and epilogue (warp w: TMEM lanes of quarter w % 4), 8-11 codes and queries into
+// shared memory, 12 issues the products, 13 reads the page table and scales ahead.
+#pragma once
+
+#include <cfloat>
+
+#include "attn_prefill.cuh"
+#include "attn_prefill2.cuh"
+#include "attn_rows.cuh"
+#include "common.cuh"
+#include "kv8.cuh"
+
+namespace lb2 {
+namespace kv8chunk {
+
+constexpr int BM = 128, BN = 128;  // rows of a row tile, keys of a key tile
+constexpr int MAX_B = 1024;        // sequences a launch
+constexpr int THREADS = 512;
+constexpr int CONV_WARP = 8, MMA_WARP = 12, TABLE_WARP = 13;
+constexpr int TABLES = 8;          // key tiles whose page ids and scales are held
+constexpr float TOP = 7.f;         // a weight at the running maximum is 2^TOP
+constexpr int STATUS = arows::STATUS_CHUNK;  // lb2_status: 140 lengths and page ids, 141.. waits
+
+template <int D>
+struct Cfg {
+  static constexpr bool WIDE = D == 256;
+  static constexpr int QT = WIDE ? 1 : 2;         // row tiles of an item
+  static constexpr int RB = BM * QT;
+  static constexpr int DS = D < 128 ? D : 128;    // dims of a stage
+  static constexpr int SPT = D / DS;              // stages of a K (or V) tile
+  static constexpr int STAGE = BN * DS * 2;
+  static constexpr int NS = D == 64 ? 6 : 4;
+  static constexpr int QTILE = BM * D * 2;
+  static constexpr int K_OFF = QT * QTILE;
+  static constexpr int TAB_OFF = K_OFF + NS * STAGE;           // [TABLES][8] float4 of a 16-key slice's scales
+  static constexpr int ID_OFF = TAB_OFF + TABLES * 8 * 16;     // [TABLES][8] page ids
+  static constexpr int FAR_OFF = ID_OFF + TABLES * 8 * 4;      // [TABLES] the slices whose weights' sums are formed apart
+  static constexpr int FAC_OFF = FAR_OFF + TABLES * 4;         // [2 items][RB] the rows' score factors
+  static constexpr int ML_OFF = FAC_OFF + 2 * RB * 4;          // [2][128] float2
+  static constexpr int MSH_OFF = ML_OFF + 2 * BM * 8;          // [128] the shared maximum
+  static constexpr int PREFIX_OFF = MSH_OFF + BM * 4;          // [MAX_B + 3] int64
+  static constexpr int BAR_OFF = PREFIX_OFF + (MAX_B + 3) * 8;
+  static constexpr int SMEM = BAR_OFF + 512 + 1024;
+  static constexpr int O_COL = 2 * BN;            // O, or the two warpgroups' O at O_COL and O_COL + D
+  static_assert(PREFIX_OFF % 8 == 0 && SMEM <= 232448, "shared memory budget");
+  static_assert(O_COL + QT * D <= 512, "TMEM budget");
+};
+
+struct Params {
+  arows::ChunkParams c;
+  float* ws_o;   // [2 grid][D][RB]
+  float* ws_ml;  // [2 grid][2][RB]
+  int4* rec;     // [grid][2]: the item that the CTA begins and does not end
+  int G;
+  int lpage;
+  int first, last;       // the launch has the call's first, last sequences
+  int wide_q, wide_o;    // 16-byte query loads; bytes an output store may take: 32, 16 or 0 (an element)
+  int flip;              // a negative scale: the queries' signs
+  int min_units;         // units a CTA at least
+  float scale_log2;
+};
+
+// The sequences as ranges of rows: range 0 the rows before the first, range b + 1 sequence b, the last the rows behind (both
+// without keys).
+struct Range {
+  int lo, n, len;
+};
+
+__device__ __forceinline__ Range range_of(const Params& p, int r) {
+  const int B = p.c.a.B, T = p.c.a.T;
+  Range x{0, 0, 0};
+  if (r == 0) {
+    if (p.first) x.n = min(max(p.c.cu[0], 0), T);
+  } else if (r == B + 1) {
+    x.lo = min(max(p.c.cu[B], 0), T);
+    if (p.last) x.n = T - x.lo;
+  } else {
+    const arows::ChunkRange c = arows::chunk_range(p.c, r - 1, STATUS, false);
+    x.lo = c.lo, x.n = c.hi - c.lo, x.len = c.len;
+  }
+  return x;
+}
+
+struct Block {
+  int rows, horizon, tiles, units;
+  bool pair;
+};
+
+template <int RB>
+__device__ __forceinline__ Block block_of(const Params& p, const Range& x, int k) {
+  Block b;
+  b.rows = min(RB, x.n * p.G - k * RB);
+  const int last = (k * RB + b.rows - 1) / p.G;  // token
+  b.horizon = p.c.a.causal ? max(x.len - (x.n - 1 - last), 0) : x.len;
+  if (x.len == 0) b.horizon = 0;
+  b.tiles = max(1, (b.horizon + BN - 1) / BN);
+  b.pair = RB > BM && b.rows > BM;
+  b.units = b.pair ? 2 * b.tiles : b.tiles;
+  return b;
+}
+
+// What a CTA does of one item: key tiles kt0 .. kt0 + nt - 1.
+struct Piece {
+  int b, lo, n, len, hk, f0, rows, horizon, kt0, nt, units;
+  bool pair, whole;
+  int slot;    // of its partial, where it is not the whole item
+  int nparts;  // of an item that it begins and does not end, else 0
+};
+
+// The CTA's pieces in order, each warp for itself. prefix[r]: units of the ranges before r.
+template <int RB>
+struct Sched {
+  const Params& p;
+  const int64_t* prefix;
+  int64_t total, runs, at, p0, p1;  // at: the current item's first unit; [p0, p1): the CTA's run
+  int r, hk, k, nb;
+  Range x;
+
+  __device__ __forceinline__ int64_t cut(int64_t c) const { return c * total / runs; }
+
+  __device__ __forceinline__ Sched(const Params& p_, const int64_t* prefix_) : p(p_), prefix(prefix_) {
+    const int NR = p.c.a.B + 2, lane = threadIdx.x & 31;
+    total = prefix[NR];
+    runs = max(int64_t(1), min(int64_t(gridDim.x), total / p.min_units));
+    const int64_t c = blockIdx.x;
+    p0 = c < runs ? cut(c) : 0;
+    p1 = c < runs ? cut(c + 1) : 0;
+    r = hk = k = nb = 0;
+    at = 0;
+    if (p0 >= p1) return;
+    int lo = 0, hi = NR;  // the last range with prefix <= p0 that is not empty
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (prefix[mid] <= p0) lo = mid; else hi = mid;
+    }
+    enter(lo);
+    const int64_t each = (prefix[r + 1] - prefix[r]) / p.c.a.Hkv;
+    hk = int((p0 - at) / each);
+    at += hk * each;
+    for (int k0 = 0; k0 < nb; k0 += 32) {  // 32 blocks at a time
+      const int own = k0 + lane < nb ? block_of<RB>(p, x, k0 + lane).units : 0;
+      int64_t sum = own;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t y = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += y;
+      }
+      const uint32_t past = __ballot_sync(0xffffffffu, k0 + lane < nb && at + sum > p0);
+      if (past) {
+        const int l = __ffs(past) - 1;
+        at += __shfl_sync(0xffffffffu, sum - own, l);
+        k = k0 + l;
+        break;
+      }
+      at += __shfl_sync(0xffffffffu, sum, 31);
+    }
+  }
+
+  __device__ __forceinline__ void enter(int range) {
+    r = range;
+    x = range_of(p, r);
+    nb = (x.n * p.G + RB - 1) / RB;
+    at = prefix[r];
+  }
+
+  __device__ __forceinline__ bool next(Piece& w) {
+    while (at < p1) {
+      const Block b = block_of<RB>(p, x, k);
+      int64_t a = max(p0 - at, int64_t(0)), z = min(p1 - at, int64_t(b.units));
+      if (b.pair) a &= ~int64_t(1), z &= ~int64_t(1);  // (runs are two units at least: a cut parts no pair)
+      w.b = r - 1, w.lo = x.lo, w.n = x.n, w.len = x.len, w.hk = hk;
+      w.f0 = k * RB, w.rows = b.rows, w.horizon = b.horizon, w.pair = b.pair;
+      w.kt0 = int(b.pair ? a >> 1 : a);
+      w.units = int(z - a);
+      w.nt = b.pair ? w.units >> 1 : w.units;
+      w.whole = a == 0 && z == b.units;
+      w.slot = 2 * int(blockIdx.x) + (a == 0 ? 1 : 0);
+      w.nparts = 0;
+      if (a == 0 && !w.whole) w.nparts = int(((at + b.units) * runs - 1) / total) - int(blockIdx.x) + 1;
+      at += b.units;
+      if (++k == nb) {
+        k = 0;
+        if (++hk == p.c.a.Hkv) {
+          hk = 0;
+          int rr = r + 1;
+          while (rr < p.c.a.B + 2 && prefix[rr + 1] == prefix[rr]) ++rr;
+          if (rr < p.c.a.B + 2) enter(rr);
+        }
+      }
+      if (w.units > 0) return true;
+    }
+    return false;
+  }
+};
+
+// Entry e of a piece's 2 nt fills of the operand ring: which (V or K) and key tile. The order is the products': with pairs
+// K_0 V_0 K_1 V_1 .., else K_0 K_1 V_0 K_2 V_1 .. V_{nt-1}.
+__device__ __forceinline__ void entry(bool pair, int nt, int e, int& kind, int& t) {
+  if (pair) kind = e & 1, t = e >> 1;
+  else if (e == 0) kind = 0, t = 0;
+  else if (e == 2 * nt - 1) kind = 1, t = nt - 1;
+  else kind = 1 - (e & 1), t = kind ? (e - 2) >> 1 : (e + 1) >> 1;
+}
+__device__ __forceinline__ int k_entry(bool pair, int t) { return pair ? 2 * t : t == 0 ? 0 : 2 * t - 1; }
+__device__ __forceinline__ int v_entry(bool pair, int nt, int t) { return pair ? 2 * t + 1 : t == nt - 1 ? 2 * nt - 1 : 2 * t + 2; }
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// l 2^x, x <= 0, in two steps: l reaches 2^115 where V scales are far apart, and 2^x alone may be 0.
+__device__ __forceinline__ float shrink(float l, float x) {
+  const float h = prefill::ex2f(0.5f * x);
+  return l * h * h;
+}
+
+template <int N>
+__device__ __forceinline__ void reg_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void reg_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+// A bounded wait that gives up at once when some role of the CTA has.
+__device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int where) {
+  if (mbar_try_wait(bar, parity)) return true;
+  uint64_t t0 = 0;
+  for (uint32_t i = 1;; ++i) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((i & 255u) == 0) {
+      if (*abort_flag) return false;
+      const uint64_t now = globaltimer_ns();
+      if (t0 == 0) {
+        t0 = now;
+      } else if (now - t0 > kWaitNs) {
+        report_timeout(where);
+        *abort_flag = 1;
+        return false;
+      }
+    }
+  }
+}
+
+// The second look at folded row f of an item, by one warp: where its output has NaN columns and one of the keys behind it that
+// its item's products took holds a NaN there, the row again, reading only what it sees.
+template <typename T, int D>
+__device__ __noinline__ void row_again(const Params& p, int b, int lo, int n, int len, int hk, int f, int horizon) {
+  constexpr int E = D / 32;
+  const arows::PagedParams& a = p.c.a;
+  const int lane = threadIdx.x & 31, t = f / p.G, h = hk * p.G + f % p.G;
+  const int seen = a.causal ? max(len - (n - 1 - t), 0) : len;
+  T* o = static_cast<T*>(a.o) + h * a.o_st[1] + int64_t(lo + t) * a.o_st[2] + lane * E;
+  bool bad[E], any = false;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const float x = to_f<T>(o[e]);
+    any |= bad[e] = x != x;
+  }
+  if (!__any_sync(0xffffffffu, any)) return;
+  arows::PagedKeys<E> keys{a.pages, a.scales, a.table + b * a.table_st, a.Hkv, hk, a.page, a.num_pages, lane * E};
+  any = false;
+  for (int i = seen; i < horizon; ++i) {
+    float k[E], v[E];
+    keys.load(i, k, v);
+#pragma unroll
+    for (int e = 0; e < E; ++e) any |= bad[e] && v[e] != v[e];
+  }
+  if (!__any_sync(0xffffffffu, any)) return;
+  const T* q = static_cast<const T*>(a.q) + h * a.q_st[1] + int64_t(lo + t) * a.q_st[2] + lane * E;
+  float x[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) x[e] = to_f<T>(q[e]);
+  arows::attend_row<E>(keys, seen, a.scale, x);
+#pragma unroll
+  for (int e = 0; e < E; ++e) o[e] = from_f<T>(x[e]);
+}
+
+// 32 output values of a row, in the widest stores that its alignment allows.
+template <typename T>
+__device__ __forceinline__ void store32(T* o, const float* v, float f, int wide) {
+  if (wide) {
+    uint32_t w[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) w[e] = pack2<T>(v[2 * e] * f, v[2 * e + 1] * f);
+    if (wide == 32) {
+#pragma unroll
+      for (int e = 0; e < 16; e += 8)
+        asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(o + 2 * e), "r"(w[e]), "r"(w[e + 1]),
+                     "r"(w[e + 2]), "r"(w[e + 3]), "r"(w[e + 4]), "r"(w[e + 5]), "r"(w[e + 6]), "r"(w[e + 7])
+                     : "memory");
+    } else {
+#pragma unroll
+      for (int e = 0; e < 16; e += 4) *reinterpret_cast<uint4*>(o + 2 * e) = make_uint4(w[e], w[e + 1], w[e + 2], w[e + 3]);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 32; ++e) o[e] = from_f<T>(v[e] * f);
+  }
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
+  using C = Cfg<D>;
+  constexpr int RB = C::RB, NS = C::NS, SPT = C::SPT;
+  constexpr uint32_t IDESC_S = prefill::idesc_f16(0, 0, 0, BM, BN);
+  constexpr uint32_t IDESC_PV = prefill::idesc_f16(0, 0, 1, BM, C::DS);
+
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  float4* tab = reinterpret_cast<float4*>(sm + C::TAB_OFF);
+  int* ids = reinterpret_cast<int*>(sm + C::ID_OFF);
+  uint32_t* far_s = reinterpret_cast<uint32_t*>(sm + C::FAR_OFF);
+  float* fac_s = reinterpret_cast<float*>(sm + C::FAC_OFF);
+  float2* ml_s = reinterpret_cast<float2*>(sm + C::ML_OFF);
+  volatile float* m_sh = reinterpret_cast<volatile float*>(sm + C::MSH_OFF);
+  int64_t* prefix = reinterpret_cast<int64_t*>(sm + C::PREFIX_OFF);
+  uint64_t* full = reinterpret_cast<uint64_t*>(sm + C::BAR_OFF);  // [NS] a stage's operand is in
+  uint64_t* empty = full + NS;           // [NS] its products are done
+  uint64_t* q_full = empty + NS;
+  uint64_t* q_empty = q_full + 1;        // the item's last S has read Q
+  uint64_t* s_full = q_empty + 1;        // [2]
+  uint64_t* p_full = s_full + 2;         // [2]
+  uint64_t* o_done = p_full + 2;         // [2] the buffer's P V is complete
+  uint64_t* o_free = o_done + 2;         // the epilogue has read O
+  uint64_t* tab_full = o_free + 1;       // [TABLES]
+  uint64_t* tab_empty = tab_full + TABLES;
+  uint64_t* token = tab_empty + TABLES;  // [2 warpgroups][4 quarters]: the shared maximum after the group's unit
+  uint64_t* drain = token + 8;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile int* again = abort_flag + 1;
+  static_assert((2 * NS + 2 + 6 + 1 + 2 * TABLES + 8 + 1) * 8 + 12 <= 512, "barrier area");
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < NS; ++i) {
+      mbar_init(&full[i], 4);
+      mbar_init(&empty[i], 1);
+    }
+    mbar_init(q_full, 4);
+    mbar_init(q_empty, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 4);
+      mbar_init(&o_done[i], 1);
+    }
+    mbar_init(o_free, 8);
+    for (int i = 0; i < TABLES; ++i) {
+      mbar_init(&tab_full[i], 1);
+      mbar_init(&tab_empty[i], 12);  // four warps' V loads and eight softmax warps (four, twice, where one group has the tile)
+    }
+    for (int i = 0; i < 8; ++i) mbar_init(&token[i], 1);
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    *again = 0;
+    fence_barrier_init();
+  }
+  if (warp == MMA_WARP) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  // A programmatic dependent of the stream's previous kernel: global memory is read only past this point.
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  {
+    const int NR = p.c.a.B + 2;
+    for (int r = warp; r < NR; r += THREADS / 32) {
+      const Range x = range_of(p, r);
+      if (blockIdx.x == 0 && lane == 0 && r > 0 && r <= p.c.a.B) arows::chunk_range(p.c, r - 1, STATUS, true);
+      const int nb = (x.n * p.G + RB - 1) / RB;
+      int64_t s = 0;
+      for (int k = lane; k < nb; k += 32) s += block_of<RB>(p, x, k).units;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+      if (lane == 0) prefix[r + 1] = s * p.c.a.Hkv;
+    }
+    __syncthreads();
+    if (warp == 0) {
+      int64_t run = 0;
+      for (int r0 = 0; r0 < NR; r0 += 32) {
+        int64_t x = r0 + lane < NR ? prefix[r0 + lane + 1] : 0;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+          if (lane >= o) x += y;
+        }
+        if (r0 + lane < NR) prefix[r0 + lane + 1] = run + x;
+        run += __shfl_sync(0xffffffffu, x, 31);
+      }
+      if (lane == 0) prefix[0] = 0;
+    }
+  }
+  prefill::tc_fence_before();
+  __syncthreads();
+  prefill::tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  Piece w;
+
+  if (warp >= CONV_WARP + 4) {
+    reg_dec<56>();
+    Sched<RB> sched(p, prefix);
+    if (warp == MMA_WARP) {
+      // ---------------------------------------------------------------------------------- MMA issuer
+      int pieces = 0, base = 0, g0 = 0, g1 = 0;  // pieces and ring entries so far; units of each buffer so far
+      bool ok = true;
+      while (ok && sched.next(w)) {
+        if (elect_one()) {
+          ok = wait_or_abort(q_full, pieces & 1, abort_flag, 141);
+          const uint32_t q_addr = smem_u32(sm), k0 = smem_u32(sm + C::K_OFF);
+          auto scores = [&](int i) {
+            const int t = w.pair ? i >> 1 : i, e = (base + k_entry(w.pair, t)) * SPT;
+            const uint32_t q = q_addr + (w.pair ? (i & 1) * C::QTILE : 0);
+#pragma unroll
+            for (int h = 0; h < SPT; ++h) {
+              const int st = (e + h) % NS;
+              if (!ok || !(ok = wait_or_abort(&full[st], ((e + h) / NS) & 1, abort_flag, 142))) return;
+              prefill::tc_fence_after();
+              const uint32_t k = k0 + st * C::STAGE;
+#pragma unroll
+              for (int kk = 0; kk < C::DS / 16; ++kk)
+                prefill::umma_ss(tmem + (i & 1) * BN,
+                                 prefill::sdesc(q + ((kk >> 2) + h * (C::DS / 64)) * BM * 128 + (kk & 3) * 32, 16, 1024),
+                                 prefill::sdesc(k + (kk >> 2) * BN * 128 + (kk & 3) * 32, 16, 1024), IDESC_S,
+                                 h + kk > 0 ? 1u : 0u);
+              if (!w.pair || (i & 1)) prefill::umma_commit(&empty[st]);
+            }
+            prefill::umma_commit(&s_full[i & 1]);
+            if (i == w.units - 1) prefill::umma_commit(q_empty);
+          };
+          if (ok) scores(0);
+          if (ok && w.units > 1) scores(1);
+          for (int i = 0; ok && i < w.units; ++i) {
+            const int t = w.pair ? i >> 1 : i, e = (base + v_entry(w.pair, w.nt, t)) * SPT;
+            ok = wait_or_abort(&p_full[i & 1], ((i & 1 ? g1 : g0) + (i >> 1)) & 1, abort_flag, 143);
+            if (ok && i == 0 && pieces > 0) ok = wait_or_abort(o_free, (pieces - 1) & 1, abort_flag, 144);
+            const bool own = !C::WIDE;  // each buffer its O
+            const uint32_t o = tmem + C::O_COL + (own && (i & 1) ? D : 0);
+#pragma unroll
+            for (int h = 0; h < SPT; ++h) {
+              const int st = (e + h) % NS;
+              if (ok) ok = wait_or_abort(&full[st], ((e + h) / NS) & 1, abort_flag, 145);
+              if (!ok) break;
+              prefill::tc_fence_after();
+              const uint32_t v = k0 + st * C::STAGE;
+#pragma unroll
+              for (int kk = 0; kk < BN / 16; ++kk)
+                prefill::umma_ts(o + h * C::DS, tmem + (i & 1) * BN + kk * 8,
+                                 prefill::sdesc(v + kk * 16 * 128, BN * 128, 1024), IDESC_PV,
+                                 (own ? i > 1 : i > 0) || kk > 0 ? 1u : 0u);
+              if (!w.pair || (i & 1)) prefill::umma_commit(&empty[st]);
+            }
+            if (!ok) break;
+            prefill::umma_commit(&o_done[i & 1]);
+            if (i + 2 < w.units) scores(i + 2);
+          }
+        }
+        ok = __all_sync(0xffffffffu, ok && !*abort_flag);
+        ++pieces;
+        base += 2 * w.nt;
+        g0 += (w.units + 1) >> 1;
+        g1 += w.units >> 1;
+      }
+      if (elect_one()) {
+        prefill::umma_commit(drain);
+        mbar_wait(drain, 0, 146);
+      }
+      __syncwarp();
+    } else if (warp == TABLE_WARP) {
+      // ---------------------------------------------------------------------------------- page ids and scales, ahead
+      // A slice of 16 keys: its K scale; its V scale's logarithm, for the maximum not below -100; the factor that takes a sum
+      // of its weights to l's scale, 1 / s_v; and the logarithm itself. Where s_v is so small, or so far below a scale
+      // before it in the piece, that weights of fp32's full range times 1 / s_v could miss keys that count in l, the
+      // factor is 0 and the slice is marked: its sum is formed apart.
+      int g = 0;
+      bool ok = true;
+      while (ok && sched.next(w)) {
+        const int32_t* row = p.c.a.table + int64_t(max(w.b, 0)) * p.c.a.table_st;
+        float most = -INFINITY;
+        for (int t = 0; ok && t < w.nt; ++t, ++g) {
+          const int s = g % TABLES, per = min(8, BN >> p.lpage);  // pages a tile
+          const int key = (w.kt0 + t) * BN + lane * 16;  // lanes 0 .. 7: a slice
+          int id = -1;
+          float ks = 0.f, vl = -INFINITY;
+          if (lane < 8 && key < w.horizon) {
+            id = row[key >> p.lpage];
+            if (id < 0 || id >= p.c.a.num_pages) {
+              report_bad_index(STATUS);
+              id = -1;
+            } else {
+              const float* sc = p.c.a.scales + int64_t(id) * 2 * p.c.a.Hkv + w.hk;
+              ks = sc[0], vl = log2f(sc[p.c.a.Hkv]);
+            }
+          }
+          float hi = vl;
+#pragma unroll
+          for (int o = 1; o < 8; o <<= 1) hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+          most = fmaxf(most, hi);
+          const bool apart = lane < 8 && key < w.horizon && vl < fmaxf(-100.f, most - 64.f);
+          const float4 f = make_float4(ks, fmaxf(vl, -100.f), apart ? 0.f : exp2f(-fmaxf(vl, -100.f)), vl);
+          const uint32_t marked = __ballot_sync(0xffffffffu, apart);
+          if (g >= TABLES) {
+            if (lane == 0) ok = wait_or_abort(&tab_empty[s], ((g / TABLES) - 1) & 1, abort_flag, 147);
+            ok = __shfl_sync(0xffffffffu, int(ok), 0) != 0;
+            if (!ok) break;
+          }
+          if (lane < 8) tab[s * 8 + lane] = f;
+          if (lane == 0) far_s[s] = marked;
+          const int pg = __shfl_sync(0xffffffffu, id, (lane * 8 / per) & 7);  // the tile's page `lane`
+          if (lane < per) ids[s * 8 + lane] = pg;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&tab_full[s]);
+        }
+      }
+    }
+  } else if (warp >= CONV_WARP) {
+    // ------------------------------------------------------------------------------------ codes into operand tiles
+    reg_dec<104>();
+    Sched<RB> sched(p, prefix);
+    constexpr int UPR = C::DS / 16;       // 16-code units a key and stage
+    constexpr int LD = BN * UPR / 128;    // units a thread and stage
+    constexpr int RSTEP = 128 / UPR;      // keys between a thread's units
+    const int tid = threadIdx.x - CONV_WARP * 32, u = tid % UPR, r0 = tid / UPR;
+    const int page = 1 << p.lpage;
+    // where the thread's unit of key r0 goes in a stage, its two 16-byte halves ordered so that eight lanes fill 128 bytes
+    const int swap = UPR == 8 ? u >> 2 : 0;
+    const uint32_t box = uint32_t(u >> 2) * (BN * 128);
+    const uint32_t c0 = (((2 * (u & 3) + swap) ^ (r0 & 7)) << 4), c1 = (((2 * (u & 3) + 1 - swap) ^ (r0 & 7)) << 4);
+    const uint32_t dst0 = box + r0 * 128 + c0, dst1 = box + r0 * 128 + c1;  // (RSTEP is a multiple of 8)
+    static_assert(RSTEP % 8 == 0, "the swizzle of a thread's rows is one");
+    int pieces = 0, g = 0, gt = 0;  // pieces, stages and tiles so far
+    bool ok = true;
+    while (ok && sched.next(w)) {
+      // ---- queries: rows as they lie, f16, K-major swizzled; and the rows' score factors
+      if (pieces > 0) ok = wait_or_abort(q_empty, (pieces - 1) & 1, abort_flag, 148);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      {
+        constexpr int LPR = D / 8;          // lanes a row
+        constexpr int RPP = 128 / LPR;      // rows a pass
+        constexpr int HOLD = 4;             // passes whose loads are in flight
+        const int qr = tid / LPR, qc = tid % LPR;
+        const int tiles = w.pair ? 2 * BM : BM;
+        const uint32_t boxq = uint32_t(qc >> 3) * (BM * 128);
+        const T* qh = static_cast<const T*>(p.c.a.q) + int64_t(w.hk) * p.G * p.c.a.q_st[1] + int64_t(w.lo) * p.c.a.q_st[2] + qc * 8;
+        float* fac = fac_s + (pieces & 1) * RB;
+        for (int b0 = 0; b0 < tiles; b0 += RPP * HOLD) {
+          uint4 raw[HOLD];
+#pragma unroll
+          for (int i = 0; i < HOLD; ++i) {
+            const int r = b0 + i * RPP + qr, f = w.f0 + r;
+            raw[i] = make_uint4(0, 0, 0, 0);
+            if (r < w.rows) {
+              const int t = f / p.G;
+              const T* src = qh + (f - t * p.G) * p.c.a.q_st[1] + t * p.c.a.q_st[2];
+              if (p.wide_q) {
+                raw[i] = *reinterpret_cast<const uint4*>(src);
+              } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) reinterpret_cast<T*>(&raw[i])[e] = src[e];
+              }
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < HOLD; ++i) {
+            const int r = b0 + i * RPP + qr;
+            uint4 x = raw[i];
+            float f = p.scale_log2;
+            if constexpr (!std::is_same<T, __half>::value) {
+              const __nv_bfloat162* h2 = reinterpret_cast<const __nv_bfloat162*>(&x);
+              __nv_bfloat162 m2 = __hmax2(__hmax2(__habs2(h2[0]), __habs2(h2[1])), __hmax2(__habs2(h2[2]), __habs2(h2[3])));
+              float mx = fmaxf(fmaxf(__low2float(m2), __high2float(m2)), 0.f);  // (NaN is passed over)
+#pragma unroll
+              for (int o = LPR / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+              // times 2^(14 - ex), the largest value's exponent to 14; undone by the factor, in two powers
+              const int ex = mx > 0.f ? min(max((__float_as_int(mx) >> 23) - 127, -112), 127) : 14;
+              const float up = __uint_as_float(uint32_t(127 + 14 - ex) << 23);
+              uint32_t* wx = reinterpret_cast<uint32_t*>(&x);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float2 v = __bfloat1622float2(h2[e]);
+                wx[e] = pack2<__half>(v.x * up, v.y * up);
+              }
+              const int d = ex - 14;
+              f = f * __uint_as_float(uint32_t(127 + d / 2) << 23) * __uint_as_float(uint32_t(127 + d - d / 2) << 23);
+            }
+            if (p.flip) x.x ^= 0x80008000u, x.y ^= 0x80008000u, x.z ^= 0x80008000u, x.w ^= 0x80008000u;
+            const int tile = r / BM, rr = r % BM;
+            *reinterpret_cast<uint4*>(sm + tile * C::QTILE + boxq + rr * 128 + (((qc & 7) ^ (rr & 7)) << 4)) = x;
+            if (qc == 0) fac[r] = f;
+          }
+        }
+        fence_proxy_async_shared();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(q_full);
+      }
+      // ---- codes: stage by stage, the next two stages' loads in flight
+      const int fills = 2 * w.nt * SPT;
+      uint4 buf[2][LD];
+      int tabs = 0;  // tiles of the piece whose ids are known to be in
+      auto load = [&](int s, uint4* x) {
+        int kind, t;
+        entry(w.pair, w.nt, s / SPT, kind, t);
+        const int slot = (gt + t) % TABLES;
+        if (t >= tabs) {
+          if (ok) ok = wait_or_abort(&tab_full[slot], ((gt + t) / TABLES) & 1, abort_flag, 149);
+          tabs = t + 1;
+        }
+        const int key0 = (w.kt0 + t) * BN;
+        const uint8_t* from = p.c.a.pages + (s % SPT) * C::DS + u * 16;
+#pragma unroll
+        for (int i = 0; i < LD; ++i) {
+          const int r = r0 + i * RSTEP;
+          const int id = ids[slot * 8 + (r >> p.lpage)];
+          x[i] = make_uint4(0, 0, 0, 0);
+          if (ok && id >= 0 && key0 + r < w.horizon)
+            x[i] = *reinterpret_cast<const uint4*>(from + ((int64_t(id) * 2 + kind) * p.c.a.Hkv + w.hk) * (page * D) + (r & (page - 1)) * D);
+        }
+        if (kind == 1 && s % SPT == SPT - 1) {  // the tile's ids have been used
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&tab_empty[slot]);
+        }
+      };
+      auto put = [&](const uint4* x) {
+        const int st = g % NS;
+        if (ok && g >= NS) ok = wait_or_abort(&empty[st], ((g / NS) - 1) & 1, abort_flag, 150);
+        uint8_t* d = sm + C::K_OFF + st * C::STAGE;
+#pragma unroll
+        for (int i = 0; i < LD; ++i) {
+          uint32_t h[8];
+          kv8::dec4(x[i].x, h[0], h[1]);
+          kv8::dec4(x[i].y, h[2], h[3]);
+          kv8::dec4(x[i].z, h[4], h[5]);
+          kv8::dec4(x[i].w, h[6], h[7]);
+          const uint4 a = make_uint4(h[0], h[1], h[2], h[3]), b = make_uint4(h[4], h[5], h[6], h[7]);
+          *reinterpret_cast<uint4*>(d + dst0 + i * RSTEP * 128) = swap ? b : a;
+          *reinterpret_cast<uint4*>(d + dst1 + i * RSTEP * 128) = swap ? a : b;
+        }
+        fence_proxy_async_shared();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&full[st]);
+        ++g;
+      };
+      load(0, buf[0]);
+      load(1, buf[1]);  // (a piece has two fills at least)
+      for (int s = 0; ok && s < fills; s += 2) {
+        put(buf[0]);
+        if (s + 2 < fills) load(s + 2, buf[0]);
+        put(buf[1]);
+        if (s + 3 < fills) load(s + 3, buf[1]);
+        ok = __all_sync(0xffffffffu, ok);
+      }
+      ++pieces;
+      gt += w.nt;
+    }
+    if (!ok) *abort_flag = 1;
+  } else {
+    // ------------------------------------------------------------------------------------ softmax, epilogue
+    reg_inc<176>();
+    Sched<RB> sched(p, prefix);
+    const int wg = warp >> 2, quarter = warp & 3, r = 32 * quarter + lane;
+    const uint32_t lane_base = tmem + (uint32_t(32 * quarter) << 16);
+    const uint32_t s_col = lane_base + wg * BN;
+    const uint32_t o_col = lane_base + C::O_COL + (C::WIDE ? 0 : wg * D);
+    int pieces = 0, gt = 0, cnt[2] = {0, 0};  // pieces, tiles, units of each buffer so far
+    bool ok = true;
+    int4 rec0 = make_int4(0, 0, 0, 0), rec1 = rec0;
+    while (sched.next(w)) {
+      const int row = r + (w.pair ? wg * BM : 0);  // in the item
+      const bool live = row < w.rows;
+      const int tok = (w.f0 + row) / p.G;
+      const int lim = !live ? -1 : (p.c.a.causal ? w.len - (w.n - 1 - tok) : w.len) - 1;  // the last key that the row sees
+      float m = -FLT_MAX, l = 0.f, fac = 0.f;
+      for (int i = wg; i < w.units; i += 2) {
+        const int t = w.pair ? i >> 1 : i, slot = (gt + t) % TABLES;
+        const int own = cnt[wg] + (i >> 1);  // the buffer's units before this one
+        if (ok) ok = wait_or_abort(&s_full[wg], own & 1, abort_flag, 151);
+        ok = __all_sync(0xffffffffu, ok);
+        prefill::tc_fence_after();
+        float s[BN];
+#pragma unroll
+        for (int c = 0; c < BN; c += 32) prefill::tmem_ld32(s_col + c, s + c);
+        if (i < 2) fac = fac_s[(pieces & 1) * RB + row];
+        const float4* sc = tab + slot * 8;
+        prefill::tmem_wait_ld();
+        const int over = lim - (w.kt0 + t) * BN;  // the last column that the row sees
+        if (__any_sync(0xffffffffu, over < BN - 1)) {
+#pragma unroll
+          for (int c = 0; c < BN; ++c)
+            if (c > over) s[c] = -INFINITY;
+        }
+        // the row's largest score with the values' scale (a factor is never 0: -inf times it stays -inf)
+        float top = -INFINITY;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          const float4 f = sc[q];
+          const float* x = s + 16 * q;
+          float a = max3(x[0], x[1], x[2]), b = max3(x[3], x[4], x[5]);
+          a = max3(a, x[6], x[7]), b = max3(b, x[8], x[9]);
+          a = max3(a, x[10], x[11]), b = max3(b, x[12], x[13]);
+          a = max3(a, x[14], x[15]);
+          top = fmaxf(top, fmaf(fmaxf(a, b), fmaxf(fac * f.x, FLT_MIN), f.y));
+        }
+        bool began;  // O holds something
+        if constexpr (C::WIDE) {
+          began = i > 0;
+          if (i > 0) {  // the maximum after the unit before
+            if (ok) ok = wait_or_abort(&token[(1 - wg) * 4 + quarter], (cnt[1 - wg] + ((i - 1) >> 1)) & 1, abort_flag, 152);
+            const float now = m_sh[r];
+            if (now != m) {
+              l = shrink(l, m - now);
+              m = now;
+            }
+          }
+        } else {
+          began = i > 1;
+        }
+        const bool move = top > m + (TOP + 8.f);
+        if (__any_sync(0xffffffffu, move)) {
+          const float now = move ? top - TOP : m, corr = move ? prefill::ex2f(m - now) : 1.f;
+          if (began) {
+            const int prev = C::WIDE ? 1 - wg : wg;  // the buffer of the O product before
+            const int nth = C::WIDE ? cnt[1 - wg] + ((i - 1) >> 1) : own - 1;
+            if (ok) ok = wait_or_abort(&o_done[prev], nth & 1, abort_flag, 153);
+            ok = __all_sync(0xffffffffu, ok);
+            prefill::tc_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < D; c += 16) {
+              float ov[16];
+              prefill2::tmem_ld16(o_col + c, ov);
+              prefill::tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 16; ++e) ov[e] *= corr;
+              prefill::tmem_st16(o_col + c, reinterpret_cast<const uint32_t*>(ov));
+            }
+            prefill::tmem_wait_st();
+          }
+          l = shrink(l, m - now);
+          m = now;
+        }
+        if constexpr (C::WIDE) {
+          m_sh[r] = m;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&token[wg * 4 + quarter]);
+        }
+        if (const uint32_t marked = far_s[slot]) {
+#pragma unroll
+          for (int q = 0; q < 8; ++q)
+            if (marked >> q & 1) {
+              const float mul = fmaxf(fac * sc[q].x, FLT_MIN);
+#pragma unroll
+              for (int c = 0; c < 16; ++c) l += prefill::ex2f(fmaf(s[16 * q + c], mul, -m));
+            }
+        }
+        // weights
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          uint32_t pk[32];
+#pragma unroll
+          for (int qq = 0; qq < 4; ++qq) {
+            const int q = half * 4 + qq;
+            const float4 f = sc[q];
+            const float mul = fmaxf(fac * f.x, FLT_MIN), add = f.w - m;
+            float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int c = 0; c < 16; c += 2) {
+              float2 x = kv8::fma2(make_float2(s[16 * q + c], s[16 * q + c + 1]), make_float2(mul, mul), make_float2(add, add));
+              x.x = prefill::ex2f(x.x), x.y = prefill::ex2f(x.y);
+              sum.x += x.x, sum.y += x.y;
+              pk[qq * 8 + c / 2] = pack2<__half>(x.x, x.y);
+            }
+            l = fmaf(sum.x + sum.y, f.z, l);
+          }
+          prefill::tmem_st32(s_col + half * 32, reinterpret_cast<const float*>(pk));
+        }
+        prefill::tmem_wait_st();
+        prefill::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&p_full[wg]);
+          mbar_arrive(&tab_empty[slot]);
+          if (!w.pair) mbar_arrive(&tab_empty[slot]);
+        }
+      }
+      // -------------------------------------------------------------------------------- the piece's end
+      const int n0 = (w.units + 1) >> 1, n1 = w.units >> 1;
+      float f0 = 1.f, f1 = 0.f;  // factors of this group's O, or of O 0 and O 1
+      if (w.pair) {
+        if (ok) ok = wait_or_abort(&o_done[wg], (cnt[wg] + n0 - 1) & 1, abort_flag, 154);
+      } else {
+        ml_s[wg * BM + r] = make_float2(m, l);
+        asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");
+        const float2 x = ml_s[r], y = ml_s[BM + r];
+        m = fmaxf(x.x, y.x);  // (a shared maximum never falls, so it is the later one)
+        f0 = prefill::ex2f(x.x - m);
+        f1 = n1 ? prefill::ex2f(y.x - m) : 0.f;
+        l = shrink(x.y, x.x - m) + (n1 ? shrink(y.y, y.x - m) : 0.f);
+        if (C::WIDE) f0 = 1.f;
+        asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");  // (read before the next piece's are written)
+        if (ok) ok = wait_or_abort(&o_done[0], (cnt[0] + n0 - 1) & 1, abort_flag, 155);
+        if (ok && n1) ok = wait_or_abort(&o_done[1], (cnt[1] + n1 - 1) & 1, abort_flag, 156);
+      }
+      ok = __all_sync(0xffffffffu, ok);
+      prefill::tc_fence_after();
+      const int first = w.pair ? 0 : wg * (D / 2), count = w.pair ? D : D / 2;  // this thread's columns of O
+      const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+      const uint32_t oc = w.pair ? o_col : lane_base + C::O_COL;
+      T* out = static_cast<T*>(p.c.a.o) + int64_t(w.hk * p.G + (w.f0 + row) % p.G) * p.c.a.o_st[1] + int64_t(w.lo + tok) * p.c.a.o_st[2];
+      float* part = p.ws_o + int64_t(w.slot) * (D * RB) + row;
+#pragma unroll 1
+      for (int c = first; c < first + count; c += 32) {
+        float ov[32];
+        prefill::tmem_ld32(oc + c, ov);
+        prefill::tmem_wait_ld();
+        if (!C::WIDE && !w.pair) {
+          if (n1) {
+            float o1[32];
+            prefill::tmem_ld32(oc + D + c, o1);
+            prefill::tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) ov[e] = ov[e] * f0 + o1[e] * f1;
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) ov[e] *= f0;
+          }
+        }
+        if (!live || !ok) continue;
+        if (w.whole) {
+          float sum = 0.f;  // (finite unless some value is not)
+#pragma unroll
+          for (int e = 0; e < 32; ++e) sum = fmaf(ov[e], 0.f, sum);
+          if (sum != sum && l == l) *again = 1;
+          store32<T>(out + c, ov, inv, p.wide_o);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) part[(c + e) * RB] = ov[e];
+        }
+      }
+      prefill::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(o_free);
+      if (!w.whole && (w.pair || wg == 0)) {
+        p.ws_ml[int64_t(w.slot) * 2 * RB + row] = m;
+        p.ws_ml[int64_t(w.slot) * 2 * RB + RB + row] = l;
+      }
+      if (w.nparts) rec0 = make_int4(w.nparts, w.b, w.lo, w.n), rec1 = make_int4(w.len, w.hk, w.f0, w.rows);
+      ++pieces;
+      gt += w.nt;
+      cnt[0] += n0;
+      cnt[1] += n1;
+    }
+    if (!ok) *abort_flag = 1, rec0.x = 0;
+    if (threadIdx.x == 0) {
+      p.rec[2 * blockIdx.x] = rec0;
+      p.rec[2 * blockIdx.x + 1] = rec1;
+    }
+  }
+
+  prefill::tc_fence_before();
+  __syncthreads();
+  if (warp == MMA_WARP) {
+    prefill::tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+  }
+  // The second look (rare), when nothing waits for this CTA any more: its whole items' rows, a warp a row.
+  if (*again && !*abort_flag) {
+    Sched<RB> sched(p, prefix);
+    while (sched.next(w))
+      for (int x = warp; w.whole && x < w.rows; x += THREADS / 32)
+        row_again<T, D>(p, w.b, w.lo, w.n, w.len, w.hk, w.f0 + x, w.horizon);
+  }
+}
+
+// Merges an item's parts: block (CTA that begins it, 32 of its rows), a lane a row, the warps sharing the columns.
+template <typename T, int D>
+__global__ void __launch_bounds__(128) combine_kernel(const Params p) {
+  constexpr int RB = Cfg<D>::RB;
+  __shared__ float s_m[4][32], s_l[4][32];
+  __shared__ int s_nan;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int4 a = p.rec[2 * blockIdx.x], e4 = p.rec[2 * blockIdx.x + 1];
+  const int parts = a.x, r0 = blockIdx.y * 32, rows = e4.w;
+  if (parts == 0 || r0 >= rows) return;
+  if (threadIdx.x == 0) s_nan = 0;
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, row = r0 + lane;
+  auto slot = [&](int i) { return i == 0 ? 2 * int64_t(blockIdx.x) + 1 : 2 * (int64_t(blockIdx.x) + i); };
+  // the row's maximum and sum: the warps share the parts
+  float M = -FLT_MAX, L = 0.f;
+  for (int i = w; i < parts; i += 4) M = fmaxf(M, p.ws_ml[slot(i) * 2 * RB + row]);
+  s_m[w][lane] = M;
+  __syncthreads();
+  M = fmaxf(fmaxf(s_m[0][lane], s_m[1][lane]), fmaxf(s_m[2][lane], s_m[3][lane]));
+  for (int i = w; i < parts; i += 4)
+    L += shrink(p.ws_ml[slot(i) * 2 * RB + RB + row], p.ws_ml[slot(i) * 2 * RB + row] - M);
+  s_l[w][lane] = L;
+  __syncthreads();
+  L = (s_l[0][lane] + s_l[1][lane]) + (s_l[2][lane] + s_l[3][lane]);
+  const float inv = L > 0.f || L != L ? 1.f / L : 0.f;
+  const int f = e4.z + row, tok = f / p.G;
+  T* out = static_cast<T*>(p.c.a.o) + int64_t(e4.y * p.G + f % p.G) * p.c.a.o_st[1] + int64_t(a.z + tok) * p.c.a.o_st[2];
+  const bool live = row < rows;
+  for (int c = w * 32; c < D; c += 128) {
+    float x[32];
+#pragma unroll
+    for (int e = 0; e < 32; ++e) x[e] = 0.f;
+    for (int i = 0; live && i < parts; ++i) {
+      const float g = prefill::ex2f(p.ws_ml[slot(i) * 2 * RB + row] - M);
+      const float* src = p.ws_o + slot(i) * (D * RB) + row;
+#pragma unroll
+      for (int e = 0; e < 32; ++e) x[e] = fmaf(src[(c + e) * RB], g, x[e]);
+    }
+    float sum = 0.f;
+#pragma unroll
+    for (int e = 0; e < 32; ++e) sum = fmaf(x[e], 0.f, sum);
+    if (live) {
+      if (sum != sum && L == L) s_nan = 1;
+      store32<T>(out + c, x, inv, p.wide_o);
+    }
+  }
+  __syncthreads();
+  if (!s_nan) return;
+  const Range x{a.z, a.w, e4.x};
+  const Block b = block_of<RB>(p, x, e4.z / RB);
+  for (int i = r0 + w; i < min(r0 + 32, rows); i += 4) row_again<T, D>(p, a.y, a.z, a.w, e4.x, e4.y, e4.z + i, b.horizon);
+}
+
+}  // namespace kv8chunk
+}  // namespace lb2

@@ -29,6 +29,7 @@
 #include "kv8_pages.cuh"
 #include "attn_rows.cuh"
 #include "kv8_attend.cuh"
+#include "kv8_chunk.cuh"
 
 namespace lb2 {
 
@@ -1827,10 +1828,100 @@ static int chunk_rows(const arows::ChunkParams& p, int D, cudaStream_t st) {
   return LB2_OK;
 }
 
+namespace lb2 {
+namespace kv8chunk {
+
+// Partials of two pieces a CTA, and what the merge reads of the items.
+struct Plan {
+  int grid;
+  size_t ml, rec, total;
+};
+
+static Plan plan(int D) {
+  Plan pl{};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  pl.grid = sm_count(dev);
+  const size_t rb = D == 256 ? Cfg<256>::RB : Cfg<128>::RB;
+  pl.ml = size_t(2) * pl.grid * rb * D * sizeof(float);
+  pl.rec = pl.ml + size_t(2) * pl.grid * rb * 2 * sizeof(float);
+  pl.total = pl.rec + size_t(2) * pl.grid * sizeof(int4);
+  return pl;
+}
+
+template <typename T, int D>
+static int launch(const Params& p, int grid, cudaStream_t st) {
+  using C = Cfg<D>;
+  static int attr_dev = -1;
+  int dev = 0;
+  LB2_CUDA(cudaGetDevice(&dev));
+  if (attr_dev != dev) {
+    LB2_CUDA(cudaFuncSetAttribute(chunk_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+    attr_dev = dev;
+  }
+  cudaLaunchAttribute pdl[1];
+  pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  pdl[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = C::SMEM;
+  cfg.stream = st;
+  cfg.attrs = pdl;
+  cfg.numAttrs = 1;
+  LB2_CUDA(cudaLaunchKernelEx(&cfg, chunk_kernel<T, D>, p));
+  cfg.gridDim = dim3(static_cast<unsigned>(grid), C::RB / 32);
+  cfg.blockDim = dim3(128);
+  cfg.dynamicSmemBytes = 0;
+  LB2_CUDA(cudaLaunchKernelEx(&cfg, combine_kernel<T, D>, p));
+  return LB2_OK;
+}
+
+static int run(const arows::ChunkParams& c, int D, int dtype, void* workspace, cudaStream_t st) {
+  Params p{};
+  const Plan pl = plan(D);
+  p.c = c;
+  p.ws_o = static_cast<float*>(workspace);
+  p.ws_ml = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + pl.ml);
+  p.rec = reinterpret_cast<int4*>(static_cast<uint8_t*>(workspace) + pl.rec);
+  const arows::PagedParams& a = c.a;
+  p.G = a.Hq / a.Hkv;
+  p.lpage = a.page == 16 ? 4 : a.page == 32 ? 5 : a.page == 64 ? 6 : 7;
+  p.wide_q = aligned16(a.q) && a.q_st[1] % 8 == 0 && a.q_st[2] % 8 == 0;
+  p.wide_o = 0;
+  for (int n = 16; n <= 32; n *= 2)
+    if (reinterpret_cast<uintptr_t>(a.o) % n == 0 && a.o_st[1] * 2 % n == 0 && a.o_st[2] * 2 % n == 0) p.wide_o = n;
+  p.flip = std::signbit(a.scale);
+  p.scale_log2 = std::fabs(a.scale) * 1.4426950408889634f;
+  p.min_units = 2;
+  for (int b0 = 0; b0 < a.B; b0 += MAX_B) {
+    Params x = p;
+    x.c.a.B = std::min(MAX_B, a.B - b0);
+    x.c.a.table = a.table + b0 * a.table_st;
+    x.c.a.kv_len = a.kv_len + b0;
+    x.c.cu = c.cu + b0;
+    x.first = b0 == 0;
+    x.last = b0 + MAX_B >= a.B;
+    int rc;
+    if (dtype == LB2_BF16)
+      rc = D == 64 ? launch<__nv_bfloat16, 64>(x, pl.grid, st)
+                   : D == 128 ? launch<__nv_bfloat16, 128>(x, pl.grid, st) : launch<__nv_bfloat16, 256>(x, pl.grid, st);
+    else
+      rc = D == 64 ? launch<__half, 64>(x, pl.grid, st)
+                   : D == 128 ? launch<__half, 128>(x, pl.grid, st) : launch<__half, 256>(x, pl.grid, st);
+    if (rc) return rc;
+  }
+  return LB2_OK;
+}
+
+}  // namespace kv8chunk
+}  // namespace lb2
+
 extern "C" {
 
 size_t lb2_kv8_attend_packed_workspace_size(int B, int Hq, int Hkv, int T, int D) {
-  return 0;
+  if (B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || T <= 0 || (D != 64 && D != 128 && D != 256)) return 0;
+  return kv8chunk::plan(D).total;
 }
 
 int lb2_kv8_attend_packed(const void* q, const int64_t* q_st, const uint8_t* pages, const float* scales,
@@ -1863,7 +1954,11 @@ int lb2_kv8_attend_packed(const void* q, const int64_t* q_st, const uint8_t* pag
   p.a.scale = scale;
   p.cu = cu;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return dtype == LB2_F32 ? chunk_rows<float>(p, D, st) : dtype == LB2_BF16 ? chunk_rows<__nv_bfloat16>(p, D, st) : chunk_rows<__half>(p, D, st);
+  if (dtype == LB2_F32) return chunk_rows<float>(p, D, st);
+  LB2_CHECK_ARG(workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0 &&
+                    workspace_bytes >= lb2_kv8_attend_packed_workspace_size(B, Hq, Hkv, T, D),
+                "kv8_attend_packed: workspace too small or not 256-byte aligned");
+  return kv8chunk::run(p, D, dtype, workspace, st);
 }
 
 // ------------------------------------------------------------------------------------------------ pages moved about
