@@ -30,7 +30,7 @@
 // again reading only what it sees.
 //
 // Roles (512 threads): warps 0-3, 4-7 softmax and epilogue (warp w: TMEM lanes of quarter w % 4), 8-11 codes and queries into
-// shared memory, 12 issues the products, 13 reads the page table and scales ahead.
+// shared memory, 12 issues the products, 13 reads the page table and scales ahead, 14 lists the CTA's pieces of work.
 #pragma once
 
 #include <cfloat>
@@ -47,10 +47,20 @@ namespace kv8chunk {
 constexpr int BM = 128, BN = 128;  // rows of a row tile, keys of a key tile
 constexpr int MAX_B = 1024;        // sequences a launch
 constexpr int THREADS = 512;
-constexpr int CONV_WARP = 8, MMA_WARP = 12, TABLE_WARP = 13;
+constexpr int CONV_WARP = 8, MMA_WARP = 12, TABLE_WARP = 13, PLAN_WARP = 14;
+constexpr int PIECES = 4;          // pieces of work listed ahead
 constexpr int TABLES = 8;          // key tiles whose page ids and scales are held
 constexpr float TOP = 7.f;         // a weight at the running maximum is 2^TOP
 constexpr int STATUS = arows::STATUS_CHUNK;  // lb2_status: 140 lengths and page ids, 141.. waits
+
+// What a CTA does of one item: key tiles kt0 .. kt0 + nt - 1. No units: the end of the list.
+struct Piece {
+  int b, lo, n, len, hk, f0, rows, horizon, kt0, nt, units;
+  int pair, whole;
+  int slot;    // of its partial, where it is not the whole item
+  int nparts;  // of an item that it begins and does not end, else 0
+  int pad;
+};
 
 template <int D>
 struct Cfg {
@@ -70,7 +80,8 @@ struct Cfg {
   static constexpr int ML_OFF = FAC_OFF + 2 * RB * 4;          // [2][128] float2
   static constexpr int MSH_OFF = ML_OFF + 2 * BM * 8;          // [128] the shared maximum
   static constexpr int PREFIX_OFF = MSH_OFF + BM * 4;          // [MAX_B + 3] int64
-  static constexpr int BAR_OFF = PREFIX_OFF + (MAX_B + 3) * 8;
+  static constexpr int PIECE_OFF = PREFIX_OFF + (MAX_B + 3) * 8;  // [PIECES] Piece
+  static constexpr int BAR_OFF = PIECE_OFF + PIECES * int(sizeof(Piece));
   static constexpr int SMEM = BAR_OFF + 512 + 1024;
   static constexpr int O_COL = 2 * BN;            // O, or the two warpgroups' O at O_COL and O_COL + D
   static_assert(PREFIX_OFF % 8 == 0 && SMEM <= 232448, "shared memory budget");
@@ -130,15 +141,7 @@ __device__ __forceinline__ Block block_of(const Params& p, const Range& x, int k
   return b;
 }
 
-// What a CTA does of one item: key tiles kt0 .. kt0 + nt - 1.
-struct Piece {
-  int b, lo, n, len, hk, f0, rows, horizon, kt0, nt, units;
-  bool pair, whole;
-  int slot;    // of its partial, where it is not the whole item
-  int nparts;  // of an item that it begins and does not end, else 0
-};
-
-// The CTA's pieces in order, each warp for itself. prefix[r]: units of the ranges before r.
+// The CTA's pieces in order, found by one warp. prefix[r]: units of the ranges before r.
 template <int RB>
 struct Sched {
   const Params& p;
@@ -247,6 +250,7 @@ __device__ __forceinline__ float shrink(float l, float x) {
   return l * h * h;
 }
 
+// (Once a warp: a second change needs a barrier of its warpgroup first.)
 template <int N>
 __device__ __forceinline__ void reg_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N>
@@ -345,6 +349,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
   float2* ml_s = reinterpret_cast<float2*>(sm + C::ML_OFF);
   volatile float* m_sh = reinterpret_cast<volatile float*>(sm + C::MSH_OFF);
   int64_t* prefix = reinterpret_cast<int64_t*>(sm + C::PREFIX_OFF);
+  Piece* list = reinterpret_cast<Piece*>(sm + C::PIECE_OFF);
   uint64_t* full = reinterpret_cast<uint64_t*>(sm + C::BAR_OFF);  // [NS] a stage's operand is in
   uint64_t* empty = full + NS;           // [NS] its products are done
   uint64_t* q_full = empty + NS;
@@ -356,11 +361,15 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
   uint64_t* tab_full = o_free + 1;       // [TABLES]
   uint64_t* tab_empty = tab_full + TABLES;
   uint64_t* token = tab_empty + TABLES;  // [2 warpgroups][4 quarters]: the shared maximum after the group's unit
-  uint64_t* drain = token + 8;
+  uint64_t* piece_full = token + 8;      // [PIECES]
+  uint64_t* piece_empty = piece_full + PIECES;
+  uint64_t* meet = piece_empty + PIECES;  // [4 quarters]: the two softmax warps of the same rows
+  uint64_t* written = meet + 4;          // the softmax warps are done
+  uint64_t* drain = written + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* again = abort_flag + 1;
-  static_assert((2 * NS + 2 + 6 + 1 + 2 * TABLES + 8 + 1) * 8 + 12 <= 512, "barrier area");
+  static_assert((2 * NS + 2 + 6 + 1 + 2 * TABLES + 8 + 2 * PIECES + 4 + 2) * 8 + 12 <= 512, "barrier area");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -381,6 +390,12 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
       mbar_init(&tab_empty[i], 12);  // four warps' V loads and eight softmax warps (four, twice, where one group has the tile)
     }
     for (int i = 0; i < 8; ++i) mbar_init(&token[i], 1);
+    for (int i = 0; i < PIECES; ++i) {
+      mbar_init(&piece_full[i], 1);
+      mbar_init(&piece_empty[i], 14);  // eight softmax warps, four of the codes, the products', the tables'
+    }
+    for (int i = 0; i < 4; ++i) mbar_init(&meet[i], 2);
+    mbar_init(written, 8);
     mbar_init(drain, 1);
     *abort_flag = 0;
     *again = 0;
@@ -425,22 +440,49 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
   prefill::tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  Piece w;
+  // Piece number i of the list (the end of it, or a wait that gave up: false); done with, its place is free.
+  auto piece = [&](int i) {
+    bool ok = wait_or_abort(&piece_full[i % PIECES], (i / PIECES) & 1, abort_flag, 157);
+    ok = __all_sync(0xffffffffu, ok);
+    return ok && list[i % PIECES].units > 0;
+  };
+  auto piece_done = [&](int i) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&piece_empty[i % PIECES]);
+  };
 
   if (warp >= CONV_WARP + 4) {
     reg_dec<56>();
-    Sched<RB> sched(p, prefix);
-    if (warp == MMA_WARP) {
+    if (warp == PLAN_WARP) {
+      // ---------------------------------------------------------------------------------- the list of pieces
+      Sched<RB> sched(p, prefix);
+      Piece w;
+      bool more = true;
+      for (int i = 0; more; ++i) {
+        more = sched.next(w);
+        if (!more) w.units = 0;
+        bool ok = i < PIECES || wait_or_abort(&piece_empty[i % PIECES], ((i / PIECES) - 1) & 1, abort_flag, 158);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        if (lane == 0) {
+          list[i % PIECES] = w;
+          mbar_arrive(&piece_full[i % PIECES]);
+        }
+        __syncwarp();
+      }
+    } else if (warp == MMA_WARP) {
       // ---------------------------------------------------------------------------------- MMA issuer
       int pieces = 0, base = 0, g0 = 0, g1 = 0;  // pieces and ring entries so far; units of each buffer so far
       bool ok = true;
-      while (ok && sched.next(w)) {
+      while (ok && piece(pieces)) {
+        const Piece& w = list[pieces % PIECES];
+        const bool pair = w.pair;
+        const int nt = w.nt, units = w.units;
         if (elect_one()) {
           ok = wait_or_abort(q_full, pieces & 1, abort_flag, 141);
           const uint32_t q_addr = smem_u32(sm), k0 = smem_u32(sm + C::K_OFF);
           auto scores = [&](int i) {
-            const int t = w.pair ? i >> 1 : i, e = (base + k_entry(w.pair, t)) * SPT;
-            const uint32_t q = q_addr + (w.pair ? (i & 1) * C::QTILE : 0);
+            const int t = pair ? i >> 1 : i, e = (base + k_entry(pair, t)) * SPT;
+            const uint32_t q = q_addr + (pair ? (i & 1) * C::QTILE : 0);
 #pragma unroll
             for (int h = 0; h < SPT; ++h) {
               const int st = (e + h) % NS;
@@ -453,15 +495,15 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
                                  prefill::sdesc(q + ((kk >> 2) + h * (C::DS / 64)) * BM * 128 + (kk & 3) * 32, 16, 1024),
                                  prefill::sdesc(k + (kk >> 2) * BN * 128 + (kk & 3) * 32, 16, 1024), IDESC_S,
                                  h + kk > 0 ? 1u : 0u);
-              if (!w.pair || (i & 1)) prefill::umma_commit(&empty[st]);
+              if (!pair || (i & 1)) prefill::umma_commit(&empty[st]);
             }
             prefill::umma_commit(&s_full[i & 1]);
-            if (i == w.units - 1) prefill::umma_commit(q_empty);
+            if (i == units - 1) prefill::umma_commit(q_empty);
           };
           if (ok) scores(0);
-          if (ok && w.units > 1) scores(1);
-          for (int i = 0; ok && i < w.units; ++i) {
-            const int t = w.pair ? i >> 1 : i, e = (base + v_entry(w.pair, w.nt, t)) * SPT;
+          if (ok && units > 1) scores(1);
+          for (int i = 0; ok && i < units; ++i) {
+            const int t = pair ? i >> 1 : i, e = (base + v_entry(pair, nt, t)) * SPT;
             ok = wait_or_abort(&p_full[i & 1], ((i & 1 ? g1 : g0) + (i >> 1)) & 1, abort_flag, 143);
             if (ok && i == 0 && pieces > 0) ok = wait_or_abort(o_free, (pieces - 1) & 1, abort_flag, 144);
             const bool own = !C::WIDE;  // each buffer its O
@@ -478,18 +520,19 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
                 prefill::umma_ts(o + h * C::DS, tmem + (i & 1) * BN + kk * 8,
                                  prefill::sdesc(v + kk * 16 * 128, BN * 128, 1024), IDESC_PV,
                                  (own ? i > 1 : i > 0) || kk > 0 ? 1u : 0u);
-              if (!w.pair || (i & 1)) prefill::umma_commit(&empty[st]);
+              if (!pair || (i & 1)) prefill::umma_commit(&empty[st]);
             }
             if (!ok) break;
             prefill::umma_commit(&o_done[i & 1]);
-            if (i + 2 < w.units) scores(i + 2);
+            if (i + 2 < units) scores(i + 2);
           }
         }
         ok = __all_sync(0xffffffffu, ok && !*abort_flag);
+        piece_done(pieces);
         ++pieces;
-        base += 2 * w.nt;
-        g0 += (w.units + 1) >> 1;
-        g1 += w.units >> 1;
+        base += 2 * nt;
+        g0 += (units + 1) >> 1;
+        g1 += units >> 1;
       }
       if (elect_one()) {
         prefill::umma_commit(drain);
@@ -502,51 +545,72 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
       // of its weights to l's scale, 1 / s_v; and the logarithm itself. Where s_v is so small, or so far below a scale
       // before it in the piece, that weights of fp32's full range times 1 / s_v could miss keys that count in l, the
       // factor is 0 and the slice is marked: its sum is formed apart.
+      // Four tiles at a time, a lane a slice, the next four asked for while these wait for their places.
       int g = 0;
       bool ok = true;
-      while (ok && sched.next(w)) {
+      const int per = min(8, BN >> p.lpage);  // pages a tile
+      for (int i = 0; ok && piece(i); ++i) {
+        const Piece& w = list[i % PIECES];
         const int32_t* row = p.c.a.table + int64_t(max(w.b, 0)) * p.c.a.table_st;
+        const int key0 = w.kt0 * BN, horizon = w.horizon, hk = w.hk, nt = w.nt;
         float most = -INFINITY;
-        for (int t = 0; ok && t < w.nt; ++t, ++g) {
-          const int s = g % TABLES, per = min(8, BN >> p.lpage);  // pages a tile
-          const int key = (w.kt0 + t) * BN + lane * 16;  // lanes 0 .. 7: a slice
-          int id = -1;
-          float ks = 0.f, vl = -INFINITY;
-          if (lane < 8 && key < w.horizon) {
+        auto fetch = [&](int t, int& id, float& ks, float& vs) {
+          const int key = key0 + t * BN + lane * 16;
+          id = -1, ks = 0.f, vs = 0.f;
+          if (key < horizon && t + (lane >> 3) < nt) {
             id = row[key >> p.lpage];
             if (id < 0 || id >= p.c.a.num_pages) {
               report_bad_index(STATUS);
               id = -1;
             } else {
-              const float* sc = p.c.a.scales + int64_t(id) * 2 * p.c.a.Hkv + w.hk;
-              ks = sc[0], vl = log2f(sc[p.c.a.Hkv]);
+              const float* sc = p.c.a.scales + int64_t(id) * 2 * p.c.a.Hkv + hk;
+              ks = sc[0], vs = sc[p.c.a.Hkv];
             }
           }
+        };
+        int id;
+        float ks, vs;
+        fetch(0, id, ks, vs);
+        for (int t = 0; ok && t < nt; t += 4) {
+          const int cid = id;
+          const float cks = ks, vl = log2f(vs);
+          const bool held = cid >= 0;
+          fetch(t + 4, id, ks, vs);
+          // the largest scale up to each tile
           float hi = vl;
 #pragma unroll
           for (int o = 1; o < 8; o <<= 1) hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-          most = fmaxf(most, hi);
-          const bool apart = lane < 8 && key < w.horizon && vl < fmaxf(-100.f, most - 64.f);
-          const float4 f = make_float4(ks, fmaxf(vl, -100.f), apart ? 0.f : exp2f(-fmaxf(vl, -100.f)), vl);
-          const uint32_t marked = __ballot_sync(0xffffffffu, apart);
-          if (g >= TABLES) {
-            if (lane == 0) ok = wait_or_abort(&tab_empty[s], ((g / TABLES) - 1) & 1, abort_flag, 147);
-            ok = __shfl_sync(0xffffffffu, int(ok), 0) != 0;
-            if (!ok) break;
+#pragma unroll
+          for (int o = 8; o < 32; o <<= 1) {
+            const float y = __shfl_up_sync(0xffffffffu, hi, o);
+            if (lane >= o) hi = fmaxf(hi, y);
           }
-          if (lane < 8) tab[s * 8 + lane] = f;
-          if (lane == 0) far_s[s] = marked;
-          const int pg = __shfl_sync(0xffffffffu, id, (lane * 8 / per) & 7);  // the tile's page `lane`
-          if (lane < per) ids[s * 8 + lane] = pg;
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&tab_full[s]);
+          hi = fmaxf(hi, most);
+          most = __shfl_sync(0xffffffffu, hi, 31);
+          const bool apart = held && vl < fmaxf(-100.f, hi - 64.f);
+          const float4 f = make_float4(cks, fmaxf(vl, -100.f), apart ? 0.f : exp2f(-fmaxf(vl, -100.f)), vl);
+          const uint32_t marked = __ballot_sync(0xffffffffu, apart);
+          const int pg = __shfl_sync(0xffffffffu, cid, (lane & 24) | ((lane & 7) * 8 / per & 7));  // the tile's page lane % 8
+          for (int j = 0; j < min(4, nt - t); ++j, ++g) {
+            const int s = g % TABLES;
+            if (g >= TABLES) ok = wait_or_abort(&tab_empty[s], ((g / TABLES) - 1) & 1, abort_flag, 147);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            if (lane >> 3 == j) {
+              tab[s * 8 + (lane & 7)] = f;
+              if ((lane & 7) < per) ids[s * 8 + (lane & 7)] = pg;
+              if ((lane & 7) == 0) far_s[s] = marked >> (8 * j) & 255u;
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&tab_full[s]);
+          }
         }
+        piece_done(i);
       }
     }
   } else if (warp >= CONV_WARP) {
     // ------------------------------------------------------------------------------------ codes into operand tiles
     reg_dec<104>();
-    Sched<RB> sched(p, prefix);
     constexpr int UPR = C::DS / 16;       // 16-code units a key and stage
     constexpr int LD = BN * UPR / 128;    // units a thread and stage
     constexpr int RSTEP = 128 / UPR;      // keys between a thread's units
@@ -560,7 +624,10 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
     static_assert(RSTEP % 8 == 0, "the swizzle of a thread's rows is one");
     int pieces = 0, g = 0, gt = 0;  // pieces, stages and tiles so far
     bool ok = true;
-    while (ok && sched.next(w)) {
+    while (ok && piece(pieces)) {
+      const Piece& w = list[pieces % PIECES];
+      const int horizon = w.horizon, hk = w.hk, nt = w.nt, kt0 = w.kt0;
+      const bool pair = w.pair;
       // ---- queries: rows as they lie, f16, K-major swizzled; and the rows' score factors
       if (pieces > 0) ok = wait_or_abort(q_empty, (pieces - 1) & 1, abort_flag, 148);
       if (!__all_sync(0xffffffffu, ok)) break;
@@ -569,9 +636,9 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
         constexpr int RPP = 128 / LPR;      // rows a pass
         constexpr int HOLD = 4;             // passes whose loads are in flight
         const int qr = tid / LPR, qc = tid % LPR;
-        const int tiles = w.pair ? 2 * BM : BM;
+        const int tiles = pair ? 2 * BM : BM;
         const uint32_t boxq = uint32_t(qc >> 3) * (BM * 128);
-        const T* qh = static_cast<const T*>(p.c.a.q) + int64_t(w.hk) * p.G * p.c.a.q_st[1] + int64_t(w.lo) * p.c.a.q_st[2] + qc * 8;
+        const T* qh = static_cast<const T*>(p.c.a.q) + int64_t(hk) * p.G * p.c.a.q_st[1] + int64_t(w.lo) * p.c.a.q_st[2] + qc * 8;
         float* fac = fac_s + (pieces & 1) * RB;
         for (int b0 = 0; b0 < tiles; b0 += RPP * HOLD) {
           uint4 raw[HOLD];
@@ -624,26 +691,26 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
         if (lane == 0) mbar_arrive(q_full);
       }
       // ---- codes: stage by stage, the next two stages' loads in flight
-      const int fills = 2 * w.nt * SPT;
+      const int fills = 2 * nt * SPT;
       uint4 buf[2][LD];
       int tabs = 0;  // tiles of the piece whose ids are known to be in
       auto load = [&](int s, uint4* x) {
         int kind, t;
-        entry(w.pair, w.nt, s / SPT, kind, t);
+        entry(pair, nt, s / SPT, kind, t);
         const int slot = (gt + t) % TABLES;
         if (t >= tabs) {
           if (ok) ok = wait_or_abort(&tab_full[slot], ((gt + t) / TABLES) & 1, abort_flag, 149);
           tabs = t + 1;
         }
-        const int key0 = (w.kt0 + t) * BN;
+        const int key0 = (kt0 + t) * BN;
         const uint8_t* from = p.c.a.pages + (s % SPT) * C::DS + u * 16;
 #pragma unroll
         for (int i = 0; i < LD; ++i) {
           const int r = r0 + i * RSTEP;
           const int id = ids[slot * 8 + (r >> p.lpage)];
           x[i] = make_uint4(0, 0, 0, 0);
-          if (ok && id >= 0 && key0 + r < w.horizon)
-            x[i] = *reinterpret_cast<const uint4*>(from + ((int64_t(id) * 2 + kind) * p.c.a.Hkv + w.hk) * (page * D) + (r & (page - 1)) * D);
+          if (ok && id >= 0 && key0 + r < horizon)
+            x[i] = *reinterpret_cast<const uint4*>(from + ((int64_t(id) * 2 + kind) * p.c.a.Hkv + hk) * (page * D) + (r & (page - 1)) * D);
         }
         if (kind == 1 && s % SPT == SPT - 1) {  // the tile's ids have been used
           __syncwarp();
@@ -679,29 +746,38 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
         if (s + 3 < fills) load(s + 3, buf[1]);
         ok = __all_sync(0xffffffffu, ok);
       }
+      piece_done(pieces);
       ++pieces;
-      gt += w.nt;
+      gt += nt;
     }
     if (!ok) *abort_flag = 1;
   } else {
     // ------------------------------------------------------------------------------------ softmax, epilogue
     reg_inc<176>();
-    Sched<RB> sched(p, prefix);
     const int wg = warp >> 2, quarter = warp & 3, r = 32 * quarter + lane;
     const uint32_t lane_base = tmem + (uint32_t(32 * quarter) << 16);
     const uint32_t s_col = lane_base + wg * BN;
     const uint32_t o_col = lane_base + C::O_COL + (C::WIDE ? 0 : wg * D);
-    int pieces = 0, gt = 0, cnt[2] = {0, 0};  // pieces, tiles, units of each buffer so far
+    int pieces = 0, gt = 0, cnt[2] = {0, 0}, met = 0;  // pieces, tiles, units of each buffer so far; meetings
+    auto meet_other = [&](bool& ok) {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&meet[quarter]);
+      if (ok) ok = wait_or_abort(&meet[quarter], met & 1, abort_flag, 159);
+      ++met;
+    };
     bool ok = true;
     int4 rec0 = make_int4(0, 0, 0, 0), rec1 = rec0;
-    while (sched.next(w)) {
-      const int row = r + (w.pair ? wg * BM : 0);  // in the item
+    while (piece(pieces)) {
+      const Piece& w = list[pieces % PIECES];
+      const bool pair = w.pair;
+      const int units = w.units, kt0 = w.kt0;
+      const int row = r + (pair ? wg * BM : 0);  // in the item
       const bool live = row < w.rows;
       const int tok = (w.f0 + row) / p.G;
       const int lim = !live ? -1 : (p.c.a.causal ? w.len - (w.n - 1 - tok) : w.len) - 1;  // the last key that the row sees
       float m = -FLT_MAX, l = 0.f, fac = 0.f;
-      for (int i = wg; i < w.units; i += 2) {
-        const int t = w.pair ? i >> 1 : i, slot = (gt + t) % TABLES;
+      for (int i = wg; i < units; i += 2) {
+        const int t = pair ? i >> 1 : i, slot = (gt + t) % TABLES;
         const int own = cnt[wg] + (i >> 1);  // the buffer's units before this one
         if (ok) ok = wait_or_abort(&s_full[wg], own & 1, abort_flag, 151);
         ok = __all_sync(0xffffffffu, ok);
@@ -712,7 +788,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
         if (i < 2) fac = fac_s[(pieces & 1) * RB + row];
         const float4* sc = tab + slot * 8;
         prefill::tmem_wait_ld();
-        const int over = lim - (w.kt0 + t) * BN;  // the last column that the row sees
+        const int over = lim - (kt0 + t) * BN;  // the last column that the row sees
         if (__any_sync(0xffffffffu, over < BN - 1)) {
 #pragma unroll
           for (int c = 0; c < BN; ++c)
@@ -808,32 +884,32 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
         if (lane == 0) {
           mbar_arrive(&p_full[wg]);
           mbar_arrive(&tab_empty[slot]);
-          if (!w.pair) mbar_arrive(&tab_empty[slot]);
+          if (!pair) mbar_arrive(&tab_empty[slot]);
         }
       }
       // -------------------------------------------------------------------------------- the piece's end
-      const int n0 = (w.units + 1) >> 1, n1 = w.units >> 1;
+      const int n0 = (units + 1) >> 1, n1 = units >> 1;
       float f0 = 1.f, f1 = 0.f;  // factors of this group's O, or of O 0 and O 1
-      if (w.pair) {
+      if (pair) {
         if (ok) ok = wait_or_abort(&o_done[wg], (cnt[wg] + n0 - 1) & 1, abort_flag, 154);
       } else {
         ml_s[wg * BM + r] = make_float2(m, l);
-        asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");
+        meet_other(ok);
         const float2 x = ml_s[r], y = ml_s[BM + r];
         m = fmaxf(x.x, y.x);  // (a shared maximum never falls, so it is the later one)
         f0 = prefill::ex2f(x.x - m);
         f1 = n1 ? prefill::ex2f(y.x - m) : 0.f;
         l = shrink(x.y, x.x - m) + (n1 ? shrink(y.y, y.x - m) : 0.f);
         if (C::WIDE) f0 = 1.f;
-        asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");  // (read before the next piece's are written)
+        meet_other(ok);  // (read before the next piece's are written)
         if (ok) ok = wait_or_abort(&o_done[0], (cnt[0] + n0 - 1) & 1, abort_flag, 155);
         if (ok && n1) ok = wait_or_abort(&o_done[1], (cnt[1] + n1 - 1) & 1, abort_flag, 156);
       }
       ok = __all_sync(0xffffffffu, ok);
       prefill::tc_fence_after();
-      const int first = w.pair ? 0 : wg * (D / 2), count = w.pair ? D : D / 2;  // this thread's columns of O
+      const int first = pair ? 0 : wg * (D / 2), count = pair ? D : D / 2;  // this thread's columns of O
       const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-      const uint32_t oc = w.pair ? o_col : lane_base + C::O_COL;
+      const uint32_t oc = pair ? o_col : lane_base + C::O_COL;
       T* out = static_cast<T*>(p.c.a.o) + int64_t(w.hk * p.G + (w.f0 + row) % p.G) * p.c.a.o_st[1] + int64_t(w.lo + tok) * p.c.a.o_st[2];
       float* part = p.ws_o + int64_t(w.slot) * (D * RB) + row;
 #pragma unroll 1
@@ -841,7 +917,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
         float ov[32];
         prefill::tmem_ld32(oc + c, ov);
         prefill::tmem_wait_ld();
-        if (!C::WIDE && !w.pair) {
+        if (!C::WIDE && !pair) {
           if (n1) {
             float o1[32];
             prefill::tmem_ld32(oc + D + c, o1);
@@ -868,11 +944,12 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
       prefill::tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(o_free);
-      if (!w.whole && (w.pair || wg == 0)) {
+      if (!w.whole && (pair || wg == 0)) {
         p.ws_ml[int64_t(w.slot) * 2 * RB + row] = m;
         p.ws_ml[int64_t(w.slot) * 2 * RB + RB + row] = l;
       }
       if (w.nparts) rec0 = make_int4(w.nparts, w.b, w.lo, w.n), rec1 = make_int4(w.len, w.hk, w.f0, w.rows);
+      piece_done(pieces);
       ++pieces;
       gt += w.nt;
       cnt[0] += n0;
@@ -883,20 +960,24 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
       p.rec[2 * blockIdx.x] = rec0;
       p.rec[2 * blockIdx.x + 1] = rec1;
     }
+    // The second look (rare), when all of the CTA's rows are written: its whole items' rows, a warp a row.
+    __syncwarp();
+    if (lane == 0) mbar_arrive(written);
+    if (ok) ok = wait_or_abort(written, 0, abort_flag, 160);
+    if (__all_sync(0xffffffffu, ok) && *again) {
+      Sched<RB> sched(p, prefix);
+      Piece y;
+      while (sched.next(y))
+        for (int x = warp; y.whole && x < y.rows; x += CONV_WARP)
+          row_again<T, D>(p, y.b, y.lo, y.n, y.len, y.hk, y.f0 + x, y.horizon);
+    }
   }
 
   prefill::tc_fence_before();
   __syncthreads();
   if (warp == MMA_WARP) {
     prefill::tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
-  }
-  // The second look (rare), when nothing waits for this CTA any more: its whole items' rows, a warp a row.
-  if (*again && !*abort_flag) {
-    Sched<RB> sched(p, prefix);
-    while (sched.next(w))
-      for (int x = warp; w.whole && x < w.rows; x += THREADS / 32)
-        row_again<T, D>(p, w.b, w.lo, w.n, w.len, w.hk, w.f0 + x, w.horizon);
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(*tmem_slot), "r"(512));
   }
 }
 
