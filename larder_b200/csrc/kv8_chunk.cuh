@@ -74,8 +74,8 @@ struct Cfg {
   static constexpr int QTILE = BM * D * 2;
   static constexpr int K_OFF = QT * QTILE;
   static constexpr int TAB_OFF = K_OFF + NS * STAGE;           // [TABLES][8] float4 of a 16-key slice's scales
-  static constexpr int ID_OFF = TAB_OFF + TABLES * 8 * 16;     // [TABLES][8] page ids
-  static constexpr int FAR_OFF = ID_OFF + TABLES * 8 * 4;      // [TABLES] the slices whose weights' sums are formed apart
+  static constexpr int ID_OFF = TAB_OFF + TABLES * 8 * 16;     // [TABLES][8] int64: where the pages' K of the head begin; -1: none
+  static constexpr int FAR_OFF = ID_OFF + TABLES * 8 * 8;      // [TABLES] the slices whose weights' sums are formed apart
   static constexpr int FAC_OFF = FAR_OFF + TABLES * 4;         // [2 items][RB] the rows' score factors
   static constexpr int ML_OFF = FAC_OFF + 2 * RB * 4;          // [2][128] float2
   static constexpr int MSH_OFF = ML_OFF + 2 * BM * 8;          // [128] the shared maximum
@@ -244,17 +244,31 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+
+// Waits for the loads from tensor memory so far; the values of one of them pass through, so that no use of them moves ahead.
+__device__ __forceinline__ void wait_ld32(float* v) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
+                 "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]),
+                 "+f"(v[15]), "+f"(v[16]), "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]),
+                 "+f"(v[22]), "+f"(v[23]), "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]),
+                 "+f"(v[29]), "+f"(v[30]), "+f"(v[31])
+               :
+               : "memory");
+}
+
 // l 2^x, x <= 0, in two steps: l reaches 2^115 where V scales are far apart, and 2^x alone may be 0.
 __device__ __forceinline__ float shrink(float l, float x) {
   const float h = prefill::ex2f(0.5f * x);
   return l * h * h;
 }
-
-// (Once a warp: a second change needs a barrier of its warpgroup first.)
-template <int N>
-__device__ __forceinline__ void reg_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
-template <int N>
-__device__ __forceinline__ void reg_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
 // A bounded wait that gives up at once when some role of the CTA has.
 __device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int where) {
@@ -343,7 +357,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   float4* tab = reinterpret_cast<float4*>(sm + C::TAB_OFF);
-  int* ids = reinterpret_cast<int*>(sm + C::ID_OFF);
+  int64_t* at_s = reinterpret_cast<int64_t*>(sm + C::ID_OFF);
   uint32_t* far_s = reinterpret_cast<uint32_t*>(sm + C::FAR_OFF);
   float* fac_s = reinterpret_cast<float*>(sm + C::FAC_OFF);
   float2* ml_s = reinterpret_cast<float2*>(sm + C::ML_OFF);
@@ -452,7 +466,6 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
   };
 
   if (warp >= CONV_WARP + 4) {
-    reg_dec<56>();
     if (warp == PLAN_WARP) {
       // ---------------------------------------------------------------------------------- the list of pieces
       Sched<RB> sched(p, prefix);
@@ -479,21 +492,23 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
         const int nt = w.nt, units = w.units;
         if (elect_one()) {
           ok = wait_or_abort(q_full, pieces & 1, abort_flag, 141);
-          const uint32_t q_addr = smem_u32(sm), k0 = smem_u32(sm + C::K_OFF);
+          // operands' descriptors: the K-major tiles' (Q, K) and the MN-major V's; tiles differ in the low word's address
+          const uint64_t q_desc = prefill::sdesc(smem_u32(sm), 16, 1024), k_desc = prefill::sdesc(smem_u32(sm + C::K_OFF), 16, 1024),
+                         v_desc = prefill::sdesc(smem_u32(sm + C::K_OFF), BN * 128, 1024);
           auto scores = [&](int i) {
             const int t = pair ? i >> 1 : i, e = (base + k_entry(pair, t)) * SPT;
-            const uint32_t q = q_addr + (pair ? (i & 1) * C::QTILE : 0);
+            const uint64_t q = q_desc + (pair && (i & 1) ? C::QTILE >> 4 : 0);
 #pragma unroll
             for (int h = 0; h < SPT; ++h) {
               const int st = (e + h) % NS;
               if (!ok || !(ok = wait_or_abort(&full[st], ((e + h) / NS) & 1, abort_flag, 142))) return;
               prefill::tc_fence_after();
-              const uint32_t k = k0 + st * C::STAGE;
+              const uint64_t k = k_desc + st * (C::STAGE >> 4);
 #pragma unroll
               for (int kk = 0; kk < C::DS / 16; ++kk)
                 prefill::umma_ss(tmem + (i & 1) * BN,
-                                 prefill::sdesc(q + ((kk >> 2) + h * (C::DS / 64)) * BM * 128 + (kk & 3) * 32, 16, 1024),
-                                 prefill::sdesc(k + (kk >> 2) * BN * 128 + (kk & 3) * 32, 16, 1024), IDESC_S,
+                                 q + ((((kk >> 2) + h * (C::DS / 64)) * BM * 128 + (kk & 3) * 32) >> 4),
+                                 k + (((kk >> 2) * BN * 128 + (kk & 3) * 32) >> 4), IDESC_S,
                                  h + kk > 0 ? 1u : 0u);
               if (!pair || (i & 1)) prefill::umma_commit(&empty[st]);
             }
@@ -514,11 +529,11 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
               if (ok) ok = wait_or_abort(&full[st], ((e + h) / NS) & 1, abort_flag, 145);
               if (!ok) break;
               prefill::tc_fence_after();
-              const uint32_t v = k0 + st * C::STAGE;
+              const uint64_t v = v_desc + st * (C::STAGE >> 4);
 #pragma unroll
               for (int kk = 0; kk < BN / 16; ++kk)
                 prefill::umma_ts(o + h * C::DS, tmem + (i & 1) * BN + kk * 8,
-                                 prefill::sdesc(v + kk * 16 * 128, BN * 128, 1024), IDESC_PV,
+                                 v + ((kk * 16 * 128) >> 4), IDESC_PV,
                                  (own ? i > 1 : i > 0) || kk > 0 ? 1u : 0u);
               if (!pair || (i & 1)) prefill::umma_commit(&empty[st]);
             }
@@ -598,7 +613,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
             if (!ok) break;
             if (lane >> 3 == j) {
               tab[s * 8 + (lane & 7)] = f;
-              if ((lane & 7) < per) ids[s * 8 + (lane & 7)] = pg;
+              if ((lane & 7) < per) at_s[s * 8 + (lane & 7)] = pg < 0 ? -1 : (int64_t(pg) * 2 * p.c.a.Hkv + hk) * (D << p.lpage);
               if ((lane & 7) == 0) far_s[s] = marked >> (8 * j) & 255u;
             }
             __syncwarp();
@@ -610,12 +625,12 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
     }
   } else if (warp >= CONV_WARP) {
     // ------------------------------------------------------------------------------------ codes into operand tiles
-    reg_dec<104>();
     constexpr int UPR = C::DS / 16;       // 16-code units a key and stage
     constexpr int LD = BN * UPR / 128;    // units a thread and stage
     constexpr int RSTEP = 128 / UPR;      // keys between a thread's units
     const int tid = threadIdx.x - CONV_WARP * 32, u = tid % UPR, r0 = tid / UPR;
     const int page = 1 << p.lpage;
+    const int64_t kv_off = int64_t(p.c.a.Hkv) * (D << p.lpage);  // from a page's K to its V
     // where the thread's unit of key r0 goes in a stage, its two 16-byte halves ordered so that eight lanes fill 128 bytes
     const int swap = UPR == 8 ? u >> 2 : 0;
     const uint32_t box = uint32_t(u >> 2) * (BN * 128);
@@ -702,15 +717,15 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
           if (ok) ok = wait_or_abort(&tab_full[slot], ((gt + t) / TABLES) & 1, abort_flag, 149);
           tabs = t + 1;
         }
-        const int key0 = (kt0 + t) * BN;
-        const uint8_t* from = p.c.a.pages + (s % SPT) * C::DS + u * 16;
+        const int end = horizon - (kt0 + t) * BN;  // keys of the tile that some row sees
+        const uint8_t* from = p.c.a.pages + kind * kv_off + (s % SPT) * C::DS;
+        const int64_t* at = at_s + slot * 8;
 #pragma unroll
         for (int i = 0; i < LD; ++i) {
           const int r = r0 + i * RSTEP;
-          const int id = ids[slot * 8 + (r >> p.lpage)];
+          const int64_t o = at[r >> p.lpage];
           x[i] = make_uint4(0, 0, 0, 0);
-          if (ok && id >= 0 && key0 + r < horizon)
-            x[i] = *reinterpret_cast<const uint4*>(from + ((int64_t(id) * 2 + kind) * p.c.a.Hkv + hk) * (page * D) + (r & (page - 1)) * D);
+          if (ok && o >= 0 && r < end) x[i] = *reinterpret_cast<const uint4*>(from + o + ((r & (page - 1)) * D + u * 16));
         }
         if (kind == 1 && s % SPT == SPT - 1) {  // the tile's ids have been used
           __syncwarp();
@@ -723,14 +738,13 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
         uint8_t* d = sm + C::K_OFF + st * C::STAGE;
 #pragma unroll
         for (int i = 0; i < LD; ++i) {
-          uint32_t h[8];
-          kv8::dec4(x[i].x, h[0], h[1]);
-          kv8::dec4(x[i].y, h[2], h[3]);
-          kv8::dec4(x[i].z, h[4], h[5]);
-          kv8::dec4(x[i].w, h[6], h[7]);
-          const uint4 a = make_uint4(h[0], h[1], h[2], h[3]), b = make_uint4(h[4], h[5], h[6], h[7]);
-          *reinterpret_cast<uint4*>(d + dst0 + i * RSTEP * 128) = swap ? b : a;
-          *reinterpret_cast<uint4*>(d + dst1 + i * RSTEP * 128) = swap ? a : b;
+          uint4 a, b;
+          kv8::dec4(swap ? x[i].z : x[i].x, a.x, a.y);
+          kv8::dec4(swap ? x[i].w : x[i].y, a.z, a.w);
+          kv8::dec4(swap ? x[i].x : x[i].z, b.x, b.y);
+          kv8::dec4(swap ? x[i].y : x[i].w, b.z, b.w);
+          *reinterpret_cast<uint4*>(d + dst0 + i * RSTEP * 128) = a;
+          *reinterpret_cast<uint4*>(d + dst1 + i * RSTEP * 128) = b;
         }
         fence_proxy_async_shared();
         __syncwarp();
@@ -753,7 +767,6 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
     if (!ok) *abort_flag = 1;
   } else {
     // ------------------------------------------------------------------------------------ softmax, epilogue
-    reg_inc<176>();
     const int wg = warp >> 2, quarter = warp & 3, r = 32 * quarter + lane;
     const uint32_t lane_base = tmem + (uint32_t(32 * quarter) << 16);
     const uint32_t s_col = lane_base + wg * BN;
@@ -782,29 +795,40 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
         if (ok) ok = wait_or_abort(&s_full[wg], own & 1, abort_flag, 151);
         ok = __all_sync(0xffffffffu, ok);
         prefill::tc_fence_after();
-        float s[BN];
-#pragma unroll
-        for (int c = 0; c < BN; c += 32) prefill::tmem_ld32(s_col + c, s + c);
-        if (i < 2) fac = fac_s[(pieces & 1) * RB + row];
-        const float4* sc = tab + slot * 8;
-        prefill::tmem_wait_ld();
         const int over = lim - (kt0 + t) * BN;  // the last column that the row sees
-        if (__any_sync(0xffffffffu, over < BN - 1)) {
+        // Masked tiles are few: their scores are masked in place, so that all tiles share one short piece of code.
+        for (int c = max(__reduce_min_sync(0xffffffffu, over + 1), 0) & ~15; c < BN; c += 16) {
+          float x[16];
+          prefill2::tmem_ld16(s_col + c, x);
+          prefill::tmem_wait_ld();
 #pragma unroll
-          for (int c = 0; c < BN; ++c)
-            if (c > over) s[c] = -INFINITY;
+          for (int e = 0; e < 16; ++e) x[e] = c + e > over ? -INFINITY : x[e];
+          prefill::tmem_st16(s_col + c, reinterpret_cast<const uint32_t*>(x));
+          prefill::tmem_wait_st();
         }
         // the row's largest score with the values' scale (a factor is never 0: -inf times it stays -inf)
-        float top = -INFINITY;
-#pragma unroll
-        for (int q = 0; q < 8; ++q) {
-          const float4 f = sc[q];
-          const float* x = s + 16 * q;
+        if (i < 2) fac = fac_s[(pieces & 1) * RB + row];
+        const float4* sc = tab + slot * 8;
+        float top = -INFINITY, sa[32], sb[32];
+        auto largest = [&](const float* x, int q) {
+          const float2 f = *reinterpret_cast<const float2*>(sc + q);
           float a = max3(x[0], x[1], x[2]), b = max3(x[3], x[4], x[5]);
           a = max3(a, x[6], x[7]), b = max3(b, x[8], x[9]);
           a = max3(a, x[10], x[11]), b = max3(b, x[12], x[13]);
           a = max3(a, x[14], x[15]);
           top = fmaxf(top, fmaf(fmaxf(a, b), fmaxf(fac * f.x, FLT_MIN), f.y));
+        };
+        prefill::tmem_ld32(s_col, sa);
+#pragma unroll
+        for (int c = 0; c < 4; c += 2) {
+          wait_ld32(sa);
+          prefill::tmem_ld32(s_col + 32 * c + 32, sb);
+          largest(sa, 2 * c);
+          largest(sa + 16, 2 * c + 1);
+          wait_ld32(sb);
+          prefill::tmem_ld32(s_col + (c == 0 ? 64 : 0), sa);  // (at last the weights' first columns)
+          largest(sb, 2 * c + 2);
+          largest(sb + 16, 2 * c + 3);
         }
         bool began;  // O holds something
         if constexpr (C::WIDE) {
@@ -848,35 +872,42 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
           __syncwarp();
           if (lane == 0) mbar_arrive(&token[wg * 4 + quarter]);
         }
-        if (const uint32_t marked = far_s[slot]) {
+        for (uint32_t marked = far_s[slot]; marked; marked &= marked - 1) {  // (rare)
+          const int q = __ffs(marked) - 1;
+          const float mul = fmaxf(fac * sc[q].x, FLT_MIN);
+          float x[16];
+          prefill2::tmem_ld16(s_col + 16 * q, x);
+          prefill::tmem_wait_ld();
 #pragma unroll
-          for (int q = 0; q < 8; ++q)
-            if (marked >> q & 1) {
-              const float mul = fmaxf(fac * sc[q].x, FLT_MIN);
-#pragma unroll
-              for (int c = 0; c < 16; ++c) l += prefill::ex2f(fmaf(s[16 * q + c], mul, -m));
-            }
+          for (int e = 0; e < 16; ++e) l += prefill::ex2f(fmaf(x[e], mul, -m));
         }
-        // weights
+        // weights, 32 columns at a time, the next ones' scores on their way; P_i takes the place of scores already read
+        auto weights = [&](const float* x, int c) {
+          uint32_t pk[16];
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          uint32_t pk[32];
-#pragma unroll
-          for (int qq = 0; qq < 4; ++qq) {
-            const int q = half * 4 + qq;
-            const float4 f = sc[q];
+          for (int h = 0; h < 2; ++h) {
+            const float4 f = sc[2 * c + h];
             const float mul = fmaxf(fac * f.x, FLT_MIN), add = f.w - m;
             float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-            for (int c = 0; c < 16; c += 2) {
-              float2 x = kv8::fma2(make_float2(s[16 * q + c], s[16 * q + c + 1]), make_float2(mul, mul), make_float2(add, add));
-              x.x = prefill::ex2f(x.x), x.y = prefill::ex2f(x.y);
-              sum.x += x.x, sum.y += x.y;
-              pk[qq * 8 + c / 2] = pack2<__half>(x.x, x.y);
+            for (int e = 0; e < 16; e += 2) {
+              float2 y = kv8::fma2(make_float2(x[16 * h + e], x[16 * h + e + 1]), make_float2(mul, mul), make_float2(add, add));
+              y.x = prefill::ex2f(y.x), y.y = prefill::ex2f(y.y);
+              sum = add2(sum, y);
+              pk[8 * h + e / 2] = pack2<__half>(y.x, y.y);
             }
             l = fmaf(sum.x + sum.y, f.z, l);
           }
-          prefill::tmem_st32(s_col + half * 32, reinterpret_cast<const float*>(pk));
+          prefill::tmem_st16(s_col + 16 * c, pk);
+        };
+#pragma unroll 1
+        for (int c = 0; c < 4; c += 2) {
+          wait_ld32(sa);
+          prefill::tmem_ld32(s_col + 32 * c + 32, sb);
+          weights(sa, c);
+          wait_ld32(sb);
+          if (c == 0) prefill::tmem_ld32(s_col + 64, sa);
+          weights(sb, c + 1);
         }
         prefill::tmem_wait_st();
         prefill::tc_fence_before();
