@@ -270,6 +270,17 @@ __device__ __forceinline__ float shrink(float l, float x) {
   return l * h * h;
 }
 
+// 16 bytes, or zeros where they are not wanted, without a branch.
+__device__ __forceinline__ uint4 load_if(const uint8_t* p, bool want) {
+  uint4 x;
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %5, 0;\n\tmov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\tmov.b32 %2, 0;\n\tmov.b32 %3, 0;\n\t"
+      "@q ld.global.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
+      : "=&r"(x.x), "=&r"(x.y), "=&r"(x.z), "=&r"(x.w)
+      : "l"(p), "r"(uint32_t(want)));
+  return x;
+}
+
 // A bounded wait that gives up at once when some role of the CTA has.
 __device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int where) {
   if (mbar_try_wait(bar, parity)) return true;
@@ -720,12 +731,13 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
         const int end = horizon - (kt0 + t) * BN;  // keys of the tile that some row sees
         const uint8_t* from = p.c.a.pages + kind * kv_off + (s % SPT) * C::DS;
         const int64_t* at = at_s + slot * 8;
+        int64_t o[LD];
+#pragma unroll
+        for (int i = 0; i < LD; ++i) o[i] = at[(r0 + i * RSTEP) >> p.lpage];
 #pragma unroll
         for (int i = 0; i < LD; ++i) {
           const int r = r0 + i * RSTEP;
-          const int64_t o = at[r >> p.lpage];
-          x[i] = make_uint4(0, 0, 0, 0);
-          if (ok && o >= 0 && r < end) x[i] = *reinterpret_cast<const uint4*>(from + o + ((r & (page - 1)) * D + u * 16));
+          x[i] = load_if(from + o[i] + ((r & (page - 1)) * D + u * 16), ok && o[i] >= 0 && r < end);
         }
         if (kind == 1 && s % SPT == SPT - 1) {  // the tile's ids have been used
           __syncwarp();
