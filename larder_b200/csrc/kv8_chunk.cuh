@@ -29,8 +29,8 @@
 // row that comes out NaN is looked at again at the end (row_again), and where a value that it does not see is to blame, taken
 // again reading only what it sees.
 //
-// Roles (512 threads): warps 0-3, 4-7 softmax and epilogue (warp w: TMEM lanes of quarter w % 4), 8-11 codes and queries into
-// shared memory, 12 issues the products, 13 reads the page table and scales ahead, 14 lists the CTA's pieces of work.
+// Roles (640 threads): warps 0-3, 4-7 softmax and epilogue (warp w: TMEM lanes of quarter w % 4), 8-15 codes and queries into
+// shared memory, 16 issues the products, 17 reads the page table and scales ahead, 18 lists the CTA's pieces of work.
 #pragma once
 
 #include <cfloat>
@@ -46,8 +46,9 @@ namespace kv8chunk {
 
 constexpr int BM = 128, BN = 128;  // rows of a row tile, keys of a key tile
 constexpr int MAX_B = 1024;        // sequences a launch
-constexpr int THREADS = 512;
-constexpr int CONV_WARP = 8, MMA_WARP = 12, TABLE_WARP = 13, PLAN_WARP = 14;
+constexpr int THREADS = 640;
+constexpr int CONV_WARP = 8, CONV_WARPS = 8, MMA_WARP = 16, TABLE_WARP = 17, PLAN_WARP = 18;
+constexpr int CT = CONV_WARPS * 32;  // threads that turn codes into operands
 constexpr int PIECES = 4;          // pieces of work listed ahead
 constexpr int TABLES = 8;          // key tiles whose page ids and scales are held
 constexpr float TOP = 7.f;         // a weight at the running maximum is 2^TOP
@@ -281,6 +282,14 @@ __device__ __forceinline__ uint4 load_if(const uint8_t* p, bool want) {
   return x;
 }
 
+// Registers a thread: 640 are launched with 96 each, of which the softmax warps take more. (Once a warp: a second change would
+// need a barrier of its warpgroup first.)
+template <int N>
+__device__ __forceinline__ void reg_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void reg_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+static_assert(256 * 128 + 384 * 72 <= THREADS * 96, "a split above what was launched would wait forever");
+
 // A bounded wait that gives up at once when some role of the CTA has.
 __device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int where) {
   if (mbar_try_wait(bar, parity)) return true;
@@ -399,10 +408,10 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < NS; ++i) {
-      mbar_init(&full[i], 4);
+      mbar_init(&full[i], CONV_WARPS);
       mbar_init(&empty[i], 1);
     }
-    mbar_init(q_full, 4);
+    mbar_init(q_full, CONV_WARPS);
     mbar_init(q_empty, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
@@ -412,12 +421,12 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
     mbar_init(o_free, 8);
     for (int i = 0; i < TABLES; ++i) {
       mbar_init(&tab_full[i], 1);
-      mbar_init(&tab_empty[i], 12);  // four warps' V loads and eight softmax warps (four, twice, where one group has the tile)
+      mbar_init(&tab_empty[i], CONV_WARPS + 8);  // the V loads and eight softmax warps (four, twice, where one group has the tile)
     }
     for (int i = 0; i < 8; ++i) mbar_init(&token[i], 1);
     for (int i = 0; i < PIECES; ++i) {
       mbar_init(&piece_full[i], 1);
-      mbar_init(&piece_empty[i], 14);  // eight softmax warps, four of the codes, the products', the tables'
+      mbar_init(&piece_empty[i], CONV_WARPS + 10);  // eight softmax warps, the products', the tables'
     }
     for (int i = 0; i < 4; ++i) mbar_init(&meet[i], 2);
     mbar_init(written, 8);
@@ -476,7 +485,8 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
     if (lane == 0) mbar_arrive(&piece_empty[i % PIECES]);
   };
 
-  if (warp >= CONV_WARP + 4) {
+  if (warp >= CONV_WARP + CONV_WARPS) {
+    reg_dec<72>();
     if (warp == PLAN_WARP) {
       // ---------------------------------------------------------------------------------- the list of pieces
       Sched<RB> sched(p, prefix);
@@ -636,9 +646,10 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
     }
   } else if (warp >= CONV_WARP) {
     // ------------------------------------------------------------------------------------ codes into operand tiles
+    reg_dec<72>();
     constexpr int UPR = C::DS / 16;       // 16-code units a key and stage
-    constexpr int LD = BN * UPR / 128;    // units a thread and stage
-    constexpr int RSTEP = 128 / UPR;      // keys between a thread's units
+    constexpr int LD = BN * UPR / CT;     // units a thread and stage
+    constexpr int RSTEP = CT / UPR;       // keys between a thread's units
     const int tid = threadIdx.x - CONV_WARP * 32, u = tid % UPR, r0 = tid / UPR;
     const int page = 1 << p.lpage;
     const int64_t kv_off = int64_t(p.c.a.Hkv) * (D << p.lpage);  // from a page's K to its V
@@ -659,7 +670,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
       if (!__all_sync(0xffffffffu, ok)) break;
       {
         constexpr int LPR = D / 8;          // lanes a row
-        constexpr int RPP = 128 / LPR;      // rows a pass
+        constexpr int RPP = CT / LPR;       // rows a pass
         constexpr int HOLD = 4;             // passes whose loads are in flight
         const int qr = tid / LPR, qc = tid % LPR;
         const int tiles = pair ? 2 * BM : BM;
@@ -779,6 +790,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
     if (!ok) *abort_flag = 1;
   } else {
     // ------------------------------------------------------------------------------------ softmax, epilogue
+    reg_inc<128>();
     const int wg = warp >> 2, quarter = warp & 3, r = 32 * quarter + lane;
     const uint32_t lane_base = tmem + (uint32_t(32 * quarter) << 16);
     const uint32_t s_col = lane_base + wg * BN;
