@@ -30,7 +30,7 @@
 // again reading only what it sees.
 //
 // Roles (640 threads): warps 0-3, 4-7 softmax and epilogue (warp w: TMEM lanes of quarter w % 4), 8-15 codes and queries into
-// shared memory, 16 issues the products, 17 reads the page table and scales ahead, 18 lists the CTA's pieces of work.
+// shared memory, 16 and 19 issue the products P V and S, 17 reads the page table and scales ahead, 18 lists the CTA's pieces.
 #pragma once
 
 #include <cfloat>
@@ -45,9 +45,10 @@ namespace lb2 {
 namespace kv8chunk {
 
 constexpr int BM = 128, BN = 128;  // rows of a row tile, keys of a key tile
+constexpr int BH = 64;             // keys of a unit: half a key tile
 constexpr int MAX_B = 1024;        // sequences a launch
 constexpr int THREADS = 640;
-constexpr int CONV_WARP = 8, CONV_WARPS = 8, MMA_WARP = 16, TABLE_WARP = 17, PLAN_WARP = 18;
+constexpr int CONV_WARP = 8, CONV_WARPS = 8, MMA_WARP = 16, TABLE_WARP = 17, PLAN_WARP = 18, SCORE_WARP = 19;
 constexpr int CT = CONV_WARPS * 32;  // threads that turn codes into operands
 constexpr int PIECES = 4;          // pieces of work listed ahead
 constexpr int TABLES = 8;          // key tiles whose page ids and scales are held
@@ -82,8 +83,9 @@ struct Cfg {
   static constexpr int MSH_OFF = ML_OFF + 2 * BM * 8;          // [128] the shared maximum
   static constexpr int PREFIX_OFF = MSH_OFF + BM * 4;          // [MAX_B + 3] int64
   static constexpr int PIECE_OFF = PREFIX_OFF + (MAX_B + 3) * 8;  // [PIECES] Piece
+  static constexpr int BAR_BYTES = 640;
   static constexpr int BAR_OFF = PIECE_OFF + PIECES * int(sizeof(Piece));
-  static constexpr int SMEM = BAR_OFF + 512 + 1024;
+  static constexpr int SMEM = BAR_OFF + BAR_BYTES + 1024;
   static constexpr int O_COL = 2 * BN;            // O, or the two warpgroups' O at O_COL and O_COL + D
   static_assert(PREFIX_OFF % 8 == 0 && SMEM <= 232448, "shared memory budget");
   static_assert(O_COL + QT * D <= 512, "TMEM budget");
@@ -153,7 +155,7 @@ struct Sched {
 
   __device__ __forceinline__ int64_t cut(int64_t c) const { return c * total / runs; }
 
-  __device__ __forceinline__ Sched(const Params& p_, const int64_t* prefix_) : p(p_), prefix(prefix_) {
+  __device__ __noinline__ Sched(const Params& p_, const int64_t* prefix_) : p(p_), prefix(prefix_) {
     const int NR = p.c.a.B + 2, lane = threadIdx.x & 31;
     total = prefix[NR];
     runs = max(int64_t(1), min(int64_t(gridDim.x), total / p.min_units));
@@ -198,7 +200,7 @@ struct Sched {
     at = prefix[r];
   }
 
-  __device__ __forceinline__ bool next(Piece& w) {
+  __device__ __noinline__ bool next(Piece& w) {
     while (at < p1) {
       const Block b = block_of<RB>(p, x, k);
       int64_t a = max(p0 - at, int64_t(0)), z = min(p1 - at, int64_t(b.units));
@@ -265,6 +267,31 @@ __device__ __forceinline__ void wait_ld32(float* v) {
                : "memory");
 }
 
+// The products and commits of attn_prefill.cuh, issued by the lane whose `lead` is set; a, b: the descriptors' low words, HI
+// the high word that all operands here share (stride 1024 bytes, version 1, 128-byte swizzle).
+constexpr uint32_t DESC_HI = (1024 >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ void mma_ss(uint32_t lead, uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 x, y;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "mov.b64 x, {%1, %6};\n\tmov.b64 y, {%2, %6};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(lead), "n"(DESC_HI));
+}
+__device__ __forceinline__ void mma_ts(uint32_t lead, uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 y;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "mov.b64 y, {%2, %6};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(lead), "n"(DESC_HI));
+}
+__device__ __forceinline__ void mma_commit(uint32_t lead, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)),
+      "r"(lead)
+      : "memory");
+}
+
 // l 2^x, x <= 0, in two steps: l reaches 2^115 where V scales are far apart, and 2^x alone may be 0.
 __device__ __forceinline__ float shrink(float l, float x) {
   const float h = prefill::ex2f(0.5f * x);
@@ -290,24 +317,26 @@ template <int N>
 __device__ __forceinline__ void reg_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 static_assert(256 * 128 + 384 * 72 <= THREADS * 96, "a split above what was launched would wait forever");
 
-// A bounded wait that gives up at once when some role of the CTA has.
+// A wait's look at the clock, out of line, as the roles' loops together should stay small (an SM's instruction cache holds
+// some thousand instructions near the schedulers, and five roles share it). since: 0 at a wait's first look, then what this
+// returned; 1: give up, some role has or the wait's time is over.
+__device__ __noinline__ uint32_t wait_check(uint32_t since, volatile int* abort_flag, int where) {
+  if (*abort_flag) return 1;
+  const uint32_t now = uint32_t(globaltimer_ns() >> 16) | 2u;  // 66 us
+  if (since == 0) return now;
+  if (now - since <= uint32_t(kWaitNs >> 16)) return since;
+  report_timeout(where);
+  *abort_flag = 1;
+  return 1;
+}
+
+// A bounded wait that gives up at once when some role of the CTA has. With HINT the waiting thread sleeps between polls.
+template <uint32_t HINT = 1000>
 __device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int where) {
-  if (mbar_try_wait(bar, parity)) return true;
-  uint64_t t0 = 0;
-  for (uint32_t i = 1;; ++i) {
-    if (mbar_try_wait(bar, parity)) return true;
-    if ((i & 255u) == 0) {
-      if (*abort_flag) return false;
-      const uint64_t now = globaltimer_ns();
-      if (t0 == 0) {
-        t0 = now;
-      } else if (now - t0 > kWaitNs) {
-        report_timeout(where);
-        *abort_flag = 1;
-        return false;
-      }
-    }
-  }
+  uint32_t since = 0, n = 0;
+  while (!(HINT ? mbar_try_wait_hint(bar, parity, HINT) : mbar_try_wait(bar, parity)))
+    if ((++n & 63u) == 0 && (since = wait_check(since, abort_flag, where)) == 1u) return false;
+  return true;
 }
 
 // The second look at folded row f of an item, by one warp: where its output has NaN columns and one of the keys behind it that
@@ -371,7 +400,7 @@ template <typename T, int D>
 __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
   using C = Cfg<D>;
   constexpr int RB = C::RB, NS = C::NS, SPT = C::SPT;
-  constexpr uint32_t IDESC_S = prefill::idesc_f16(0, 0, 0, BM, BN);
+  constexpr uint32_t IDESC_S = prefill::idesc_f16(0, 0, 0, BM, BH);
   constexpr uint32_t IDESC_PV = prefill::idesc_f16(0, 0, 1, BM, C::DS);
 
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -388,10 +417,10 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
   uint64_t* empty = full + NS;           // [NS] its products are done
   uint64_t* q_full = empty + NS;
   uint64_t* q_empty = q_full + 1;        // the item's last S has read Q
-  uint64_t* s_full = q_empty + 1;        // [2]
-  uint64_t* p_full = s_full + 2;         // [2]
-  uint64_t* o_done = p_full + 2;         // [2] the buffer's P V is complete
-  uint64_t* o_free = o_done + 2;         // the epilogue has read O
+  uint64_t* s_full = q_empty + 1;        // [4] the unit's S is complete
+  uint64_t* p_full = s_full + 4;         // [4]
+  uint64_t* o_done = p_full + 4;         // [4] its P V is complete
+  uint64_t* o_free = o_done + 4;         // the epilogue has read O
   uint64_t* tab_full = o_free + 1;       // [TABLES]
   uint64_t* tab_empty = tab_full + TABLES;
   uint64_t* token = tab_empty + TABLES;  // [2 warpgroups][4 quarters]: the shared maximum after the group's unit
@@ -400,20 +429,20 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
   uint64_t* meet = piece_empty + PIECES;  // [4 quarters]: the two softmax warps of the same rows
   uint64_t* written = meet + 4;          // the softmax warps are done
   uint64_t* drain = written + 1;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* again = abort_flag + 1;
-  static_assert((2 * NS + 2 + 6 + 1 + 2 * TABLES + 8 + 2 * PIECES + 4 + 2) * 8 + 12 <= 512, "barrier area");
+  static_assert((2 * NS + 2 + 12 + 1 + 2 * TABLES + 8 + 2 * PIECES + 4 + 3) * 8 + 12 <= C::BAR_BYTES, "barrier area");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < NS; ++i) {
-      mbar_init(&full[i], CONV_WARPS);
+      mbar_init(&full[i], 4);
       mbar_init(&empty[i], 1);
     }
     mbar_init(q_full, CONV_WARPS);
     mbar_init(q_empty, 1);
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < 4; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 4);
       mbar_init(&o_done[i], 1);
@@ -421,16 +450,17 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
     mbar_init(o_free, 8);
     for (int i = 0; i < TABLES; ++i) {
       mbar_init(&tab_full[i], 1);
-      mbar_init(&tab_empty[i], CONV_WARPS + 8);  // the V loads and eight softmax warps (four, twice, where one group has the tile)
+      mbar_init(&tab_empty[i], 4 * SPT + 8);  // the V loads and the softmax warps
     }
     for (int i = 0; i < 8; ++i) mbar_init(&token[i], 1);
     for (int i = 0; i < PIECES; ++i) {
       mbar_init(&piece_full[i], 1);
-      mbar_init(&piece_empty[i], CONV_WARPS + 10);  // eight softmax warps, the products', the tables'
+      mbar_init(&piece_empty[i], CONV_WARPS + 11);  // eight softmax warps, the products' two, the tables'
     }
     for (int i = 0; i < 4; ++i) mbar_init(&meet[i], 2);
     mbar_init(written, 8);
-    mbar_init(drain, 1);
+    mbar_init(&drain[0], 1);
+    mbar_init(&drain[1], 1);
     *abort_flag = 0;
     *again = 0;
     fence_barrier_init();
@@ -503,76 +533,79 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
         }
         __syncwarp();
       }
-    } else if (warp == MMA_WARP) {
-      // ---------------------------------------------------------------------------------- MMA issuer
-      int pieces = 0, base = 0, g0 = 0, g1 = 0;  // pieces and ring entries so far; units of each buffer so far
+    } else if (warp == MMA_WARP || warp == SCORE_WARP) {
+      // ---------------------------------------------------------------------------------- MMA issuers
+      // One warp issues the S products, one the P V, so that neither's waits hold up the other's. Each walks the units as a
+      // whole, with values that are the same in all lanes; one lane's predicate issues.
+      const bool scores = warp == SCORE_WARP;
+      const uint32_t lead = elect_one();
+      auto uni = [](int x) { return __shfl_sync(0xffffffffu, x, 0); };
+      auto wait = [&](uint64_t* bar, uint32_t parity, int where) {
+        return __all_sync(0xffffffffu, wait_or_abort<0>(bar, parity, abort_flag, where)) != 0;
+      };
+      const uint32_t tm = uni(tmem);
+      int pieces = 0, base = 0, g01 = 0, g23 = 0;  // pieces and ring entries so far; units of each buffer so far
       bool ok = true;
       while (ok && piece(pieces)) {
-        const Piece& w = list[pieces % PIECES];
-        const bool pair = w.pair;
-        const int nt = w.nt, units = w.units;
-        if (elect_one()) {
-          ok = wait_or_abort(q_full, pieces & 1, abort_flag, 141);
-          // operands' descriptors: the K-major tiles' (Q, K) and the MN-major V's; tiles differ in the low word's address
-          const uint64_t q_desc = prefill::sdesc(smem_u32(sm), 16, 1024), k_desc = prefill::sdesc(smem_u32(sm + C::K_OFF), 16, 1024),
-                         v_desc = prefill::sdesc(smem_u32(sm + C::K_OFF), BN * 128, 1024);
-          auto scores = [&](int i) {
-            const int t = pair ? i >> 1 : i, e = (base + k_entry(pair, t)) * SPT;
-            const uint64_t q = q_desc + (pair && (i & 1) ? C::QTILE >> 4 : 0);
-#pragma unroll
-            for (int h = 0; h < SPT; ++h) {
-              const int st = (e + h) % NS;
-              if (!ok || !(ok = wait_or_abort(&full[st], ((e + h) / NS) & 1, abort_flag, 142))) return;
-              prefill::tc_fence_after();
-              const uint64_t k = k_desc + st * (C::STAGE >> 4);
-#pragma unroll
-              for (int kk = 0; kk < C::DS / 16; ++kk)
-                prefill::umma_ss(tmem + (i & 1) * BN,
-                                 q + ((((kk >> 2) + h * (C::DS / 64)) * BM * 128 + (kk & 3) * 32) >> 4),
-                                 k + (((kk >> 2) * BN * 128 + (kk & 3) * 32) >> 4), IDESC_S,
-                                 h + kk > 0 ? 1u : 0u);
-              if (!pair || (i & 1)) prefill::umma_commit(&empty[st]);
-            }
-            prefill::umma_commit(&s_full[i & 1]);
-            if (i == units - 1) prefill::umma_commit(q_empty);
-          };
-          if (ok) scores(0);
-          if (ok && units > 1) scores(1);
-          for (int i = 0; ok && i < units; ++i) {
-            const int t = pair ? i >> 1 : i, e = (base + v_entry(pair, nt, t)) * SPT;
-            ok = wait_or_abort(&p_full[i & 1], ((i & 1 ? g1 : g0) + (i >> 1)) & 1, abort_flag, 143);
-            if (ok && i == 0 && pieces > 0) ok = wait_or_abort(o_free, (pieces - 1) & 1, abort_flag, 144);
-            const bool own = !C::WIDE;  // each buffer its O
-            const uint32_t o = tmem + C::O_COL + (own && (i & 1) ? D : 0);
-#pragma unroll
-            for (int h = 0; h < SPT; ++h) {
-              const int st = (e + h) % NS;
-              if (ok) ok = wait_or_abort(&full[st], ((e + h) / NS) & 1, abort_flag, 145);
-              if (!ok) break;
-              prefill::tc_fence_after();
-              const uint64_t v = v_desc + st * (C::STAGE >> 4);
-#pragma unroll
-              for (int kk = 0; kk < BN / 16; ++kk)
-                prefill::umma_ts(o + h * C::DS, tmem + (i & 1) * BN + kk * 8,
-                                 v + ((kk * 16 * 128) >> 4), IDESC_PV,
-                                 (own ? i > 1 : i > 0) || kk > 0 ? 1u : 0u);
-              if (!pair || (i & 1)) prefill::umma_commit(&empty[st]);
-            }
-            if (!ok) break;
-            prefill::umma_commit(&o_done[i & 1]);
-            if (i + 2 < units) scores(i + 2);
-          }
+        const bool pair = uni(list[pieces % PIECES].pair) != 0;
+        const int nt = uni(list[pieces % PIECES].nt), units = (pair ? 4 : 2) * nt;
+        // operands' descriptors: the K-major tiles' (Q, K) and the MN-major V's; tiles differ in the low word's address
+        const uint32_t q_desc = smem_u32(sm) >> 4 | 1u << 16;
+        const uint32_t s_desc = smem_u32(sm + C::K_OFF) >> 4 | uint32_t(scores ? 16 >> 4 : BN * 128 >> 4) << 16;
+        if (scores) {
+          ok = wait(q_full, pieces & 1, 141);
+        } else if (pieces > 0) {
+          ok = wait(o_free, (pieces - 1) & 1, 144);
         }
-        ok = __all_sync(0xffffffffu, ok && !*abort_flag);
+#pragma unroll 1
+        for (int i = 0; ok && i < units; ++i) {
+          const int ht = pair ? i >> 1 : i, half = ht & 1, buf = i & 3, nth = (i & 2 ? g23 : g01) + (i >> 2);
+          const int e = (base + (scores ? k_entry(pair, ht >> 1) : v_entry(pair, nt, ht >> 1))) * SPT;
+          const bool begins = half == 0 && (!pair || !(i & 1)), ends = half && (!pair || (i & 1));  // the tile's units
+          if (scores) {  // S overwrites the buffer's last P: its P V is done
+            if (nth > 0) ok = wait(&o_done[buf], (nth - 1) & 1, 161);
+          } else {
+            ok = wait(&p_full[buf], nth & 1, 143);
+          }
+          const uint32_t q = q_desc + (pair && (i & 1) ? C::QTILE >> 4 : 0);
+          const bool own = !C::WIDE;  // each warpgroup its O
+          const uint32_t o = tm + C::O_COL + (own && (i & 1) ? D : 0);
+#pragma unroll
+          for (int h = 0; h < SPT; ++h) {
+            const int st = (e + h) % NS;
+            if (begins && ok) ok = wait(&full[st], ((e + h) / NS) & 1, 142);
+            if (!ok) break;
+            prefill::tc_fence_after();
+            const uint32_t x = s_desc + st * (C::STAGE >> 4) + half * (BH * 128 >> 4);
+            if (scores) {
+#pragma unroll 1
+              for (uint32_t bx = 0; bx < C::DS / 64; ++bx)
+#pragma unroll
+                for (uint32_t kk = 0; kk < 4; ++kk)
+                  mma_ss(lead, tm + buf * BH, q + (((h * (C::DS / 64) + bx) * BM * 128 + kk * 32) >> 4),
+                         x + ((bx * BN * 128 + kk * 32) >> 4), IDESC_S, h + bx + kk > 0 ? 1u : 0u);
+            } else {
+#pragma unroll
+              for (int kk = 0; kk < BH / 16; ++kk)
+                mma_ts(lead, o + h * C::DS, tm + buf * BH + kk * 8, x + ((kk * 16 * 128) >> 4), IDESC_PV,
+                       (own ? i > 1 : i > 0) || kk > 0 ? 1u : 0u);
+            }
+            if (ends) mma_commit(lead, &empty[st]);
+          }
+          if (!ok) break;
+          mma_commit(lead, scores ? &s_full[buf] : &o_done[buf]);
+          if (scores && i == units - 1) mma_commit(lead, q_empty);
+        }
+        ok = ok && __all_sync(0xffffffffu, !*abort_flag);
         piece_done(pieces);
         ++pieces;
         base += 2 * nt;
-        g0 += (units + 1) >> 1;
-        g1 += units >> 1;
+        g01 += (units + 2) >> 2;
+        g23 += units >> 2;
       }
-      if (elect_one()) {
-        prefill::umma_commit(drain);
-        mbar_wait(drain, 0, 146);
+      if (lead) {
+        prefill::umma_commit(&drain[scores]);
+        mbar_wait(&drain[scores], 0, 146);
       }
       __syncwarp();
     } else if (warp == TABLE_WARP) {
@@ -648,9 +681,10 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
     // ------------------------------------------------------------------------------------ codes into operand tiles
     reg_dec<72>();
     constexpr int UPR = C::DS / 16;       // 16-code units a key and stage
-    constexpr int LD = BN * UPR / CT;     // units a thread and stage
-    constexpr int RSTEP = CT / UPR;       // keys between a thread's units
-    const int tid = threadIdx.x - CONV_WARP * 32, u = tid % UPR, r0 = tid / UPR;
+    constexpr int LD = BN * UPR / 128;    // units a thread and stage
+    constexpr int RSTEP = 128 / UPR;      // keys between a thread's units
+    const int tid = threadIdx.x - CONV_WARP * 32, ti = tid & 127, u = ti % UPR, r0 = ti / UPR;
+    const int group = tid >> 7;  // the two warpgroups take the stages in turn
     const int page = 1 << p.lpage;
     const int64_t kv_off = int64_t(p.c.a.Hkv) * (D << p.lpage);  // from a page's K to its V
     // where the thread's unit of key r0 goes in a stage, its two 16-byte halves ordered so that eight lanes fill 128 bytes
@@ -727,11 +761,11 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
         __syncwarp();
         if (lane == 0) mbar_arrive(q_full);
       }
-      // ---- codes: stage by stage, the next two stages' loads in flight
-      const int fills = 2 * nt * SPT;
-      uint4 buf[2][LD];
-      int tabs = 0;  // tiles of the piece whose ids are known to be in
-      auto load = [&](int s, uint4* x) {
+      // ---- codes: a stage's loads, and behind the other group's stage its operand
+      const int fills = 2 * nt * SPT;  // (even: each group's turns go on from piece to piece)
+      int tabs = 0;  // tiles of the piece whose places are known to be in
+#pragma unroll 1
+      for (int s = group; s < fills; s += 2) {
         int kind, t;
         entry(pair, nt, s / SPT, kind, t);
         const int slot = (gt + t) % TABLES;
@@ -739,25 +773,22 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
           if (ok) ok = wait_or_abort(&tab_full[slot], ((gt + t) / TABLES) & 1, abort_flag, 149);
           tabs = t + 1;
         }
-        const int end = horizon - (kt0 + t) * BN;  // keys of the tile that some row sees
-        const uint8_t* from = p.c.a.pages + kind * kv_off + (s % SPT) * C::DS;
+        const int end = ok ? horizon - (kt0 + t) * BN : 0;  // keys of the tile that some row sees
+        const uint8_t* from = p.c.a.pages + kind * kv_off + (s % SPT) * C::DS + u * 16;
         const int64_t* at = at_s + slot * 8;
-        int64_t o[LD];
-#pragma unroll
-        for (int i = 0; i < LD; ++i) o[i] = at[(r0 + i * RSTEP) >> p.lpage];
+        uint4 x[LD];
 #pragma unroll
         for (int i = 0; i < LD; ++i) {
           const int r = r0 + i * RSTEP;
-          x[i] = load_if(from + o[i] + ((r & (page - 1)) * D + u * 16), ok && o[i] >= 0 && r < end);
+          const int64_t o = at[r >> p.lpage];
+          x[i] = load_if(from + o + (r & (page - 1)) * D, o >= 0 && r < end);
         }
-        if (kind == 1 && s % SPT == SPT - 1) {  // the tile's ids have been used
+        if (kind == 1) {  // the tile's places have been used
           __syncwarp();
           if (lane == 0) mbar_arrive(&tab_empty[slot]);
         }
-      };
-      auto put = [&](const uint4* x) {
-        const int st = g % NS;
-        if (ok && g >= NS) ok = wait_or_abort(&empty[st], ((g / NS) - 1) & 1, abort_flag, 150);
+        const int gs = g + s, st = gs % NS;
+        if (ok && gs >= NS) ok = wait_or_abort(&empty[st], ((gs / NS) - 1) & 1, abort_flag, 150);
         uint8_t* d = sm + C::K_OFF + st * C::STAGE;
 #pragma unroll
         for (int i = 0; i < LD; ++i) {
@@ -772,17 +803,9 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
         fence_proxy_async_shared();
         __syncwarp();
         if (lane == 0) mbar_arrive(&full[st]);
-        ++g;
-      };
-      load(0, buf[0]);
-      load(1, buf[1]);  // (a piece has two fills at least)
-      for (int s = 0; ok && s < fills; s += 2) {
-        put(buf[0]);
-        if (s + 2 < fills) load(s + 2, buf[0]);
-        put(buf[1]);
-        if (s + 3 < fills) load(s + 3, buf[1]);
-        ok = __all_sync(0xffffffffu, ok);
       }
+      g += fills;
+      ok = __all_sync(0xffffffffu, ok);
       piece_done(pieces);
       ++pieces;
       gt += nt;
@@ -793,9 +816,8 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
     reg_inc<128>();
     const int wg = warp >> 2, quarter = warp & 3, r = 32 * quarter + lane;
     const uint32_t lane_base = tmem + (uint32_t(32 * quarter) << 16);
-    const uint32_t s_col = lane_base + wg * BN;
     const uint32_t o_col = lane_base + C::O_COL + (C::WIDE ? 0 : wg * D);
-    int pieces = 0, gt = 0, cnt[2] = {0, 0}, met = 0;  // pieces, tiles, units of each buffer so far; meetings
+    int pieces = 0, gt = 0, g01 = 0, g23 = 0, met = 0;  // pieces, tiles, units of each buffer so far; meetings
     auto meet_other = [&](bool& ok) {
       __syncwarp();
       if (lane == 0) mbar_arrive(&meet[quarter]);
@@ -807,21 +829,27 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
     while (piece(pieces)) {
       const Piece& w = list[pieces % PIECES];
       const bool pair = w.pair;
-      const int units = w.units, kt0 = w.kt0;
+      const int units = (pair ? 4 : 2) * w.nt, kt0 = w.kt0;
+      const int done = g01 + g23;  // each warpgroup's units before the piece's
       const int row = r + (pair ? wg * BM : 0);  // in the item
       const bool live = row < w.rows;
       const int tok = (w.f0 + row) / p.G;
       const int lim = !live ? -1 : (p.c.a.causal ? w.len - (w.n - 1 - tok) : w.len) - 1;  // the last key that the row sees
       float m = -FLT_MAX, l = 0.f, fac = 0.f;
+      // Waits for the P V of the piece's unit n. (Barriers are waited for within one phase of where they are: S_i comes after
+      // the P V of unit i - 4, the buffer's last.)
+      auto pv_done = [&](int n) {
+        return wait_or_abort(&o_done[n & 3], ((n & 2 ? g23 : g01) + (n >> 2)) & 1, abort_flag, 153);
+      };
       for (int i = wg; i < units; i += 2) {
-        const int t = pair ? i >> 1 : i, slot = (gt + t) % TABLES;
-        const int own = cnt[wg] + (i >> 1);  // the buffer's units before this one
-        if (ok) ok = wait_or_abort(&s_full[wg], own & 1, abort_flag, 151);
+        const int ht = pair ? i >> 1 : i, t = ht >> 1, half = ht & 1, slot = (gt + t) % TABLES;
+        const uint32_t s_col = lane_base + (i & 3) * BH;
+        if (ok) ok = wait_or_abort(&s_full[i & 3], ((i & 2 ? g23 : g01) + (i >> 2)) & 1, abort_flag, 151);
         ok = __all_sync(0xffffffffu, ok);
         prefill::tc_fence_after();
-        const int over = lim - (kt0 + t) * BN;  // the last column that the row sees
+        const int over = lim - (kt0 + t) * BN - half * BH;  // the last column that the row sees
         // Masked tiles are few: their scores are masked in place, so that all tiles share one short piece of code.
-        for (int c = max(__reduce_min_sync(0xffffffffu, over + 1), 0) & ~15; c < BN; c += 16) {
+        for (int c = max(__reduce_min_sync(0xffffffffu, over + 1), 0) & ~15; c < BH; c += 16) {
           float x[16];
           prefill2::tmem_ld16(s_col + c, x);
           prefill::tmem_wait_ld();
@@ -832,8 +860,8 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
         }
         // the row's largest score with the values' scale (a factor is never 0: -inf times it stays -inf)
         if (i < 2) fac = fac_s[(pieces & 1) * RB + row];
-        const float4* sc = tab + slot * 8;
-        float top = -INFINITY, sa[32], sb[32];
+        const float4* sc = tab + slot * 8 + half * 4;
+        float top = -INFINITY, s[BH];
         auto largest = [&](const float* x, int q) {
           const float2 f = *reinterpret_cast<const float2*>(sc + q);
           float a = max3(x[0], x[1], x[2]), b = max3(x[3], x[4], x[5]);
@@ -842,23 +870,17 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
           a = max3(a, x[14], x[15]);
           top = fmaxf(top, fmaf(fmaxf(a, b), fmaxf(fac * f.x, FLT_MIN), f.y));
         };
-        prefill::tmem_ld32(s_col, sa);
+        prefill::tmem_ld32(s_col, s);
+        prefill::tmem_ld32(s_col + 32, s + 32);
+        wait_ld32(s);
+        wait_ld32(s + 32);
 #pragma unroll
-        for (int c = 0; c < 4; c += 2) {
-          wait_ld32(sa);
-          prefill::tmem_ld32(s_col + 32 * c + 32, sb);
-          largest(sa, 2 * c);
-          largest(sa + 16, 2 * c + 1);
-          wait_ld32(sb);
-          prefill::tmem_ld32(s_col + (c == 0 ? 64 : 0), sa);  // (at last the weights' first columns)
-          largest(sb, 2 * c + 2);
-          largest(sb + 16, 2 * c + 3);
-        }
+        for (int q = 0; q < 4; ++q) largest(s + 16 * q, q);
         bool began;  // O holds something
         if constexpr (C::WIDE) {
           began = i > 0;
           if (i > 0) {  // the maximum after the unit before
-            if (ok) ok = wait_or_abort(&token[(1 - wg) * 4 + quarter], (cnt[1 - wg] + ((i - 1) >> 1)) & 1, abort_flag, 152);
+            if (ok) ok = wait_or_abort(&token[(1 - wg) * 4 + quarter], (done + ((i - 1) >> 1)) & 1, abort_flag, 152);
             const float now = m_sh[r];
             if (now != m) {
               l = shrink(l, m - now);
@@ -872,9 +894,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
         if (__any_sync(0xffffffffu, move)) {
           const float now = move ? top - TOP : m, corr = move ? prefill::ex2f(m - now) : 1.f;
           if (began) {
-            const int prev = C::WIDE ? 1 - wg : wg;  // the buffer of the O product before
-            const int nth = C::WIDE ? cnt[1 - wg] + ((i - 1) >> 1) : own - 1;
-            if (ok) ok = wait_or_abort(&o_done[prev], nth & 1, abort_flag, 153);
+            if (ok) ok = pv_done(i - (C::WIDE ? 1 : 2));
             ok = __all_sync(0xffffffffu, ok);
             prefill::tc_fence_after();
 #pragma unroll 1
@@ -896,7 +916,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
           __syncwarp();
           if (lane == 0) mbar_arrive(&token[wg * 4 + quarter]);
         }
-        for (uint32_t marked = far_s[slot]; marked; marked &= marked - 1) {  // (rare)
+        for (uint32_t marked = far_s[slot] >> (4 * half) & 15u; marked; marked &= marked - 1) {  // (rare)
           const int q = __ffs(marked) - 1;
           const float mul = fmaxf(fac * sc[q].x, FLT_MIN);
           float x[16];
@@ -905,60 +925,47 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
 #pragma unroll
           for (int e = 0; e < 16; ++e) l += prefill::ex2f(fmaf(x[e], mul, -m));
         }
-        // weights, 32 columns at a time, the next ones' scores on their way; P_i takes the place of scores already read
-        auto weights = [&](const float* x, int c) {
-          uint32_t pk[16];
+        // weights; P_i takes the place of S_i
+        uint32_t pk[32];
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float4 f = sc[2 * c + h];
-            const float mul = fmaxf(fac * f.x, FLT_MIN), add = f.w - m;
-            float2 sum = make_float2(0.f, 0.f);
+        for (int q = 0; q < 4; ++q) {
+          const float4 f = sc[q];
+          const float mul = fmaxf(fac * f.x, FLT_MIN), add = f.w - m;
+          float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-            for (int e = 0; e < 16; e += 2) {
-              float2 y = kv8::fma2(make_float2(x[16 * h + e], x[16 * h + e + 1]), make_float2(mul, mul), make_float2(add, add));
-              y.x = prefill::ex2f(y.x), y.y = prefill::ex2f(y.y);
-              sum = add2(sum, y);
-              pk[8 * h + e / 2] = pack2<__half>(y.x, y.y);
-            }
-            l = fmaf(sum.x + sum.y, f.z, l);
+          for (int e = 0; e < 16; e += 2) {
+            float2 y = kv8::fma2(make_float2(s[16 * q + e], s[16 * q + e + 1]), make_float2(mul, mul), make_float2(add, add));
+            y.x = prefill::ex2f(y.x), y.y = prefill::ex2f(y.y);
+            sum = add2(sum, y);
+            pk[8 * q + e / 2] = pack2<__half>(y.x, y.y);
           }
-          prefill::tmem_st16(s_col + 16 * c, pk);
-        };
-#pragma unroll 1
-        for (int c = 0; c < 4; c += 2) {
-          wait_ld32(sa);
-          prefill::tmem_ld32(s_col + 32 * c + 32, sb);
-          weights(sa, c);
-          wait_ld32(sb);
-          if (c == 0) prefill::tmem_ld32(s_col + 64, sa);
-          weights(sb, c + 1);
+          l = fmaf(sum.x + sum.y, f.z, l);
         }
+        prefill::tmem_st32(s_col, reinterpret_cast<const float*>(pk));
         prefill::tmem_wait_st();
         prefill::tc_fence_before();
         __syncwarp();
         if (lane == 0) {
-          mbar_arrive(&p_full[wg]);
-          mbar_arrive(&tab_empty[slot]);
-          if (!pair) mbar_arrive(&tab_empty[slot]);
+          mbar_arrive(&p_full[i & 3]);
+          if (half || !pair) mbar_arrive(&tab_empty[slot]);
         }
       }
       // -------------------------------------------------------------------------------- the piece's end
-      const int n0 = (units + 1) >> 1, n1 = units >> 1;
       float f0 = 1.f, f1 = 0.f;  // factors of this group's O, or of O 0 and O 1
       if (pair) {
-        if (ok) ok = wait_or_abort(&o_done[wg], (cnt[wg] + n0 - 1) & 1, abort_flag, 154);
+        if (ok) ok = pv_done(units - 2 + wg);
       } else {
         ml_s[wg * BM + r] = make_float2(m, l);
         meet_other(ok);
         const float2 x = ml_s[r], y = ml_s[BM + r];
         m = fmaxf(x.x, y.x);  // (a shared maximum never falls, so it is the later one)
         f0 = prefill::ex2f(x.x - m);
-        f1 = n1 ? prefill::ex2f(y.x - m) : 0.f;
-        l = shrink(x.y, x.x - m) + (n1 ? shrink(y.y, y.x - m) : 0.f);
+        f1 = prefill::ex2f(y.x - m);
+        l = shrink(x.y, x.x - m) + shrink(y.y, y.x - m);
         if (C::WIDE) f0 = 1.f;
         meet_other(ok);  // (read before the next piece's are written)
-        if (ok) ok = wait_or_abort(&o_done[0], (cnt[0] + n0 - 1) & 1, abort_flag, 155);
-        if (ok && n1) ok = wait_or_abort(&o_done[1], (cnt[1] + n1 - 1) & 1, abort_flag, 156);
+        if (ok) ok = pv_done(units - 2);
+        if (ok) ok = pv_done(units - 1);
       }
       ok = __all_sync(0xffffffffu, ok);
       prefill::tc_fence_after();
@@ -973,16 +980,11 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
         prefill::tmem_ld32(oc + c, ov);
         prefill::tmem_wait_ld();
         if (!C::WIDE && !pair) {
-          if (n1) {
-            float o1[32];
-            prefill::tmem_ld32(oc + D + c, o1);
-            prefill::tmem_wait_ld();
+          float o1[32];
+          prefill::tmem_ld32(oc + D + c, o1);
+          prefill::tmem_wait_ld();
 #pragma unroll
-            for (int e = 0; e < 32; ++e) ov[e] = ov[e] * f0 + o1[e] * f1;
-          } else {
-#pragma unroll
-            for (int e = 0; e < 32; ++e) ov[e] *= f0;
-          }
+          for (int e = 0; e < 32; ++e) ov[e] = ov[e] * f0 + o1[e] * f1;
         }
         if (!live || !ok) continue;
         if (w.whole) {
@@ -1007,8 +1009,8 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
       piece_done(pieces);
       ++pieces;
       gt += w.nt;
-      cnt[0] += n0;
-      cnt[1] += n1;
+      g01 += (units + 2) >> 2;
+      g23 += units >> 2;
     }
     if (!ok) *abort_flag = 1, rec0.x = 0;
     if (threadIdx.x == 0) {
