@@ -1963,6 +1963,42 @@ int lb2_kv8_attend_packed(const void* q, const int64_t* q_st, const uint8_t* pag
 
 // ------------------------------------------------------------------------------------------------ pages moved about
 
+}  // extern "C"
+
+template <typename Kern, typename P>
+static int kv8_go(Kern kern, dim3 grid, int threads, cudaStream_t st, const P& p) {
+  cudaLaunchAttribute pdl[1];
+  pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  pdl[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
+  cfg.stream = st;
+  cfg.attrs = pdl;
+  cfg.numAttrs = 1;
+  LB2_CUDA(cudaLaunchKernelEx(&cfg, kern, p));
+  return LB2_OK;
+}
+
+static int kv8_compact_run(const kv8::CompactParams& p, int D, int page, dim3 grid, cudaStream_t st) {
+  const int units = page * D / 16;  // 64 .. 2048, over 64 to 512 threads of 1 to 4
+  auto go = [&](auto d) {
+    constexpr int N = decltype(d)::value;
+    switch (units) {
+      case 64: return kv8_go(kv8::compact_kernel<64, 1, N>, grid, 64, st, p);
+      case 128: return kv8_go(kv8::compact_kernel<128, 1, N>, grid, 128, st, p);
+      case 256: return kv8_go(kv8::compact_kernel<128, 2, N>, grid, 128, st, p);
+      case 512: return kv8_go(kv8::compact_kernel<256, 2, N>, grid, 256, st, p);
+      case 1024: return kv8_go(kv8::compact_kernel<512, 2, N>, grid, 512, st, p);
+      default: return kv8_go(kv8::compact_kernel<512, 4, N>, grid, 512, st, p);
+    }
+  };
+  return D == 64 ? go(std::integral_constant<int, 64>()) : D == 128 ? go(std::integral_constant<int, 128>())
+                                                                      : go(std::integral_constant<int, 256>());
+}
+
+extern "C" {
+
 int lb2_kv8_copy(const uint8_t* from_pages, const float* from_scales, int from_num, uint8_t* to_pages, float* to_scales,
                  int to_num, const int32_t* src, const int32_t* dst, int n, int Hkv, int page, int D, void* stream) {
   int rc = kv8_shape(0, Hkv, 0, D, page, from_num, 1, "kv8_copy");
@@ -1976,11 +2012,12 @@ int lb2_kv8_copy(const uint8_t* from_pages, const float* from_scales, int from_n
   kv8::CopyParams p{from_pages, from_scales, to_pages, to_scales, src, dst, n, from_num, to_num, 2 * Hkv,
                     int64_t(2) * Hkv * page * D};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const unsigned parts = static_cast<unsigned>((p.bytes / 16 + kv8::COPY_THREADS * kv8::COPY_HELD - 1) / (kv8::COPY_THREADS * kv8::COPY_HELD));
   for (int i = 0; i < n; i += 65535) {
     kv8::CopyParams c = p;
     c.src += i, c.dst += i;
-    kv8::copy_kernel<<<dim3(8, unsigned(std::min(n - i, 65535))), kv8::COPY_THREADS, 0, st>>>(c);
-    LB2_CUDA(cudaGetLastError());
+    const int rc = kv8_go(kv8::copy_kernel, dim3(parts, unsigned(std::min(n - i, 65535))), kv8::COPY_THREADS, st, c);
+    if (rc) return rc;
   }
   return LB2_OK;
 }
@@ -2006,9 +2043,11 @@ int lb2_kv8_compact(uint8_t* pages, float* scales, const int32_t* table, int64_t
   p.interleaved = interleaved != 0;
   const int64_t pieces = int64_t(T) / page + B;
   LB2_CHECK_ARG(pieces < (int64_t(1) << 31), "kv8_compact: too many tokens");
-  kv8::compact_any_kernel<<<dim3(unsigned(pieces), unsigned(2 * Hkv)), 128, 0, static_cast<cudaStream_t>(stream)>>>(p);
-  LB2_CUDA(cudaGetLastError());
-  return LB2_OK;
+  p.hpb = 1;
+  if (R % 16) return kv8_go(kv8::compact_any_kernel, dim3(unsigned(pieces), unsigned(2 * Hkv)), 128, static_cast<cudaStream_t>(stream), p);
+  // heads a block while every SM keeps two blocks: they share the block's start and the angles
+  while (p.hpb < 8 && pieces * 2 * ((Hkv + 2 * p.hpb - 1) / (2 * p.hpb)) >= 148 * 2) p.hpb *= 2;
+  return kv8_compact_run(p, D, page, dim3(unsigned(pieces), unsigned(2 * ((Hkv + p.hpb - 1) / p.hpb))), static_cast<cudaStream_t>(stream));
 }
 
 // ------------------------------------------------------------------------------------------------ packed prompts
