@@ -61,7 +61,7 @@ struct CompactParams {
   int B, Hkv, T, D, R, num_pages, max_pages, max_to;
   int lpage;  // log2 of page
   int interleaved;
-  int hpb;    // heads a block takes in turn
+  int planes;  // (K or V, head) pairs a block takes
 };
 
 // The page that block piece i writes: of sequence b, its moved tokens [t0, t0 + n), into page `id` (out of range: none).
@@ -73,39 +73,49 @@ struct CompactPiece {
 
 // Sequence b's pieces start at cu[b] / page + b, which leaves room for its pages (n tokens fill at most n / page + 1).
 __device__ __forceinline__ bool compact_piece(const CompactParams& p, int i, CompactPiece& w) {
-  auto base = [&](int s) { return (min(max(p.cu[s], 0), p.T) >> p.lpage) + s; };
-  int lo = 0, hi = p.B;  // base(lo) <= i, and base(hi) > i or hi == B
-  while (hi - lo > 1) {
-    const int step = (hi - lo + 31) / 32, s = lo + (threadIdx.x & 31) * step;
-    const uint32_t le = __ballot_sync(0xffffffffu, s < hi && (s == lo || base(s) <= i));
-    const int k = 31 - __clz(le);
-    lo += k * step;
-    hi = min(hi, lo + step);
+  auto base = [&](int c, int s) { return (min(max(c, 0), p.T) >> p.lpage) + s; };
+  const int lane = threadIdx.x & 31;
+  int lo = 0, c0, c1, s0;
+  if (p.B < 32) {  // a lane a sequence: one round of loads
+    const int c = p.cu[min(lane, p.B)], s = p.start[min(lane, p.B - 1)];
+    lo = 31 - __clz(__ballot_sync(0xffffffffu, lane < p.B && (lane == 0 || base(c, lane) <= i)));
+    c0 = __shfl_sync(0xffffffffu, c, lo), c1 = __shfl_sync(0xffffffffu, c, lo + 1), s0 = __shfl_sync(0xffffffffu, s, lo);
+  } else {
+    int hi = p.B;  // base(lo) <= i, and base(hi) > i or hi == B
+    while (hi - lo > 1) {
+      const int step = (hi - lo + 31) / 32, s = lo + lane * step;
+      const uint32_t le = __ballot_sync(0xffffffffu, s < hi && (s == lo || base(p.cu[s], s) <= i));
+      const int k = 31 - __clz(le);
+      lo += k * step;
+      hi = min(hi, lo + step);
+    }
+    c0 = p.cu[lo], c1 = p.cu[lo + 1], s0 = p.start[lo];
   }
   w.b = lo;
-  const int j = i - base(lo), page = 1 << p.lpage;
-  const int c0 = p.cu[lo], c1 = p.cu[lo + 1], r0 = min(max(c0, 0), p.T), n = min(max(c1, r0), p.T) - r0;
+  const int j = i - base(c0, lo), page = 1 << p.lpage, r0 = min(max(c0, 0), p.T), n = min(max(c1, r0), p.T) - r0;
   const bool lead = threadIdx.x == 0;
   if (lead && j == 0 && (c0 != r0 || c1 != r0 + n)) report_bad_index(STATUS_COMPACT);
   if (j < 0 || int64_t(j) << p.lpage >= n) return false;
   w.t0 = j << p.lpage;
   w.n = min(n - w.t0, page);
   w.row0 = r0 + w.t0;
-  const int s0 = p.start[lo];
   w.first = int64_t(s0) + w.t0;
   const int64_t pj = w.first >> p.lpage;
   w.id = s0 >= 0 && (s0 & (page - 1)) == 0 && pj < p.max_to ? p.to[lo * p.to_st + pj] : -1;
+  return true;
+}
+
+// (Apart from the search: the loads of the page id and of the tokens' positions then run at once.)
+__device__ __forceinline__ bool compact_page(const CompactParams& p, const CompactPiece& w) {
   if (w.id >= 0 && w.id < p.num_pages) return true;
-  if (lead) report_bad_index(STATUS_COMPACT);
+  if (threadIdx.x == 0) report_bad_index(STATUS_COMPACT);
   return false;
 }
 
-// Where token t of the piece lies: its page's first (page, K / V, head) slot for head 0 of K and the row in it; -1 where it
-// cannot be read. pos: its old position.
-__device__ __forceinline__ int64_t compact_slot(const CompactParams& p, const CompactPiece& w, int t, int& pos) {
-  pos = p.keep[w.row0 + t];
+// The first (page, K / V, head) slot of the page that holds sequence b's position; -1 where it cannot be read.
+__device__ __forceinline__ int64_t compact_slot(const CompactParams& p, int b, int pos) {
   const int j = pos >> p.lpage;
-  const int id = pos >= 0 && j < p.max_pages ? p.table[w.b * p.table_st + j] : -1;
+  const int id = pos >= 0 && j < p.max_pages ? p.table[b * p.table_st + j] : -1;
   if (id < 0 || id >= p.num_pages) {
     report_bad_index(STATUS_COMPACT);
     return -1;
@@ -118,13 +128,13 @@ __global__ void __launch_bounds__(128) compact_any_kernel(const CompactParams p)
   __shared__ float red[4];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   CompactPiece w;
-  if (!compact_piece(p, blockIdx.x, w)) return;
+  if (!compact_piece(p, blockIdx.x, w) || !compact_page(p, w)) return;
   const int kind = blockIdx.y & 1, h = blockIdx.y >> 1, D = p.D, page = 1 << p.lpage;
   const int rot = kind == 0 ? p.R : 0, R2 = rot >> 1, cnt = w.n * D;
   auto value = [&](int i) {
     const int t = i / D, d = i - t * D;
-    int pos;
-    const int64_t s = compact_slot(p, w, t, pos);
+    const int pos = p.keep[w.row0 + t];
+    const int64_t s = compact_slot(p, w.b, pos);
     if (s < 0) return 0.f;
     const int64_t slot = s + kind * p.Hkv + h;
     const uint8_t* x = p.pages + (slot * page + (pos & (page - 1))) * D;
@@ -162,136 +172,213 @@ __global__ void __launch_bounds__(128) compact_any_kernel(const CompactParams p)
         enc4(value(i) * inv, value(i + 1) * inv, value(i + 2) * inv, value(i + 3) * inv);
 }
 
-// Rotated dims in whole units of 16. A block takes a page of K or of V and p.hpb heads in turn; a thread holds U units, a unit
-// being 16 of a token's dims whose partners under the rotation lie in it too: 8 dims and the 8 that they are paired with (half
-// layout), or 16 in a row. So the codes are read once, the angles of a page are formed once for the block's heads, and
-// between the two the page's largest magnitude is found in registers; the next head's codes are on their way meanwhile.
-template <int THREADS, int U, int D>
-__global__ void __launch_bounds__(THREADS) compact_kernel(const CompactParams p) {
-  constexpr int UPR = D / 16;  // units a token
-  __shared__ uint32_t red[2][THREADS / 32];
+// (cos, sin) of `frac` 2^-64 turns, from its upper 32 bits: the nearest quarter turn, and Taylor's series on the rest, |x| <=
+// pi / 4: to x^9 and x^8, which leave out 2e-9 and 3e-8. Half the instructions of sincospi, which set the kernel's pace.
+__device__ __forceinline__ float2 quarter_cs(uint64_t frac) {
+  const uint32_t hi = uint32_t(frac >> 32), q = (hi + 0x20000000u) >> 30;
+  const float x = float(int32_t(hi - (q << 30))) * 1.4629180792671596e-9f;  // 2 pi / 2^32
+  const float x2 = x * x;
+  float s = fmaf(x2, 1.f / 362880.f, -1.f / 5040.f);
+  s = fmaf(x2, s, 1.f / 120.f);
+  s = fmaf(x2, s, -1.f / 6.f);
+  s = fmaf(x * x2, s, x);
+  float c = fmaf(x2, 1.f / 40320.f, -1.f / 720.f);
+  c = fmaf(x2, c, 1.f / 24.f);
+  c = fmaf(x2, c, -0.5f);
+  c = fmaf(x2, c, 1.f);
+  const float a = q & 1 ? s : c, b = q & 1 ? c : s;
+  return make_float2(__uint_as_float(__float_as_uint(a) ^ (((q + 1) & 2) << 30)), __uint_as_float(__float_as_uint(b) ^ ((q & 2) << 30)));
+}
+
+// The largest finite magnitude of 16 codes times f.
+__device__ __noinline__ float held_max(uint2 a, uint2 b, float f) {
+  float m = 0.f;
+  for (int k = 0; k < 4; ++k) {
+    uint32_t lo, hi;
+    dec4(k == 0 ? a.x : k == 1 ? a.y : k == 2 ? b.x : b.y, lo, hi);
+    const float2 x = half2_f(lo), y = half2_f(hi);
+    m = fmaxf(fmaxf(m, fmaxf(finite_abs(x.x * f), finite_abs(x.y * f))), fmaxf(finite_abs(y.x * f), finite_abs(y.y * f)));
+  }
+  return m;
+}
+
+// Four codes times r, to the nearest codes.
+__device__ __forceinline__ uint32_t times(uint32_t c, __half2 r) {
+  uint32_t lo, hi, x;
+  dec4(c, lo, hi);
+  const __half2 a = __hmul2(*reinterpret_cast<__half2*>(&lo), r), b = __hmul2(*reinterpret_cast<__half2*>(&hi), r);
+  asm("{\n\t.reg .b16 lo, hi;\n\tcvt.rn.satfinite.e4m3x2.f16x2 lo, %1;\n\tcvt.rn.satfinite.e4m3x2.f16x2 hi, %2;\n\tmov.b32 %0, {lo, hi};\n\t}"
+      : "=r"(x)
+      : "r"(*reinterpret_cast<const uint32_t*>(&a)), "r"(*reinterpret_cast<const uint32_t*>(&b)));
+  return x;
+}
+
+// Rotated dims in whole units of 16. A block takes a page of p.planes (K or V, head) pairs; a thread holds a unit of U tokens'
+// dims, a unit being 16 of a token's dims whose partners under the rotation lie in it too: 8 dims and the 8 that they are
+// paired with (half layout), or 16 in a row. So the codes are read once, the angles of a page are formed once for the block's
+// heads, and the page's largest magnitude is found in between.
+// A block begins with a chain of four loads (bounds, positions, pages, codes), some 4 us, and needs few instructions after it:
+// what counts is the bytes in flight, so H planes' codes are asked for at once, and one barrier serves their maxima.
+template <int THREADS, int U, int H, int D, bool TURN>
+__global__ void __launch_bounds__(THREADS, U == 1 || !TURN ? 768 / THREADS : 1) compact_kernel(const CompactParams p) {
+  constexpr int UPR = D / 16, WARPS = THREADS / 32;
+  __shared__ uint32_t red[2][H][WARPS];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   CompactPiece w;
   if (!compact_piece(p, blockIdx.x, w)) return;
-  const int groups = (p.Hkv + p.hpb - 1) / p.hpb, kind = blockIdx.y >= groups;
-  const int h0 = (int(blockIdx.y) - kind * groups) * p.hpb, h1 = min(h0 + p.hpb, p.Hkv);
-  const int page = 1 << p.lpage, tid = threadIdx.x, turned = kind == 0 ? p.R / 16 : 0;
-  const int64_t head = int64_t(page) * D;  // codes of a head's page
-  const uint8_t* src[U];                   // the unit's codes of head h0 (null: nothing to read)
+  const int l0 = blockIdx.y * p.planes, l1 = min(l0 + p.planes, 2 * p.Hkv);
+  const int page = 1 << p.lpage, tid = threadIdx.x, turned = TURN && l0 < p.Hkv ? p.R / 16 : 0;
+  const int head = page * D;  // codes of a plane of a page
+  int pos[U];
+#pragma unroll
+  for (int i = 0; i < U; ++i) pos[i] = (i * THREADS + tid) / UPR < w.n ? p.keep[w.row0 + (i * THREADS + tid) / UPR] : 0;
+  if (!compact_page(p, w)) return;
+  const uint8_t* src[U];  // the unit's codes of plane 0 (null: nothing to read)
   const float* sc[U];
-  int a0[U], a1[U], pos[U];                // where its two halves lie in a row; its old position
-  int64_t dst[U];
+  int at[U], by[U];       // where the unit's first half lies in a plane; how far the second one is from it
   bool live[U];
 #pragma unroll
   for (int i = 0; i < U; ++i) {
     const int x = i * THREADS + tid, t = x / UPR, q = x % UPR;
     live[i] = t < w.n;
-    a0[i] = 16 * q, a1[i] = 16 * q + 8;
-    if (q < turned && !p.interleaved) a0[i] = 8 * q, a1[i] = p.R / 2 + 8 * q;
+    const bool halves = q < turned && !p.interleaved;
+    const int d0 = halves ? 8 * q : 16 * q;
+    by[i] = halves ? p.R / 2 : 8;
+    at[i] = t * D + d0;
     src[i] = nullptr;
     sc[i] = nullptr;
-    pos[i] = 0;
     if (live[i]) {
-      const int64_t s = compact_slot(p, w, t, pos[i]);
-      if (s >= 0) {
-        const int64_t slot = s + kind * p.Hkv + h0;
-        src[i] = p.pages + slot * head + (pos[i] & (page - 1)) * D;
+      const int64_t slot = compact_slot(p, w.b, pos[i]);
+      if (slot >= 0) {
+        src[i] = p.pages + slot * head + (pos[i] & (page - 1)) * D + d0;
         sc[i] = p.scales + slot;
       }
     }
-    dst[i] = ((int64_t(w.id) * 2 + kind) * p.Hkv + h0) * head + t * D;
   }
-  uint2 c[U][2];
-  float f[U];
-  auto load = [&](int h) {
+  uint2 c[H][U][2];
+  float f[H][U];
+  float2 z[TURN ? U : 1][8];  // the unit's angles
+  // a turned unit's codes as values, turned (its scale is left out: a power of two)
+  auto values = [&](const uint2* x, int i, bool turn_it, float* y) {
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
-      c[i][0] = c[i][1] = make_uint2(0, 0);
-      f[i] = 0.f;
-      if (src[i]) {
-        const uint8_t* x = src[i] + (h - h0) * head;
-        c[i][0] = *reinterpret_cast<const uint2*>(x + a0[i]);
-        c[i][1] = *reinterpret_cast<const uint2*>(x + a1[i]);
-        f[i] = sc[i][h - h0];
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        uint32_t lo, hi;
+        dec4(e ? x[k].y : x[k].x, lo, hi);
+        const float2 a = half2_f(lo), b = half2_f(hi);
+        float* o = y + 8 * k + 4 * e;
+        o[0] = a.x, o[1] = a.y, o[2] = b.x, o[3] = b.y;
       }
+    if (!TURN || !turn_it || (i * THREADS + tid) % UPR >= turned) return;
+    auto turn = [](float& a, float& b, float2 r) {
+      const float x = a;
+      a = x * r.x - b * r.y;
+      b = b * r.x + x * r.y;
+    };
+    if (p.interleaved) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) turn(y[2 * e], y[2 * e + 1], z[TURN ? i : 0][e]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) turn(y[e], y[8 + e], z[TURN ? i : 0][e]);
     }
   };
-  load(h0);
-  float2 z[U][8];  // the unit's angles
-  if (turned) {
+  int round = 0;
+#pragma unroll 1
+  for (int l = l0; l < l1; l += H, round ^= 1) {
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const int x = i * THREADS + tid, t = x / UPR, q = x % UPR;
-      if (!live[i] || q >= turned) continue;
-      const uint64_t by = uint64_t(w.first + t - pos[i]);
+    for (int h = 0; h < H; ++h)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) z[i][e] = rope::turn_cs(by * p.turns[8 * q + e]);
-    }
-  }
-  for (int h = h0; h < h1; ++h) {
-    float y[U][16];
-    float m = 0.f;
-#pragma unroll
-    for (int i = 0; i < U; ++i) {
-#pragma unroll
-      for (int k = 0; k < 2; ++k)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          uint32_t lo, hi;
-          dec4(e ? c[i][k].y : c[i][k].x, lo, hi);
-          const float2 a = half2_f(lo), b = half2_f(hi);
-          float* o = y[i] + 8 * k + 4 * e;
-          o[0] = a.x * f[i], o[1] = a.y * f[i], o[2] = b.x * f[i], o[3] = b.y * f[i];
-        }
-    }
-    if (h + 1 < h1) load(h + 1);
-#pragma unroll
-    for (int i = 0; i < U; ++i) {
-      if (turned && (i * THREADS + tid) % UPR < turned) {
-        auto turn = [](float& a, float& b, float2 z) {
-          const float x = a;
-          a = x * z.x - b * z.y;
-          b = b * z.x + x * z.y;
-        };
-        if (p.interleaved) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) turn(y[i][2 * e], y[i][2 * e + 1], z[i][e]);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) turn(y[i][e], y[i][8 + e], z[i][e]);
+      for (int i = 0; i < U; ++i) {
+        c[h][i][0] = c[h][i][1] = make_uint2(0, 0);
+        f[h][i] = 0.f;
+        if (src[i] && l + h < l1) {
+          // (K's planes hold units as they are turned, V's 16 dims in a row)
+          const int64_t o = int64_t(l + h) * head;
+          const bool v = l + h >= p.Hkv && by[i] != 8;
+          const uint8_t* x = src[i] + o + (v ? (at[i] % D) : 0);
+          c[h][i][0] = *reinterpret_cast<const uint2*>(x);
+          c[h][i][1] = *reinterpret_cast<const uint2*>(x + (v ? 8 : by[i]));
+          f[h][i] = sc[i][l + h];
         }
       }
+    if (TURN && turned && l == l0) {
 #pragma unroll
-      for (int e = 0; e < 16; e += 2) m = max3_abs(m, y[i][e], y[i][e + 1]);  // (NaN is passed over)
+      for (int i = 0; i < U; ++i) {
+        const int x = i * THREADS + tid, q = x % UPR;
+        if (!live[i] || q >= turned) continue;
+        const uint64_t shift = uint64_t(w.first + x / UPR - pos[i]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) z[TURN ? i : 0][e] = quarter_cs(shift * p.turns[8 * q + e]);
+      }
     }
-    if (m == INFINITY) {  // rare: held infinities of a page whose scale is near fp32's end
-      m = 0.f;
 #pragma unroll
-      for (int i = 0; i < U; ++i)
+    for (int h = 0; h < H; ++h) {
+      const bool turn_it = TURN && turned && l + h < p.Hkv;
+      float m = 0.f;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) m = fmaxf(m, finite_abs(y[i][e]));
+      for (int i = 0; i < U; ++i) {
+        float mi = 0.f;
+        if (turn_it) {
+          float y[16];
+          values(c[h][i], i, true, y);
+#pragma unroll
+          for (int e = 0; e < 16; e += 2) mi = max3_abs(mi, y[e], y[e + 1]);  // (NaN is passed over)
+        } else {  // codes as they lie: in f16, two a step
+          __half2 m2 = __float2half2_rn(0.f);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            uint32_t x[2];
+            const uint2 u = c[h][i][k >> 1];
+            dec4(k & 1 ? u.y : u.x, x[0], x[1]);
+            m2 = __hmax2(m2, __hmax2(__habs2(*reinterpret_cast<__half2*>(&x[0])), __habs2(*reinterpret_cast<__half2*>(&x[1]))));
+          }
+          mi = fmaxf(__low2float(m2), __high2float(m2));
+        }
+        mi *= f[h][i];
+        if (!(mi < INFINITY)) mi = held_max(c[h][i][0], c[h][i][1], f[h][i]);  // rare: held infinities near fp32's end
+        m = fmaxf(m, mi);
+      }
+      const uint32_t wm = __reduce_max_sync(0xffffffffu, __float_as_uint(m));
+      if ((tid & 31) == 0) red[round][h][tid >> 5] = wm;
     }
-    const int turn = (h - h0) & 1;
-    const uint32_t wm = __reduce_max_sync(0xffffffffu, __float_as_uint(m));
-    if ((tid & 31) == 0) red[turn][tid >> 5] = wm;
     __syncthreads();
-    uint32_t all = red[turn][0];
 #pragma unroll
-    for (int k = 1; k < THREADS / 32; ++k) all = max(all, red[turn][k]);
-    const float now = scale_of(__uint_as_float(all)), inv = scale_inv(now);
-    if (tid == 0) p.scales[(int64_t(w.id) * 2 + kind) * p.Hkv + h] = now;
+    for (int h = 0; h < H; ++h) {
+      if (l + h >= l1) break;
+      const bool turn_it = TURN && turned && l + h < p.Hkv;
+      uint32_t all = red[round][h][0];
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
-      if (!live[i]) continue;
-      uint8_t* o = p.pages + dst[i] + (h - h0) * head;
-      uint2 e[2];
+      for (int k = 1; k < WARPS; ++k) all = max(all, red[round][h][k]);
+      const float now = scale_of(__uint_as_float(all)), inv = scale_inv(now);
+      const int64_t slot = int64_t(w.id) * 2 * p.Hkv + l + h;
+      if (tid == 0) p.scales[slot] = now;
+      uint8_t* out = p.pages + slot * head;
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const float* v = y[i] + 8 * k;
-        e[k] = make_uint2(enc4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv), enc4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv));
+      for (int i = 0; i < U; ++i) {
+        if (!live[i]) continue;
+        const float r = f[h][i] * inv;  // what the codes are multiplied by
+        uint2 e[2];
+        if (turn_it || !(r <= 32768.f) || (__float_as_uint(f[h][i]) & 0x7fffffu) != 0) {
+          float v[16];
+          values(c[h][i], i, turn_it, v);
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const float* x = v + 8 * k;
+            e[k] = make_uint2(enc4(x[0] * r, x[1] * r, x[2] * r, x[3] * r), enc4(x[4] * r, x[5] * r, x[6] * r, x[7] * r));
+          }
+        } else {
+          // a power of two times a code in f16: exact down to 2^-21, and below 2^-10 every code is 0
+          const __half2 r2 = __float2half2_rn(r);
+#pragma unroll
+          for (int k = 0; k < 2; ++k) e[k] = make_uint2(times(c[h][i][k].x, r2), times(c[h][i][k].y, r2));
+        }
+        const bool v = l + h >= p.Hkv && by[i] != 8;
+        const int o = at[i] + (v ? at[i] % D : 0);
+        *reinterpret_cast<uint2*>(out + o) = e[0];
+        *reinterpret_cast<uint2*>(out + o + (v ? 8 : by[i])) = e[1];
       }
-      *reinterpret_cast<uint2*>(o + a0[i]) = e[0];
-      *reinterpret_cast<uint2*>(o + a1[i]) = e[1];
     }
   }
 }

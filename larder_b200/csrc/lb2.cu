@@ -1981,20 +1981,25 @@ static int kv8_go(Kern kern, dim3 grid, int threads, cudaStream_t st, const P& p
 }
 
 static int kv8_compact_run(const kv8::CompactParams& p, int D, int page, dim3 grid, cudaStream_t st) {
-  const int units = page * D / 16;  // 64 .. 2048, over 64 to 512 threads of 1 to 4
-  auto go = [&](auto d) {
+  const int units = page * D / 16;  // 64 .. 2048, a thread each up to 512
+  auto go = [&](auto d, auto t) {
     constexpr int N = decltype(d)::value;
+    constexpr bool TURN = decltype(t)::value;
     switch (units) {
-      case 64: return kv8_go(kv8::compact_kernel<64, 1, N>, grid, 64, st, p);
-      case 128: return kv8_go(kv8::compact_kernel<128, 1, N>, grid, 128, st, p);
-      case 256: return kv8_go(kv8::compact_kernel<128, 2, N>, grid, 128, st, p);
-      case 512: return kv8_go(kv8::compact_kernel<256, 2, N>, grid, 256, st, p);
-      case 1024: return kv8_go(kv8::compact_kernel<512, 2, N>, grid, 512, st, p);
-      default: return kv8_go(kv8::compact_kernel<512, 4, N>, grid, 512, st, p);
+      case 64: return kv8_go(kv8::compact_kernel<64, 1, 4, N, TURN>, grid, 64, st, p);
+      case 128: return kv8_go(kv8::compact_kernel<128, 1, 4, N, TURN>, grid, 128, st, p);
+      case 256: return kv8_go(kv8::compact_kernel<256, 1, 4, N, TURN>, grid, 256, st, p);
+      case 512: return kv8_go(kv8::compact_kernel<256, 2, 2, N, TURN>, grid, 256, st, p);
+      case 1024: return kv8_go(kv8::compact_kernel<512, 2, 2, N, TURN>, grid, 512, st, p);
+      default: return kv8_go(kv8::compact_kernel<512, 4, 1, N, TURN>, grid, 512, st, p);
     }
   };
-  return D == 64 ? go(std::integral_constant<int, 64>()) : D == 128 ? go(std::integral_constant<int, 128>())
-                                                                      : go(std::integral_constant<int, 256>());
+  auto by_dim = [&](auto t) {
+    return D == 64    ? go(std::integral_constant<int, 64>(), t)
+           : D == 128 ? go(std::integral_constant<int, 128>(), t)
+                      : go(std::integral_constant<int, 256>(), t);
+  };
+  return p.R ? by_dim(std::true_type()) : by_dim(std::false_type());
 }
 
 extern "C" {
@@ -2043,11 +2048,12 @@ int lb2_kv8_compact(uint8_t* pages, float* scales, const int32_t* table, int64_t
   p.interleaved = interleaved != 0;
   const int64_t pieces = int64_t(T) / page + B;
   LB2_CHECK_ARG(pieces < (int64_t(1) << 31), "kv8_compact: too many tokens");
-  p.hpb = 1;
   if (R % 16) return kv8_go(kv8::compact_any_kernel, dim3(unsigned(pieces), unsigned(2 * Hkv)), 128, static_cast<cudaStream_t>(stream), p);
-  // heads a block while every SM keeps two blocks: they share the block's start and the angles
-  while (p.hpb < 8 && pieces * 2 * ((Hkv + 2 * p.hpb - 1) / (2 * p.hpb)) >= 148 * 2) p.hpb *= 2;
-  return kv8_compact_run(p, D, page, dim3(unsigned(pieces), unsigned(2 * ((Hkv + p.hpb - 1) / p.hpb))), static_cast<cudaStream_t>(stream));
+  // planes a block: all of a page's where that leaves every SM eight blocks, fewer for small calls (1030 tokens of 8 heads x
+  // 128 leave 17 pages: a plane a block)
+  const int64_t want = std::max<int64_t>(1, std::min<int64_t>(2 * Hkv, (148 * 8 + pieces - 1) / pieces));
+  p.planes = int((2 * Hkv + want - 1) / want);
+  return kv8_compact_run(p, D, page, dim3(unsigned(pieces), unsigned((2 * Hkv + p.planes - 1) / p.planes)), static_cast<cudaStream_t>(stream));
 }
 
 // ------------------------------------------------------------------------------------------------ packed prompts
