@@ -202,6 +202,12 @@ __device__ __noinline__ float held_max(uint2 a, uint2 b, float f) {
   return m;
 }
 
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
 // Four codes times r, to the nearest codes.
 __device__ __forceinline__ uint32_t times(uint32_t c, __half2 r) {
   uint32_t lo, hi, x;
@@ -219,9 +225,10 @@ __device__ __forceinline__ uint32_t times(uint32_t c, __half2 r) {
 // heads, and the page's largest magnitude is found in between.
 // A block begins with a chain of four loads (bounds, positions, pages, codes), some 4 us, and needs few instructions after it:
 // what counts is the bytes in flight, so H planes' codes are asked for at once, and one barrier serves their maxima.
-template <int THREADS, int U, int H, int D, bool TURN>
-__global__ void __launch_bounds__(THREADS, U == 1 || !TURN ? 768 / THREADS : 1) compact_kernel(const CompactParams p) {
+template <int THREADS, int U, int H, int D, int LAYOUT>  // LAYOUT: 0 no turns, 1 halves, 2 interleaved
+__global__ void __launch_bounds__(THREADS, U == 1 || !LAYOUT ? 768 / THREADS : 1) compact_kernel(const CompactParams p) {
   constexpr int UPR = D / 16, WARPS = THREADS / 32;
+  constexpr bool TURN = LAYOUT != 0;
   __shared__ uint32_t red[2][H][WARPS];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   CompactPiece w;
@@ -235,16 +242,18 @@ __global__ void __launch_bounds__(THREADS, U == 1 || !TURN ? 768 / THREADS : 1) 
   if (!compact_page(p, w)) return;
   const uint8_t* src[U];  // the unit's codes of plane 0 (null: nothing to read)
   const float* sc[U];
-  int at[U], by[U];       // where the unit's first half lies in a plane; how far the second one is from it
+  int at[U], by[U];       // where the unit's first half lies in a plane of K; how far the second one is from it
+  int more[U];            // and how far on the unit lies in a plane of V
   bool live[U];
 #pragma unroll
   for (int i = 0; i < U; ++i) {
     const int x = i * THREADS + tid, t = x / UPR, q = x % UPR;
     live[i] = t < w.n;
-    const bool halves = q < turned && !p.interleaved;
+    const bool halves = LAYOUT == 1 && q < turned;
     const int d0 = halves ? 8 * q : 16 * q;
     by[i] = halves ? p.R / 2 : 8;
     at[i] = t * D + d0;
+    more[i] = 16 * q - d0;
     src[i] = nullptr;
     sc[i] = nullptr;
     if (live[i]) {
@@ -257,31 +266,26 @@ __global__ void __launch_bounds__(THREADS, U == 1 || !TURN ? 768 / THREADS : 1) 
   }
   uint2 c[H][U][2];
   float f[H][U];
-  float2 z[TURN ? U : 1][8];  // the unit's angles
-  // a turned unit's codes as values, turned (its scale is left out: a power of two)
-  auto values = [&](const uint2* x, int i, bool turn_it, float* y) {
+  float2 zc[TURN ? U : 1][4], zs[TURN ? U : 1][4];  // the unit's angles: cosines and sines of pairs 2 e, 2 e + 1
+  // a turned unit's codes as values, turned (its scale is left out: a power of two); in pairs y[e], y[4 + e] of what is turned
+  // together, each two neighbours
+  auto values = [&](const uint2* x, int i, bool turn_it, float2* y) {
+    uint32_t w[8];
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
+    for (int k = 0; k < 2; ++k) dec4(x[k].x, w[4 * k], w[4 * k + 1]), dec4(x[k].y, w[4 * k + 2], w[4 * k + 3]);
+    constexpr bool mixed = LAYOUT == 2;  // two neighbours are a pair
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        uint32_t lo, hi;
-        dec4(e ? x[k].y : x[k].x, lo, hi);
-        const float2 a = half2_f(lo), b = half2_f(hi);
-        float* o = y + 8 * k + 4 * e;
-        o[0] = a.x, o[1] = a.y, o[2] = b.x, o[3] = b.y;
-      }
+    for (int e = 0; e < 4; ++e) {
+      const float2 a = half2_f(w[mixed ? 2 * e : e]), b = half2_f(w[mixed ? 2 * e + 1 : 4 + e]);
+      y[e] = mixed ? make_float2(a.x, b.x) : a;
+      y[4 + e] = mixed ? make_float2(a.y, b.y) : b;
+    }
     if (!TURN || !turn_it || (i * THREADS + tid) % UPR >= turned) return;
-    auto turn = [](float& a, float& b, float2 r) {
-      const float x = a;
-      a = x * r.x - b * r.y;
-      b = b * r.x + x * r.y;
-    };
-    if (p.interleaved) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) turn(y[2 * e], y[2 * e + 1], z[TURN ? i : 0][e]);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) turn(y[e], y[8 + e], z[TURN ? i : 0][e]);
+    for (int e = 0; e < 4; ++e) {
+      const float2 c = zc[TURN ? i : 0][e], s = zs[TURN ? i : 0][e], a = y[e], b = y[4 + e];
+      y[e] = fma2(a, c, mul2(b, make_float2(-s.x, -s.y)));
+      y[4 + e] = fma2(b, c, mul2(a, s));
     }
   };
   int round = 0;
@@ -295,9 +299,8 @@ __global__ void __launch_bounds__(THREADS, U == 1 || !TURN ? 768 / THREADS : 1) 
         f[h][i] = 0.f;
         if (src[i] && l + h < l1) {
           // (K's planes hold units as they are turned, V's 16 dims in a row)
-          const int64_t o = int64_t(l + h) * head;
-          const bool v = l + h >= p.Hkv && by[i] != 8;
-          const uint8_t* x = src[i] + o + (v ? (at[i] % D) : 0);
+          const bool v = l + h >= p.Hkv;
+          const uint8_t* x = src[i] + int64_t(l + h) * head + (v ? more[i] : 0);
           c[h][i][0] = *reinterpret_cast<const uint2*>(x);
           c[h][i][1] = *reinterpret_cast<const uint2*>(x + (v ? 8 : by[i]));
           f[h][i] = sc[i][l + h];
@@ -310,7 +313,10 @@ __global__ void __launch_bounds__(THREADS, U == 1 || !TURN ? 768 / THREADS : 1) 
         if (!live[i] || q >= turned) continue;
         const uint64_t shift = uint64_t(w.first + x / UPR - pos[i]);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) z[TURN ? i : 0][e] = quarter_cs(shift * p.turns[8 * q + e]);
+        for (int e = 0; e < 4; ++e) {
+          const float2 a = quarter_cs(shift * p.turns[8 * q + 2 * e]), b = quarter_cs(shift * p.turns[8 * q + 2 * e + 1]);
+          zc[TURN ? i : 0][e] = make_float2(a.x, b.x), zs[TURN ? i : 0][e] = make_float2(a.y, b.y);
+        }
       }
     }
 #pragma unroll
@@ -321,23 +327,24 @@ __global__ void __launch_bounds__(THREADS, U == 1 || !TURN ? 768 / THREADS : 1) 
       for (int i = 0; i < U; ++i) {
         float mi = 0.f;
         if (turn_it) {
-          float y[16];
+          float2 y[8];
           values(c[h][i], i, true, y);
 #pragma unroll
-          for (int e = 0; e < 16; e += 2) mi = max3_abs(mi, y[e], y[e + 1]);  // (NaN is passed over)
-        } else {  // codes as they lie: in f16, two a step
-          __half2 m2 = __float2half2_rn(0.f);
+          for (int e = 0; e < 8; ++e) mi = max3_abs(mi, y[e].x, y[e].y);  // (NaN is passed over)
+        } else {  // codes rise with their magnitudes
+          uint32_t m2 = 0;
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            uint32_t x[2];
-            const uint2 u = c[h][i][k >> 1];
-            dec4(k & 1 ? u.y : u.x, x[0], x[1]);
-            m2 = __hmax2(m2, __hmax2(__habs2(*reinterpret_cast<__half2*>(&x[0])), __habs2(*reinterpret_cast<__half2*>(&x[1]))));
+            const uint32_t u = k & 1 ? c[h][i][k >> 1].y : c[h][i][k >> 1].x;
+            m2 = max_u16x2(m2, max_u16x2(u & 0x7f007f00u, u << 8 & 0x7f007f00u));
           }
-          mi = fmaxf(__low2float(m2), __high2float(m2));
+          const uint32_t top = max(m2 >> 16, m2 & 0xffffu);
+          uint32_t lo, hi;
+          dec4(top >> 8, lo, hi);
+          mi = top == 0x7f00u ? INFINITY : half2_f(lo).x;  // (NaN codes: looked at again)
         }
         mi *= f[h][i];
-        if (!(mi < INFINITY)) mi = held_max(c[h][i][0], c[h][i][1], f[h][i]);  // rare: held infinities near fp32's end
+        if (!(mi < INFINITY)) mi = held_max(c[h][i][0], c[h][i][1], f[h][i]);  // rare: NaN, or infinities near fp32's end
         m = fmaxf(m, mi);
       }
       const uint32_t wm = __reduce_max_sync(0xffffffffu, __float_as_uint(m));
@@ -361,21 +368,32 @@ __global__ void __launch_bounds__(THREADS, U == 1 || !TURN ? 768 / THREADS : 1) 
         const float r = f[h][i] * inv;  // what the codes are multiplied by
         uint2 e[2];
         if (turn_it || !(r <= 32768.f) || (__float_as_uint(f[h][i]) & 0x7fffffu) != 0) {
-          float v[16];
-          values(c[h][i], i, turn_it, v);
+          float2 y[8];
+          values(c[h][i], i, turn_it, y);
+          const float2 r2 = make_float2(r, r);
 #pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const float* x = v + 8 * k;
-            e[k] = make_uint2(enc4(x[0] * r, x[1] * r, x[2] * r, x[3] * r), enc4(x[4] * r, x[5] * r, x[6] * r, x[7] * r));
+          for (int e = 0; e < 8; ++e) y[e] = mul2(y[e], r2);
+          if (LAYOUT == 2) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+              e[k] = make_uint2(enc4(y[2 * k].x, y[4 + 2 * k].x, y[2 * k].y, y[4 + 2 * k].y),
+                                enc4(y[2 * k + 1].x, y[5 + 2 * k].x, y[2 * k + 1].y, y[5 + 2 * k].y));
+          } else {
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+              e[k] = make_uint2(enc4(y[4 * k].x, y[4 * k].y, y[4 * k + 1].x, y[4 * k + 1].y),
+                                enc4(y[4 * k + 2].x, y[4 * k + 2].y, y[4 * k + 3].x, y[4 * k + 3].y));
           }
+        } else if (r == 1.f) {
+          e[0] = c[h][i][0], e[1] = c[h][i][1];
         } else {
           // a power of two times a code in f16: exact down to 2^-21, and below 2^-10 every code is 0
           const __half2 r2 = __float2half2_rn(r);
 #pragma unroll
           for (int k = 0; k < 2; ++k) e[k] = make_uint2(times(c[h][i][k].x, r2), times(c[h][i][k].y, r2));
         }
-        const bool v = l + h >= p.Hkv && by[i] != 8;
-        const int o = at[i] + (v ? at[i] % D : 0);
+        const bool v = l + h >= p.Hkv;
+        const int o = at[i] + (v ? more[i] : 0);
         *reinterpret_cast<uint2*>(out + o) = e[0];
         *reinterpret_cast<uint2*>(out + o + (v ? 8 : by[i])) = e[1];
       }

@@ -1984,14 +1984,14 @@ static int kv8_compact_run(const kv8::CompactParams& p, int D, int page, dim3 gr
   const int units = page * D / 16;  // 64 .. 2048, a thread each up to 512
   auto go = [&](auto d, auto t) {
     constexpr int N = decltype(d)::value;
-    constexpr bool TURN = decltype(t)::value;
+    constexpr int L = decltype(t)::value;
     switch (units) {
-      case 64: return kv8_go(kv8::compact_kernel<64, 1, 4, N, TURN>, grid, 64, st, p);
-      case 128: return kv8_go(kv8::compact_kernel<128, 1, 4, N, TURN>, grid, 128, st, p);
-      case 256: return kv8_go(kv8::compact_kernel<256, 1, 4, N, TURN>, grid, 256, st, p);
-      case 512: return kv8_go(kv8::compact_kernel<256, 2, 2, N, TURN>, grid, 256, st, p);
-      case 1024: return kv8_go(kv8::compact_kernel<512, 2, 2, N, TURN>, grid, 512, st, p);
-      default: return kv8_go(kv8::compact_kernel<512, 4, 1, N, TURN>, grid, 512, st, p);
+      case 64: return kv8_go(kv8::compact_kernel<64, 1, 4, N, L>, grid, 64, st, p);
+      case 128: return kv8_go(kv8::compact_kernel<128, 1, 4, N, L>, grid, 128, st, p);
+      case 256: return kv8_go(kv8::compact_kernel<256, 1, 4, N, L>, grid, 256, st, p);
+      case 512: return kv8_go(kv8::compact_kernel<256, 2, 2, N, L>, grid, 256, st, p);
+      case 1024: return kv8_go(kv8::compact_kernel<512, 2, 2, N, L>, grid, 512, st, p);
+      default: return kv8_go(kv8::compact_kernel<512, 4, 1, N, L>, grid, 512, st, p);
     }
   };
   auto by_dim = [&](auto t) {
@@ -1999,7 +1999,8 @@ static int kv8_compact_run(const kv8::CompactParams& p, int D, int page, dim3 gr
            : D == 128 ? go(std::integral_constant<int, 128>(), t)
                       : go(std::integral_constant<int, 256>(), t);
   };
-  return p.R ? by_dim(std::true_type()) : by_dim(std::false_type());
+  return !p.R ? by_dim(std::integral_constant<int, 0>())
+              : p.interleaved ? by_dim(std::integral_constant<int, 2>()) : by_dim(std::integral_constant<int, 1>());
 }
 
 extern "C" {
