@@ -52,6 +52,7 @@ constexpr int CONV_WARP = 8, CONV_WARPS = 8, MMA_WARP = 16, TABLE_WARP = 17, PLA
 constexpr int CT = CONV_WARPS * 32;  // threads that turn codes into operands
 constexpr int PIECES = 4;          // pieces of work listed ahead
 constexpr int TABLES = 8;          // key tiles whose page ids and scales are held
+constexpr uint32_t WHOLE = 256;    // a tile whose 128 keys are all there
 constexpr float TOP = 7.f;         // a weight at the running maximum is 2^TOP
 constexpr int STATUS = arows::STATUS_CHUNK;  // lb2_status: 140 lengths and page ids, 141.. waits
 
@@ -296,6 +297,13 @@ __device__ __forceinline__ void mma_commit(uint32_t lead, uint64_t* bar) {
 __device__ __forceinline__ float shrink(float l, float x) {
   const float h = prefill::ex2f(0.5f * x);
   return l * h * h;
+}
+
+// 16 bytes of codes. (volatile: the loads stay ahead of the wait behind them)
+__device__ __forceinline__ uint4 ld_codes(const uint8_t* p) {
+  uint4 x;
+  asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "l"(p));
+  return x;
 }
 
 // 16 bytes, or zeros where they are not wanted, without a branch.
@@ -659,6 +667,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
           const bool apart = held && vl < fmaxf(-100.f, hi - 64.f);
           const float4 f = make_float4(cks, fmaxf(vl, -100.f), apart ? 0.f : exp2f(-fmaxf(vl, -100.f)), vl);
           const uint32_t marked = __ballot_sync(0xffffffffu, apart);
+          const uint32_t whole = __ballot_sync(0xffffffffu, held && key0 + t * BN + lane * 16 + 15 < horizon);
           const int pg = __shfl_sync(0xffffffffu, cid, (lane & 24) | ((lane & 7) * 8 / per & 7));  // the tile's page lane % 8
           for (int j = 0; j < min(4, nt - t); ++j, ++g) {
             const int s = g % TABLES;
@@ -668,7 +677,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
             if (lane >> 3 == j) {
               tab[s * 8 + (lane & 7)] = f;
               if ((lane & 7) < per) at_s[s * 8 + (lane & 7)] = pg < 0 ? -1 : (int64_t(pg) * 2 * p.c.a.Hkv + hk) * (D << p.lpage);
-              if ((lane & 7) == 0) far_s[s] = marked >> (8 * j) & 255u;
+              if ((lane & 7) == 0) far_s[s] = (marked >> (8 * j) & 255u) | ((whole >> (8 * j) & 255u) == 255u ? WHOLE : 0u);
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(&tab_full[s]);
@@ -680,19 +689,14 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
   } else if (warp >= CONV_WARP) {
     // ------------------------------------------------------------------------------------ codes into operand tiles
     reg_dec<72>();
-    constexpr int UPR = C::DS / 16;       // 16-code units a key and stage
-    constexpr int LD = BN * UPR / 128;    // units a thread and stage
-    constexpr int RSTEP = 128 / UPR;      // keys between a thread's units
-    const int tid = threadIdx.x - CONV_WARP * 32, ti = tid & 127, u = ti % UPR, r0 = ti / UPR;
+    // A thread takes units of 16 codes: unit ul + 4 h of keys r0, r0 + 32, .. Eight lanes that store 16 bytes each then fill 128:
+    // four units of two keys, whose swizzles are apart.
+    constexpr int UH = C::DS / 64, LD = 4 * UH;  // 64-dim boxes, units a thread and stage
+    const int tid = threadIdx.x - CONV_WARP * 32, ul = tid & 3, r0 = (tid & 127) >> 2;
     const int group = tid >> 7;  // the two warpgroups take the stages in turn
     const int page = 1 << p.lpage;
     const int64_t kv_off = int64_t(p.c.a.Hkv) * (D << p.lpage);  // from a page's K to its V
-    // where the thread's unit of key r0 goes in a stage, its two 16-byte halves ordered so that eight lanes fill 128 bytes
-    const int swap = UPR == 8 ? u >> 2 : 0;
-    const uint32_t box = uint32_t(u >> 2) * (BN * 128);
-    const uint32_t c0 = (((2 * (u & 3) + swap) ^ (r0 & 7)) << 4), c1 = (((2 * (u & 3) + 1 - swap) ^ (r0 & 7)) << 4);
-    const uint32_t dst0 = box + r0 * 128 + c0, dst1 = box + r0 * 128 + c1;  // (RSTEP is a multiple of 8)
-    static_assert(RSTEP % 8 == 0, "the swizzle of a thread's rows is one");
+    const uint32_t dst0 = r0 * 128 + ((2 * ul ^ (r0 & 7)) << 4), dst1 = r0 * 128 + (((2 * ul + 1) ^ (r0 & 7)) << 4);
     int pieces = 0, g = 0, gt = 0;  // pieces, stages and tiles so far
     bool ok = true;
     while (ok && piece(pieces)) {
@@ -774,14 +778,26 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
           tabs = t + 1;
         }
         const int end = ok ? horizon - (kt0 + t) * BN : 0;  // keys of the tile that some row sees
-        const uint8_t* from = p.c.a.pages + kind * kv_off + (s % SPT) * C::DS + u * 16;
+        const uint8_t* from = p.c.a.pages + kind * kv_off + (s % SPT) * C::DS + ul * 16;
         const int64_t* at = at_s + slot * 8;
-        uint4 x[LD];
+        const uint8_t* x0[4];
 #pragma unroll
-        for (int i = 0; i < LD; ++i) {
-          const int r = r0 + i * RSTEP;
-          const int64_t o = at[r >> p.lpage];
-          x[i] = load_if(from + o + (r & (page - 1)) * D, o >= 0 && r < end);
+        for (int k = 0; k < 4; ++k) {
+          const int r = r0 + 32 * k;
+          x0[k] = from + at[r >> p.lpage] + (r & (page - 1)) * D;
+        }
+        uint4 x[LD];
+        if (ok && (far_s[slot] & WHOLE)) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int h = 0; h < UH; ++h) x[k * UH + h] = ld_codes(x0[k] + 64 * h);
+        } else {  // the tile's last keys, or a page that is none, are zeros
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int h = 0; h < UH; ++h)
+              x[k * UH + h] = load_if(x0[k] + 64 * h, r0 + 32 * k < end && at[(r0 + 32 * k) >> p.lpage] >= 0);
         }
         if (kind == 1) {  // the tile's places have been used
           __syncwarp();
@@ -791,15 +807,18 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
         if (ok && gs >= NS) ok = wait_or_abort(&empty[st], ((gs / NS) - 1) & 1, abort_flag, 150);
         uint8_t* d = sm + C::K_OFF + st * C::STAGE;
 #pragma unroll
-        for (int i = 0; i < LD; ++i) {
-          uint4 a, b;
-          kv8::dec4(swap ? x[i].z : x[i].x, a.x, a.y);
-          kv8::dec4(swap ? x[i].w : x[i].y, a.z, a.w);
-          kv8::dec4(swap ? x[i].x : x[i].z, b.x, b.y);
-          kv8::dec4(swap ? x[i].y : x[i].w, b.z, b.w);
-          *reinterpret_cast<uint4*>(d + dst0 + i * RSTEP * 128) = a;
-          *reinterpret_cast<uint4*>(d + dst1 + i * RSTEP * 128) = b;
-        }
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int h = 0; h < UH; ++h) {
+            const uint4 c = x[k * UH + h];
+            uint4 a, b;
+            kv8::dec4(c.x, a.x, a.y);
+            kv8::dec4(c.y, a.z, a.w);
+            kv8::dec4(c.z, b.x, b.y);
+            kv8::dec4(c.w, b.z, b.w);
+            *reinterpret_cast<uint4*>(d + dst0 + h * (BN * 128) + k * (32 * 128)) = a;
+            *reinterpret_cast<uint4*>(d + dst1 + h * (BN * 128) + k * (32 * 128)) = b;
+          }
         fence_proxy_async_shared();
         __syncwarp();
         if (lane == 0) mbar_arrive(&full[st]);
@@ -858,43 +877,33 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
           prefill::tmem_st16(s_col + c, reinterpret_cast<const uint32_t*>(x));
           prefill::tmem_wait_st();
         }
-        // the row's largest score with the values' scale (a factor is never 0: -inf times it stays -inf)
         if (i < 2) fac = fac_s[(pieces & 1) * RB + row];
         const float4* sc = tab + slot * 8 + half * 4;
-        float top = -INFINITY, s[BH];
-        auto largest = [&](const float* x, int q) {
-          const float2 f = *reinterpret_cast<const float2*>(sc + q);
-          float a = max3(x[0], x[1], x[2]), b = max3(x[3], x[4], x[5]);
-          a = max3(a, x[6], x[7]), b = max3(b, x[8], x[9]);
-          a = max3(a, x[10], x[11]), b = max3(b, x[12], x[13]);
-          a = max3(a, x[14], x[15]);
-          top = fmaxf(top, fmaf(fmaxf(a, b), fmaxf(fac * f.x, FLT_MIN), f.y));
-        };
+        float s[BH];
         prefill::tmem_ld32(s_col, s);
         prefill::tmem_ld32(s_col + 32, s + 32);
         wait_ld32(s);
         wait_ld32(s + 32);
+        // The row's largest score with the values' scale (a factor is never 0: -inf times it stays -inf).
+        auto largest = [&] {
+          float top = -INFINITY;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) largest(s + 16 * q, q);
-        bool began;  // O holds something
-        if constexpr (C::WIDE) {
-          began = i > 0;
-          if (i > 0) {  // the maximum after the unit before
-            if (ok) ok = wait_or_abort(&token[(1 - wg) * 4 + quarter], (done + ((i - 1) >> 1)) & 1, abort_flag, 152);
-            const float now = m_sh[r];
-            if (now != m) {
-              l = shrink(l, m - now);
-              m = now;
-            }
+          for (int q = 0; q < 4; ++q) {
+            const float2 f = *reinterpret_cast<const float2*>(sc + q);
+            const float* x = s + 16 * q;
+            float a = max3(x[0], x[1], x[2]), b = max3(x[3], x[4], x[5]);
+            a = max3(a, x[6], x[7]), b = max3(b, x[8], x[9]);
+            a = max3(a, x[10], x[11]), b = max3(b, x[12], x[13]);
+            a = max3(a, x[14], x[15]);
+            top = fmaxf(top, fmaf(fmaxf(a, b), fmaxf(fac * f.x, FLT_MIN), f.y));
           }
-        } else {
-          began = i > 1;
-        }
-        const bool move = top > m + (TOP + 8.f);
-        if (__any_sync(0xffffffffu, move)) {
-          const float now = move ? top - TOP : m, corr = move ? prefill::ex2f(m - now) : 1.f;
-          if (began) {
-            if (ok) ok = pv_done(i - (C::WIDE ? 1 : 2));
+          return top;
+        };
+        // The maximum moves to `now`: what was summed against the old one follows. `prev`: the unit whose P V must be done.
+        auto move_to = [&](float now, int prev) {
+          const float corr = prefill::ex2f(m - now);
+          if (prev >= 0) {  // O holds something
+            if (ok) ok = pv_done(prev);
             ok = __all_sync(0xffffffffu, ok);
             prefill::tc_fence_after();
 #pragma unroll 1
@@ -910,20 +919,22 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
           }
           l = shrink(l, m - now);
           m = now;
+        };
+        const float top = largest();
+        if (C::WIDE && i > 0) {  // the maximum after the unit before
+          if (ok) ok = wait_or_abort(&token[(1 - wg) * 4 + quarter], (done + ((i - 1) >> 1)) & 1, abort_flag, 152);
+          const float now = m_sh[r];
+          if (now != m) {
+            l = shrink(l, m - now);
+            m = now;
+          }
         }
-        if constexpr (C::WIDE) {
+        const bool move = top > m + (TOP + 8.f);
+        if (__any_sync(0xffffffffu, move)) move_to(move ? top - TOP : m, i - (C::WIDE ? 1 : 2));
+        if (C::WIDE) {
           m_sh[r] = m;
           __syncwarp();
           if (lane == 0) mbar_arrive(&token[wg * 4 + quarter]);
-        }
-        for (uint32_t marked = far_s[slot] >> (4 * half) & 15u; marked; marked &= marked - 1) {  // (rare)
-          const int q = __ffs(marked) - 1;
-          const float mul = fmaxf(fac * sc[q].x, FLT_MIN);
-          float x[16];
-          prefill2::tmem_ld16(s_col + 16 * q, x);
-          prefill::tmem_wait_ld();
-#pragma unroll
-          for (int e = 0; e < 16; ++e) l += prefill::ex2f(fmaf(x[e], mul, -m));
         }
         // weights; P_i takes the place of S_i
         uint32_t pk[32];
@@ -940,6 +951,15 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
             pk[8 * q + e / 2] = pack2<__half>(y.x, y.y);
           }
           l = fmaf(sum.x + sum.y, f.z, l);
+        }
+        for (uint32_t marked = far_s[slot] >> (4 * half) & 15u; marked; marked &= marked - 1) {  // (rare)
+          const int q = __ffs(marked) - 1;
+          const float mul = fmaxf(fac * sc[q].x, FLT_MIN);
+          float x[16];
+          prefill2::tmem_ld16(s_col + 16 * q, x);
+          prefill::tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 16; ++e) l += prefill::ex2f(fmaf(x[e], mul, -m));
         }
         prefill::tmem_st32(s_col, reinterpret_cast<const float*>(pk));
         prefill::tmem_wait_st();

@@ -226,7 +226,7 @@ __device__ __forceinline__ uint32_t times(uint32_t c, __half2 r) {
 // A block begins with a chain of four loads (bounds, positions, pages, codes), some 4 us, and needs few instructions after it:
 // what counts is the bytes in flight, so H planes' codes are asked for at once, and one barrier serves their maxima.
 template <int THREADS, int U, int H, int D, int LAYOUT>  // LAYOUT: 0 no turns, 1 halves, 2 interleaved
-__global__ void __launch_bounds__(THREADS, U == 1 || !LAYOUT ? 768 / THREADS : 1) compact_kernel(const CompactParams p) {
+__global__ void __launch_bounds__(THREADS, !LAYOUT ? 1024 / THREADS : U == 1 ? 768 / THREADS : 1) compact_kernel(const CompactParams p) {
   constexpr int UPR = D / 16, WARPS = THREADS / 32;
   constexpr bool TURN = LAYOUT != 0;
   __shared__ uint32_t red[2][H][WARPS];
