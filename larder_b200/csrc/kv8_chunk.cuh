@@ -350,17 +350,18 @@ __device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, vo
 // The second look at folded row f of an item, by one warp: where its output has NaN columns and one of the keys behind it that
 // its item's products took holds a NaN there, the row again, reading only what it sees.
 template <typename T, int D>
-__device__ __noinline__ void row_again(const Params& p, int b, int lo, int n, int len, int hk, int f, int horizon) {
+__device__ __noinline__ void row_again(const Params& p, int b, int lo, int n, int len, int hk, int f, int horizon, int c0, int c1) {
   constexpr int E = D / 32;
   const arows::PagedParams& a = p.c.a;
   const int lane = threadIdx.x & 31, t = f / p.G, h = hk * p.G + f % p.G;
+  const bool mine = lane * E >= c0 && lane * E < c1;  // columns c0 .. c1 - 1
   const int seen = a.causal ? max(len - (n - 1 - t), 0) : len;
   T* o = static_cast<T*>(a.o) + h * a.o_st[1] + int64_t(lo + t) * a.o_st[2] + lane * E;
   bool bad[E], any = false;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     const float x = to_f<T>(o[e]);
-    any |= bad[e] = x != x;
+    any |= bad[e] = mine && x != x;
   }
   if (!__any_sync(0xffffffffu, any)) return;
   arows::PagedKeys<E> keys{a.pages, a.scales, a.table + b * a.table_st, a.Hkv, hk, a.page, a.num_pages, lane * E};
@@ -378,7 +379,8 @@ __device__ __noinline__ void row_again(const Params& p, int b, int lo, int n, in
   for (int e = 0; e < E; ++e) x[e] = to_f<T>(q[e]);
   arows::attend_row<E>(keys, seen, a.scale, x);
 #pragma unroll
-  for (int e = 0; e < E; ++e) o[e] = from_f<T>(x[e]);
+  for (int e = 0; e < E; ++e)
+    if (mine) o[e] = from_f<T>(x[e]);
 }
 
 // 32 output values of a row, in the widest stores that its alignment allows.
@@ -1046,7 +1048,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
       Piece y;
       while (sched.next(y))
         for (int x = warp; y.whole && x < y.rows; x += CONV_WARP)
-          row_again<T, D>(p, y.b, y.lo, y.n, y.len, y.hk, y.f0 + x, y.horizon);
+          row_again<T, D>(p, y.b, y.lo, y.n, y.len, y.hk, y.f0 + x, y.horizon, 0, D);
     }
   }
 
@@ -1058,58 +1060,61 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
   }
 }
 
-// Merges an item's parts: block (CTA that begins it, 32 of its rows), a lane a row, the warps sharing the columns.
+// Merges an item's parts: a block for the CTA that begins it and 16 pieces of 32 rows x 32 columns, a warp each, a lane a row.
+// Two parts' loads are in flight at once. (A block a piece, with the parts shared by its warps, took 18 to 40 us a call: most
+// of the many blocks have nothing to do.)
+constexpr int COMBINE_WARPS = 16;
+
 template <typename T, int D>
-__global__ void __launch_bounds__(128) combine_kernel(const Params p) {
+__global__ void __launch_bounds__(COMBINE_WARPS * 32) combine_kernel(const Params p) {
   constexpr int RB = Cfg<D>::RB;
-  __shared__ float s_m[4][32], s_l[4][32];
-  __shared__ int s_nan;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int4 a = p.rec[2 * blockIdx.x], e4 = p.rec[2 * blockIdx.x + 1];
-  const int parts = a.x, r0 = blockIdx.y * 32, rows = e4.w;
+  const int lane = threadIdx.x & 31, task = blockIdx.y * COMBINE_WARPS + (threadIdx.x >> 5);
+  const int parts = a.x, r0 = task / (D / 32) * 32, c0 = task % (D / 32) * 32, rows = e4.w, row = r0 + lane;
   if (parts == 0 || r0 >= rows) return;
-  if (threadIdx.x == 0) s_nan = 0;
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, row = r0 + lane;
+  const float* ml = p.ws_ml + row;
+  const float* ws = p.ws_o + int64_t(c0) * RB + row;
   auto slot = [&](int i) { return i == 0 ? 2 * int64_t(blockIdx.x) + 1 : 2 * (int64_t(blockIdx.x) + i); };
-  // the row's maximum and sum: the warps share the parts
-  float M = -FLT_MAX, L = 0.f;
-  for (int i = w; i < parts; i += 4) M = fmaxf(M, p.ws_ml[slot(i) * 2 * RB + row]);
-  s_m[w][lane] = M;
-  __syncthreads();
-  M = fmaxf(fmaxf(s_m[0][lane], s_m[1][lane]), fmaxf(s_m[2][lane], s_m[3][lane]));
-  for (int i = w; i < parts; i += 4)
-    L += shrink(p.ws_ml[slot(i) * 2 * RB + RB + row], p.ws_ml[slot(i) * 2 * RB + row] - M);
-  s_l[w][lane] = L;
-  __syncthreads();
-  L = (s_l[0][lane] + s_l[1][lane]) + (s_l[2][lane] + s_l[3][lane]);
+  float M = -FLT_MAX, L = 0.f, x[32];
+#pragma unroll
+  for (int e = 0; e < 32; ++e) x[e] = 0.f;
+  for (int i = 0; i < parts; i += 2) {
+    float y[2][32], m[2], l[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int64_t s = slot(min(i + k, parts - 1));
+      m[k] = ml[s * 2 * RB], l[k] = ml[s * 2 * RB + RB];
+#pragma unroll
+      for (int e = 0; e < 32; ++e) y[k][e] = ws[s * (D * RB) + e * RB];
+    }
+    if (i + 1 == parts) m[1] = -FLT_MAX, l[1] = 0.f;
+    const float now = fmaxf(M, fmaxf(m[0], m[1]));
+    const float f = prefill::ex2f(M - now), g0 = prefill::ex2f(m[0] - now);
+    const float g1 = i + 1 == parts ? 0.f : prefill::ex2f(m[1] - now);
+    L = shrink(L, M - now) + shrink(l[0], m[0] - now) + shrink(l[1], m[1] - now);
+    M = now;
+#pragma unroll
+    for (int e = 0; e < 32; ++e) x[e] = fmaf(y[0][e], g0, x[e] * f);
+    if (i + 1 < parts)
+#pragma unroll
+      for (int e = 0; e < 32; ++e) x[e] = fmaf(y[1][e], g1, x[e]);
+  }
   const float inv = L > 0.f || L != L ? 1.f / L : 0.f;
   const int f = e4.z + row, tok = f / p.G;
-  T* out = static_cast<T*>(p.c.a.o) + int64_t(e4.y * p.G + f % p.G) * p.c.a.o_st[1] + int64_t(a.z + tok) * p.c.a.o_st[2];
-  const bool live = row < rows;
-  for (int c = w * 32; c < D; c += 128) {
-    float x[32];
+  float sum = 0.f;  // (finite unless some value is not)
 #pragma unroll
-    for (int e = 0; e < 32; ++e) x[e] = 0.f;
-    for (int i = 0; live && i < parts; ++i) {
-      const float g = prefill::ex2f(p.ws_ml[slot(i) * 2 * RB + row] - M);
-      const float* src = p.ws_o + slot(i) * (D * RB) + row;
-#pragma unroll
-      for (int e = 0; e < 32; ++e) x[e] = fmaf(src[(c + e) * RB], g, x[e]);
-    }
-    float sum = 0.f;
-#pragma unroll
-    for (int e = 0; e < 32; ++e) sum = fmaf(x[e], 0.f, sum);
-    if (live) {
-      if (sum != sum && L == L) s_nan = 1;
-      store32<T>(out + c, x, inv, p.wide_o);
-    }
-  }
-  __syncthreads();
-  if (!s_nan) return;
-  const Range x{a.z, a.w, e4.x};
-  const Block b = block_of<RB>(p, x, e4.z / RB);
-  for (int i = r0 + w; i < min(r0 + 32, rows); i += 4) row_again<T, D>(p, a.y, a.z, a.w, e4.x, e4.y, e4.z + i, b.horizon);
+  for (int e = 0; e < 32; ++e) sum = fmaf(x[e], 0.f, sum);
+  if (row < rows)
+    store32<T>(static_cast<T*>(p.c.a.o) + int64_t(e4.y * p.G + f % p.G) * p.c.a.o_st[1] + int64_t(a.z + tok) * p.c.a.o_st[2] + c0, x,
+               inv, p.wide_o);
+  uint32_t nan = __ballot_sync(0xffffffffu, row < rows && sum != sum && L == L);
+  if (nan == 0) return;
+  __syncwarp();
+  const Block b = block_of<RB>(p, Range{a.z, a.w, e4.x}, e4.z / RB);
+  for (; nan; nan &= nan - 1)
+    row_again<T, D>(p, a.y, a.z, a.w, e4.x, e4.y, e4.z + r0 + __ffs(nan) - 1, b.horizon, c0, c0 + 32);
 }
 
 }  // namespace kv8chunk

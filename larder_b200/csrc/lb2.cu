@@ -1870,8 +1870,8 @@ static int launch(const Params& p, int grid, cudaStream_t st) {
   cfg.attrs = pdl;
   cfg.numAttrs = 1;
   LB2_CUDA(cudaLaunchKernelEx(&cfg, chunk_kernel<T, D>, p));
-  cfg.gridDim = dim3(static_cast<unsigned>(grid), C::RB / 32);
-  cfg.blockDim = dim3(128);
+  cfg.gridDim = dim3(static_cast<unsigned>(grid), C::RB / 32 * (D / 32) / COMBINE_WARPS);
+  cfg.blockDim = dim3(COMBINE_WARPS * 32);
   cfg.dynamicSmemBytes = 0;
   LB2_CUDA(cudaLaunchKernelEx(&cfg, combine_kernel<T, D>, p));
   return LB2_OK;
