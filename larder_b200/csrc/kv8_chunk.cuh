@@ -150,17 +150,28 @@ template <int RB>
 struct Sched {
   const Params& p;
   const int64_t* prefix;
-  int64_t total, runs, at, p0, p1;  // at: the current item's first unit; [p0, p1): the CTA's run
+  int64_t each, at, p0, p1;  // units a run; the current item's first unit; the CTA's run [p0, p1)
+  int more;                  // the first so many runs have one unit more
   int r, hk, k, nb;
   Range x;
 
-  __device__ __forceinline__ int64_t cut(int64_t c) const { return c * total / runs; }
+  __device__ __forceinline__ int64_t cut(int c) const { return c * each + min(c, more); }
+  // The run of a unit.
+  __device__ __forceinline__ int run_of(int64_t u) const {
+    const int64_t first = more * (each + 1);
+    return int(u < first ? div(u, each + 1) : more + div(u - first, each));
+  }
+  // (64-bit divisions take a few hundred clocks: they are kept for calls that need them)
+  static __device__ __forceinline__ int64_t div(int64_t a, int64_t b) {
+    return ((a | b) >> 32) == 0 ? int64_t(uint32_t(a) / uint32_t(b)) : a / b;
+  }
 
   __device__ __noinline__ Sched(const Params& p_, const int64_t* prefix_) : p(p_), prefix(prefix_) {
     const int NR = p.c.a.B + 2, lane = threadIdx.x & 31;
-    total = prefix[NR];
-    runs = max(int64_t(1), min(int64_t(gridDim.x), total / p.min_units));
-    const int64_t c = blockIdx.x;
+    const int64_t total = prefix[NR];
+    const int runs = int(max(int64_t(1), min(int64_t(gridDim.x), div(total, p.min_units)))), c = blockIdx.x;
+    each = div(total, runs);
+    more = int(total - each * runs);
     p0 = c < runs ? cut(c) : 0;
     p1 = c < runs ? cut(c + 1) : 0;
     r = hk = k = nb = 0;
@@ -172,9 +183,9 @@ struct Sched {
       if (prefix[mid] <= p0) lo = mid; else hi = mid;
     }
     enter(lo);
-    const int64_t each = (prefix[r + 1] - prefix[r]) / p.c.a.Hkv;
-    hk = int((p0 - at) / each);
-    at += hk * each;
+    const int64_t of_head = div(prefix[r + 1] - prefix[r], p.c.a.Hkv);
+    hk = int(div(p0 - at, of_head));
+    at += hk * of_head;
     for (int k0 = 0; k0 < nb; k0 += 32) {  // 32 blocks at a time
       const int own = k0 + lane < nb ? block_of<RB>(p, x, k0 + lane).units : 0;
       int64_t sum = own;
@@ -214,7 +225,7 @@ struct Sched {
       w.whole = a == 0 && z == b.units;
       w.slot = 2 * int(blockIdx.x) + (a == 0 ? 1 : 0);
       w.nparts = 0;
-      if (a == 0 && !w.whole) w.nparts = int(((at + b.units) * runs - 1) / total) - int(blockIdx.x) + 1;
+      if (a == 0 && !w.whole) w.nparts = run_of(at + b.units - 1) - int(blockIdx.x) + 1;
       at += b.units;
       if (++k == nb) {
         k = 0;
@@ -713,54 +724,69 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
         constexpr int RPP = CT / LPR;       // rows a pass
         constexpr int HOLD = 4;             // passes whose loads are in flight
         const int qr = tid / LPR, qc = tid % LPR;
-        const int tiles = pair ? 2 * BM : BM;
-        const uint32_t boxq = uint32_t(qc >> 3) * (BM * 128);
+        const int rows = w.rows, tiles = pair ? 2 * BM : BM;
+        const uint32_t dq = uint32_t(qc >> 3) * (BM * 128) + (((qc & 7) ^ (qr & 7)) << 4);  // (RPP is a multiple of 8)
+        // the thread's row as (token, query head), stepped from pass to pass
+        const int st = RPP / p.G, sg = RPP % p.G;
+        int tq = (w.f0 + qr) / p.G, gq = (w.f0 + qr) % p.G;
         const T* qh = static_cast<const T*>(p.c.a.q) + int64_t(hk) * p.G * p.c.a.q_st[1] + int64_t(w.lo) * p.c.a.q_st[2] + qc * 8;
         float* fac = fac_s + (pieces & 1) * RB;
-        for (int b0 = 0; b0 < tiles; b0 += RPP * HOLD) {
+#pragma unroll 1
+        for (int b0 = qr; b0 < tiles; b0 += RPP * HOLD) {
           uint4 raw[HOLD];
 #pragma unroll
           for (int i = 0; i < HOLD; ++i) {
-            const int r = b0 + i * RPP + qr, f = w.f0 + r;
             raw[i] = make_uint4(0, 0, 0, 0);
-            if (r < w.rows) {
-              const int t = f / p.G;
-              const T* src = qh + (f - t * p.G) * p.c.a.q_st[1] + t * p.c.a.q_st[2];
+            if (b0 + i * RPP < rows) {
+              const T* src = qh + gq * p.c.a.q_st[1] + tq * p.c.a.q_st[2];
               if (p.wide_q) {
                 raw[i] = *reinterpret_cast<const uint4*>(src);
               } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) reinterpret_cast<T*>(&raw[i])[e] = src[e];
+                for (int e = 0; e < 8; e += 2) {
+                  const uint32_t lo = reinterpret_cast<const uint16_t*>(src)[e], hi = reinterpret_cast<const uint16_t*>(src)[e + 1];
+                  (e == 0 ? raw[i].x : e == 2 ? raw[i].y : e == 4 ? raw[i].z : raw[i].w) = lo | hi << 16;
+                }
               }
             }
+            tq += st, gq += sg;
+            if (gq >= p.G) gq -= p.G, ++tq;
+          }
+          [[maybe_unused]] uint32_t mx[HOLD];
+          if constexpr (!std::is_same<T, __half>::value) {  // the rows' largest magnitudes (bits of bf16 values rise with them)
+#pragma unroll
+            for (int i = 0; i < HOLD; ++i) {
+              const __nv_bfloat162* h2 = reinterpret_cast<const __nv_bfloat162*>(&raw[i]);
+              const __nv_bfloat162 m2 = __hmax2(__hmax2(__habs2(h2[0]), __habs2(h2[1])), __hmax2(__habs2(h2[2]), __habs2(h2[3])));
+              const uint32_t m = *reinterpret_cast<const uint32_t*>(&m2);  // (NaN is passed over, unless both are)
+              mx[i] = max(m >> 16, m & 0xffffu);
+              mx[i] = mx[i] > 0x7f80u ? 0u : mx[i];
+            }
+#pragma unroll
+            for (int o = LPR / 2; o > 0; o >>= 1)
+#pragma unroll
+              for (int i = 0; i < HOLD; ++i) mx[i] = max(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], o));
           }
 #pragma unroll
           for (int i = 0; i < HOLD; ++i) {
-            const int r = b0 + i * RPP + qr;
+            const int r = b0 + i * RPP;
             uint4 x = raw[i];
             float f = p.scale_log2;
             if constexpr (!std::is_same<T, __half>::value) {
-              const __nv_bfloat162* h2 = reinterpret_cast<const __nv_bfloat162*>(&x);
-              __nv_bfloat162 m2 = __hmax2(__hmax2(__habs2(h2[0]), __habs2(h2[1])), __hmax2(__habs2(h2[2]), __habs2(h2[3])));
-              float mx = fmaxf(fmaxf(__low2float(m2), __high2float(m2)), 0.f);  // (NaN is passed over)
-#pragma unroll
-              for (int o = LPR / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
               // times 2^(14 - ex), the largest value's exponent to 14; undone by the factor, in two powers
-              const int ex = mx > 0.f ? min(max((__float_as_int(mx) >> 23) - 127, -112), 127) : 14;
+              const int ex = mx[i] ? min(max(int(mx[i] >> 7) - 127, -112), 127) : 14;
               const float up = __uint_as_float(uint32_t(127 + 14 - ex) << 23);
               uint32_t* wx = reinterpret_cast<uint32_t*>(&x);
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const float2 v = __bfloat1622float2(h2[e]);
-                wx[e] = pack2<__half>(v.x * up, v.y * up);
-              }
+              for (int e = 0; e < 4; ++e)
+                wx[e] = pack2<__half>(__uint_as_float(wx[e] << 16) * up, __uint_as_float(wx[e] & 0xffff0000u) * up);
               const int d = ex - 14;
               f = f * __uint_as_float(uint32_t(127 + d / 2) << 23) * __uint_as_float(uint32_t(127 + d - d / 2) << 23);
             }
             if (p.flip) x.x ^= 0x80008000u, x.y ^= 0x80008000u, x.z ^= 0x80008000u, x.w ^= 0x80008000u;
-            const int tile = r / BM, rr = r % BM;
-            *reinterpret_cast<uint4*>(sm + tile * C::QTILE + boxq + rr * 128 + (((qc & 7) ^ (rr & 7)) << 4)) = x;
-            if (qc == 0) fac[r] = f;
+            if (r < tiles) {
+              *reinterpret_cast<uint4*>(sm + (r / BM) * C::QTILE + dq + (r % BM) * 128) = x;
+              if (qc == 0) fac[r] = f;
+            }
           }
         }
         fence_proxy_async_shared();
@@ -855,7 +881,8 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
       const int row = r + (pair ? wg * BM : 0);  // in the item
       const bool live = row < w.rows;
       const int tok = (w.f0 + row) / p.G;
-      const int lim = !live ? -1 : (p.c.a.causal ? w.len - (w.n - 1 - tok) : w.len) - 1;  // the last key that the row sees
+      // the last key that the row sees (rows past the item's are zeros; nothing of them is kept)
+      const int lim = !live ? w.horizon - 1 : (p.c.a.causal ? w.len - (w.n - 1 - tok) : w.len) - 1;
       float m = -FLT_MAX, l = 0.f, fac = 0.f;
       // Waits for the P V of the piece's unit n. (Barriers are waited for within one phase of where they are: S_i comes after
       // the P V of unit i - 4, the buffer's last.)
