@@ -83,7 +83,8 @@ struct Cfg {
   static constexpr int ML_OFF = FAC_OFF + 2 * RB * 4;          // [2][128] float2
   static constexpr int MSH_OFF = ML_OFF + 2 * BM * 8;          // [128] the shared maximum
   static constexpr int PREFIX_OFF = MSH_OFF + BM * 4;          // [MAX_B + 3] int64
-  static constexpr int PIECE_OFF = PREFIX_OFF + (MAX_B + 3) * 8;  // [PIECES] Piece
+  static constexpr int RANGE_OFF = PREFIX_OFF + (MAX_B + 3) * 8;  // [MAX_B + 2] Range
+  static constexpr int PIECE_OFF = (RANGE_OFF + (MAX_B + 2) * 12 + 15) / 16 * 16;  // [PIECES] Piece
   static constexpr int BAR_BYTES = 640;
   static constexpr int BAR_OFF = PIECE_OFF + PIECES * int(sizeof(Piece));
   static constexpr int SMEM = BAR_OFF + BAR_BYTES + 1024;
@@ -94,7 +95,7 @@ struct Cfg {
 
 struct Params {
   arows::ChunkParams c;
-  float* ws_o;   // [2 grid][D][RB]
+  float* ws_o;   // [2 grid][D / 4][RB][4]
   float* ws_ml;  // [2 grid][2][RB]
   int4* rec;     // [grid][2]: the item that the CTA begins and does not end
   int G;
@@ -150,6 +151,7 @@ template <int RB>
 struct Sched {
   const Params& p;
   const int64_t* prefix;
+  const Range* ranges;
   int64_t each, at, p0, p1;  // units a run; the current item's first unit; the CTA's run [p0, p1)
   int more;                  // the first so many runs have one unit more
   int r, hk, k, nb;
@@ -166,7 +168,7 @@ struct Sched {
     return ((a | b) >> 32) == 0 ? int64_t(uint32_t(a) / uint32_t(b)) : a / b;
   }
 
-  __device__ __noinline__ Sched(const Params& p_, const int64_t* prefix_) : p(p_), prefix(prefix_) {
+  __device__ __noinline__ Sched(const Params& p_, const int64_t* prefix_, const Range* ranges_) : p(p_), prefix(prefix_), ranges(ranges_) {
     const int NR = p.c.a.B + 2, lane = threadIdx.x & 31;
     const int64_t total = prefix[NR];
     const int runs = int(max(int64_t(1), min(int64_t(gridDim.x), div(total, p.min_units)))), c = blockIdx.x;
@@ -207,7 +209,7 @@ struct Sched {
 
   __device__ __forceinline__ void enter(int range) {
     r = range;
-    x = range_of(p, r);
+    x = ranges[r];
     nb = (x.n * p.G + RB - 1) / RB;
     at = prefix[r];
   }
@@ -433,6 +435,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
   float2* ml_s = reinterpret_cast<float2*>(sm + C::ML_OFF);
   volatile float* m_sh = reinterpret_cast<volatile float*>(sm + C::MSH_OFF);
   int64_t* prefix = reinterpret_cast<int64_t*>(sm + C::PREFIX_OFF);
+  Range* ranges = reinterpret_cast<Range*>(sm + C::RANGE_OFF);
   Piece* list = reinterpret_cast<Piece*>(sm + C::PIECE_OFF);
   uint64_t* full = reinterpret_cast<uint64_t*>(sm + C::BAR_OFF);  // [NS] a stage's operand is in
   uint64_t* empty = full + NS;           // [NS] its products are done
@@ -502,7 +505,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
       for (int k = lane; k < nb; k += 32) s += block_of<RB>(p, x, k).units;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-      if (lane == 0) prefix[r + 1] = s * p.c.a.Hkv;
+      if (lane == 0) prefix[r + 1] = s * p.c.a.Hkv, ranges[r] = x;
     }
     __syncthreads();
     if (warp == 0) {
@@ -540,7 +543,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
     reg_dec<72>();
     if (warp == PLAN_WARP) {
       // ---------------------------------------------------------------------------------- the list of pieces
-      Sched<RB> sched(p, prefix);
+      Sched<RB> sched(p, prefix, ranges);
       Piece w;
       bool more = true;
       for (int i = 0; more; ++i) {
@@ -1022,7 +1025,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
       const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
       const uint32_t oc = pair ? o_col : lane_base + C::O_COL;
       T* out = static_cast<T*>(p.c.a.o) + int64_t(w.hk * p.G + (w.f0 + row) % p.G) * p.c.a.o_st[1] + int64_t(w.lo + tok) * p.c.a.o_st[2];
-      float* part = p.ws_o + int64_t(w.slot) * (D * RB) + row;
+      float* part = p.ws_o + int64_t(w.slot) * (D * RB) + 4 * row;
 #pragma unroll 1
       for (int c = first; c < first + count; c += 32) {
         float ov[32];
@@ -1044,7 +1047,8 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
           store32<T>(out + c, ov, inv, p.wide_o);
         } else {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) part[(c + e) * RB] = ov[e];
+          for (int e = 0; e < 32; e += 4)
+            *reinterpret_cast<float4*>(part + (c + e) * RB) = make_float4(ov[e], ov[e + 1], ov[e + 2], ov[e + 3]);
         }
       }
       prefill::tc_fence_before();
@@ -1071,7 +1075,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
     if (lane == 0) mbar_arrive(written);
     if (ok) ok = wait_or_abort(written, 0, abort_flag, 160);
     if (__all_sync(0xffffffffu, ok) && *again) {
-      Sched<RB> sched(p, prefix);
+      Sched<RB> sched(p, prefix, ranges);
       Piece y;
       while (sched.next(y))
         for (int x = warp; y.whole && x < y.rows; x += CONV_WARP)
@@ -1102,7 +1106,7 @@ __global__ void __launch_bounds__(COMBINE_WARPS * 32) combine_kernel(const Param
   const int parts = a.x, r0 = task / (D / 32) * 32, c0 = task % (D / 32) * 32, rows = e4.w, row = r0 + lane;
   if (parts == 0 || r0 >= rows) return;
   const float* ml = p.ws_ml + row;
-  const float* ws = p.ws_o + int64_t(c0) * RB + row;
+  const float* ws = p.ws_o + int64_t(c0) * RB + 4 * row;
   auto slot = [&](int i) { return i == 0 ? 2 * int64_t(blockIdx.x) + 1 : 2 * (int64_t(blockIdx.x) + i); };
   float M = -FLT_MAX, L = 0.f, x[32];
 #pragma unroll
@@ -1114,7 +1118,10 @@ __global__ void __launch_bounds__(COMBINE_WARPS * 32) combine_kernel(const Param
       const int64_t s = slot(min(i + k, parts - 1));
       m[k] = ml[s * 2 * RB], l[k] = ml[s * 2 * RB + RB];
 #pragma unroll
-      for (int e = 0; e < 32; ++e) y[k][e] = ws[s * (D * RB) + e * RB];
+      for (int e = 0; e < 32; e += 4) {
+        const float4 v = *reinterpret_cast<const float4*>(ws + s * (D * RB) + e * RB);
+        y[k][e] = v.x, y[k][e + 1] = v.y, y[k][e + 2] = v.z, y[k][e + 3] = v.w;
+      }
     }
     if (i + 1 == parts) m[1] = -FLT_MAX, l[1] = 0.f;
     const float now = fmaxf(M, fmaxf(m[0], m[1]));
