@@ -54,6 +54,7 @@ constexpr int PIECES = 4;          // pieces of work listed ahead
 constexpr int TABLES = 8;          // key tiles whose page ids and scales are held
 constexpr uint32_t WHOLE = 256;    // a tile whose 128 keys are all there
 constexpr float TOP = 7.f;         // a weight at the running maximum is 2^TOP
+constexpr int STATUS_PLAN = 158;
 constexpr int STATUS = arows::STATUS_CHUNK;  // lb2_status: 140 lengths and page ids, 141.. waits
 
 // What a CTA does of one item: key tiles kt0 .. kt0 + nt - 1. No units: the end of the list.
@@ -345,7 +346,8 @@ __device__ __noinline__ uint32_t wait_check(uint32_t since, volatile int* abort_
   if (*abort_flag) return 1;
   const uint32_t now = uint32_t(globaltimer_ns() >> 16) | 2u;  // 66 us
   if (since == 0) return now;
-  if (now - since <= uint32_t(kWaitNs >> 16)) return since;
+  // (the list's warp waits for whole pieces of work: its bound is for the others to have failed to end theirs)
+  if (now - since <= uint32_t(kWaitNs >> 16) * (where == STATUS_PLAN ? 64u : 1u)) return since;
   report_timeout(where);
   *abort_flag = 1;
   return 1;
@@ -549,7 +551,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
       for (int i = 0; more; ++i) {
         more = sched.next(w);
         if (!more) w.units = 0;
-        bool ok = i < PIECES || wait_or_abort(&piece_empty[i % PIECES], ((i / PIECES) - 1) & 1, abort_flag, 158);
+        bool ok = i < PIECES || wait_or_abort(&piece_empty[i % PIECES], ((i / PIECES) - 1) & 1, abort_flag, STATUS_PLAN);
         if (!__all_sync(0xffffffffu, ok)) break;
         if (lane == 0) {
           list[i % PIECES] = w;
@@ -667,7 +669,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
         for (int t = 0; ok && t < nt; t += 4) {
           const int cid = id;
           const float cks = ks, vl = log2f(vs);
-          const bool held = cid >= 0;
+          const bool held = cid >= 0, there = key0 + t * BN + lane * 16 < horizon && t + (lane >> 3) < nt;
           fetch(t + 4, id, ks, vs);
           // the largest scale up to each tile
           float hi = vl;
@@ -680,7 +682,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
           }
           hi = fmaxf(hi, most);
           most = __shfl_sync(0xffffffffu, hi, 31);
-          const bool apart = held && vl < fmaxf(-100.f, hi - 64.f);
+          const bool apart = there && vl < fmaxf(-100.f, hi - 64.f);  // (also a page that is none: it counts as zeros)
           const float4 f = make_float4(cks, fmaxf(vl, -100.f), apart ? 0.f : exp2f(-fmaxf(vl, -100.f)), vl);
           const uint32_t marked = __ballot_sync(0xffffffffu, apart);
           const uint32_t whole = __ballot_sync(0xffffffffu, held && key0 + t * BN + lane * 16 + 15 < horizon);

@@ -674,6 +674,15 @@ def kv8_append(pages, scales, k, v, table, start, lens=None, cu=None, turns=None
         check(rc, "kv8_append")
 
 
+_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+def _elsewhere(dev, call, *args):
+    """A call for tensors of another device than the current one, made there."""
+    with torch.cuda.device(dev):
+        return call(*args)
+
+
 _KV8_WS = {}  # (B, Hq, Hkv, T, D, page, max_pages, device index) -> workspace bytes
 
 
@@ -718,6 +727,8 @@ def kv8_attend_packed(q, pages, scales, table, kv_len, cu, scale, causal=True, o
     own among them, already appended). causal: each row sees the tokens up to its own. For inference: the result is in no
     autograd graph."""
     (num_pages, _, Hkv, page, D), (B, max_pages), dev = _kv8_pool(pages, scales, table, "kv8_attend_packed")
+    if dev != _device():
+        return _elsewhere(dev, kv8_attend_packed, q, pages, scales, table, kv_len, cu, scale, causal, out)
     qs, qst = q.shape, q.stride()
     if len(qs) != 4 or qs[0] != 1 or qs[3] != D or q.get_device() != dev or qst[3] != 1:
         raise ValueError("kv8_attend_packed: q must be [1, Hq, T, D] for the cache's D and device, with a unit last stride")
@@ -762,6 +773,8 @@ def kv8_copy(pages, scales, src, dst, into=None):
             raise ValueError("kv8_copy: scales must be contiguous fp32 [num_pages, 2, Hkv]")
         if p.get_device() != dev or s.get_device() != dev:
             raise ValueError("kv8_copy: the pools must be on one device")
+    if dev != _device():
+        return _elsewhere(dev, kv8_copy, pages, scales, src, dst, into)
     n = src.numel()
     _int32(src, (n,), dev, "kv8_copy: src")
     _int32(dst, (n,), dev, "kv8_copy: dst")
@@ -777,6 +790,8 @@ def kv8_compact(pages, scales, table, keep, cu, to, start, turns=None, layout="h
     [B], page beginnings) in the pages to[b] (int32 [B, max_to], entry j for positions j * page and on), keys turned by the
     difference of the positions when turns is given. No page may be written twice, or both read and written."""
     (num_pages, _, Hkv, page, D), (B, max_pages), dev = _kv8_pool(pages, scales, table, "kv8_compact")
+    if dev != _device():
+        return _elsewhere(dev, kv8_compact, pages, scales, table, keep, cu, to, start, turns, layout)
     T, ts = keep.numel(), to.shape
     _int32(keep, (T,), dev, "kv8_compact: keep")
     _int32(cu, (B + 1,), dev, "kv8_compact: cu")

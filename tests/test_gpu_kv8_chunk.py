@@ -387,6 +387,48 @@ def test_bad_lengths_bounds_and_pages():
                 assert ops.status() != 0
 
 
+@pytest.mark.parametrize("dtype", [BF, HF, F])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_a_page_that_is_none_counts_as_zeros(d, dtype):
+    """Its keys' scores are 0 and their weights count; a page whose scales are 0 is such a page too."""
+    lens, counts = [300], [140]
+    pages, scales, table = cache(lens, 2, 32, d)
+    q = queries(4, 140, d, dtype)
+    p, s = pages.clone(), scales.clone()
+    for j in (1, 8):
+        p.view(torch.uint8)[int(table[0, j])], s[int(table[0, j])] = 0, 0.0
+    o, a = expect(q, p, s, table, lens, counts, 0.1)
+    close(ops.kv8_attend_packed(q, p, s, table, i32(lens), i32([0, 140]), 0.1), o, a, dtype)
+    assert ops.status() == 0
+    t = table.clone()
+    t[0, 1], t[0, 8] = -7, pages.shape[0]
+    close(ops.kv8_attend_packed(q, pages, scales, t, i32(lens), i32([0, 140]), 0.1), o, a, dtype)
+    assert ops.status() != 0
+
+
+def test_beside_the_other_kernels_of_the_cache():
+    """Calls of several kernels that hold tensor memory, on several streams at once."""
+    lens, counts = [900, 333, 64], [200, 33, 64]
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    work = []
+    for d, dtype in ((64, BF), (128, HF), (256, BF)):
+        pages, scales, table = cache(lens, 2, 32, d)
+        q = queries(8, 297, d, dtype)
+        k = queries(2, 297, d, dtype, seed=3)
+        args = (q, pages, scales, table, i32(lens), i32(starts(counts)), 0.1)
+        cu = args[5]
+        work.append((lambda args=args: ops.kv8_attend_packed(*args)))
+        work.append((lambda q=q, k=k, cu=cu: ops.attn_packed(q, k, k, 0.1, cu)))
+    first = [w() for w in work]
+    torch.cuda.synchronize()
+    outs = []
+    for i in range(24):
+        with torch.cuda.stream(streams[i % 4]):
+            outs.append((i % len(work), work[i % len(work)]()))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, first[i]) for i, o in outs) and ops.status() == 0
+
+
 def test_refusals():
     pages, scales, table = cache([100], 2, 16, 128)
     q, n, cu = queries(4, 10, 128, BF), i32([100]), i32([0, 10])
