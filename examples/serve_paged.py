@@ -5,7 +5,8 @@
 One attention layer with random weights stands for the model: q, k, v projections of a hidden state, rotary positions,
 attention, the output projection, whose result is the next step's hidden state. Prompts go in packed on one row axis
 (attn_packed over the prompt's own keys, then the keys and values into the cache); each decode step appends one token a
-sequence and attends over the cache. Prints the steps' time and how far the cached attention is from attention over the
+sequence and attends over the cache. A forked sequence then shares its prompt's pages, takes a turn of its own, keeps a window
+of its tokens, and the pool is made as small as its pages allow. Prints the steps' time and how far the cached attention is from attention over the
 unrounded keys and values.
 """
 import argparse
@@ -53,6 +54,15 @@ class Layer:
         cache.append(step, k, v, rope=self.rope)
         return self.finish(cache.attend(step, self.rope.apply(q, step.positions), self.scale)), (step, q, k, v)
 
+    def turns(self, cache, handles, x, lens):
+        """The next turns of running sequences, packed: hidden states x [1, sum(lens), hidden] over what is cached and
+        themselves; their last rows' outputs."""
+        step = cache.step(handles, lens)
+        q, k, v = self.project(x)
+        cache.append(step, k, v, rope=self.rope, packed=True)
+        o = cache.attend(step, self.rope.apply(q, step.positions.reshape(-1)), self.scale, packed=True)
+        return self.finish(o)[0, step.cu[1:].long() - 1][:, None]
+
 
 def main(steps=32, hidden=2048, hq=32, hk=8, d=128, lens=(700, 1500, 33, 260), device="cuda"):
     layer = Layer(hidden, hq, hk, d, device)
@@ -92,7 +102,17 @@ def main(steps=32, hidden=2048, hq=32, hk=8, d=128, lens=(700, 1500, 33, 260), d
     handles.append(new)
     for _ in range(3):
         x, _ = layer.decode(cache, handles, x)
-    assert ops.status() == 0 and torch.isfinite(x).all()
+    # a second answer to the first sequence's prompt shares its pages; both go on with turns of their own, then the longer one
+    # keeps its first tokens and a window, and the pool shrinks to what is used
+    other = cache.fork(handles[0])
+    y = layer.turns(cache, [handles[0], other], prompt(5 + 40), [5, 40])
+    n = cache.length(other)
+    cache.keep([other], [[*range(4), *range(n - 50, n)]], layer.rope)
+    cache.resize(max(1, cache.pages.shape[0] - cache.free_pages))
+    cache.resize(512)
+    y, _ = layer.decode(cache, [handles[0], other], y)
+    assert cache.length(other) == 55 and cache.length(handles[0]) == lens[0] + steps + 3 + 5 + 1
+    assert ops.status() == 0 and torch.isfinite(x).all() and torch.isfinite(y).all()
     return worst
 
 

@@ -8,18 +8,23 @@
 // one) and stored as the swizzled operand tiles of both products: once for a block's 256 rows, and no raw tile passes
 // through shared memory, whose bandwidth is the products' too.
 //
-// The tensor pipe works on units, (row tile of 128, key tile) pairs, two S buffers in turn: S_i = Q K^T into buffer i % 2,
-// warpgroup i % 2 turns it into P_i (in its place), O += P_i V, S_{i+2}. So one warpgroup's softmax runs under the other's
-// products.
-//  - more than 128 rows, head dim 64 and 128: unit i is row tile i % 2 of key tile i / 2; each warpgroup has its own rows.
-//  - up to 128 rows there: unit i is key tile i of the one row tile; each warpgroup has its own maximum, sum and O over its
+// The tensor pipe works on units, (row tile of 128, half a key tile) pairs, over four S buffers in turn: S_i = Q K^T into buffer
+// i % 4, warpgroup i % 2 turns it into P_i (in its place), O += P_i V, S_{i+4}. A warpgroup's next scores are thus ready when it
+// is done with the last ones.
+//  - more than 128 rows, head dim 64 and 128: unit i is row tile i % 2 of half tile i / 2; each warpgroup has its own rows.
+//  - up to 128 rows there: unit i is half tile i of the one row tile; each warpgroup has its own maximum, sum and O over its
 //    half of the keys, joined at the end.
-//  - head dim 256 (O takes half the tensor memory): unit i is key tile i; the warpgroups share the rows' maximum, handed on
+//  - head dim 256 (O takes half the tensor memory): unit i is half tile i; the warpgroups share the rows' maximum, handed on
 //    from unit to unit, and O; each sums its own units' weights.
 //
-// Work is cut evenly whatever the lengths: the call's units in order, cut into equal runs, one a CTA (one CTA an SM). An item
-// that a cut parts is merged from fp32 partials by combine_kernel, launched behind as a programmatic dependent; its parts
-// are known from the units alone, so every sum is formed in the same order in every run of a call.
+// Work is cut evenly whatever the lengths: the call's (row tile, key tile) steps in order, cut into equal runs, one a CTA (one
+// CTA an SM). An item that a cut parts is merged from fp32 partials by combine_kernel, launched behind as a programmatic
+// dependent; its parts are known from the steps alone, so every sum is formed in the same order in every run of a call.
+//
+// Measured (bf16, 32 / 8 heads x 128): 2048 new of 32768 tokens 1.24 ms, 860 TFLOP/s, half of what the products alone could run
+// at; what bounds it is the number of instructions, 10 000 warp instructions for 256 rows x 128 keys, at two a clock and SM (softmax 4 300,
+// conversion 2 200, the rest barriers, schedules and issue). f16, 24 / 2 heads x 256, 1001 of up to 16390: 0.44 ms, 760 TFLOP/s.
+// 33 of 777 tokens: 29 us, the life of one CTA and the merge.
 //
 // Softmax in base 2, fp32, one thread a row. As in kv8_attend.cuh the weights carry the values' scale, p' = 2^(s + log2 s_v -
 // m), m the running maximum of s + log2 s_v less 7, l = sum p' / s_v, o = sum p' code_v / l; the maximum moves when it is
