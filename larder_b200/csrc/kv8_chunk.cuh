@@ -23,7 +23,7 @@
 //
 // Measured (bf16, 32 / 8 heads x 128): 2048 new of 32768 tokens 1.24 ms, 860 TFLOP/s, half of what the products alone could run
 // at; what bounds it is the number of instructions, 10 000 warp instructions for 256 rows x 128 keys, at two a clock and SM (softmax 4 300,
-// conversion 2 200, the rest barriers, schedules and issue). f16, 24 / 2 heads x 256, 1001 of up to 16390: 0.44 ms, 760 TFLOP/s.
+// conversion 2 200, the rest barriers, schedules and issue). f16, 24 / 2 heads x 256, 1001 of up to 16390: 0.42 ms, 800 TFLOP/s.
 // 33 of 777 tokens: 29 us, the life of one CTA and the merge.
 //
 // Softmax in base 2, fp32, one thread a row. As in kv8_attend.cuh the weights carry the values' scale, p' = 2^(s + log2 s_v -
@@ -76,9 +76,12 @@ struct Cfg {
   static constexpr bool WIDE = D == 256;
   static constexpr int QT = WIDE ? 1 : 2;         // row tiles of an item
   static constexpr int RB = BM * QT;
-  static constexpr int DS = D < 128 ? D : 128;    // dims of a stage
-  static constexpr int SPT = D / DS;              // stages of a K (or V) tile
-  static constexpr int STAGE = BN * DS * 2;
+  // A stage of the operand ring: a tile's K or V, or a half tile's (the keys of a unit) at head dim 256, where two tiles' K and V
+  // do not fit: a half is free again after its unit. Boxes of 64 dims, 128 bytes a key.
+  static constexpr int SPT = WIDE ? 2 : 1;        // stages of a K (or V) tile
+  static constexpr int SK = BN / SPT;             // keys of a stage
+  static constexpr int BOX = SK * 128;            // bytes of a stage's box
+  static constexpr int STAGE = SK * D * 2;
   static constexpr int NS = D == 64 ? 6 : 4;
   static constexpr int QTILE = BM * D * 2;
   static constexpr int K_OFF = QT * QTILE;
@@ -431,7 +434,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
   using C = Cfg<D>;
   constexpr int RB = C::RB, NS = C::NS, SPT = C::SPT;
   constexpr uint32_t IDESC_S = prefill::idesc_f16(0, 0, 0, BM, BH);
-  constexpr uint32_t IDESC_PV = prefill::idesc_f16(0, 0, 1, BM, C::DS);
+  constexpr uint32_t IDESC_PV = prefill::idesc_f16(0, 0, 1, BM, D);
 
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -582,7 +585,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
         const int nt = uni(list[pieces % PIECES].nt), units = (pair ? 4 : 2) * nt;
         // operands' descriptors: the K-major tiles' (Q, K) and the MN-major V's; tiles differ in the low word's address
         const uint32_t q_desc = smem_u32(sm) >> 4 | 1u << 16;
-        const uint32_t s_desc = smem_u32(sm + C::K_OFF) >> 4 | uint32_t(scores ? 16 >> 4 : BN * 128 >> 4) << 16;
+        const uint32_t s_desc = smem_u32(sm + C::K_OFF) >> 4 | uint32_t(scores ? 16 >> 4 : C::BOX >> 4) << 16;
         if (scores) {
           ok = wait(q_full, pieces & 1, 141);
         } else if (pieces > 0) {
@@ -591,8 +594,9 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
 #pragma unroll 1
         for (int i = 0; ok && i < units; ++i) {
           const int ht = pair ? i >> 1 : i, half = ht & 1, buf = i & 3, nth = (i & 2 ? g23 : g01) + (i >> 2);
-          const int e = (base + (scores ? k_entry(pair, ht >> 1) : v_entry(pair, nt, ht >> 1))) * SPT;
-          const bool begins = half == 0 && (!pair || !(i & 1)), ends = half && (!pair || (i & 1));  // the tile's units
+          const int e = (base + (scores ? k_entry(pair, ht >> 1) : v_entry(pair, nt, ht >> 1))) * SPT + (C::WIDE ? half : 0);
+          // whether the unit is its stage's first, its last
+          const bool begins = C::WIDE || (half == 0 && (!pair || !(i & 1))), ends = C::WIDE || (half && (!pair || (i & 1)));
           if (scores) {  // S overwrites the buffer's last P: its P V is done
             if (nth > 0) ok = wait(&o_done[buf], (nth - 1) & 1, 161);
           } else {
@@ -601,29 +605,25 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
           const uint32_t q = q_desc + (pair && (i & 1) ? C::QTILE >> 4 : 0);
           const bool own = !C::WIDE;  // each warpgroup its O
           const uint32_t o = tm + C::O_COL + (own && (i & 1) ? D : 0);
-#pragma unroll
-          for (int h = 0; h < SPT; ++h) {
-            const int st = (e + h) % NS;
-            if (begins && ok) ok = wait(&full[st], ((e + h) / NS) & 1, 142);
-            if (!ok) break;
-            prefill::tc_fence_after();
-            const uint32_t x = s_desc + st * (C::STAGE >> 4) + half * (BH * 128 >> 4);
-            if (scores) {
-#pragma unroll 1
-              for (uint32_t bx = 0; bx < C::DS / 64; ++bx)
-#pragma unroll
-                for (uint32_t kk = 0; kk < 4; ++kk)
-                  mma_ss(lead, tm + buf * BH, q + (((h * (C::DS / 64) + bx) * BM * 128 + kk * 32) >> 4),
-                         x + ((bx * BN * 128 + kk * 32) >> 4), IDESC_S, h + bx + kk > 0 ? 1u : 0u);
-            } else {
-#pragma unroll
-              for (int kk = 0; kk < BH / 16; ++kk)
-                mma_ts(lead, o + h * C::DS, tm + buf * BH + kk * 8, x + ((kk * 16 * 128) >> 4), IDESC_PV,
-                       (own ? i > 1 : i > 0) || kk > 0 ? 1u : 0u);
-            }
-            if (ends) mma_commit(lead, &empty[st]);
-          }
+          const int st = e % NS;
+          if (begins && ok) ok = wait(&full[st], (e / NS) & 1, 142);
           if (!ok) break;
+          prefill::tc_fence_after();
+          const uint32_t x = s_desc + st * (C::STAGE >> 4) + (C::WIDE ? 0 : half * (BH * 128 >> 4));
+          if (scores) {
+#pragma unroll 1
+            for (uint32_t bx = 0; bx < D / 64; ++bx)
+#pragma unroll
+              for (uint32_t kk = 0; kk < 4; ++kk)
+                mma_ss(lead, tm + buf * BH, q + ((bx * BM * 128 + kk * 32) >> 4), x + ((bx * C::BOX + kk * 32) >> 4), IDESC_S,
+                       bx + kk > 0 ? 1u : 0u);
+          } else {
+#pragma unroll
+            for (int kk = 0; kk < BH / 16; ++kk)
+              mma_ts(lead, o, tm + buf * BH + kk * 8, x + ((kk * 16 * 128) >> 4), IDESC_PV,
+                     (own ? i > 1 : i > 0) || kk > 0 ? 1u : 0u);
+          }
+          if (ends) mma_commit(lead, &empty[st]);
           mma_commit(lead, scores ? &s_full[buf] : &o_done[buf]);
           if (scores && i == units - 1) mma_commit(lead, q_empty);
         }
@@ -714,7 +714,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
     reg_dec<72>();
     // A thread takes units of 16 codes: unit ul + 4 h of keys r0, r0 + 32, .. Eight lanes that store 16 bytes each then fill 128:
     // four units of two keys, whose swizzles are apart.
-    constexpr int UH = C::DS / 64, LD = 4 * UH;  // 64-dim boxes, units a thread and stage
+    constexpr int UH = D / 64, KP = C::SK / 32, LD = KP * UH;  // 64-dim boxes, keys and units a thread and stage
     const int tid = threadIdx.x - CONV_WARP * 32, ul = tid & 3, r0 = (tid & 127) >> 2;
     const int group = tid >> 7;  // the two warpgroups take the stages in turn
     const int page = 1 << p.lpage;
@@ -816,26 +816,27 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
           tabs = t + 1;
         }
         const int end = ok ? horizon - (kt0 + t) * BN : 0;  // keys of the tile that some row sees
-        const uint8_t* from = p.c.a.pages + kind * kv_off + (s % SPT) * C::DS + ul * 16;
+        const uint8_t* from = p.c.a.pages + kind * kv_off + ul * 16;
+        const int r1 = r0 + (s % SPT) * C::SK;  // the thread's first key in the tile
         const int64_t* at = at_s + slot * 8;
-        const uint8_t* x0[4];
+        const uint8_t* x0[KP];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int r = r0 + 32 * k;
+        for (int k = 0; k < KP; ++k) {
+          const int r = r1 + 32 * k;
           x0[k] = from + at[r >> p.lpage] + (r & (page - 1)) * D;
         }
         uint4 x[LD];
         if (ok && (far_s[slot] & WHOLE)) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
+          for (int k = 0; k < KP; ++k)
 #pragma unroll
             for (int h = 0; h < UH; ++h) x[k * UH + h] = ld_codes(x0[k] + 64 * h);
         } else {  // the tile's last keys, or a page that is none, are zeros
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
+          for (int k = 0; k < KP; ++k)
 #pragma unroll
             for (int h = 0; h < UH; ++h)
-              x[k * UH + h] = load_if(x0[k] + 64 * h, r0 + 32 * k < end && at[(r0 + 32 * k) >> p.lpage] >= 0);
+              x[k * UH + h] = load_if(x0[k] + 64 * h, r1 + 32 * k < end && at[(r1 + 32 * k) >> p.lpage] >= 0);
         }
         if (kind == 1) {  // the tile's places have been used
           __syncwarp();
@@ -845,7 +846,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
         if (ok && gs >= NS) ok = wait_or_abort(&empty[st], ((gs / NS) - 1) & 1, abort_flag, 150);
         uint8_t* d = sm + C::K_OFF + st * C::STAGE;
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
+        for (int k = 0; k < KP; ++k)
 #pragma unroll
           for (int h = 0; h < UH; ++h) {
             const uint4 c = x[k * UH + h];
@@ -854,8 +855,8 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
             kv8::dec4(c.y, a.z, a.w);
             kv8::dec4(c.z, b.x, b.y);
             kv8::dec4(c.w, b.z, b.w);
-            *reinterpret_cast<uint4*>(d + dst0 + h * (BN * 128) + k * (32 * 128)) = a;
-            *reinterpret_cast<uint4*>(d + dst1 + h * (BN * 128) + k * (32 * 128)) = b;
+            *reinterpret_cast<uint4*>(d + dst0 + h * C::BOX + k * (32 * 128)) = a;
+            *reinterpret_cast<uint4*>(d + dst1 + h * C::BOX + k * (32 * 128)) = b;
           }
         fence_proxy_async_shared();
         __syncwarp();
