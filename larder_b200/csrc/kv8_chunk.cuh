@@ -45,6 +45,7 @@
 #include "attn_rows.cuh"
 #include "common.cuh"
 #include "kv8.cuh"
+#include "wait_clock.cuh"
 
 namespace lb2 {
 namespace kv8chunk {
@@ -352,10 +353,9 @@ static_assert(256 * 128 + 384 * 72 <= THREADS * 96, "a split above what was laun
 // returned; 1: give up, some role has or the wait's time is over.
 __device__ __noinline__ uint32_t wait_check(uint32_t since, volatile int* abort_flag, int where) {
   if (*abort_flag) return 1;
-  const uint32_t now = uint32_t(globaltimer_ns() >> 16) | 2u;  // 66 us
-  if (since == 0) return now;
   // (the list's warp waits for whole pieces of work: its bound is for the others to have failed to end theirs)
-  if (now - since <= uint32_t(kWaitNs >> 16) * (where == STATUS_PLAN ? 64u : 1u)) return since;
+  since = wait_look(since, globaltimer_ns(), kWaitNs * (where == STATUS_PLAN ? 64u : 1u));
+  if (since != 1u) return since;
   report_timeout(where);
   *abort_flag = 1;
   return 1;
