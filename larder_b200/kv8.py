@@ -99,6 +99,12 @@ class Cache:
         if any(n is None or s < n for s in self._pending.get(handle, ())):
             raise ValueError(f"kv8: sequence {handle} has tokens that a step reserved and that were not appended")
 
+    def _lacks(self, step, where=lambda h, s: True):
+        """The step's append was refused: its tokens count, but the pages do not hold them."""
+        for h, s, n in step.spans:
+            if n and h in self._seqs and where(h, s):
+                self._missing.setdefault(h, set()).add(s)
+
     def length(self, handle):
         return self._seqs[handle][1]
 
@@ -280,10 +286,14 @@ class Cache:
         """The step's new tokens: k / v [B, hk, T, d] where every sequence has T of them, or, packed, [1, hk, rows, d].
         Keys are rotated by their positions when a Rope is given. After a refused append the step's tokens still count:
         append them again, or trim them away; attend refuses sequences that lack them."""
-        self._current(step)
-        for h, s, n in step.spans if self._forked else ():
-            if n and h in self._seqs and any(self._refs[i] > 1 for i in self._seqs[h][0][s // self.page:-(-(s + n) // self.page)]):
-                raise ValueError(f"kv8: sequence {h} shares the pages of this step since it was made")
+        try:
+            self._current(step)
+            for h, s, n in step.spans if self._forked else ():
+                if n and h in self._seqs and any(self._refs[i] > 1 for i in self._seqs[h][0][s // self.page:-(-(s + n) // self.page)]):
+                    raise ValueError(f"kv8: sequence {h} shares the pages of this step since it was made")
+        except ValueError:  # (tokens that it appended before are there as they were)
+            self._lacks(step, lambda h, s: s in self._pending.get(h, ()))
+            raise
         try:
             kw = {} if rope is None else {"turns": rope.turns, "layout": rope.layout, "amp": rope.amp}
             if packed:
@@ -293,10 +303,8 @@ class Cache:
             elif any(c != k.shape[2] for c in step.counts):
                 raise ValueError("kv8: sequences with different counts go in packed")
             ops.kv8_append(self.pages, self.scales, k, v, step.table, step.start, **kw)
-        except Exception:  # the step's tokens count, but the pages do not hold them
-            for h, s, n in step.spans:
-                if n and h in self._seqs:
-                    self._missing.setdefault(h, set()).add(s)
+        except Exception:
+            self._lacks(step)
             raise
         for h, s, n in step.spans:
             if n:
