@@ -19,9 +19,19 @@ Pages are handed out on the host; the device sees a page table a step. A page ma
 alike: it is copied for the one that appends into it. The codes, the rounding and what the kernels check are
 lb2_kv8_append's, lb2_kv8_attend's, lb2_kv8_attend_packed's, lb2_kv8_copy's and lb2_kv8_compact's.
 """
+import weakref
+
 import torch
 
 from . import ops
+
+
+class _Use:
+    """What a step relies on: each sequence's tokens up to ends[handle]; why[handle]: what has happened to them since."""
+    __slots__ = ("ends", "why", "__weakref__")
+
+    def __init__(self, spans):
+        self.ends, self.why = {h: s + n for h, s, n in spans}, {}
 
 
 class Step:
@@ -29,11 +39,11 @@ class Step:
     cu int32 [B + 1] (row offsets of the new tokens packed), positions int32 (of the new tokens: [B, T] where every
     sequence has T, else packed [rows])."""
 
-    def __init__(self, table, start, kv_len, cu, positions, counts, spans=(), made=0):
+    def __init__(self, table, start, kv_len, cu, positions, counts, spans=(), use=None):
         self.table, self.start, self.kv_len, self.cu = table, start, kv_len, cu
         self.positions, self.counts = positions, counts
         self.spans = spans  # (handle, tokens before the call, new tokens) of each sequence, on the host
-        self.made = made    # the cache's count of moves when its table was made
+        self.use = _Use(spans) if use is None else use
 
 
 class Cache:
@@ -49,8 +59,7 @@ class Cache:
         self._refs = [0] * num_pages  # sequences that hold each page
         self._missing = {}  # handle -> first positions of the steps whose append was refused
         self._pending = {}  # handle -> first positions of the steps whose append has not been made
-        self._moves = 0     # times that pages of sequences were exchanged for others
-        self._moved = {}    # handle -> the count at its last one
+        self._uses = weakref.WeakSet()  # of the steps that are still held
         self._forked = False  # some pages may be shared
         self._next = 0
 
@@ -68,8 +77,9 @@ class Cache:
     def drop(self, handle):
         """Ends a sequence; its pages may be handed out again where no other sequence holds them."""
         self._release(reversed(self._seqs.pop(handle)[0]))
-        for d in (self._missing, self._pending, self._moved):
+        for d in (self._missing, self._pending):
             d.pop(handle, None)
+        self._overtake(handle, 0, f"sequence {handle} was dropped")
 
     def _take(self):
         i = self._free.pop()
@@ -82,17 +92,20 @@ class Cache:
             if not self._refs[i]:
                 self._free.append(i)
 
-    def _move(self, handles):
-        """The handles' pages have been exchanged: tables of steps made before no longer name them."""
-        self._moves += 1
-        for h in handles:
-            self._moved[h] = self._moves
+    def _overtake(self, handle, n, why):
+        """A sequence's tokens from position n on are no longer where steps made before have them."""
+        for use in list(self._uses):
+            if use.ends.get(handle, 0) > n:
+                use.why.setdefault(handle, why)
 
-    def _current(self, step):
-        if self._moves > step.made:
-            for h, _, _ in step.spans:
-                if self._moved.get(h, 0) > step.made:
-                    raise ValueError(f"kv8: sequence {h}'s pages have moved since this step was made")
+    def _moved(self, handle, n):
+        self._overtake(handle, n, f"sequence {handle}'s pages have moved")
+
+    def _current(self, step, new=False):
+        """Refuses a step whose tokens (new: its new ones) are no longer where it has them."""
+        for h, _, n in step.spans if step.use.why else ():
+            if h in step.use.why and (n or not new):
+                raise ValueError(f"kv8: {step.use.why[h]} since this step was made")
 
     def _settled(self, handle, n=None):
         """Refuses a sequence among whose first n tokens (all) some were reserved by a step and not appended."""
@@ -191,7 +204,7 @@ class Cache:
             for ids, now, (h, at, same) in zip(old, new, moves):
                 self._release(reversed(ids[same // self.page:]))
                 self._seqs[h] = [now, len(at)]
-            self._move([h for h, _, _ in moves])
+                self._moved(h, same)
         moved = {h for h, _, _ in moves}
         for h, at in zip(handles, positions):
             if h not in moved:
@@ -216,7 +229,8 @@ class Cache:
         self._refs = [self._refs[i] for i in used] + [0] * (num_pages - len(used))
         self._free = list(range(num_pages - 1, len(used) - 1, -1))
         self.pages, self.scales = pages, scales
-        self._move(self._seqs)
+        for h in self._seqs:
+            self._moved(h, -1)
 
     def step(self, handles, counts):
         """Reserves room for counts[i] new tokens of handles[i] and returns the call's Step. Nothing is reserved, and a
@@ -239,8 +253,7 @@ class Cache:
             self._refs[i] -= 1
             self._seqs[h][0][j] = self._take()
             dst.append(self._seqs[h][0][j])
-        if copies:
-            self._move([h for h, _, _ in copies])
+            self._moved(h, j * self.page)
         start = []
         for h, c, n in zip(handles, counts, need):
             seq = self._seqs[h]
@@ -279,17 +292,19 @@ class Cache:
             raise
         table, start_t, len_t, cu_t, pos = t
         same = B and all(c == counts[0] for c in counts)
-        return Step(table.view(B, width), start_t, len_t, cu_t, pos.view(B, counts[0]) if same else pos, list(counts),
-                    list(zip(handles, start, counts)), self._moves)
+        step = Step(table.view(B, width), start_t, len_t, cu_t, pos.view(B, counts[0]) if same else pos, list(counts),
+                    list(zip(handles, start, counts)))
+        self._uses.add(step.use)
+        return step
 
     def append(self, step, k, v, rope=None, packed=False):
         """The step's new tokens: k / v [B, hk, T, d] where every sequence has T of them, or, packed, [1, hk, rows, d].
         Keys are rotated by their positions when a Rope is given. After a refused append the step's tokens still count:
         append them again, or trim them away; attend refuses sequences that lack them."""
         try:
-            self._current(step)
+            self._current(step, new=True)
             for h, s, n in step.spans if self._forked else ():
-                if n and h in self._seqs and any(self._refs[i] > 1 for i in self._seqs[h][0][s // self.page:-(-(s + n) // self.page)]):
+                if n and any(self._refs[i] > 1 for i in self._seqs[h][0][s // self.page:-(-(s + n) // self.page)]):
                     raise ValueError(f"kv8: sequence {h} shares the pages of this step since it was made")
         except ValueError:  # (tokens that it appended before are there as they were)
             self._lacks(step, lambda h, s: s in self._pending.get(h, ()))

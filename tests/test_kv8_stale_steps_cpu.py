@@ -61,3 +61,63 @@ def test_a_refused_append_of_tokens_that_are_there_changes_nothing(names):
     with pytest.raises(ValueError, match="moved"):
         c.append(s, rows(10), rows(10))
     assert held(names, c, a) == [2, 4, 6] and c.attend(c.step([a], [0]), q(), 1.0) == "o"
+
+
+def test_a_dropped_sequence_writes_into_no_page(names):
+    c = make()
+    a = c.add()
+    put(c, [a], [range(10)])
+    s, done = c.step([a], [3]), c.step([a], [0])
+    b = c.fork(a, 10)
+    c.drop(a)
+    put(c, [b], [[11, 12, 13]])  # in the page that b now holds alone
+    for call in (lambda: c.append(s, rows(3), rows(3)), lambda: c.attend(s, q(), 1.0), lambda: c.attend(done, q(), 1.0)):
+        with pytest.raises(ValueError, match="dropped"):
+            call()
+    assert held(names, c, b) == list(range(10)) + [11, 12, 13]
+
+
+def test_a_step_with_a_dropped_sequence_among_others(names):
+    c = make()
+    a, b = c.add(), c.add()
+    put(c, [a, b], [range(20), range(30)])
+    both, one = c.step([a, b], [1, 2]), c.step([a, b], [0, 1])
+    c.drop(a)
+    with pytest.raises(ValueError, match="dropped"):
+        c.append(both, rows(3), rows(3), packed=True)
+    with pytest.raises(ValueError, match="not appended"):  # b lacks its tokens of that step
+        c.attend(c.step([b], [0]), q(), 1.0)
+    c.append(one, rows(1), rows(1), packed=True)  # no new tokens of a
+    for step in (both, one):  # a's pages may be another's
+        with pytest.raises(ValueError, match="dropped"):
+            c.attend(step, q(2), 1.0)
+    whole(c)
+
+
+def test_a_dropped_sequence_and_a_pool_of_another_size(names):
+    c = make()
+    a, b = c.add(), c.add()
+    s = c.step([a], [40])
+    put(c, [b], [range(40)])
+    c.drop(a)
+    c.resize(4)  # b's pages now have the ids that a's step names
+    with pytest.raises(ValueError):
+        c.append(s, rows(40), rows(40))
+    assert held(names, c, b) == list(range(40))
+
+
+def test_only_the_steps_that_reach_what_moved_are_refused(names):
+    c = make()
+    a = c.add()
+    early = put(c, [a], [range(16)])
+    late = put(c, [a], [range(16, 40)])
+    c.fork(a)
+    put(c, [a], [[40]])  # the third page is copied for a
+    assert c.attend(early, q(), 1.0) == "o"
+    with pytest.raises(ValueError, match="moved"):
+        c.attend(late, q(), 1.0)
+    c.keep([a], [list(range(20)) + [30]])
+    assert c.attend(early, q(), 1.0) == "o"  # the first page stayed where it was
+    c.resize(12)
+    with pytest.raises(ValueError, match="moved"):
+        c.attend(early, q(), 1.0)
