@@ -122,7 +122,8 @@ class Cache:
         return self._seqs[handle][1]
 
     def trim(self, handle, n):
-        """Forgets a sequence's tokens from position n on (rejected drafts). The kept page's scale stays as it is."""
+        """Forgets a sequence's tokens from position n on (rejected drafts). The kept page's scale stays as it is. Steps that
+        reach past n are refused from now on."""
         ids, have = self._seqs[handle]
         if not 0 <= n <= have:
             raise ValueError(f"kv8: cannot trim a sequence of {have} tokens to {n}")
@@ -130,6 +131,7 @@ class Cache:
         self._release(reversed(ids[keep:]))
         del ids[keep:]
         self._seqs[handle][1] = n
+        self._overtake(handle, n, f"sequence {handle} was cut to {n} tokens")
         for d in (self._missing, self._pending):
             for s in [s for s in d.get(handle, ()) if s >= n]:
                 self._found(d, handle, s)

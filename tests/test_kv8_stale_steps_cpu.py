@@ -121,3 +121,77 @@ def test_only_the_steps_that_reach_what_moved_are_refused(names):
     c.resize(12)
     with pytest.raises(ValueError, match="moved"):
         c.attend(early, q(), 1.0)
+
+
+def test_a_step_cut_away_writes_into_no_page(names):
+    c = make()
+    a, b = c.add(), c.add()
+    s = c.step([a], [20])
+    c.trim(a, 0)
+    put(c, [b], [range(20)])  # in the pages that a's step names
+    for call in (lambda: c.append(s, rows(20), rows(20)), lambda: c.attend(s, q(), 1.0)):
+        with pytest.raises(ValueError, match="cut"):
+            call()
+    assert held(names, c, b) == list(range(20))
+    assert c.attend(put(c, [a], [[1, 2]]), q(), 1.0) == "o"  # nothing of the refused step is left
+
+
+def test_a_step_cut_in_the_middle_before_its_append(names):
+    c = make()
+    a, b = c.add(), c.add()
+    s = c.step([a], [40])
+    c.trim(a, 20)
+    put(c, [b], [range(20)])
+    with pytest.raises(ValueError, match="cut"):
+        c.append(s, rows(40), rows(40))
+    assert held(names, c, b) == list(range(20))
+    with pytest.raises(ValueError, match="not appended"):
+        c.attend(c.step([a], [0]), q(), 1.0)
+    c.trim(a, 0)
+    assert c.attend(put(c, [a], [range(3)]), q(), 1.0) == "o"
+
+
+def test_cut_and_grown_again(names):
+    """The length alone does not tell: the tokens are another step's."""
+    c = make()
+    a = c.add()
+    early, s = put(c, [a], [range(10)]), c.step([a], [30])
+    c.trim(a, 10)
+    now = put(c, [a], [range(100, 130)])
+    with pytest.raises(ValueError, match="cut"):
+        c.append(s, rows(30), rows(30))
+    assert held(names, c, a) == list(range(10)) + list(range(100, 130))
+    assert c.attend(early, q(), 1.0) == c.attend(now, q(), 1.0) == "o"
+    c.trim(a, 40)  # nothing is forgotten
+    assert c.attend(now, q(), 1.0) == "o"
+
+
+def test_kept_prefixes_cut_the_steps_behind_them(names):
+    c = make()
+    a, b = c.add(), c.add()
+    s, early = put(c, [a], [range(40)]), c.step([a], [0])
+    c.keep([a], [range(16)])  # nothing moves
+    put(c, [b], [range(24)])
+    for step in (s, early):
+        with pytest.raises(ValueError, match="cut"):
+            c.attend(step, q(), 1.0)
+    c.drop(a)
+    whole(c)
+
+
+def test_drafts_round_by_round(names):
+    """A step of drafts, its attention, the rejected ones trimmed: the steps of later rounds are as before."""
+    c = make()
+    a, b = c.add(), c.add()
+    put(c, [a, b], [range(30), range(5)])
+    want = {a: list(range(30)), b: list(range(5))}
+    for i in range(12):
+        drafts = {h: [1000 * (h + 1) + 10 * i + j for j in range(4)] for h in (a, b)}
+        s = put(c, [a, b], [drafts[a], drafts[b]])
+        assert c.attend(s, q(2), 1.0) == "o"
+        for h, n in ((a, i % 5), (b, (i + 2) % 5)):
+            want[h] += drafts[h][:n]
+            c.trim(h, len(want[h]))
+            assert held(names, c, h) == want[h]
+    whole(c)
+    assert len(c._uses) <= 1  # only steps that someone holds
