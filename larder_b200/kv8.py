@@ -255,7 +255,6 @@ class Cache:
             self._refs[i] -= 1
             self._seqs[h][0][j] = self._take()
             dst.append(self._seqs[h][0][j])
-            self._moved(h, j * self.page)
         start = []
         for h, c, n in zip(handles, counts, need):
             seq = self._seqs[h]
@@ -292,6 +291,8 @@ class Cache:
                 self._seqs[h][0][j] = i
                 self._refs[i] += 1
             raise
+        for h, j, _ in copies:
+            self._moved(h, j * self.page)
         table, start_t, len_t, cu_t, pos = t
         same = B and all(c == counts[0] for c in counts)
         step = Step(table.view(B, width), start_t, len_t, cu_t, pos.view(B, counts[0]) if same else pos, list(counts),

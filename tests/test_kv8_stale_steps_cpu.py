@@ -195,3 +195,17 @@ def test_drafts_round_by_round(names):
             assert held(names, c, h) == want[h]
     whole(c)
     assert len(c._uses) <= 1  # only steps that someone holds
+
+
+def test_a_refused_step_overtakes_nothing(names):
+    c = make()
+    a = c.add()
+    s = put(c, [a], [range(20)])
+    c.fork(a)
+    names["fail"] = "copy"
+    with pytest.raises(ValueError, match="refused"):
+        c.step([a], [1])
+    assert c.attend(s, q(), 1.0) == "o"  # its pages are where they were
+    c.step([a], [1])
+    with pytest.raises(ValueError, match="moved"):
+        c.attend(s, q(), 1.0)
