@@ -108,8 +108,9 @@ class Cache:
                 raise ValueError(f"kv8: {step.use.why[h]} since this step was made")
 
     def _settled(self, handle, n=None):
-        """Refuses a sequence among whose first n tokens (all) some were reserved by a step and not appended."""
-        if any(n is None or s < n for s in self._pending.get(handle, ())):
+        """Refuses a sequence among whose first n tokens (all) some were reserved by a step and not appended, or were to be
+        appended again and that was refused."""
+        if any(n is None or s < n for d in (self._pending, self._missing) for s in d.get(handle, ())):
             raise ValueError(f"kv8: sequence {handle} has tokens that a step reserved and that were not appended")
 
     def _lacks(self, step, where=lambda h, s: True):
@@ -218,7 +219,7 @@ class Cache:
         used = [i for i, r in enumerate(self._refs) if r]
         if num_pages < 1 or len(used) > num_pages:
             raise ValueError(f"kv8: {len(used)} pages are in use, they do not fit a pool of {num_pages}")
-        for h in self._pending:
+        for h in self._seqs:
             self._settled(h)
         pages = torch.zeros((num_pages,) + self.pages.shape[1:], dtype=torch.uint8, device=self.device).view(torch.float8_e4m3fn)
         scales = torch.zeros((num_pages,) + self.scales.shape[1:], dtype=torch.float32, device=self.device)

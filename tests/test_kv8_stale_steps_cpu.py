@@ -209,3 +209,22 @@ def test_a_refused_step_overtakes_nothing(names):
     c.step([a], [1])
     with pytest.raises(ValueError, match="moved"):
         c.attend(s, q(), 1.0)
+
+
+def test_an_append_again_that_was_refused(names):
+    """attend refuses the sequence until it is put right, and nothing copies or moves what it refuses to read."""
+    c = make()
+    a = c.add()
+    put(c, [a], [range(10)])
+    s = put(c, [a], [range(10, 13)])
+    with pytest.raises(ValueError, match="different counts"):
+        c.append(s, rows(4), rows(4))
+    for call in (lambda: c.attend(s, q(), 1.0), lambda: c.fork(a), lambda: c.keep([a], [[1, 11]]), lambda: c.resize(20)):
+        with pytest.raises(ValueError, match="not appended"):
+            call()
+    assert held(names, c, c.fork(a, 10)) == list(range(10))
+    c.trim(a, 10)
+    assert c.attend(put(c, [a], [[5]]), q(), 1.0) == "o"
+    c.resize(20)
+    c.keep([a], [[1, 10]])
+    assert held(names, c, a) == [1, 5] and c.attend(c.step([a], [0]), q(), 1.0) == "o"
