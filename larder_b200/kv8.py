@@ -167,9 +167,9 @@ class Cache:
         when the pool has too few free pages (the pages moved from are free only afterwards)."""
         if len(set(handles)) != len(handles) or len(handles) != len(positions):
             raise ValueError("kv8: distinct sequences, a list of positions each")
+        positions = [list(at) for at in positions]
         moves, need = [], 0
         for h, at in zip(handles, positions):
-            at = list(at)
             have = self._seqs[h][1]
             if at and not (at[0] >= 0 and at[-1] < have and all(x < y for x, y in zip(at, at[1:]))):
                 raise ValueError(f"kv8: positions to keep must rise within 0 .. {have - 1}")

@@ -333,3 +333,14 @@ def test_cpu_tensors_are_refused():
                  lambda: kv8.ops.kv8_compact(pages, scales, table, n, cu, table, n)):
         with pytest.raises(ValueError, match="CUDA"):
             call()
+
+
+def test_keep_takes_any_iterable_of_positions(names):
+    c = make()
+    a, b = c.add(), c.add()
+    put(c, [a, b], [range(40), range(100, 140)])
+    c.keep([a, b], [iter([3, 4]), (i for i in range(2))])
+    assert held(names, c, a) == [3, 4] and held(names, c, b) == [100, 101]
+    with pytest.raises(TypeError):
+        c.keep([a, b], [[1], 5])
+    assert c.length(a) == c.length(b) == 2
