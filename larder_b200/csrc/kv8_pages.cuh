@@ -1,6 +1,8 @@
 // Pages of the paged 8-bit cache (kv8.cuh) moved about: whole pages copied, and sequences compacted to the tokens kept.
 #pragma once
 
+#include <cfloat>
+
 #include "common.cuh"
 #include "kv8.cuh"
 #include "rope.cuh"
@@ -374,7 +376,9 @@ __global__ void __launch_bounds__(THREADS, !LAYOUT ? 1024 / THREADS : U == 1 ? 7
         if (turn_it || !(r <= 32768.f) || (__float_as_uint(f[h][i]) & 0x7fffffu) != 0) {
           float2 y[8];
           values(c[h][i], i, turn_it, y);
-          const float2 r2 = make_float2(r, r);
+          // (past fp32's range only where all codes are zeros or NaN: zeros stay zeros)
+          const float rf = r > FLT_MAX ? FLT_MAX : r;
+          const float2 r2 = make_float2(rf, rf);
 #pragma unroll
           for (int e = 0; e < 8; ++e) y[e] = mul2(y[e], r2);
           if (LAYOUT == 2) {
