@@ -28,7 +28,8 @@
 //
 // Softmax in base 2, fp32, one thread a row. As in kv8_attend.cuh the weights carry the values' scale, p' = 2^(s + log2 s_v -
 // m), m the running maximum of s + log2 s_v less 7, l = sum p' / s_v, o = sum p' code_v / l; the maximum moves when it is
-// passed by more than 8, so p' reaches 2^15, the upper end of f16, and keeps f16's 11 bits down to 2^-21 of the largest. bf16 queries go to f16 exactly, a row shifted by a power of two that the score's factor undoes.
+// passed by more than 8, so p' reaches 2^15, the upper end of f16, and keeps f16's 11 bits down to 2^-21 of the largest; scores
+// too large for that arithmetic take a path of their own (loud_weights). bf16 queries go to f16 exactly, a row shifted by a power of two that the score's factor undoes.
 //
 // A NaN code under a weight of 0 would spread to rows that do not see it. Keys past an item's horizon are stored as zeros; a
 // row that comes out NaN is looked at again at the end (row_again), and where a value that it does not see is to blame, taken
@@ -60,6 +61,7 @@ constexpr int PIECES = 4;          // pieces of work listed ahead
 constexpr int TABLES = 8;          // key tiles whose page ids and scales are held
 constexpr uint32_t WHOLE = 256;    // a tile whose 128 keys are all there
 constexpr float TOP = 7.f;         // a weight at the running maximum is 2^TOP
+constexpr float LOUD = 1 << 20;    // from a maximum of this size on, fp32 numbers are 2^-3 and more apart
 constexpr int STATUS_PLAN = 158;
 constexpr int STATUS = arows::STATUS_CHUNK;  // lb2_status: 140 lengths and page ids, 141.. waits
 
@@ -320,6 +322,42 @@ __device__ __forceinline__ void mma_commit(uint32_t lead, uint64_t* bar) {
 __device__ __forceinline__ float shrink(float l, float x) {
   const float h = prefill::ex2f(0.5f * x);
   return l * h * h;
+}
+
+// A row whose maximum is so large that the roundings of the maximum and of a weight's exponent, each half a step between fp32
+// numbers of that size, could lift weights past f16's range, or all of them out of it. (The look for such rows takes 1 % of 2048
+// new of 32768 tokens, 1.21 -> 1.23 ms; a branch in the loop of the weights instead, or their loop twice, 3 to 5 %.)
+__device__ __forceinline__ bool is_loud(float m) { return fabsf(m) >= LOUD && m != -FLT_MAX; }
+
+// The weights of a unit with loud rows, out of line: exponents are the scores as the maximum saw them, each rounded once, less the
+// maximum, so that none is above what the maximum may lag by. P takes the place of S; l with the weights' sum.
+__device__ __noinline__ float loud_weights(uint32_t s_col, const float4* sc, uint32_t marked, float fac, float m, float l) {
+#pragma unroll 1
+  for (int c = 0; c < BH; c += 32) {
+    float x[32];
+    uint32_t pk[16];
+    prefill::tmem_ld32(s_col + c, x);
+    prefill::tmem_wait_ld();
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const float4 f = sc[c / 16 + q];
+      const float mul = fmaxf(fac * f.x, FLT_MIN);
+      float sum = 0.f;
+#pragma unroll
+      for (int e = 0; e < 16; e += 2) {
+        const float a = x[16 * q + e], b = x[16 * q + e + 1];
+        const float y = prefill::ex2f(fmaf(a, mul, f.w) - m), z = prefill::ex2f(fmaf(b, mul, f.w) - m);
+        sum += y + z;
+        pk[8 * q + e / 2] = pack2<__half>(y, z);
+        if (marked >> (c / 16 + q) & 1u)
+          l += prefill::ex2f(fmaf(a, mul, f.y) - m - f.y) + prefill::ex2f(fmaf(b, mul, f.y) - m - f.y);
+      }
+      l = fmaf(sum, f.z, l);
+    }
+    prefill::tmem_st16(s_col + c / 2, pk);
+    prefill::tmem_wait_st();
+  }
+  return l;
 }
 
 // 16 bytes of codes. (volatile: the loads stay ahead of the wait behind them)
@@ -895,6 +933,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
       // the last key that the row sees (rows past the item's are zeros; nothing of them is kept)
       const int lim = !live ? w.horizon - 1 : (p.c.a.causal ? w.len - (w.n - 1 - tok) : w.len) - 1;
       float m = -FLT_MAX, l = 0.f, fac = 0.f;
+      bool far = false;  // the row is loud
       // Waits for the P V of the piece's unit n. (Barriers are waited for within one phase of where they are: S_i comes after
       // the P V of unit i - 4, the buffer's last.)
       auto pv_done = [&](int n) {
@@ -967,41 +1006,50 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const Params p) {
           if (now != m) {
             l = shrink(l, m - now);
             m = now;
+            far = is_loud(m);
           }
         }
-        const bool move = top > m + (TOP + 8.f);
-        if (__any_sync(0xffffffffu, move)) move_to(move ? top - TOP : m, i - (C::WIDE ? 1 : 2));
+        const bool move = top - m > TOP + 8.f;
+        bool loud = false;  // of some of the warp's rows
+        if (__any_sync(0xffffffffu, move || far)) {
+          move_to(move ? top - TOP : m, i - (C::WIDE ? 1 : 2));
+          far = is_loud(m);
+          loud = __any_sync(0xffffffffu, far);
+          if (loud) l = loud_weights(s_col, sc, far_s[slot] >> (4 * half), fac, m, l);
+        }
         if (C::WIDE) {
           m_sh[r] = m;
           __syncwarp();
           if (lane == 0) mbar_arrive(&token[wg * 4 + quarter]);
         }
         // weights; P_i takes the place of S_i
-        uint32_t pk[32];
+        if (!loud) {
+          uint32_t pk[32];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const float4 f = sc[q];
-          const float mul = fmaxf(fac * f.x, FLT_MIN), add = f.w - m;
-          float2 sum = make_float2(0.f, 0.f);
+          for (int q = 0; q < 4; ++q) {
+            const float4 f = sc[q];
+            const float mul = fmaxf(fac * f.x, FLT_MIN), add = f.w - m;
+            float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-          for (int e = 0; e < 16; e += 2) {
-            float2 y = kv8::fma2(make_float2(s[16 * q + e], s[16 * q + e + 1]), make_float2(mul, mul), make_float2(add, add));
-            y.x = prefill::ex2f(y.x), y.y = prefill::ex2f(y.y);
-            sum = add2(sum, y);
-            pk[8 * q + e / 2] = pack2<__half>(y.x, y.y);
+            for (int e = 0; e < 16; e += 2) {
+              float2 y = kv8::fma2(make_float2(s[16 * q + e], s[16 * q + e + 1]), make_float2(mul, mul), make_float2(add, add));
+              y.x = prefill::ex2f(y.x), y.y = prefill::ex2f(y.y);
+              sum = add2(sum, y);
+              pk[8 * q + e / 2] = pack2<__half>(y.x, y.y);
+            }
+            l = fmaf(sum.x + sum.y, f.z, l);
           }
-          l = fmaf(sum.x + sum.y, f.z, l);
-        }
-        for (uint32_t marked = far_s[slot] >> (4 * half) & 15u; marked; marked &= marked - 1) {  // (rare)
-          const int q = __ffs(marked) - 1;
-          const float mul = fmaxf(fac * sc[q].x, FLT_MIN);
-          float x[16];
-          prefill2::tmem_ld16(s_col + 16 * q, x);
-          prefill::tmem_wait_ld();
+          for (uint32_t marked = far_s[slot] >> (4 * half) & 15u; marked; marked &= marked - 1) {  // (rare)
+            const int q = __ffs(marked) - 1;
+            const float mul = fmaxf(fac * sc[q].x, FLT_MIN);
+            float x[16];
+            prefill2::tmem_ld16(s_col + 16 * q, x);
+            prefill::tmem_wait_ld();
 #pragma unroll
-          for (int e = 0; e < 16; ++e) l += prefill::ex2f(fmaf(x[e], mul, -m));
+            for (int e = 0; e < 16; ++e) l += prefill::ex2f(fmaf(x[e], mul, -m));
+          }
+          prefill::tmem_st32(s_col, reinterpret_cast<const float*>(pk));
         }
-        prefill::tmem_st32(s_col, reinterpret_cast<const float*>(pk));
         prefill::tmem_wait_st();
         prefill::tc_fence_before();
         __syncwarp();
