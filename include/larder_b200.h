@@ -395,7 +395,8 @@ int lb2_kv8_attend(const void* q, const int64_t* q_st, const uint8_t* pages, con
  * kv_len[b] cached tokens (int32 [B]; already appended). o = softmax(scale q K^T) V; causal: row i of n sees keys
  * 0 .. kv_len[b] - n + i, else all kv_len[b]; a row that sees none gives zeros, as do rows of no sequence (before cu[0],
  * from cu[B] on).
- *   q, o [Hq, T, D], strides [0..1] for H, T; unit on D; dtype LB2_BF16 / F16, or LB2_F32 (exact CUDA-core kernel);
+ *   q, o [Hq, T, D], strides [0..1] for H, T; unit on D; dtype LB2_BF16 / F16, or LB2_F32 (exact CUDA-core kernel); o
+ *   apart from q: rows that a later token's NaN code reached are taken again from q;
  *   pages, scales, table as lb2_kv8_append; page, D as lb2_kv8_attend; T Hq < 2^30; any finite scale.
  *   workspace: lb2_kv8_attend_packed_workspace_size() bytes, 256-byte aligned, any contents; shared as lb2_kv8_attend's.
  * Codes past kv_len are never used, nor does a later token's value reach a row that does not see it, NaN codes among them.

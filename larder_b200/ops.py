@@ -725,7 +725,7 @@ def kv8_attend_packed(q, pages, scales, table, kv_len, cu, scale, causal=True, o
     """Attention of packed chunks of new tokens over the paged 8-bit cache (lb2_kv8_attend_packed): q [1, Hq, T, D], sequence
     b's rows cu[b] .. cu[b + 1] - 1 (cu int32 [B + 1]) being the last of its kv_len[b] cached tokens (int32 [B], the call's
     own among them, already appended). causal: each row sees the tokens up to its own. For inference: the result is in no
-    autograd graph."""
+    autograd graph. out must not overlap q."""
     (num_pages, _, Hkv, page, D), (B, max_pages), dev = _kv8_pool(pages, scales, table, "kv8_attend_packed")
     if dev != _device():
         return _elsewhere(dev, kv8_attend_packed, q, pages, scales, table, kv_len, cu, scale, causal, out)
@@ -742,6 +742,8 @@ def kv8_attend_packed(q, pages, scales, table, kv_len, cu, scale, causal=True, o
     else:
         _out_like(out, q, "kv8_attend_packed")
         ost = out.stride()
+        if T and out.data_ptr() == q.data_ptr():
+            raise ValueError("kv8_attend_packed: out must not be q's memory (some rows are read a second time)")
     n = lib().lb2_kv8_attend_packed_workspace_size(B, Hq, Hkv, T, D)
     stream = _stream_of(dev)
     ws = _scratch(n or 1, stream)
