@@ -646,12 +646,23 @@ def _kv8_pool(pages, scales, table, what):
     return ps, ts, dev
 
 
+_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+def _elsewhere(dev, call, *args):
+    """A call for tensors of another device than the current one, made there."""
+    with torch.cuda.device(dev):
+        return call(*args)
+
+
 def kv8_append(pages, scales, k, v, table, start, lens=None, cu=None, turns=None, layout="half", amp=1.0):
     """Appends k / v [B, Hkv, T, D] to the paged 8-bit cache in place (lb2_kv8_append): sequence b's tokens become its
     positions start[b] onwards (start int32 [B]), keys rotated by them when turns is given. lens int32 [B]: only the
     first lens[b] tokens of each. cu int32 [B + 1]: k / v are [1, Hkv, T, D] and sequence b's tokens are rows cu[b] to
     cu[b + 1] - 1."""
     (num_pages, _, Hkv, page, D), (B, max_pages), dev = _kv8_pool(pages, scales, table, "kv8_append")
+    if dev != _device():
+        return _elsewhere(dev, kv8_append, pages, scales, k, v, table, start, lens, cu, turns, layout, amp)
     ks, kst, vst = k.shape, k.stride(), v.stride()
     if (len(ks) != 4 or ks != v.shape or k.dtype is not v.dtype or k.get_device() != dev or v.get_device() != dev
             or kst[3] != 1 or vst[3] != 1):
@@ -674,15 +685,6 @@ def kv8_append(pages, scales, k, v, table, start, lens=None, cu=None, turns=None
         check(rc, "kv8_append")
 
 
-_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
-
-
-def _elsewhere(dev, call, *args):
-    """A call for tensors of another device than the current one, made there."""
-    with torch.cuda.device(dev):
-        return call(*args)
-
-
 _KV8_WS = {}  # (B, Hq, Hkv, T, D, page, max_pages, device index) -> workspace bytes
 
 
@@ -691,6 +693,8 @@ def kv8_attend(q, pages, scales, table, kv_len, scale, causal=True, out=None):
     [B] counts the call's own tokens, which are already appended. causal: row t sees keys 0 .. kv_len - T + t. For
     inference: the result is in no autograd graph."""
     (num_pages, _, Hkv, page, D), (B, max_pages), dev = _kv8_pool(pages, scales, table, "kv8_attend")
+    if dev != _device():
+        return _elsewhere(dev, kv8_attend, q, pages, scales, table, kv_len, scale, causal, out)
     qs, qst = q.shape, q.stride()
     if len(qs) != 4 or qs[0] != B or qs[3] != D or q.get_device() != dev or qst[3] != 1:
         raise ValueError("kv8_attend: q must be [B, Hq, T, D] for the table's B and the cache's D and device, with a unit "
