@@ -397,6 +397,7 @@ int lb2_kv8_attend(const void* q, const int64_t* q_st, const uint8_t* pages, con
  * from cu[B] on).
  *   q, o [Hq, T, D], strides [0..1] for H, T; unit on D; dtype LB2_BF16 / F16, or LB2_F32 (exact CUDA-core kernel); o
  *   apart from q: rows that a later token's NaN code reached are taken again from q;
+ *   bf16 queries are held in f16, each row shifted: exactly down to 2^-31 of the row's largest value, within 2^-39 of it below;
  *   pages, scales, table as lb2_kv8_append; page, D as lb2_kv8_attend; T Hq < 2^30; any finite scale.
  *   workspace: lb2_kv8_attend_packed_workspace_size() bytes, 256-byte aligned, any contents; shared as lb2_kv8_attend's.
  * Codes past kv_len are never used, nor does a later token's value reach a row that does not see it, NaN codes among them.

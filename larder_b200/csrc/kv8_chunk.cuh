@@ -29,7 +29,9 @@
 // Softmax in base 2, fp32, one thread a row. As in kv8_attend.cuh the weights carry the values' scale, p' = 2^(s + log2 s_v -
 // m), m the running maximum of s + log2 s_v less 7, l = sum p' / s_v, o = sum p' code_v / l; the maximum moves when it is
 // passed by more than 8, so p' reaches 2^15, the upper end of f16, and keeps f16's 11 bits down to 2^-21 of the largest; scores
-// too large for that arithmetic take a path of their own (loud_weights). bf16 queries go to f16 exactly, a row shifted by a power of two that the score's factor undoes.
+// too large for that arithmetic take a path of their own (loud_weights). bf16 queries go to f16, a row shifted by a power of two
+// that the score's factor undoes, its largest value to [2^14, 2^15): exactly down to 2^-31 of that value, and off by 2^-39 of it at
+// most below (half a step of f16's subnormals).
 //
 // A NaN code under a weight of 0 would spread to rows that do not see it. Keys past an item's horizon are stored as zeros; a
 // row that comes out NaN is looked at again at the end (row_again), and where a value that it does not see is to blame, taken
