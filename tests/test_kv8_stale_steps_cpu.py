@@ -1,9 +1,13 @@
 """kv8.Cache on the host, steps that what happened since has overtaken: which appends and attends are refused, and that none of
 them reaches pages or tokens that are not the step's."""
+import random
+
 import pytest
 import torch
 
-from test_kv8_shared_cpu import D, HK, held, make, names, put, whole  # noqa: F401 (names: the kernels' stand-ins)
+from larder_b200 import kv8
+
+from test_kv8_shared_cpu import D, HK, PAGE, held, make, names, put, whole  # noqa: F401 (names: the kernels' stand-ins)
 
 
 def rows(n):
@@ -228,3 +232,94 @@ def test_an_append_again_that_was_refused(names):
     c.resize(20)
     c.keep([a], [[1, 10]])
     assert held(names, c, a) == [1, 5] and c.attend(c.step([a], [0]), q(), 1.0) == "o"
+
+
+@pytest.mark.parametrize("seed", range(12))
+def test_old_steps_in_any_order(names, monkeypatch, seed):
+    """Random calls with steps held from before: an append is refused or writes its sequences' own tokens and no others, an attend
+    is refused or finds, where its step's table says, the tokens that its sequences have there now."""
+    rng = random.Random(seed)
+    c, fresh = make(20), iter(range(10 ** 6))
+    want, steps, accepted = {c.add(): []}, [], {"append": 0, "attend": 0}
+    monkeypatch.setattr(kv8.ops, "kv8_attend_packed", lambda q, pages, scales, table, *a: table)
+    lacking = {}  # handle -> positions reserved and never appended
+
+    def step(hs, counts):
+        s = c.step(hs, counts)
+        for h, n in zip(hs, counts):
+            at = len(want[h])
+            lacking.setdefault(h, set()).update(range(at, at + n))
+            want[h] += [None] * n
+        steps.append(s)
+        del steps[:-8]
+        return s
+
+    def append(s):
+        new = [[next(fresh) for _ in range(n)] for _, _, n in s.spans]
+        flat = [x for t in new for x in t]
+        k = torch.tensor(flat, dtype=torch.float64).view(1, 1, -1, 1).expand(1, HK, len(flat), D)
+        try:
+            c.append(s, k, k, packed=True)
+        except ValueError:
+            return
+        accepted["append"] += 1
+        for (h, at, n), t in zip(s.spans, new):
+            if n:
+                want[h][at:at + n] = t
+                lacking[h].difference_update(range(at, at + n))
+
+    def attend(s):
+        try:
+            table = c.attend(s, torch.zeros(1, 4, sum(s.counts), D), 1.0, packed=True)
+        except ValueError:
+            return
+        accepted["attend"] += 1
+        at = names["pools"].get(c.pages.data_ptr(), {})
+        for b, (h, first, n) in enumerate(s.spans):
+            for p in range(first + n):
+                if p not in lacking.get(h, ()):
+                    assert at[int(table[b, p // PAGE])][p % PAGE] == want[h][p]
+
+    for _ in range(400):
+        what = rng.choice(["add", "fork", "step", "step", "append", "append", "put", "attend", "attend", "trim", "keep", "drop", "resize"])
+        h = rng.choice(list(want)) if want else None
+        try:
+            if what == "add" or h is None:
+                want[c.add()] = []
+            elif what == "fork":
+                n = rng.randint(0, len(want[h]))
+                want[c.fork(h, n)] = list(want[h][:n])
+            elif what in ("step", "put"):
+                hs = rng.sample(list(want), rng.randint(1, min(3, len(want))))
+                s = step(hs, [rng.choice([0, 1, 3, 20]) for _ in hs])
+                if what == "put":
+                    append(s)
+            elif what in ("append", "attend"):
+                if steps:
+                    (append if what == "append" else attend)(rng.choice(steps))
+            elif what == "trim":
+                n = rng.randint(0, len(want[h]))
+                c.trim(h, n)
+                del want[h][n:]
+                lacking[h] = {p for p in lacking.get(h, ()) if p < n}
+            elif what == "keep":
+                at = sorted(rng.sample(range(len(want[h])), rng.randint(0, len(want[h]))))
+                c.keep([h], [at])
+                want[h] = [want[h][i] for i in at]
+                lacking[h] = set()
+            elif what == "drop":
+                c.drop(h)
+                del want[h]
+                lacking.pop(h, None)
+            else:
+                c.resize(rng.randint(14, 24))
+        except ValueError as e:
+            assert any(x in str(e) for x in ("free", "fit", "not appended")), e
+        whole(c)
+        at = names["pools"].get(c.pages.data_ptr(), {})
+        for x, t in want.items():
+            ids = c._seqs[x][0]
+            for p, v in enumerate(t):
+                if p not in lacking.get(x, ()):
+                    assert at[ids[p // PAGE]][p % PAGE] == v
+    assert accepted["append"] > 20 and accepted["attend"] > 5
