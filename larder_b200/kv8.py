@@ -27,11 +27,17 @@ from . import ops
 
 
 class _Use:
-    """What a step relies on: each sequence's tokens up to ends[handle]; why[handle]: what has happened to them since."""
-    __slots__ = ("ends", "why", "__weakref__")
+    """What a step relies on: each sequence's tokens up to the end of its span; why[handle]: what has happened to them since."""
+    __slots__ = ("spans", "ends", "why", "__weakref__")
 
     def __init__(self, spans):
-        self.ends, self.why = {h: s + n for h, s, n in spans}, {}
+        self.spans, self.ends, self.why = spans, None, {}
+
+    def overtake(self, handle, n, why):
+        if self.ends is None:
+            self.ends = {h: s + c for h, s, c in self.spans}
+        if self.ends.get(handle, 0) > n:
+            self.why.setdefault(handle, why)
 
 
 class Step:
@@ -95,8 +101,7 @@ class Cache:
     def _overtake(self, handle, n, why):
         """A sequence's tokens from position n on are no longer where steps made before have them."""
         for use in list(self._uses):
-            if use.ends.get(handle, 0) > n:
-                use.why.setdefault(handle, why)
+            use.overtake(handle, n, why)
 
     def _moved(self, handle, n):
         self._overtake(handle, n, f"sequence {handle}'s pages have moved")
